@@ -295,6 +295,69 @@ int mg_gemm_i8(const int8_t* A, int M, int K, const int8_t* W, int N, const floa
  * half away from zero (w/scale), +-127); an all-zero tensor gets scale 1. */
 int mg_quantize_f32(const float* w, long long n, int8_t* q, float* scale, int flags, void* stream);
 
+/* ---- Microscaled 4-bit numbers (no reference counterpart) ----
+ * Blocks of 32 neighbouring elements of a row: one scale byte s for 2^(s - 127) (255: the block is NaN) and 16 code bytes,
+ * element 2i in the low half of byte i. A code is the sign bit 8 and the index of the magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6.
+ * For a block whose largest magnitude is a, s = max(0, floor(log2 a) - 2 + 127); elements are rounded to the nearest value,
+ * ties to the even code, beyond 6 to 6; a block with a NaN or an infinity is NaN (s = 255).
+ * A matrix of M rows of K elements has its rows padded with zeros to Kp, the next multiple of 128: codes [M][Kp / 2] and
+ * scales [M][Kp / 32]. Device pointers: codes 16-byte aligned, scales 4-byte aligned, real arrays aligned to their element.
+ * Types of real arrays: */
+#define MG_F32 0
+#define MG_F16 1
+#define MG_BF16 2
+/* x [M][K] (row stride ldx >= K elements) to 4 bits. The padding's codes and scales are written too. With MG_PTR_DEVICE the
+ * work is enqueued on `stream` (NULL: the default stream), nothing is allocated, and the call can be captured. */
+int mg_mx4_quantize(const void* x, int type, int M, int K, long long ldx, uint8_t* codes, uint8_t* scales, int flags,
+                    void* stream);
+/* The values back, y [M][K] with row stride ldy >= K (what lies between the rows is left as it is). Exact for MG_F32, and
+ * rounded once to the nearest for the other types. */
+int mg_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* y, int type, long long ldy, int flags,
+                      void* stream);
+/* C[m][n] = sum_k A[m][k] W[n][k] for two 4-bit matrices A [M][K] and W [N][K] (both padded as above), summed in fp32 and
+ * rounded once to C's type: the 4-bit counterpart of mg_gemm_i8. C [M][N]. */
+int mg_mx4_gemm(const uint8_t* A, const uint8_t* As, int M, int K, const uint8_t* W, const uint8_t* Ws, int N, void* C,
+                int type, int flags, void* stream);
+
+/* ---- A key/value cache in 4 bits, and attention over it (no reference counterpart) ----
+ * n sequences of `heads` key/value heads of head_dim (32, 64, 96 or 128) channels, `capacity` (a multiple of 32) slots each.
+ * Position p < sinks (0 <= sinks < capacity) has slot p for good; a later one has slot sinks + (p - sinks) % ring, with
+ * ring = capacity - sinks: of the positions below a sequence's length, the cache holds the first `sinks` and the last `ring`.
+ * Planes: k and v codes [n][heads][capacity][head_dim / 2], 16-byte aligned; k_scales and v_scales
+ * [n][heads][capacity][head_dim / 32], 4-byte aligned. Memory of any contents may be used: what was not written is not seen.
+ * The caller owns the planes and keeps count of the positions. All pointers of these calls but the structs are device
+ * pointers; the calls enqueue work on `stream`, allocate nothing and can be captured. */
+typedef struct {
+    int n, heads, head_dim, capacity, sinks;
+    uint8_t *k, *k_scales, *v, *v_scales;
+} mg_kv_cache_t;
+/* Rows of a call: element (sequence s, token t, head h, channel d) at data + s * seq + t * token + h * head + d. */
+typedef struct {
+    void* data;
+    long long seq, token, head;
+} mg_kv_rows_t;
+/* Tokens of a call: token t of sequence s sits at position pos[s] + t (pos in [0, 2^30)); only the first counts[s] (0..T; NULL: T)
+ * of its T rows are there, the others are neither read nor written. */
+/* Quantises new key and value rows [n][T][heads][head_dim] into their slots. Of two tokens of a call that share a slot the
+ * later one is kept. */
+int mg_kv_write(const mg_kv_cache_t* cache, const mg_kv_rows_t* k, const mg_kv_rows_t* v, int type, int T,
+                const int32_t* pos, const int32_t* counts, void* stream);
+/* Reads rows back. lens[s]: the sequence's length (NULL: pos[s] + counts[s]). A position that the cache does not hold reads as
+ * zeros. */
+int mg_kv_read(const mg_kv_cache_t* cache, const mg_kv_rows_t* k, const mg_kv_rows_t* v, int type, int T, const int32_t* pos,
+               const int32_t* counts, const int32_t* lens, void* stream);
+/* Causal attention of query rows [n][T][q_heads][head_dim] (q_heads a multiple of the cache's heads; query head i reads head
+ * i / (q_heads / heads)) over the cache, after the call's own keys were written: sequence s has length pos[s] + counts[s], and
+ * the row at position p sees the held positions j <= p with j > p - window, or any if window <= 0, and those with j < sinks.
+ * out = sum softmax(scale q.k) v, zeros for a row that sees nothing; statistics and sums in fp32. Rows past counts[s] are left
+ * as they are. A NaN or infinity in a key or value reaches the rows that see it only. workspace: device memory of
+ * mg_kv_attention_workspace bytes, 16-byte aligned, for this call alone until it has run (calls that may overlap, and captured
+ * graphs that may, need one each); may be NULL where that is 0. */
+long long mg_kv_attention_workspace(const mg_kv_cache_t* cache, int q_heads, int T, int window);
+int mg_kv_attention(const mg_kv_cache_t* cache, const mg_kv_rows_t* q, const mg_kv_rows_t* out, int type, int q_heads, int T,
+                    const int32_t* pos, const int32_t* counts, int window, float scale, void* workspace,
+                    long long workspace_bytes, void* stream);
+
 /* Engine options, no reference counterpart: where two implementations of a stage exist, which one runs,
  * for every model of the process. Value 0 (the default) chooses automatically. Small models (state size up
  * to 128, hidden size up to 256, heads of up to 32 over spans of up to 65 keys) run sequences of up to 128 tokens

@@ -17,6 +17,7 @@ MG_ERR_DEVICE = -3
 MG_ERR_NOMEM = -4
 MG_ERR_UNSUPPORTED = -5
 MG_PTR_DEVICE = 1
+MG_F32, MG_F16, MG_BF16 = 0, 1, 2
 MG_OPT_GEMM_KERNEL, MG_OPT_ATTENTION_KERNEL, MG_OPT_SCAN_KERNEL = 0, 1, 2
 MG_GEMM_STREAM, MG_GEMM_SLAB = 1, 2
 MG_ATTN_EXACT, MG_ATTN_MFMA, MG_ATTN_FUSED = 1, 2, 3
@@ -58,6 +59,17 @@ class KernelTime(ctypes.Structure):
                 ("bytes", ctypes.c_double), ("ops", ctypes.c_double)]
 
 
+class KvCache(ctypes.Structure):
+    """mg_kv_cache_t: a 4-bit key/value cache's sizes and planes."""
+    _fields_ = [("n", _int), ("heads", _int), ("head_dim", _int), ("capacity", _int), ("sinks", _int),
+                ("k", _vp), ("k_scales", _vp), ("v", _vp), ("v_scales", _vp)]
+
+
+class KvRows(ctypes.Structure):
+    """mg_kv_rows_t: rows of a cache call and their strides in elements."""
+    _fields_ = [("data", _vp), ("seq", _ll), ("token", _ll), ("head", _ll)]
+
+
 # name -> (restype, argtypes); the exported set of include/mignon_hip.h
 SIGNATURES = {
     "mg_last_error": (ctypes.c_char_p, []),
@@ -85,6 +97,13 @@ SIGNATURES = {
     "mg_sessions_free": (None, [_vp]),
     "mg_gemm_i8": (_int, [_vp, _int, _int, _vp, _int, _vp, _vp, _vp, _int, _vp]),
     "mg_quantize_f32": (_int, [_vp, _ll, _vp, _vp, _int, _vp]),
+    "mg_mx4_quantize": (_int, [_vp, _int, _int, _int, _ll, _vp, _vp, _int, _vp]),
+    "mg_mx4_dequantize": (_int, [_vp, _vp, _int, _int, _vp, _int, _ll, _int, _vp]),
+    "mg_mx4_gemm": (_int, [_vp, _vp, _int, _int, _vp, _vp, _int, _vp, _int, _int, _vp]),
+    "mg_kv_write": (_int, [_vp, _vp, _vp, _int, _int, _vp, _vp, _vp]),
+    "mg_kv_read": (_int, [_vp, _vp, _vp, _int, _int, _vp, _vp, _vp, _vp]),
+    "mg_kv_attention_workspace": (_ll, [_vp, _int, _int, _int]),
+    "mg_kv_attention": (_int, [_vp, _vp, _vp, _int, _int, _int, _vp, _vp, _int, ctypes.c_float, _vp, _ll, _vp]),
     "mg_engine_option": (_int, [_int, _int]),
     "mg_score_sequences": (_int, [_vp, _vp, _vp, _int, _int, _vp]),
     "mg_tokenizer_load": (_int, [_u8p, ctypes.c_size_t, ctypes.POINTER(_vp)]),

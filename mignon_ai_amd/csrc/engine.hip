@@ -30,6 +30,7 @@
 #include "gemm.hpp"
 #include "kernels.hpp"
 #include "model_file.hpp"
+#include "mx4.hpp"
 #include "options.hpp"
 #include "sample.hpp"
 #include "seq.hpp"
@@ -1201,6 +1202,53 @@ int guarded(F&& f) {
         g_last_error = e.what();
         return MG_ERR_FORMAT;
     }
+}
+
+bool real_type(int type) { return type == MG_F32 || type == MG_F16 || type == MG_BF16; }
+bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
+// Elements of a 4-bit row, and channels of a product, at most.
+constexpr int kMx4MaxK = 1 << 24;
+
+KvRows kv_rows(const mg_kv_rows_t* r) {
+    KvRows x;
+    x.data = r->data; x.seq = r->seq; x.token = r->token; x.head = r->head;
+    return x;
+}
+
+// The cache of a call, checked. False: it has no sequences.
+bool kv_cache(const std::string& who, const mg_kv_cache_t* c, int T, KvCache& x) {
+    require(c, who + ": null argument");
+    require(kv_head_width(c->head_dim), who + ": head_dim " + std::to_string(c->head_dim) + " (32, 64, 96 and 128 are there)");
+    require(c->n >= 0 && c->heads > 0 && c->heads <= 4096 && T >= 0 && T < kKvMaxPos, who + ": bad shape");
+    require(c->capacity > 0 && c->capacity % 32 == 0 && c->capacity < kKvMaxPos, who + ": capacity is a multiple of 32");
+    require(c->sinks >= 0 && c->sinks < c->capacity, who + ": sinks leave no slot for later positions");
+    require((long long)c->n * std::max(T, 1) * c->heads < (1LL << 31), who + ": too many rows");
+    if (c->n == 0 || T == 0) return false;
+    require(c->k && c->k_scales && c->v && c->v_scales, who + ": null argument");
+    require(aligned(c->k, 16) && aligned(c->v, 16) && aligned(c->k_scales, 4) && aligned(c->v_scales, 4), who + ": misaligned plane");
+    x.n = c->n; x.heads = c->heads; x.dh = c->head_dim; x.cap = c->capacity; x.sinks = c->sinks;
+    x.k = c->k; x.ks = c->k_scales; x.v = c->v; x.vs = c->v_scales;
+    return true;
+}
+
+bool kv_rows_args(const std::string& who, const mg_kv_cache_t* c, const mg_kv_rows_t* k, const mg_kv_rows_t* v, int type, int T,
+                  const int32_t* pos, const int32_t* counts, KvRowsArgs& a) {
+    if (!kv_cache(who, c, T, a.c)) return false;
+    require(k && v && k->data && v->data && pos, who + ": null argument");
+    require(real_type(type), who + ": unknown type");
+    require(aligned(k->data, real_size(type)) && aligned(v->data, real_size(type)), who + ": misaligned pointer");
+    a.k = kv_rows(k); a.v = kv_rows(v);
+    a.type = type; a.T = T; a.pos = pos; a.counts = counts;
+    return true;
+}
+
+bool kv_attention_args(const std::string& who, const mg_kv_cache_t* c, int q_heads, int T, int window, KvAttnArgs& a) {
+    if (!kv_cache(who, c, T, a.c)) return false;
+    require(q_heads > 0 && q_heads <= 65536 && q_heads % c->heads == 0, who + ": q_heads is a multiple of the cache's heads");
+    require((long long)c->n * T * q_heads < (1LL << 31), who + ": too many rows");
+    a.T = T; a.group = q_heads / c->heads;
+    a.window = window >= kKvMaxPos ? 0 : std::max(window, 0);  // positions are below kKvMaxPos: such a window hides nothing
+    return true;
 }
 
 // Tokens per workspace pass of a teacher-forced batch, at most. c5's 2^21 tokens in one pass: 170.9 ms per
@@ -2479,6 +2527,146 @@ int mg_quantize_f32(const float* w, long long n, int8_t* q, float* scale, int fl
         } else {
             HIPCHECK(hipStreamSynchronize(st));  // the temporaries above are released on return
         }
+        return MG_OK;
+    });
+}
+
+int mg_mx4_quantize(const void* x, int type, int M, int K, long long ldx, uint8_t* codes, uint8_t* scales, int flags,
+                    void* stream) {
+    return guarded([&] {
+        require(x && codes && scales, "mg_mx4_quantize: null argument");
+        require(real_type(type), "mg_mx4_quantize: unknown type");
+        require(M >= 0 && K > 0 && K <= kMx4MaxK && ldx >= K, "mg_mx4_quantize: bad shape");
+        if (M == 0) return MG_OK;
+        hipStream_t st = (hipStream_t)stream;
+        const bool dev = flags & MG_PTR_DEVICE;
+        const size_t e = real_size(type), kp = round_up(K, 128), nc = M * (kp / 2), ns = M * (kp / 32);
+        Staging sg;
+        Mx4RowsArgs a;
+        a.type = type; a.M = M; a.K = K; a.ld = dev ? ldx : K;
+        a.codes = codes; a.scales = scales; a.x = x;
+        if (!dev) {
+            uint8_t* xd = sg.out<uint8_t>((size_t)M * K * e);
+            HIPCHECK(hipMemcpy2DAsync(xd, K * e, x, ldx * e, K * e, M, hipMemcpyHostToDevice, st));
+            a.x = xd;
+            a.codes = sg.out<uint8_t>(nc);
+            a.scales = sg.out<uint8_t>(ns);
+        }
+        require(aligned(a.x, e) && aligned(a.codes, 16) && aligned(a.scales, 4), "mg_mx4_quantize: misaligned pointer");
+        HIPCHECK(launch_mx4_quantize(a, st));
+        if (!dev) {
+            HIPCHECK(hipMemcpyAsync(codes, a.codes, nc, hipMemcpyDeviceToHost, st));
+            HIPCHECK(hipMemcpyAsync(scales, a.scales, ns, hipMemcpyDeviceToHost, st));
+            HIPCHECK(hipStreamSynchronize(st));
+        }
+        return MG_OK;
+    });
+}
+
+int mg_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* y, int type, long long ldy, int flags,
+                      void* stream) {
+    return guarded([&] {
+        require(y && codes && scales, "mg_mx4_dequantize: null argument");
+        require(real_type(type), "mg_mx4_dequantize: unknown type");
+        require(M >= 0 && K > 0 && K <= kMx4MaxK && ldy >= K, "mg_mx4_dequantize: bad shape");
+        if (M == 0) return MG_OK;
+        hipStream_t st = (hipStream_t)stream;
+        const bool dev = flags & MG_PTR_DEVICE;
+        const size_t e = real_size(type), kp = round_up(K, 128), nc = M * (kp / 2), ns = M * (kp / 32);
+        Staging sg;
+        Mx4RowsArgs a;
+        a.type = type; a.M = M; a.K = K; a.ld = dev ? ldy : K;
+        a.codes = const_cast<uint8_t*>(dev ? codes : sg.in(codes, nc, st));
+        a.scales = const_cast<uint8_t*>(dev ? scales : sg.in(scales, ns, st));
+        a.y = dev ? y : sg.out<uint8_t>((size_t)M * K * e);
+        require(aligned(a.y, e) && aligned(a.codes, 16) && aligned(a.scales, 4), "mg_mx4_dequantize: misaligned pointer");
+        HIPCHECK(launch_mx4_dequantize(a, st));
+        if (!dev) {
+            HIPCHECK(hipMemcpy2DAsync(y, ldy * e, a.y, K * e, K * e, M, hipMemcpyDeviceToHost, st));
+            HIPCHECK(hipStreamSynchronize(st));
+        }
+        return MG_OK;
+    });
+}
+
+int mg_mx4_gemm(const uint8_t* A, const uint8_t* As, int M, int K, const uint8_t* W, const uint8_t* Ws, int N, void* C,
+                int type, int flags, void* stream) {
+    return guarded([&] {
+        require(A && As && W && Ws && C, "mg_mx4_gemm: null argument");
+        require(real_type(type), "mg_mx4_gemm: unknown type");
+        require(M >= 0 && K > 0 && K <= kMx4MaxK && N > 0 && N <= kMx4MaxK, "mg_mx4_gemm: bad shape");
+        if (M == 0) return MG_OK;
+        hipStream_t st = (hipStream_t)stream;
+        const bool dev = flags & MG_PTR_DEVICE;
+        const size_t e = real_size(type), kp = round_up(K, 128), out = (size_t)M * N * e;
+        Staging sg;
+        Mx4GemmArgs a;
+        a.M = M; a.N = N; a.Kp = (int)kp; a.type = type;
+        a.A = dev ? A : sg.in(A, M * (kp / 2), st);
+        a.As = dev ? As : sg.in(As, M * (kp / 32), st);
+        a.W = dev ? W : sg.in(W, N * (kp / 2), st);
+        a.Ws = dev ? Ws : sg.in(Ws, N * (kp / 32), st);
+        a.C = dev ? C : sg.out<uint8_t>(out);
+        require(aligned(a.A, 16) && aligned(a.W, 16) && aligned(a.As, 4) && aligned(a.Ws, 4) && aligned(a.C, e),
+                "mg_mx4_gemm: misaligned pointer");
+        HIPCHECK(launch_mx4_gemm(a, st));
+        if (!dev) {
+            HIPCHECK(hipMemcpyAsync(C, a.C, out, hipMemcpyDeviceToHost, st));
+            HIPCHECK(hipStreamSynchronize(st));
+        }
+        return MG_OK;
+    });
+}
+
+int mg_kv_write(const mg_kv_cache_t* cache, const mg_kv_rows_t* k, const mg_kv_rows_t* v, int type, int T, const int32_t* pos,
+                const int32_t* counts, void* stream) {
+    return guarded([&] {
+        KvRowsArgs a;
+        if (!kv_rows_args("mg_kv_write", cache, k, v, type, T, pos, counts, a)) return MG_OK;
+        HIPCHECK(launch_kv_write(a, (hipStream_t)stream));
+        return MG_OK;
+    });
+}
+
+int mg_kv_read(const mg_kv_cache_t* cache, const mg_kv_rows_t* k, const mg_kv_rows_t* v, int type, int T, const int32_t* pos,
+               const int32_t* counts, const int32_t* lens, void* stream) {
+    return guarded([&] {
+        KvRowsArgs a;
+        if (!kv_rows_args("mg_kv_read", cache, k, v, type, T, pos, counts, a)) return MG_OK;
+        a.lens = lens;
+        HIPCHECK(launch_kv_read(a, (hipStream_t)stream));
+        return MG_OK;
+    });
+}
+
+long long mg_kv_attention_workspace(const mg_kv_cache_t* cache, int q_heads, int T, int window) {
+    long long bytes = 0;
+    const int rc = guarded([&] {
+        KvAttnArgs a;
+        if (kv_attention_args("mg_kv_attention_workspace", cache, q_heads, T, window, a)) bytes = (long long)kv_attention_ws_bytes(a);
+        return MG_OK;
+    });
+    return rc < 0 ? rc : bytes;
+}
+
+int mg_kv_attention(const mg_kv_cache_t* cache, const mg_kv_rows_t* q, const mg_kv_rows_t* out, int type, int q_heads, int T,
+                    const int32_t* pos, const int32_t* counts, int window, float scale, void* workspace,
+                    long long workspace_bytes, void* stream) {
+    return guarded([&] {
+        const char* who = "mg_kv_attention";
+        KvAttnArgs a;
+        if (!kv_attention_args(who, cache, q_heads, T, window, a)) return MG_OK;
+        require(q && out && q->data && out->data && pos, "mg_kv_attention: null argument");
+        require(real_type(type), "mg_kv_attention: unknown type");
+        require(aligned(q->data, real_size(type)) && aligned(out->data, real_size(type)) && aligned(workspace, 16),
+                "mg_kv_attention: misaligned pointer");
+        a.q = kv_rows(q); a.out = kv_rows(out);
+        a.type = type; a.pos = pos; a.counts = counts; a.scale = scale;
+        const size_t need = kv_attention_ws_bytes(a);
+        require(need == 0 || (workspace && workspace_bytes >= 0 && (size_t)workspace_bytes >= need),
+                "mg_kv_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) + " needed");
+        a.ws = (float*)workspace;
+        HIPCHECK(launch_kv_attention(a, (hipStream_t)stream));
         return MG_OK;
     });
 }
