@@ -76,6 +76,12 @@ void require(bool ok, const std::string& msg) {
     if (!ok) throw Error(MG_ERR_INVALID, msg);
 }
 
+// The same for calls of a few microseconds: the message is put together only when it is thrown.
+#define REQUIRE(ok, msg) \
+    do { \
+        if (!(ok)) throw Error(MG_ERR_INVALID, msg); \
+    } while (0)
+
 struct DevBuf {
     void* p = nullptr;
     size_t n = 0;
@@ -1216,36 +1222,36 @@ KvRows kv_rows(const mg_kv_rows_t* r) {
 }
 
 // The cache of a call, checked. False: it has no sequences.
-bool kv_cache(const std::string& who, const mg_kv_cache_t* c, int T, KvCache& x) {
-    require(c, who + ": null argument");
-    require(kv_head_width(c->head_dim), who + ": head_dim " + std::to_string(c->head_dim) + " (32, 64, 96 and 128 are there)");
-    require(c->n >= 0 && c->heads > 0 && c->heads <= 4096 && T >= 0 && T < kKvMaxPos, who + ": bad shape");
-    require(c->capacity > 0 && c->capacity % 32 == 0 && c->capacity < kKvMaxPos, who + ": capacity is a multiple of 32");
-    require(c->sinks >= 0 && c->sinks < c->capacity, who + ": sinks leave no slot for later positions");
-    require((long long)c->n * std::max(T, 1) * c->heads < (1LL << 31), who + ": too many rows");
+bool kv_cache(const char* who, const mg_kv_cache_t* c, int T, KvCache& x) {
+    REQUIRE(c, std::string(who) + ": null argument");
+    REQUIRE(kv_head_width(c->head_dim), std::string(who) + ": head_dim " + std::to_string(c->head_dim) + " (32, 64, 96 and 128 are there)");
+    REQUIRE(c->n >= 0 && c->heads > 0 && c->heads <= 4096 && T >= 0 && T < kKvMaxPos, std::string(who) + ": bad shape");
+    REQUIRE(c->capacity > 0 && c->capacity % 32 == 0 && c->capacity < kKvMaxPos, std::string(who) + ": capacity is a multiple of 32");
+    REQUIRE(c->sinks >= 0 && c->sinks < c->capacity, std::string(who) + ": sinks leave no slot for later positions");
+    REQUIRE((long long)c->n * std::max(T, 1) * c->heads < (1LL << 31), std::string(who) + ": too many rows");
     if (c->n == 0 || T == 0) return false;
-    require(c->k && c->k_scales && c->v && c->v_scales, who + ": null argument");
-    require(aligned(c->k, 16) && aligned(c->v, 16) && aligned(c->k_scales, 4) && aligned(c->v_scales, 4), who + ": misaligned plane");
+    REQUIRE(c->k && c->k_scales && c->v && c->v_scales, std::string(who) + ": null argument");
+    REQUIRE(aligned(c->k, 16) && aligned(c->v, 16) && aligned(c->k_scales, 4) && aligned(c->v_scales, 4), std::string(who) + ": misaligned plane");
     x.n = c->n; x.heads = c->heads; x.dh = c->head_dim; x.cap = c->capacity; x.sinks = c->sinks;
     x.k = c->k; x.ks = c->k_scales; x.v = c->v; x.vs = c->v_scales;
     return true;
 }
 
-bool kv_rows_args(const std::string& who, const mg_kv_cache_t* c, const mg_kv_rows_t* k, const mg_kv_rows_t* v, int type, int T,
+bool kv_rows_args(const char* who, const mg_kv_cache_t* c, const mg_kv_rows_t* k, const mg_kv_rows_t* v, int type, int T,
                   const int32_t* pos, const int32_t* counts, KvRowsArgs& a) {
     if (!kv_cache(who, c, T, a.c)) return false;
-    require(k && v && k->data && v->data && pos, who + ": null argument");
-    require(real_type(type), who + ": unknown type");
-    require(aligned(k->data, real_size(type)) && aligned(v->data, real_size(type)), who + ": misaligned pointer");
+    REQUIRE(k && v && k->data && v->data && pos, std::string(who) + ": null argument");
+    REQUIRE(real_type(type), std::string(who) + ": unknown type");
+    REQUIRE(aligned(k->data, real_size(type)) && aligned(v->data, real_size(type)), std::string(who) + ": misaligned pointer");
     a.k = kv_rows(k); a.v = kv_rows(v);
     a.type = type; a.T = T; a.pos = pos; a.counts = counts;
     return true;
 }
 
-bool kv_attention_args(const std::string& who, const mg_kv_cache_t* c, int q_heads, int T, int window, KvAttnArgs& a) {
+bool kv_attention_args(const char* who, const mg_kv_cache_t* c, int q_heads, int T, int window, KvAttnArgs& a) {
     if (!kv_cache(who, c, T, a.c)) return false;
-    require(q_heads > 0 && q_heads <= 65536 && q_heads % c->heads == 0, who + ": q_heads is a multiple of the cache's heads");
-    require((long long)c->n * T * q_heads < (1LL << 31), who + ": too many rows");
+    REQUIRE(q_heads > 0 && q_heads <= 65536 && q_heads % c->heads == 0, std::string(who) + ": q_heads is a multiple of the cache's heads");
+    REQUIRE((long long)c->n * T * q_heads < (1LL << 31), std::string(who) + ": too many rows");
     a.T = T; a.group = q_heads / c->heads;
     a.window = window >= kKvMaxPos ? 0 : std::max(window, 0);  // positions are below kKvMaxPos: such a window hides nothing
     return true;
@@ -2534,9 +2540,9 @@ int mg_quantize_f32(const float* w, long long n, int8_t* q, float* scale, int fl
 int mg_mx4_quantize(const void* x, int type, int M, int K, long long ldx, uint8_t* codes, uint8_t* scales, int flags,
                     void* stream) {
     return guarded([&] {
-        require(x && codes && scales, "mg_mx4_quantize: null argument");
-        require(real_type(type), "mg_mx4_quantize: unknown type");
-        require(M >= 0 && K > 0 && K <= kMx4MaxK && ldx >= K, "mg_mx4_quantize: bad shape");
+        REQUIRE(x && codes && scales, "mg_mx4_quantize: null argument");
+        REQUIRE(real_type(type), "mg_mx4_quantize: unknown type");
+        REQUIRE(M >= 0 && K > 0 && K <= kMx4MaxK && ldx >= K, "mg_mx4_quantize: bad shape");
         if (M == 0) return MG_OK;
         hipStream_t st = (hipStream_t)stream;
         const bool dev = flags & MG_PTR_DEVICE;
@@ -2552,7 +2558,7 @@ int mg_mx4_quantize(const void* x, int type, int M, int K, long long ldx, uint8_
             a.codes = sg.out<uint8_t>(nc);
             a.scales = sg.out<uint8_t>(ns);
         }
-        require(aligned(a.x, e) && aligned(a.codes, 16) && aligned(a.scales, 4), "mg_mx4_quantize: misaligned pointer");
+        REQUIRE(aligned(a.x, e) && aligned(a.codes, 16) && aligned(a.scales, 4), "mg_mx4_quantize: misaligned pointer");
         HIPCHECK(launch_mx4_quantize(a, st));
         if (!dev) {
             HIPCHECK(hipMemcpyAsync(codes, a.codes, nc, hipMemcpyDeviceToHost, st));
@@ -2566,9 +2572,9 @@ int mg_mx4_quantize(const void* x, int type, int M, int K, long long ldx, uint8_
 int mg_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* y, int type, long long ldy, int flags,
                       void* stream) {
     return guarded([&] {
-        require(y && codes && scales, "mg_mx4_dequantize: null argument");
-        require(real_type(type), "mg_mx4_dequantize: unknown type");
-        require(M >= 0 && K > 0 && K <= kMx4MaxK && ldy >= K, "mg_mx4_dequantize: bad shape");
+        REQUIRE(y && codes && scales, "mg_mx4_dequantize: null argument");
+        REQUIRE(real_type(type), "mg_mx4_dequantize: unknown type");
+        REQUIRE(M >= 0 && K > 0 && K <= kMx4MaxK && ldy >= K, "mg_mx4_dequantize: bad shape");
         if (M == 0) return MG_OK;
         hipStream_t st = (hipStream_t)stream;
         const bool dev = flags & MG_PTR_DEVICE;
@@ -2579,7 +2585,7 @@ int mg_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K,
         a.codes = const_cast<uint8_t*>(dev ? codes : sg.in(codes, nc, st));
         a.scales = const_cast<uint8_t*>(dev ? scales : sg.in(scales, ns, st));
         a.y = dev ? y : sg.out<uint8_t>((size_t)M * K * e);
-        require(aligned(a.y, e) && aligned(a.codes, 16) && aligned(a.scales, 4), "mg_mx4_dequantize: misaligned pointer");
+        REQUIRE(aligned(a.y, e) && aligned(a.codes, 16) && aligned(a.scales, 4), "mg_mx4_dequantize: misaligned pointer");
         HIPCHECK(launch_mx4_dequantize(a, st));
         if (!dev) {
             HIPCHECK(hipMemcpy2DAsync(y, ldy * e, a.y, K * e, K * e, M, hipMemcpyDeviceToHost, st));
@@ -2592,9 +2598,9 @@ int mg_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K,
 int mg_mx4_gemm(const uint8_t* A, const uint8_t* As, int M, int K, const uint8_t* W, const uint8_t* Ws, int N, void* C,
                 int type, int flags, void* stream) {
     return guarded([&] {
-        require(A && As && W && Ws && C, "mg_mx4_gemm: null argument");
-        require(real_type(type), "mg_mx4_gemm: unknown type");
-        require(M >= 0 && K > 0 && K <= kMx4MaxK && N > 0 && N <= kMx4MaxK, "mg_mx4_gemm: bad shape");
+        REQUIRE(A && As && W && Ws && C, "mg_mx4_gemm: null argument");
+        REQUIRE(real_type(type), "mg_mx4_gemm: unknown type");
+        REQUIRE(M >= 0 && K > 0 && K <= kMx4MaxK && N > 0 && N <= kMx4MaxK, "mg_mx4_gemm: bad shape");
         if (M == 0) return MG_OK;
         hipStream_t st = (hipStream_t)stream;
         const bool dev = flags & MG_PTR_DEVICE;
@@ -2607,7 +2613,7 @@ int mg_mx4_gemm(const uint8_t* A, const uint8_t* As, int M, int K, const uint8_t
         a.W = dev ? W : sg.in(W, N * (kp / 2), st);
         a.Ws = dev ? Ws : sg.in(Ws, N * (kp / 32), st);
         a.C = dev ? C : sg.out<uint8_t>(out);
-        require(aligned(a.A, 16) && aligned(a.W, 16) && aligned(a.As, 4) && aligned(a.Ws, 4) && aligned(a.C, e),
+        REQUIRE(aligned(a.A, 16) && aligned(a.W, 16) && aligned(a.As, 4) && aligned(a.Ws, 4) && aligned(a.C, e),
                 "mg_mx4_gemm: misaligned pointer");
         HIPCHECK(launch_mx4_gemm(a, st));
         if (!dev) {
@@ -2656,14 +2662,14 @@ int mg_kv_attention(const mg_kv_cache_t* cache, const mg_kv_rows_t* q, const mg_
         const char* who = "mg_kv_attention";
         KvAttnArgs a;
         if (!kv_attention_args(who, cache, q_heads, T, window, a)) return MG_OK;
-        require(q && out && q->data && out->data && pos, "mg_kv_attention: null argument");
-        require(real_type(type), "mg_kv_attention: unknown type");
-        require(aligned(q->data, real_size(type)) && aligned(out->data, real_size(type)) && aligned(workspace, 16),
+        REQUIRE(q && out && q->data && out->data && pos, "mg_kv_attention: null argument");
+        REQUIRE(real_type(type), "mg_kv_attention: unknown type");
+        REQUIRE(aligned(q->data, real_size(type)) && aligned(out->data, real_size(type)) && aligned(workspace, 16),
                 "mg_kv_attention: misaligned pointer");
         a.q = kv_rows(q); a.out = kv_rows(out);
         a.type = type; a.pos = pos; a.counts = counts; a.scale = scale;
         const size_t need = kv_attention_ws_bytes(a);
-        require(need == 0 || (workspace && workspace_bytes >= 0 && (size_t)workspace_bytes >= need),
+        REQUIRE(need == 0 || (workspace && workspace_bytes >= 0 && (size_t)workspace_bytes >= need),
                 "mg_kv_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) + " needed");
         a.ws = (float*)workspace;
         HIPCHECK(launch_kv_attention(a, (hipStream_t)stream));

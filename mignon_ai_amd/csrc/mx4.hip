@@ -2,6 +2,8 @@
 #include "mx4.hpp"
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "common.hpp"
 #include "mx4_device.hpp"
@@ -61,42 +63,339 @@ RowsGrid rows_grid(int M, int lanes) {
 // C = A W^T on v_mfma_scale_f32_16x16x128_f8f6f4. Both operands' rows are read in the instruction's layout: lane L holds row
 // (L & 15) and block L >> 4 of a 128-element step, sixteen code bytes and one scale byte.
 //
-// A workgroup of `waves` waves computes 16 channels x 16 rows, each wave over its share of the steps, and adds the waves'
-// sums in LDS, in the waves' order.
+// One 16-byte load per lane from global memory straight into LDS: lane L's bytes land at LDS offset lds + 16 L (four bytes: lds +
+// 4 L). Inline assembly, with the waits written out (vm_wait), because the compiler would wait for all such loads before any LDS
+// read. The LDS address goes through M0; the s_nop covers the wait states between a vector instruction's write of the scalar base
+// and its use, and those of M0. No register receives anything.
+__device__ __forceinline__ void lds_load16(const uint8_t* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0", "memory");
+}
+__device__ __forceinline__ void lds_load4(const uint8_t* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0", "memory");
+}
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+
+// Four neighbouring channels of a row, `left` of which exist; vec: such a run is aligned.
 template <class T>
-__global__ __launch_bounds__(512) void mx4_gemm_tile_kernel(Mx4GemmArgs a) {
-    __shared__ v4f part[7][64];
-    const int L = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int n0 = blockIdx.x * 16;
-    const int steps = a.Kp / 128;
-    for (int m0 = blockIdx.y * 16; m0 < a.M; m0 += gridDim.y * 16) {
-        const long long wr = min(n0 + (L & 15), a.N - 1), ar = min(m0 + (L & 15), a.M - 1);
-        const uint8_t* wp = a.W + wr * (a.Kp / 2) + 16 * (L >> 4);
-        const uint8_t* ap = a.A + ar * (a.Kp / 2) + 16 * (L >> 4);
-        const uint8_t* wsp = a.Ws + wr * (a.Kp / 32) + (L >> 4);
-        const uint8_t* asp = a.As + ar * (a.Kp / 32) + (L >> 4);
-        v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k = wave; k < steps; k += waves) {
-            const uint4 wq = *(const uint4*)(wp + 64LL * k), aq = *(const uint4*)(ap + 64LL * k);
-            const int ws = wsp[4 * k], as = asp[4 * k];
-            const v8i wv = {(int)wq.x, (int)wq.y, (int)wq.z, (int)wq.w, 0, 0, 0, 0};
-            const v8i av = {(int)aq.x, (int)aq.y, (int)aq.z, (int)aq.w, 0, 0, 0, 0};
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, acc, 4, 4, 0, ws, 0, as);
-        }
-        if (wave) part[wave - 1][L] = acc;
-        __syncthreads();
-        if (wave == 0) {
-            for (int w = 1; w < waves; w++) acc += part[w - 1][L];
-            // lane L: row m0 + (L & 15), channels n0 + 4 (L >> 4) .. + 3
-            const int m = m0 + (L & 15), n = n0 + 4 * (L >> 4);
-            T* out = (T*)a.C + (long long)m * a.N + n;
-            if (m < a.M)
+__device__ __forceinline__ void store4(T* out, v4f v, int left, int vec) {
+    if (vec && left >= 4) {
+        T t[4];
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (n + r < a.N) out[r] = (T)acc[r];
-        }
-        __syncthreads();
+        for (int r = 0; r < 4; r++) t[r] = (T)v[r];
+        if constexpr (sizeof(T) == 4) *(uint4*)out = *(uint4*)t;
+        else *(uint2*)out = *(uint2*)t;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (r < left) out[r] = (T)v[r];
     }
+}
+
+// A workgroup of up to NW waves computes 16 FN channels x 16 FM rows, each wave over its own share of K, and adds the waves' sums in
+// LDS, in the waves' order: for products with too few tiles to fill the chip, whose time is the latency of a tile's steps. A
+// wave's shares are runs of four steps; it loads them into four LDS slots of its own, which no other wave touches (no
+// barriers), and reloads a slot once its products were issued. Slots and scales as in the large form.
+template <int FN_, int FM_, int NW_>
+struct MxSplit {
+    static constexpr int FN = FN_, FM = FM_, NW = NW_, F = FN + FM;
+    static constexpr int wave_lds = 4 * F * 1024 + 2 * F * 256, lds = NW * wave_lds;
+    static_assert(4 * F <= 63 && lds <= 160 * 1024, "");
+};
+
+template <class S, class T>
+__global__ __launch_bounds__(S::NW * 64) void mx4_gemm_split_kernel(Mx4GemmArgs a, int vec) {
+    extern __shared__ uint8_t smem[];
+    constexpr int FN = S::FN, FM = S::FM, F = S::F;
+    const int L = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int n0 = blockIdx.x * 16 * FN, m0 = blockIdx.y * 16 * FM;
+    const int steps = a.Kp / 128;
+    const long long row = a.Kp / 2, srow = a.Kp / 32;
+    const uint8_t* cb[F];
+    const uint8_t* sb[F];
+    uint32_t co[F], so[F];
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+        const bool w = f < FN;
+        const int first = w ? n0 + 16 * f : m0 + 16 * (f - FN), last = (w ? a.N : a.M) - 1;
+        const int r0 = min(first, last), r = min(first + (L >> 2), last) - r0;
+        cb[f] = (w ? a.W : a.A) + r0 * row;
+        co[f] = (uint32_t)(r * row) + 16 * ((L & 3) ^ ((L >> 3) & 3));
+        sb[f] = (w ? a.Ws : a.As) + r0 * srow;
+        so[f] = (uint32_t)(r * srow);
+    }
+    uint8_t* mine = smem + wave * S::wave_lds;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)mine;
+    auto fetch = [&](int k) {
+        const long long at = 64LL * min(k, steps - 1);
+#pragma unroll
+        for (int f = 0; f < F; f++) lds_load16(cb[f] + at, co[f], lds0 + ((k & 3) * F + f) * 1024);
+    };
+    auto fetch_scales = [&](int c, int slot) {
+        const uint32_t at = 4 * min(4 * c + (L & 3), steps - 1);
+#pragma unroll
+        for (int f = 0; f < F; f++) lds_load4(sb[f], so[f] + at, lds0 + 4 * F * 1024 + (slot * F + f) * 256);
+    };
+    const int lane_at = (L & 15) * 64 + (((L >> 4) ^ ((L >> 1) & 3)) << 4);
+    const uint32_t pick = (L >> 4) | (((L >> 4) + 4) << 8) | 0x0c0c0000u;
+    v4f acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int j = 0; j < FM; j++) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    int sc[F];
+    auto step = [&](auto ss, auto more, int c, int next) {
+        constexpr int s = decltype(ss)::value;
+        constexpr bool MORE = decltype(more)::value;
+        // the loads issued after this step's: three steps', and the next scales
+        vm_wait<MORE ? 4 * F : (3 - s) * F>();
+        if (4 * c + s < steps) {
+            uint4 q[F];
+#pragma unroll
+            for (int f = 0; f < F; f++) q[f] = *(const uint4*)(mine + (s * F + f) * 1024 + lane_at);
+#pragma unroll
+            for (int i = 0; i < FN; i++) {
+                const v8i w = {(int)q[i].x, (int)q[i].y, (int)q[i].z, (int)q[i].w, 0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < FM; j++) {
+                    const uint4 p = q[FN + j];
+                    const v8i x = {(int)p.x, (int)p.y, (int)p.z, (int)p.w, 0, 0, 0, 0};
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc[i][j], 4, 4, s, sc[i], s, sc[FN + j]);
+                }
+            }
+        }
+        if (MORE) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot's reads are done
+            fetch(4 * next + s);
+        }
+    };
+    auto run = [&](auto more, int c, int slot) {
+        const int next = c + waves;
+        if (decltype(more)::value) fetch_scales(next, slot ^ 1);
+        vm_wait<(decltype(more)::value ? 5 : 4) * F>();  // this run's scales
+#pragma unroll
+        for (int f = 0; f < F; f++) {
+            const uint4 q = *(const uint4*)(mine + 4 * F * 1024 + (slot * F + f) * 256 + (L & 15) * 16);
+            sc[f] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(q.w, q.z, pick), __builtin_amdgcn_perm(q.y, q.x, pick), 0x05040100u);
+        }
+        step(std::integral_constant<int, 0>(), more, c, next);
+        step(std::integral_constant<int, 1>(), more, c, next);
+        step(std::integral_constant<int, 2>(), more, c, next);
+        step(std::integral_constant<int, 3>(), more, c, next);
+    };
+    const int runs = (steps + 3) / 4;  // (at least as many as waves)
+    fetch_scales(wave, 0);
+    for (int s = 0; s < 4; s++) fetch(4 * wave + s);
+    int c = wave, slot = 0;
+    for (; c + waves < runs; c += waves, slot ^= 1) run(std::true_type(), c, slot);
+    run(std::false_type(), c, slot);
+
+    // the sums, fragment by fragment over the slots; wave w adds up fragments w, w + waves, ...
+    __syncthreads();
+    v4f* part = (v4f*)smem;
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int j = 0; j < FM; j++) part[(wave * FN * FM + i * FM + j) * 64 + L] = acc[i][j];
+    __syncthreads();
+    for (int f = wave; f < FN * FM; f += waves) {
+        v4f sum = part[f * 64 + L];
+        for (int w = 1; w < waves; w++) sum += part[(w * FN * FM + f) * 64 + L];
+        const int i = f / FM, j = f - i * FM;
+        const int m = m0 + 16 * j + (L & 15), n = n0 + 16 * i + 4 * (L >> 4);
+        if (m < a.M) store4((T*)a.C + (long long)m * a.N + n, sum, a.N - n, vec);
+    }
+}
+
+// ---- Large products ----
+// A workgroup of WN x WM waves computes TN channels x TM rows, each wave its FN x FM fragments of 16 x 16, in steps of 128
+// elements of K. A step's codes come into one of four LDS slots, three steps ahead; the scales of four steps (16 bytes a row)
+// come at once into one of two. What the loads cost is lines touched, not bytes: four neighbouring lanes take the 64 bytes of
+// a row. A fragment is 16 rows of 64 bytes in LDS, a row's four blocks exchanged by (row >> 1) & 3 so that eight lanes reading
+// one block of eight rows touch all banks.
+//
+// In a step each channel fragment is read anew for the next step right after its products were issued, so that only the row
+// fragments need two sets of registers.
+template <int TN_, int TM_, int WN_, int WM_>
+struct MxTile {
+    static constexpr int TN = TN_, TM = TM_, WN = WN_, WM = WM_;
+    static constexpr int NW = WN * WM, FN = TN / 16 / WN, FM = TM / 16 / WM;
+    static constexpr int kSlots = 4;
+    static constexpr int loads = (TN + TM) / 16 / NW;  // of a wave: codes of a step, and scales of four steps
+    static constexpr int slot = (TN + TM) * 64, o_scale = kSlots * slot, scale_slot = (TN + TM) * 16;
+    static constexpr int lds = o_scale + 2 * scale_slot;
+    static_assert((TN + TM) / 16 % NW == 0 && FM <= FN, "");
+};
+
+template <class S, class T>
+__global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a, int tiles_n, int tiles_m, int vec) {
+    extern __shared__ uint8_t smem[];
+    const int L = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wn = wave % S::WN, wm = wave / S::WN;
+    // consecutive tiles stay on one XCD (its L2), in bands of eight channel tiles
+    const int tile = xcd_tile(blockIdx.x, tiles_n * tiles_m);
+    if (tile >= tiles_n * tiles_m) return;
+    const int band = tile / (8 * tiles_m), in_band = tile - band * 8 * tiles_m;
+    const int width = min(8, tiles_n - 8 * band);
+    const int n0 = (8 * band + in_band % width) * S::TN, m0 = in_band / width * S::TM;
+    const int steps = a.Kp / 128;
+    const long long row = a.Kp / 2, srow = a.Kp / 32;
+
+    // this wave's loads: 16 rows each, first of W, then of A (rows past the end: the last one, whose results are not stored)
+    const uint8_t* cb[S::loads];
+    const uint8_t* sb[S::loads];
+    uint32_t co[S::loads], so[S::loads];
+#pragma unroll
+    for (int j = 0; j < S::loads; j++) {
+        const int f = wave * S::loads + j;
+        const bool w = f < S::TN / 16;
+        const int first = w ? n0 + 16 * f : m0 + 16 * (f - S::TN / 16), last = (w ? a.N : a.M) - 1;
+        const int r0 = min(first, last), r = min(first + (L >> 2), last) - r0;
+        cb[j] = (w ? a.W : a.A) + r0 * row;
+        co[j] = (uint32_t)(r * row) + 16 * ((L & 3) ^ ((L >> 3) & 3));
+        sb[j] = (w ? a.Ws : a.As) + r0 * srow;
+        so[j] = (uint32_t)(r * srow);
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem + wave * S::loads * 1024;
+    const uint32_t lds1 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem + S::o_scale + wave * S::loads * 256;
+    // past the last step it is loaded again: the count of loads in flight stays the same
+    auto fetch = [&](int k, int slot) {
+        const long long at = 64LL * min(k, steps - 1);
+#pragma unroll
+        for (int j = 0; j < S::loads; j++) lds_load16(cb[j] + at, co[j], lds0 + slot * S::slot + 1024 * j);
+    };
+    auto fetch_scales = [&](int c, int slot) {
+        const uint32_t at = 4 * min(4 * c + (L & 3), steps - 1);
+#pragma unroll
+        for (int j = 0; j < S::loads; j++) lds_load4(sb[j], so[j] + at, lds1 + slot * S::scale_slot + 256 * j);
+    };
+    const int lane_at = (L & 15) * 64 + (((L >> 4) ^ ((L >> 1) & 3)) << 4);
+    auto read_w = [&](int slot, int i) { return *(const uint4*)(smem + slot * S::slot + (wn * S::FN + i) * 1024 + lane_at); };
+    auto read_a = [&](int slot, int j) { return *(const uint4*)(smem + slot * S::slot + (S::TN / 16 + wm * S::FM + j) * 1024 + lane_at); };
+    // the scale bytes of a lane's block in four steps, one a byte (the instruction picks one)
+    const uint32_t pick = (L >> 4) | (((L >> 4) + 4) << 8) | 0x0c0c0000u;
+    auto read_scale = [&](int slot, int r) {
+        const uint4 q = *(const uint4*)(smem + S::o_scale + slot * S::scale_slot + (r + (L & 15)) * 16);
+        return (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(q.w, q.z, pick), __builtin_amdgcn_perm(q.y, q.x, pick), 0x05040100u);
+    };
+    v4f acc[S::FN][S::FM];
+#pragma unroll
+    for (int i = 0; i < S::FN; i++)
+#pragma unroll
+        for (int j = 0; j < S::FM; j++) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    uint4 wf[S::FN], af[2][S::FM];
+    int ws[S::FN], as[S::FM];
+    auto scales = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < S::FN; i++) ws[i] = read_scale(slot, (wn * S::FN + i) * 16);
+#pragma unroll
+        for (int j = 0; j < S::FM; j++) as[j] = read_scale(slot, S::TN + (wm * S::FM + j) * 16);
+    };
+    // Only the matrix products and LDS reads of the wave itself cross a barrier: a slot is overwritten two barriers after it was
+    // read, and its reads were waited for by the products between.
+    auto barrier = [&] {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // Step k = 4 c + s. Its row fragments are in af[s & 1], its channel fragments in wf; those of step k + 1 have landed in LDS.
+    auto step = [&](auto sc, int c) {
+        constexpr int s = decltype(sc)::value;
+        const int k = 4 * c + s;
+        vm_wait<(s == 1 ? 2 : 1) * S::loads>();  // (of the step before this: its codes, and the next scales where it was the first)
+        barrier();
+        if (s == 0) fetch_scales(c + 1, (c + 1) & 1);
+        fetch(k + 3, (s + 3) & 3);
+        constexpr int next = (s + 1) & 3;
+#pragma unroll
+        for (int i = 0; i < S::FN; i++) {
+            const v8i w = {(int)wf[i].x, (int)wf[i].y, (int)wf[i].z, (int)wf[i].w, 0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < S::FM; j++) {
+                const uint4 q = af[s & 1][j];
+                const v8i x = {(int)q.x, (int)q.y, (int)q.z, (int)q.w, 0, 0, 0, 0};
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc[i][j], 4, 4, s, ws[i], s, as[j]);
+            }
+            if (i < S::FM) af[(s + 1) & 1][i] = read_a(next, i);
+            wf[i] = read_w(next, i);
+            __builtin_amdgcn_sched_group_barrier(0x008, S::FM, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if (i < S::FM) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (s == 3) scales((c + 1) & 1);
+    };
+    fetch_scales(0, 0);
+    fetch(0, 0);
+    fetch(1, 1);
+    fetch(2, 2);
+    vm_wait<2 * S::loads>();
+    barrier();
+#pragma unroll
+    for (int j = 0; j < S::FM; j++) af[0][j] = read_a(0, j);
+#pragma unroll
+    for (int i = 0; i < S::FN; i++) wf[i] = read_w(0, i);
+    scales(0);
+    const int whole = steps / 4, rest = steps - 4 * whole;
+    for (int c = 0; c < whole; c++) {
+        step(std::integral_constant<int, 0>(), c);
+        step(std::integral_constant<int, 1>(), c);
+        step(std::integral_constant<int, 2>(), c);
+        step(std::integral_constant<int, 3>(), c);
+    }
+    if (rest > 0) step(std::integral_constant<int, 0>(), whole);
+    if (rest > 1) step(std::integral_constant<int, 1>(), whole);
+    if (rest > 2) step(std::integral_constant<int, 2>(), whole);
+    vm_wait<0>();
+
+    // lane L: rows m0 + ... + (L & 15), four channels from 4 (L >> 4)
+#pragma unroll
+    for (int j = 0; j < S::FM; j++) {
+        const int m = m0 + (wm * S::FM + j) * 16 + (L & 15);
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int i = 0; i < S::FN; i++) {
+            const int n = n0 + (wn * S::FN + i) * 16 + 4 * (L >> 4);
+            store4((T*)a.C + (long long)m * a.N + n, acc[i][j], a.N - n, vec);
+        }
+    }
+}
+
+// Allows a kernel dynamic LDS above the default limit, once per device.
+hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& allowed) {
+    int dev = 0;
+    if (const hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (allowed.load() & bit) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) allowed |= bit;
+    return e;
+}
+
+// Runs of four channels of C can be stored at once.
+template <class T>
+int vec4(const Mx4GemmArgs& a) { return a.N % 4 == 0 && (uintptr_t)a.C % (4 * sizeof(T)) == 0; }
+
+template <class S, class T>
+hipError_t launch_lds_gemm(const Mx4GemmArgs& a, hipStream_t s) {
+    static std::atomic<uint64_t> allowed{0};
+    if (const hipError_t e = allow_lds((const void*)mx4_gemm_lds_kernel<S, T>, S::lds, allowed); e != hipSuccess) return e;
+    const int tn = (a.N + S::TN - 1) / S::TN, tm = (a.M + S::TM - 1) / S::TM;
+    if ((long long)tn * tm >= 1 << 22) return hipErrorInvalidValue;  // beyond a launch's 2^32 lanes with the widest workgroup
+    hipLaunchKernelGGL((mx4_gemm_lds_kernel<S, T>), dim3(xcd_grid(tn * tm)), dim3(S::NW * 64), S::lds, s, a, tn, tm, vec4<T>(a));
+    return hipGetLastError();
+}
+
+template <class S, class T>
+hipError_t launch_split_gemm(const Mx4GemmArgs& a, hipStream_t s) {
+    static std::atomic<uint64_t> allowed{0};
+    if (const hipError_t e = allow_lds((const void*)mx4_gemm_split_kernel<S, T>, S::lds, allowed); e != hipSuccess) return e;
+    const int waves = std::min(S::NW, (a.Kp / 128 + 3) / 4);
+    const dim3 grid((a.N + 16 * S::FN - 1) / (16 * S::FN), (a.M + 16 * S::FM - 1) / (16 * S::FM));
+    hipLaunchKernelGGL((mx4_gemm_split_kernel<S, T>), grid, dim3(64 * waves), waves * S::wave_lds, s, a, vec4<T>(a));
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -127,12 +426,22 @@ hipError_t launch_mx4_dequantize(const Mx4RowsArgs& a, hipStream_t s) {
 
 hipError_t launch_mx4_gemm(const Mx4GemmArgs& a, hipStream_t s) {
     if (a.M <= 0 || a.N <= 0 || a.Kp <= 0 || a.Kp % 128) return hipErrorInvalidValue;
-    const int waves = std::max(1, std::min(8, a.Kp / 128));
-    const dim3 grid((a.N + 15) / 16, std::min((a.M + 15) / 16, kMaxGridY));
+    // The largest tile of which there are enough for three quarters of the 256 CUs and which the shape fills to four fifths;
+    // where even those of 64 x 64 are too few, K is split. us at M x N x K, 256 / 128 / 64 tiles, split 32 x 32 and 16 x 16:
+    //   16384 x 4096 x 4096: 185 252 383;     2048 x 2048 x 4096: 36.8 18.2 27.5 57;    1001 x 2048 x 1152: 17.5 8.5 6.4 10.6 15.4
+    //   256 x 4096 x 4096: 33.5 15.2 9.3 14.5 19.6;    128 x 4096 x 4096: 30 14.9 8.3 7.9 10.8;    300 x 300 x 8192: 52 24 12.6 5.6 6.9
+    //   8 x 4096 x 4096: 26 13 7.6 4.8 3.5;    16 x 8192 x 4096: 27 13 7.8 5.3 4.5
+    const auto takes = [&](int tile) {
+        const long long n = (a.N + tile - 1) / tile, m = (a.M + tile - 1) / tile;
+        return n * m >= 192 && (tile == 64 || 4.0 * n * m * tile * tile <= 5.0 * a.M * a.N);
+    };
     return by_real(a.type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        hipLaunchKernelGGL((mx4_gemm_tile_kernel<T>), grid, dim3(64 * waves), 0, s, a);
-        return hipGetLastError();
+        if (a.M <= 16) return launch_split_gemm<MxSplit<1, 1, 8>, T>(a, s);
+        if (takes(256)) return launch_lds_gemm<MxTile<256, 256, 2, 4>, T>(a, s);
+        if (takes(128)) return launch_lds_gemm<MxTile<128, 128, 2, 2>, T>(a, s);
+        if (takes(64)) return launch_lds_gemm<MxTile<64, 64, 2, 2>, T>(a, s);
+        return launch_split_gemm<MxSplit<2, 2, 8>, T>(a, s);
     });
 }
 

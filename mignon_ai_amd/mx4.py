@@ -37,28 +37,19 @@ def _type(t):
     return _device_types.get(t.dtype)
 
 
-class _on:
-    """The device of a call's tensors as the current one, and the stream it goes to."""
-
-    def __init__(self, who, stream, *tensors):
-        import torch
-        dev = tensors[0].device
-        for t in tensors:
-            if not t.is_cuda or t.device != dev:
-                _invalid(f"{who}: tensors on one GPU are needed")
-        self.guard = None
-        if torch.cuda.current_device() != dev.index:
-            self.guard = torch.cuda.device(dev)
-        self.stream = torch.cuda.current_stream(dev).cuda_stream if stream is None else stream
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(who, fn, stream, tensors, args):
+    """fn(*args, stream) with the tensors' device as the current one, on `stream` (default: torch's current stream there)."""
+    import torch
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != dev or dev < 0:
+            _invalid(f"{who}: tensors on one GPU are needed")
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return _launch(who, fn, stream, tensors, args)
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
+    if rc < 0:
+        check(rc)
 
 
 def _real(who, t, name):
@@ -133,8 +124,8 @@ def mx4_quantize_device(x, codes, scales, stream=None):
     ty, M, K, ld = _real("mx4_quantize_device", x, "x")
     if _rows4("mx4_quantize_device", codes, scales, "the result") != (M, padded(K)):
         _invalid("mx4_quantize_device: codes and scales do not go with x")
-    with _on("mx4_quantize_device", stream, x, codes, scales) as st:
-        check(lib().mg_mx4_quantize(x.data_ptr(), ty, M, K, ld, codes.data_ptr(), scales.data_ptr(), MG_PTR_DEVICE, st))
+    _launch("mx4_quantize_device", lib().mg_mx4_quantize, stream, (x, codes, scales),
+            (x.data_ptr(), ty, M, K, ld, codes.data_ptr(), scales.data_ptr(), MG_PTR_DEVICE))
 
 
 def mx4_dequantize_device(codes, scales, y, stream=None):
@@ -142,8 +133,8 @@ def mx4_dequantize_device(codes, scales, y, stream=None):
     ty, M, K, ld = _real("mx4_dequantize_device", y, "y")
     if _rows4("mx4_dequantize_device", codes, scales, "the operand") != (M, padded(K)):
         _invalid("mx4_dequantize_device: codes and scales do not go with y")
-    with _on("mx4_dequantize_device", stream, y, codes, scales) as st:
-        check(lib().mg_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), M, K, y.data_ptr(), ty, ld, MG_PTR_DEVICE, st))
+    _launch("mx4_dequantize_device", lib().mg_mx4_dequantize, stream, (y, codes, scales),
+            (codes.data_ptr(), scales.data_ptr(), M, K, y.data_ptr(), ty, ld, MG_PTR_DEVICE))
 
 
 def mx4_gemm_device(A, As, W, Ws, C, stream=None):
@@ -153,9 +144,8 @@ def mx4_gemm_device(A, As, W, Ws, C, stream=None):
     ty = _type(C)
     if ty is None or ty < 0 or C.shape != (M, N) or Kp != Kw or not C.is_contiguous():
         _invalid("mx4_gemm_device: A [M][K], W [N][K] and a contiguous C [M][N] of reals are needed")
-    with _on("mx4_gemm_device", stream, A, As, W, Ws, C) as st:
-        check(lib().mg_mx4_gemm(A.data_ptr(), As.data_ptr(), M, Kp, W.data_ptr(), Ws.data_ptr(), N, C.data_ptr(), ty,
-                                MG_PTR_DEVICE, st))
+    _launch("mx4_gemm_device", lib().mg_mx4_gemm, stream, (A, As, W, Ws, C),
+            (A.data_ptr(), As.data_ptr(), M, Kp, W.data_ptr(), Ws.data_ptr(), N, C.data_ptr(), ty, MG_PTR_DEVICE))
 
 
 class KVCache:
@@ -223,22 +213,19 @@ class KVCache:
         """mg_kv_write: new rows k, v [n][T][heads][head_dim] (any strides but the last) at positions pos[s] + t, of which the
         first counts[s] (default T) are there. pos, counts: int32 [n]."""
         ty, kr, vr = self._two("KVCache.write", k, v, pos, counts)
-        with _on("KVCache.write", None, self.k, k, v, pos, *(() if counts is None else (counts,))) as st:
-            check(lib().mg_kv_write(self._p, ctypes.addressof(kr), ctypes.addressof(vr), ty, k.shape[1], pos.data_ptr(),
-                                    ptr(counts), st))
+        _launch("KVCache.write", lib().mg_kv_write, None, (self.k, k, v, pos) + (() if counts is None else (counts,)),
+                (self._p, ctypes.addressof(kr), ctypes.addressof(vr), ty, k.shape[1], pos.data_ptr(), ptr(counts)))
 
     def read(self, k, v, pos, counts=None, lens=None):
         """mg_kv_read: the rows at positions pos[s] + t into k, v; lens [n]: the sequences' lengths (default pos + counts)."""
         ty, kr, vr = self._two("KVCache.read", k, v, pos, counts, lens)
-        more = [a for a in (counts, lens) if a is not None]
-        with _on("KVCache.read", None, self.k, k, v, pos, *more) as st:
-            check(lib().mg_kv_read(self._p, ctypes.addressof(kr), ctypes.addressof(vr), ty, k.shape[1], pos.data_ptr(),
-                                   ptr(counts), ptr(lens), st))
+        more = tuple(a for a in (counts, lens) if a is not None)
+        _launch("KVCache.read", lib().mg_kv_read, None, (self.k, k, v, pos) + more,
+                (self._p, ctypes.addressof(kr), ctypes.addressof(vr), ty, k.shape[1], pos.data_ptr(), ptr(counts), ptr(lens)))
 
     def attention(self, q, out, pos, counts=None, window: int = 0, scale: float | None = None):
         """mg_kv_attention: rows q [n][T][q_heads][head_dim] at positions pos[s] + t over the cache (their own keys written
         already) into out, which is returned; scale: head_dim ** -0.5 if not given."""
-        import torch
         ty, qr = self._rows("KVCache.attention", q, "q", None)
         to, orow = self._rows("KVCache.attention", out, "out", None)
         if ty != to or q.shape != out.shape or pos is None:
@@ -246,9 +233,8 @@ class KVCache:
         self._ints("KVCache.attention", pos, counts)
         T, q_heads = q.shape[1], q.shape[2]
         need = self._workspace(q_heads, T, window)
-        with _on("KVCache.attention", None, self.k, q, out, pos, *(() if counts is None else (counts,))) as st:
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            check(lib().mg_kv_attention(self._p, ctypes.addressof(qr), ctypes.addressof(orow), ty, q_heads, T, pos.data_ptr(),
-                                        ptr(counts), window, self.head_dim ** -0.5 if scale is None else scale, ptr(ws), need,
-                                        st))
+        ws = self.k.new_empty(need) if need else None
+        _launch("KVCache.attention", lib().mg_kv_attention, None, (self.k, q, out, pos) + (() if counts is None else (counts,)),
+                (self._p, ctypes.addressof(qr), ctypes.addressof(orow), ty, q_heads, T, pos.data_ptr(), ptr(counts), window,
+                 self.head_dim ** -0.5 if scale is None else scale, ptr(ws), need))
         return out
