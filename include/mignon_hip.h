@@ -323,8 +323,8 @@ int mg_mx4_gemm(const uint8_t* A, const uint8_t* As, int M, int K, const uint8_t
  * n sequences of `heads` key/value heads of head_dim (32, 64, 96 or 128) channels, `capacity` (a multiple of 32) slots each.
  * Position p < sinks (0 <= sinks < capacity) has slot p for good; a later one has slot sinks + (p - sinks) % ring, with
  * ring = capacity - sinks: of the positions below a sequence's length, the cache holds the first `sinks` and the last `ring`.
- * Planes: k and v codes [n][heads][capacity][head_dim / 2], 16-byte aligned; k_scales and v_scales
- * [n][heads][capacity][head_dim / 32], 4-byte aligned. Memory of any contents may be used: what was not written is not seen.
+ * Planes, 16-byte aligned: k and v codes [n][heads][capacity][head_dim / 2], k_scales and v_scales
+ * [n][heads][capacity][head_dim / 32]. Memory of any contents may be used: what was not written is not seen.
  * The caller owns the planes and keeps count of the positions. All pointers of these calls but the structs are device
  * pointers; the calls enqueue work on `stream`, allocate nothing and can be captured. */
 typedef struct {

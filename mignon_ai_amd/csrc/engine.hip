@@ -1228,10 +1228,11 @@ bool kv_cache(const char* who, const mg_kv_cache_t* c, int T, KvCache& x) {
     REQUIRE(c->n >= 0 && c->heads > 0 && c->heads <= 4096 && T >= 0 && T < kKvMaxPos, std::string(who) + ": bad shape");
     REQUIRE(c->capacity > 0 && c->capacity % 32 == 0 && c->capacity < kKvMaxPos, std::string(who) + ": capacity is a multiple of 32");
     REQUIRE(c->sinks >= 0 && c->sinks < c->capacity, std::string(who) + ": sinks leave no slot for later positions");
-    REQUIRE((long long)c->n * std::max(T, 1) * c->heads < (1LL << 31), std::string(who) + ": too many rows");
+    const long long tokens = (long long)c->n * std::max(T, 1);
+    REQUIRE(tokens < (1LL << 31) && tokens * c->heads < (1LL << 31), std::string(who) + ": too many rows");
     if (c->n == 0 || T == 0) return false;
     REQUIRE(c->k && c->k_scales && c->v && c->v_scales, std::string(who) + ": null argument");
-    REQUIRE(aligned(c->k, 16) && aligned(c->v, 16) && aligned(c->k_scales, 4) && aligned(c->v_scales, 4), std::string(who) + ": misaligned plane");
+    REQUIRE(aligned(c->k, 16) && aligned(c->v, 16) && aligned(c->k_scales, 16) && aligned(c->v_scales, 16), std::string(who) + ": misaligned plane");
     x.n = c->n; x.heads = c->heads; x.dh = c->head_dim; x.cap = c->capacity; x.sinks = c->sinks;
     x.k = c->k; x.ks = c->k_scales; x.v = c->v; x.vs = c->v_scales;
     return true;

@@ -123,6 +123,21 @@ hipError_t launch_rows(const KvRowsArgs& a, hipStream_t s) {
     });
 }
 
+// Four neighbouring channels; vec: aligned.
+template <class T>
+__device__ __forceinline__ void store4(T* p, v4f v, int vec) {
+    T t[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) t[r] = (T)v[r];
+    if (vec) {
+        if constexpr (sizeof(T) == 4) *(uint4*)p = *(uint4*)t;
+        else *(uint2*)p = *(uint2*)t;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++) p[r] = t[r];
+    }
+}
+
 // ---- attention -----------------------------------------------------------------------------------------------------
 // The cache is read in tiles of 32 slots. The tiles that hold a position some row of a row tile sees, in slot order: up to
 // three runs (the sinks; the ring's part up to the newest position; the older part behind it, where the run wraps).
@@ -132,26 +147,6 @@ struct Tiles {
     __device__ __forceinline__ int count() const { return n0 + n1 + n2; }
     __device__ __forceinline__ int at(int o) const { return o < n0 ? o : o < n0 + n1 ? b1 + o - n0 : b2 + o - n0 - n1; }
 };
-// Rows at positions lo_row .. hi_row; the cache holds positions below `end`.
-__device__ __forceinline__ Tiles tiles_of(int lo_row, int hi_row, int end, int sinks, int ring, int cap, int window) {
-    Tiles r{0, 0, 0, 0, 0};
-    if (hi_row < 0) return r;
-    const int seen = min(sinks, hi_row + 1);
-    r.n0 = (seen + 31) >> 5;
-    int lo = max(sinks, end - ring);
-    if (window > 0) lo = max(lo, lo_row - window + 1);
-    if (hi_row < lo) return r;
-    const int a = kv_slot(lo, sinks, ring) >> 5, b = (kv_slot(hi_row, sinks, ring) >> 5) + 1;
-    const bool wraps = kv_slot(lo, sinks, ring) > kv_slot(hi_row, sinks, ring);
-    r.b1 = max(r.n0, wraps ? sinks >> 5 : a);
-    r.n1 = max(0, b - r.b1);
-    if (wraps) {
-        r.b2 = max(max(r.n0, r.b1 + r.n1), a);
-        r.n2 = max(0, (cap >> 5) - r.b2);
-    }
-    return r;
-}
-
 template <class T>
 struct Terms;  // bf16 parts that hold a query element, and those that a probability is split into
 template <>
@@ -191,20 +186,34 @@ __device__ __forceinline__ void split_bf16(const float x[8], v8bf out[N]) {
 // Channels of a head as the two products take them, with i = lane & 15 and g = lane >> 4.
 //   Scores, K (16 keys a product) times q: step s of DH / 32 covers, for lane group g, channels (DH / 4) g + 8 s .. + 7, so
 //   that a lane's steps are neighbouring words of a row (DH 96: channels 32 s + 8 g, since 24 do not end with a block).
-//   Output, V^T times the probabilities: channels in chunks of 16 E, lane i owning E neighbouring ones (E 8, 4, 2).
+//   Output, V^T times the probabilities: channels in chunks of 16 E, lane i owning E neighbouring ones (E 8, 4, 2): of the
+//   product's result, lane (i, g) holds row i and in element r of fragment e channel base + (4 g + r) E + e.
 template <int DH>
 struct Width {
-    static constexpr int KS = DH / 32;
+    static constexpr int KS = DH / 32, NB = DH / 32, ND = DH / 16;
     static constexpr bool kEven = DH != 96;
+    static constexpr int KW = kEven ? 1 : 3;  // scale bytes a lane needs of a key
     static constexpr int chunks = DH == 96 ? 2 : 1;
     static constexpr int E0 = DH == 96 ? 4 : DH / 16;
-    __device__ static constexpr int E(int c) { return c == 0 ? E0 : 2; }
+    __host__ __device__ static constexpr int E(int c) { return c == 0 ? E0 : 2; }
+    __host__ __device__ static constexpr int base(int c) { return c == 0 ? 0 : 64; }
+    __host__ __device__ static constexpr int d0(int c) { return c == 0 ? 0 : E0; }
     __device__ static int k_channel(int g, int s) { return kEven ? (DH / 4) * g + 8 * s : 32 * s + 8 * g; }
 };
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// A scale of the byte at bit 8 b of a word, for a conversion: it reads the exponent bits alone, so the byte is only rotated there.
+__device__ __forceinline__ float scale_at(uint32_t w, int shift) { return __uint_as_float(__builtin_amdgcn_alignbit(w, w, shift)); }
+__device__ __forceinline__ constexpr int scale_shift(int b) { return (8 * b + 9) & 31; }
+
+// Of two lanes 16 (32) apart, both their values.
 __device__ __forceinline__ float max_groups(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float sum_groups(float v) {
     v += __shfl_xor(v, 16, 64);
@@ -214,284 +223,449 @@ __device__ __forceinline__ float sum_groups(float v) {
 constexpr int kTile = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Few query rows: a wave takes 16 rows (the query heads of one key/value head, token after token) over a share of the tiles.
-//
-// Scores of 16 keys x 16 rows come out of the matrix cores with lane (i, g) holding row i and four keys; the keys of a tile
-// are assigned to the product's rows so that group g ends with keys 8 g .. 8 g + 7, the very layout in which the second
-// product takes the probabilities: they never leave their lane. V is brought into its layout (one channel of eight keys in
-// a lane) by unpacking two keys' words and exchanging halves.
-template <int DH, class T, int WAVES>
-__global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles) {
+// A tile of 32 slots as one lane of a wave holds it. K: two products of 16 keys, lane i holding slot 8 (i >> 2) + 4 h + (i & 3) of
+// the tile in product h, so that the scores of slots 8 g .. 8 g + 7 come out in lane group g. V: those eight slots, the lane's
+// channels of each.
+template <int DH>
+struct KvTile {
     using W = Width<DH>;
-    constexpr int QT = Terms<T>::q, PT = Terms<T>::p, ND = DH / 16, LD = DH + 4;
+    uint32_t k[2][W::KS];
+    uint32_t ks[2][W::KW];
+    uint32_t v[W::chunks][8];
+    uint32_t vs[2 * W::NB];
+
+    __device__ __forceinline__ void load(const uint8_t* kb, const uint8_t* ksb, const uint8_t* vb, const uint8_t* vsb, int j0, int i, int g) {
+        kb += (size_t)j0 * (DH / 2);
+        vb += (size_t)j0 * (DH / 2);
+        ksb += (size_t)j0 * W::NB;
+        vsb += (size_t)j0 * W::NB;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int key = (i >> 2) * 8 + 4 * h + (i & 3);
+            const uint8_t* p = kb + key * (DH / 2) + (W::kEven ? (DH / 8) * g : 4 * g);
+            if constexpr (DH == 128) *(u32x4*)k[h] = *(const u32x4*)p;
+            else if constexpr (DH == 64) *(u32x2*)k[h] = *(const u32x2*)p;
+            else
+#pragma unroll
+                for (int s = 0; s < W::KS; s++) k[h][s] = *(const uint32_t*)(p + 16 * s);
+#pragma unroll
+            for (int x = 0; x < W::KW; x++) ks[h][x] = ksb[key * W::NB + (W::kEven ? (DH / 4) * g / 32 : x)];
+        }
+#pragma unroll
+        for (int c = 0; c < W::chunks; c++) {
+            const uint8_t* p = vb + 8 * g * (DH / 2) + (W::base(c) + i * W::E(c)) / 2;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                v[c][e] = W::E(c) == 8 ? *(const uint32_t*)(p + e * (DH / 2)) : W::E(c) == 4 ? *(const uint16_t*)(p + e * (DH / 2)) : p[e * (DH / 2)];
+        }
+#pragma unroll
+        for (int x = 0; x < W::NB; x++) *(u32x2*)(vs + 2 * x) = *(const u32x2*)(vsb + 8 * g * W::NB + 8 * x);
+    }
+    // The scale byte of slot 8 g + e for block b, and the scale for a conversion (b of this lane's channels in chunk c).
+    __device__ __forceinline__ uint32_t v_byte(int e, int b) const {
+        const int at = e * W::NB + b;
+        return (vs[at >> 2] >> (8 * (at & 3))) & 255;
+    }
+    __device__ __forceinline__ float v_scale(int c, int e, int i) const {
+        if constexpr (DH == 128) return scale_at(vs[e], 8 * (i >> 2) + 9);
+        else if constexpr (DH == 64) return scale_at(vs[e >> 1], 16 * (e & 1) + 8 * (i >> 3) + 9);
+        else if constexpr (DH == 32) return scale_at(vs[e >> 2], scale_shift(e & 3));
+        else {
+            if (c == 1) return scale_at(vs[(3 * e + 2) >> 2], scale_shift((3 * e + 2) & 3));
+            const int at = 3 * e;  // this byte or the next
+            const float lo = scale_at(vs[at >> 2], scale_shift(at & 3)), hi = scale_at(vs[(at + 1) >> 2], scale_shift((at + 1) & 3));
+            return i & 8 ? hi : lo;
+        }
+    }
+};
+
+// Two elements of word w (byte b), scaled, as bf16.
+__device__ __forceinline__ uint32_t unpack2(uint32_t w, float s, int b) {
+    switch (b) {
+        case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+        case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+        case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+        default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+    }
+}
+
+// What a wave's rows and the slots are, for the masks. Uniform but for `at`.
+struct Seen {
+    int sinks, ring, window;
+    int last, newest;     // the last position, and its slot in the ring (-1: none is there)
+    int lo_at, hi_at;     // positions of the wave's rows
+    int at;               // of this lane's row
+    __device__ __forceinline__ int position(int j) const { return j < sinks ? j : last - (newest - j + (j > newest ? ring : 0)); }
+    __device__ __forceinline__ bool held(int j, int p) const { return j < sinks ? j <= last : p >= sinks && p <= last; }
+    // Every row sees every slot of the tile.
+    __device__ __forceinline__ bool whole(int j0) const {
+        if (j0 + 31 < sinks) return j0 + 31 <= lo_at;
+        if (j0 < sinks || (j0 <= newest && newest < j0 + 31)) return false;
+        const int p = position(j0);
+        return p >= sinks && p + 31 <= lo_at && (window <= 0 || p > hi_at - window);
+    }
+};
+
+__device__ __forceinline__ Tiles tiles_of(const Seen& q, int cap) {
+    Tiles r{0, 0, 0, 0, 0};
+    if (q.hi_at < 0) return r;
+    r.n0 = (min(q.sinks, q.hi_at + 1) + 31) >> 5;
+    int lo = max(q.sinks, q.last + 1 - q.ring);
+    if (q.window > 0) lo = max(lo, q.lo_at - q.window + 1);
+    if (q.hi_at < lo) return r;
+    // (both are within a ring of the last position: no division)
+    const auto slot = [&](int p) {
+        const int j = q.newest - (q.last - p);
+        return j < q.sinks ? j + q.ring : j;
+    };
+    const int first = slot(lo), newest = slot(q.hi_at);
+    const int a = first >> 5, b = (newest >> 5) + 1;
+    const bool wraps = first > newest;
+    r.b1 = max(r.n0, wraps ? q.sinks >> 5 : a);
+    r.n1 = max(0, b - r.b1);
+    if (wraps) {
+        r.b2 = max(max(r.n0, r.b1 + r.n1), a);
+        r.n2 = max(0, (cap >> 5) - r.b2);
+    }
+    return r;
+}
+
+// Running softmax of 16 rows, a lane's share: O^T in the second product's layout, the maximum of its row (common to the four
+// lane groups), and the sum over its own keys.
+template <int DH>
+struct RowState {
+    v4f acc[Width<DH>::ND];
+    float m, l;
+    uint32_t nan_blocks;  // careful form: bit b: a key that the row sees has NaN in channels 32 b .. 32 b + 31
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int d = 0; d < Width<DH>::ND; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        m = -INFINITY;
+        l = 0.0f;
+        nan_blocks = 0;
+    }
+};
+
+// One tile for 16 rows. Scores leave the matrix cores with lane (i, g) holding row i and slots 8 g .. 8 g + 7 of the tile, the very
+// layout in which the second product takes the probabilities: they never leave their lane. V comes into its layout (one
+// channel of eight slots in a lane) by unpacking the words of two slots and exchanging halves. CAREFUL keeps blocks of NaN
+// out of the product (they would spread over rows that do not see their key) and notes who sees them instead.
+template <int DH, class T, bool CAREFUL>
+__device__ __forceinline__ void tile_step(RowState<DH>& st, const KvTile<DH>& x, const v8bf (*qf)[Terms<T>::q], float scale,
+                                          const Seen& seen, int j0, bool whole, int i, int g) {
+    using W = Width<DH>;
+    constexpr int QT = Terms<T>::q, PT = Terms<T>::p;
+    float sc[8];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < W::KS; s++) {
+            const float ks = mx4_scale(x.ks[h][W::kEven ? 0 : s]);
+            uint32_t kw[4];
+#pragma unroll
+            for (int b = 0; b < 4; b++) kw[b] = unpack2(x.k[h][s], ks, b);
+            const v8bf kf = __builtin_bit_cast(v8bf, *(u32x4*)kw);
+#pragma unroll
+            for (int n = QT - 1; n >= 0; n--) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[s][n], d, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) sc[4 * h + r] = d[r] * scale;
+    }
+    uint32_t sees = 255, drop = 0;
+    if (!whole) {
+        sees = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int j = j0 + 8 * g + e, p = seen.position(j);
+            const bool held = seen.held(j, p);
+            const bool v = held && p <= seen.at && (j < seen.sinks || seen.window <= 0 || p > seen.at - seen.window);
+            sees |= (uint32_t)v << e;
+            drop |= (uint32_t)!held << e;  // never written, or lost: may hold anything
+            sc[e] = v ? sc[e] : -INFINITY;
+        }
+    }
+    float mt = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+    if (__any(mt > st.m)) {  // rare after the first tiles
+        const float mn = fmaxf(st.m, max_groups(mt)), al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : st.m - mn);
+        st.m = mn;
+        st.l *= al;
+#pragma unroll
+        for (int d = 0; d < W::ND; d++) st.acc[d] *= al;
+    }
+    const float mu = st.m == -INFINITY ? 0.0f : st.m;
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(sc[e] - mu);
+    st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    v8bf pf[PT];
+    split_bf16<PT>(p, pf);
+    if (CAREFUL) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+#pragma unroll
+            for (int b = 0; b < W::NB; b++)
+                if (((sees >> e) & 1) && x.v_byte(e, b) > 252u) st.nan_blocks |= 1u << b;
+    }
+#pragma unroll
+    for (int c = 0; c < W::chunks; c++) {
+        uint32_t word[8];
+        float vs[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            word[e] = x.v[c][e];
+            vs[e] = x.v_scale(c, e, i);
+            // (the writer's scales are at most 252, or 255 for NaN)
+            if ((CAREFUL && (__float_as_uint(vs[e]) >> 23 & 255) > 252u) || (!whole && (drop >> e & 1))) {
+                word[e] = 0;
+                vs[e] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < W::E(c) / 2; b++) {
+            uint32_t lo[4], hi[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t y0 = unpack2(word[2 * e], vs[2 * e], b), y1 = unpack2(word[2 * e + 1], vs[2 * e + 1], b);
+                lo[e] = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
+                hi[e] = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
+            }
+            const v8bf v0 = __builtin_bit_cast(v8bf, *(u32x4*)lo), v1 = __builtin_bit_cast(v8bf, *(u32x4*)hi);
+            const int d = W::d0(c) + 2 * b;
+#pragma unroll
+            for (int n = PT - 1; n >= 0; n--) {
+                st.acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pf[n], st.acc[d], 0, 0, 0);
+                st.acc[d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pf[n], st.acc[d + 1], 0, 0, 0);
+            }
+        }
+    }
+}
+
+// Parts of a row for the join: sums, then maximum and sum of probabilities.
+template <int DH>
+constexpr int kPart = DH + 4;
+
+// Few query rows: a wave takes 16 rows (the query heads of one key/value head, token after token) over a share of the tiles,
+// loading each tile while the one before is worked on. WAVES waves share the tiles of a row tile (of one chunk of them, with
+// a.chunks > 1) and add up what they have in LDS; with WAVES 1 a wave is alone with its row tile.
+template <int DH, class T, int WAVES>
+__global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
+    using W = Width<DH>;
+    constexpr int QT = Terms<T>::q, LD = DH + 4;
     __shared__ float s_ml[WAVES > 1 ? WAVES : 1][2][16];
-    __shared__ float s_o[WAVES > 1 ? WAVES * 16 * LD : 1];
+    __shared__ __align__(16) float s_o[WAVES > 1 ? WAVES * 16 * LD : 4];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int unit = WAVES > 1 ? blockIdx.x : blockIdx.x * 4 + wave, w = WAVES > 1 ? wave : 0;
     const int pairs = a.c.n * a.c.heads;
     if (unit >= pairs * row_tiles) return;
-    const int pair = unit / row_tiles, rt = unit - pair * row_tiles;
+    const int pair = row_tiles == 1 ? unit : unit / row_tiles, rt = unit - pair * row_tiles;
     const int s = pair / a.c.heads, h = pair - s * a.c.heads;
     const SeqSpan q = seq_span(a.pos, a.counts, s, a.T);
     const int ring = a.c.cap - a.c.sinks, sinks = a.c.sinks;
-    const int t_lo = rt * 16 / a.group;
+    const int t_lo = rt == 0 ? 0 : rt * 16 / a.group;
     if (t_lo >= q.count) return;
-    const int t_hi = min((rt * 16 + 15) / a.group, q.count - 1);
-    const Tiles tl = tiles_of(q.pos + t_lo, q.pos + t_hi, q.end, sinks, ring, a.c.cap, a.window);
+    const int t_hi = a.T == 1 ? 0 : min((rt * 16 + 15) / a.group, q.count - 1);
+
+    Seen seen;
+    seen.sinks = sinks; seen.ring = ring; seen.window = a.window;
+    seen.last = q.end - 1;
+    seen.newest = seen.last >= sinks ? kv_slot(seen.last, sinks, ring) : -1;
+    seen.lo_at = q.pos + t_lo;
+    seen.hi_at = q.pos + t_hi;
+    const Tiles tl = tiles_of(seen, a.c.cap);
     const int n_tiles = tl.count();
     const int o0 = blockIdx.y * chunk_tiles, o1 = min(n_tiles, o0 + chunk_tiles);
     if (blockIdx.y && o0 >= n_tiles) return;
 
     // this lane's row
     const int row = rt * 16 + i, rows = a.T * a.group;
-    const int t = row / a.group, head = h * a.group + (row - t * a.group);
+    const int t = a.T == 1 ? 0 : row / a.group, head = h * a.group + (row - t * a.group);
     const bool there = row < rows && t < q.count;
-    const int at = q.pos + t;
+    seen.at = q.pos + t;
     v8bf qf[W::KS][QT];
 #pragma unroll
     for (int st = 0; st < W::KS; st++) {
         float x[8] = {};
-        if (there)
-            real_load8<T, false>((const T*)a.q.data + s * a.q.seq + t * a.q.token + head * a.q.head + W::k_channel(g, st), 8, x);
+        if (there) {
+            const T* p = (const T*)a.q.data + s * a.q.seq + t * a.q.token + head * a.q.head + W::k_channel(g, st);
+            if (vec) real_load8<T, true>(p, 8, x);
+            else real_load8<T, false>(p, 8, x);
+        }
         split_bf16<QT>(x, qf[st]);
     }
     const float scale = a.scale * kLog2e;
-
-    // what the slots hold: slots of the ring up to `newest` belong to the run that ends with position end - 1
-    const int last = q.end - 1, newest = last >= sinks ? kv_slot(last, sinks, ring) : -1;
     const size_t plane = (size_t)pair * a.c.cap;
     const uint8_t* kb = a.c.k + plane * (DH / 2);
-    const uint8_t* ksb = a.c.ks + plane * (DH / 32);
+    const uint8_t* ksb = a.c.ks + plane * W::NB;
     const uint8_t* vb = a.c.v + plane * (DH / 2);
-    const uint8_t* vsb = a.c.vs + plane * (DH / 32);
+    const uint8_t* vsb = a.c.vs + plane * W::NB;
 
-    v4f acc[ND];
-#pragma unroll
-    for (int d = 0; d < ND; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;
-    uint32_t nan_blocks = 0;  // bit b: a key this row sees has NaN for channels 32 b .. 32 b + 31
-
-    for (int o = o0 + w; o < o1; o += WAVES) {
-        const int j0 = tl.at(o) * kTile;
-        // scores
-        float sc[8];
-#pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-            const int key = j0 + (i >> 2) * 8 + 4 * hf + (i & 3);
-            const uint8_t* kp = kb + (size_t)key * (DH / 2);
-            const uint8_t* kss = ksb + (size_t)key * (DH / 32);
-            v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int st = 0; st < W::KS; st++) {
-                const int c0 = W::k_channel(g, st);
-                const uint32_t word = *(const uint32_t*)(kp + c0 / 2);
-                const float ks = mx4_scale(kss[c0 / 32]);
-                uint32_t kw[4];
-                kw[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, ks, 0));
-                kw[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, ks, 1));
-                kw[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, ks, 2));
-                kw[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, ks, 3));
-                const v8bf kf = __builtin_bit_cast(v8bf, *(uint4*)kw);
-#pragma unroll
-                for (int n = QT - 1; n >= 0; n--) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[st][n], d, 0, 0, 0);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++) sc[4 * hf + r] = d[r];
+    RowState<DH> st;
+    auto sweep = [&](auto careful) {
+        st.clear();
+        int o = o0 + w;
+        if (o >= o1) return;
+        KvTile<DH> x, y;
+        int j0 = __builtin_amdgcn_readfirstlane(tl.at(o) * kTile);
+        x.load(kb, ksb, vb, vsb, j0, i, g);
+        for (; o < o1; o += WAVES) {
+            const int j1 = __builtin_amdgcn_readfirstlane(tl.at(min(o + WAVES, o1 - 1)) * kTile);
+            if (o + WAVES < o1) y.load(kb, ksb, vb, vsb, j1, i, g);
+            tile_step<DH, T, decltype(careful)::value>(st, x, qf, scale, seen, j0, seen.whole(j0), i, g);
+            x = y;
+            j0 = j1;
         }
-        // who sees what: lane (i, g) holds row i and slots j0 + 8 g + e
-        uint32_t sees = 0;
+    };
+    sweep(std::false_type());
+    {
+        // A NaN among the sums: it may come from a value that the row does not see.
+        float bad = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int j = j0 + 8 * g + e;
-            const int p = j < sinks ? j : last - (newest - j + (j > newest ? ring : 0));
-            const bool held = j < sinks ? j <= last : p >= sinks;
-            const bool v = held && p <= at && (j < sinks || a.window <= 0 || p > at - a.window);
-            sees |= (uint32_t)v << e;
-            sc[e] = v ? sc[e] * scale : -INFINITY;
-        }
-        float mt = sc[0];
+        for (int d = 0; d < W::ND; d++)
 #pragma unroll
-        for (int e = 1; e < 8; e++) mt = fmaxf(mt, sc[e]);
-        const float mn = fmaxf(m, max_groups(mt)), mu = mn == -INFINITY ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(m - mu);
-        m = mn;
-        float p[8], ps = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            p[e] = __builtin_amdgcn_exp2f(sc[e] - mu);
-            ps += p[e];
-        }
-        l = l * al + ps;
-#pragma unroll
-        for (int d = 0; d < ND; d++) acc[d] *= al;
-        v8bf pf[PT];
-        split_bf16<PT>(p, pf);
-        // output
-#pragma unroll
-        for (int c = 0; c < W::chunks; c++) {
-            const int E = c == 0 ? W::E0 : 2, base = c == 0 ? 0 : 64, dt0 = c == 0 ? 0 : W::E0;
-            const int blk = (base + i * E) / 32;
-            uint32_t word[8], sb[8];
-            uint32_t most = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const size_t key = (size_t)(j0 + 8 * g + e);
-                const uint8_t* vp = vb + key * (DH / 2) + (base + i * E) / 2;
-                word[e] = E == 8 ? *(const uint32_t*)vp : E == 4 ? *(const uint16_t*)vp : *vp;
-                sb[e] = vsb[key * (DH / 32) + blk];
-                most = max(most, sb[e]);
-            }
-            // a block of NaN stands apart: it would spread over rows that do not see its key (the writer's scales are at
-            // most 252 otherwise; slots that were never written may hold anything)
-            if (__any(most > 252u)) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const size_t key = (size_t)(j0 + 8 * g + e);
-                    for (int b = 0; b < DH / 32; b++)
-                        if (((sees >> e) & 1) && vsb[key * (DH / 32) + b] > 252u) nan_blocks |= 1u << b;
-                    if (sb[e] > 252u) { sb[e] = 0; word[e] = 0; }
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < E / 2; b++) {
-                uint32_t lo[4], hi[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    uint32_t x, y;
-                    const float s0 = mx4_scale(sb[2 * e]), s1 = mx4_scale(sb[2 * e + 1]);
-#define MX4_CVT(sel) \
-    x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word[2 * e], s0, sel)); \
-    y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word[2 * e + 1], s1, sel));
-                    if (b == 0) { MX4_CVT(0) } else if (b == 1) { MX4_CVT(1) } else if (b == 2) { MX4_CVT(2) } else { MX4_CVT(3) }
-#undef MX4_CVT
-                    lo[e] = __builtin_amdgcn_perm(y, x, 0x05040100u);
-                    hi[e] = __builtin_amdgcn_perm(y, x, 0x07060302u);
-                }
-                const v8bf v0 = __builtin_bit_cast(v8bf, *(uint4*)lo), v1 = __builtin_bit_cast(v8bf, *(uint4*)hi);
-#pragma unroll
-                for (int n = PT - 1; n >= 0; n--) {
-                    acc[dt0 + 2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pf[n], acc[dt0 + 2 * b], 0, 0, 0);
-                    acc[dt0 + 2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pf[n], acc[dt0 + 2 * b + 1], 0, 0, 0);
-                }
-            }
-        }
+            for (int r = 0; r < 4; r++) bad += st.acc[d][r] * 0.0f;
+        if (__any(bad != 0.0f)) sweep(std::true_type());
     }
-    l = sum_groups(l);
-    nan_blocks |= __shfl_xor(nan_blocks, 16, 64);
-    nan_blocks |= __shfl_xor(nan_blocks, 32, 64);
-    if (nan_blocks) {
-        // lane (i, g): row i, channels base + (4 g + r) E + e
+    st.l = sum_groups(st.l);
+    if (__any(st.nan_blocks)) {
+        st.nan_blocks |= __shfl_xor(st.nan_blocks, 16, 64);
+        st.nan_blocks |= __shfl_xor(st.nan_blocks, 32, 64);
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            const bool first = d < W::E0;
-            const int E = first ? W::E0 : 2, base = first ? 0 : 64, e = first ? d : d - W::E0;
+        for (int c = 0; c < W::chunks; c++)
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                if ((nan_blocks >> ((base + (4 * g + r) * E + e) / 32)) & 1) acc[d][r] = NAN;
-        }
+            for (int e = 0; e < W::E(c); e++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if ((st.nan_blocks >> ((W::base(c) + (4 * g + r) * W::E(c) + e) / 32)) & 1) st.acc[W::d0(c) + e][r] = NAN;
     }
-    const int chunks = (n_tiles + chunk_tiles - 1) / chunk_tiles;
-    float total = l;
-    if constexpr (WAVES > 1) {
+    const bool split = n_tiles > chunk_tiles;
+    const int keep = min(16, rows);
+    // [chunk][unit][row][kPart]
+    float* part = a.ws + (((size_t)blockIdx.y * pairs * row_tiles + unit) * keep) * kPart<DH>;
+    if constexpr (WAVES == 1) {
+        if (!there) return;
+        const float f = st.l == 0.0f ? 0.0f : 1.0f / st.l;
+        T* out = (T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head;
+#pragma unroll
+        for (int c = 0; c < W::chunks; c++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                constexpr int EM = W::E0;
+                T v[EM];
+#pragma unroll
+                for (int e = 0; e < W::E(c); e++) v[e] = (T)(st.acc[W::d0(c) + e][r] * f);
+                T* p = out + W::base(c) + (4 * g + r) * W::E(c);
+                if (vec) {
+                    if (W::E(c) * sizeof(T) >= 16) {
+#pragma unroll
+                        for (int x = 0; x < (int)(W::E(c) * sizeof(T) / 16); x++) ((u32x4*)p)[x] = ((u32x4*)v)[x];
+                    } else if (W::E(c) * sizeof(T) == 8) {
+                        *(u32x2*)p = *(u32x2*)v;
+                    } else {
+                        *(uint32_t*)p = *(uint32_t*)v;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < W::E(c); e++) p[e] = v[e];
+                }
+            }
+    } else {
         // join the waves: their sums at the largest maximum, added in the waves' order
         if (g == 0) {
-            s_ml[w][0][i] = m;
-            s_ml[w][1][i] = l;
+            s_ml[w][0][i] = st.m;
+            s_ml[w][1][i] = st.l;
         }
         __syncthreads();
         float top = -INFINITY;
 #pragma unroll
         for (int x = 0; x < WAVES; x++) top = fmaxf(top, s_ml[x][0][i]);
-        const float tu = top == -INFINITY ? 0.0f : top;
-        total = 0.0f;
+        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - top);
 #pragma unroll
-        for (int x = 0; x < WAVES; x++) total += s_ml[x][1][i] * __builtin_amdgcn_exp2f(s_ml[x][0][i] - tu);
-        const float f = __builtin_amdgcn_exp2f(m - tu);
+        for (int c = 0; c < W::chunks; c++)
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            const bool first = d < W::E0;
-            const int E = first ? W::E0 : 2, base = first ? 0 : 64, e = first ? d : d - W::E0;
+            for (int e = 0; e < W::E(c); e++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) s_o[(w * 16 + i) * LD + base + (4 * g + r) * E + e] = acc[d][r] * f;
-        }
-        m = top;
+                for (int r = 0; r < 4; r++) s_o[(w * 16 + i) * LD + W::base(c) + (4 * g + r) * W::E(c) + e] = st.acc[W::d0(c) + e][r] * f;
         __syncthreads();
-        if (w) return;
+        for (int x = threadIdx.x * 4; x < keep * DH; x += 256 * 4) {
+            const int r = x / DH, d = x - r * DH, rr = rt * 16 + r;
+            const int tt = a.T == 1 ? 0 : rr / a.group, hh = h * a.group + (rr - tt * a.group);
+            if (rr >= rows || tt >= q.count) break;
+            float most = -INFINITY, total = 0.0f;
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            const bool first = d < W::E0;
-            const int E = first ? W::E0 : 2, base = first ? 0 : 64, e = first ? d : d - W::E0;
+            for (int y = 0; y < WAVES; y++) most = fmaxf(most, s_ml[y][0][r]);
+            v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float v = 0.0f;
-#pragma unroll
-                for (int x = 0; x < WAVES; x++) v += s_o[(x * 16 + i) * LD + base + (4 * g + r) * E + e];
-                acc[d][r] = v;
+            for (int y = 0; y < WAVES; y++) {
+                total += s_ml[y][1][r] * (most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_ml[y][0][r] - most));
+                sum += *(const v4f*)(s_o + (y * 16 + r) * LD + d);
             }
-        }
-    }
-    if (!there) return;
-    float* part = nullptr;
-    T* out = nullptr;
-    float f = 1.0f;
-    if (chunks > 1) {
-        // [chunk][unit][row][DH + 2]: sums, maximum, sum of probabilities
-        const int keep = min(16, rows);
-        part = a.ws + (((size_t)blockIdx.y * pairs * row_tiles + unit) * keep + i) * (DH + 2);
-        if (g == 0) {
-            part[DH] = m;
-            part[DH + 1] = total;
-        }
-    } else {
-        out = (T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head;
-        f = total == 0.0f ? 0.0f : 1.0f / total;
-    }
-#pragma unroll
-    for (int d = 0; d < ND; d++) {
-        const bool first = d < W::E0;
-        const int E = first ? W::E0 : 2, base = first ? 0 : 64, e = first ? d : d - W::E0;
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int ch = base + (4 * g + r) * E + e;
-            if (part) part[ch] = acc[d][r];
-            else out[ch] = (T)(acc[d][r] * f);
+            if (split) {
+                *(v4f*)(part + r * kPart<DH> + d) = sum;
+                if (d == 0) {
+                    part[r * kPart<DH> + DH] = most;
+                    part[r * kPart<DH> + DH + 1] = total;
+                }
+            } else {
+                store4((T*)a.out.data + s * a.out.seq + tt * a.out.token + hh * a.out.head + d, sum * (total == 0.0f ? 0.0f : 1.0f / total), vec);
+            }
         }
     }
 }
 
-// Joins the chunks of a row tile that took more than one, in the chunks' order. A workgroup a row tile.
+// Joins the chunks of a row tile that took more than one: a workgroup a row, its lanes over channels (four each) and, in as many
+// groups as fit, over the chunks, whose sums are added in a fixed order.
 template <int DH, class T>
-__global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles) {
-    const int unit = blockIdx.x, pairs = a.c.n * a.c.heads;
+__global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
+    constexpr int LC = DH / 4, G = 256 / LC;  // lanes a group, groups
+    __shared__ float s_top[4];
+    __shared__ __align__(16) float s_sum[G][DH + 4];
+    __shared__ float s_total[G];
+    const int unit = blockIdx.x, pairs = a.c.n * a.c.heads, r = blockIdx.y;
     const int pair = unit / row_tiles, rt = unit - pair * row_tiles;
     const int s = pair / a.c.heads, h = pair - s * a.c.heads;
     const SeqSpan q = seq_span(a.pos, a.counts, s, a.T);
-    const int t_lo = rt * 16 / a.group;
-    if (t_lo >= q.count) return;
-    const int t_hi = min((rt * 16 + 15) / a.group, q.count - 1);
-    const Tiles tl = tiles_of(q.pos + t_lo, q.pos + t_hi, q.end, a.c.sinks, a.c.cap - a.c.sinks, a.c.cap, a.window);
-    const int chunks = (tl.count() + chunk_tiles - 1) / chunk_tiles;
+    const int rows = a.T * a.group, keep = min(16, rows), row = rt * 16 + r;
+    const int t = row / a.group, head = h * a.group + (row - t * a.group);
+    if (row >= rows || t >= q.count) return;
+    Seen seen;
+    seen.sinks = a.c.sinks; seen.ring = a.c.cap - a.c.sinks; seen.window = a.window;
+    seen.last = q.end - 1;
+    seen.newest = seen.last >= seen.sinks ? kv_slot(seen.last, seen.sinks, seen.ring) : -1;
+    seen.lo_at = q.pos + rt * 16 / a.group;
+    seen.hi_at = q.pos + min((rt * 16 + 15) / a.group, q.count - 1);
+    const int chunks = (tiles_of(seen, a.c.cap).count() + chunk_tiles - 1) / chunk_tiles;
     if (chunks <= 1) return;
-    const int rows = a.T * a.group, keep = min(16, rows);
-    const size_t step = (size_t)pairs * row_tiles * keep * (DH + 2);
-    for (int x = threadIdx.x; x < 16 * DH; x += 256) {
-        const int i = x / DH, d = x - i * DH, row = rt * 16 + i;
-        const int t = row / a.group, head = h * a.group + (row - t * a.group);
-        if (row >= rows || t >= q.count) break;
-        const float* part = a.ws + ((size_t)unit * keep + i) * (DH + 2);
-        float top = -INFINITY;
-        for (int c = 0; c < chunks; c++) top = fmaxf(top, part[c * step + DH]);
-        const float tu = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f, total = 0.0f;
-        for (int c = 0; c < chunks; c++) {
-            const float f = __builtin_amdgcn_exp2f(part[c * step + DH] - tu);
-            sum += part[c * step + d] * f;
+    const size_t step = (size_t)pairs * row_tiles * keep * kPart<DH>;
+    const float* part = a.ws + ((size_t)unit * keep + r) * kPart<DH>;
+    float top = -INFINITY;
+    for (int c = threadIdx.x; c < chunks; c += 256) top = fmaxf(top, part[c * step + DH]);
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    const int grp = threadIdx.x / LC, d = (threadIdx.x - grp * LC) * 4;
+    if (grp < G) {
+        v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        float total = 0.0f;
+        for (int c = grp; c < chunks; c += G) {
+            const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[c * step + DH] - top);
+            sum += *(const v4f*)(part + c * step + d) * f;
             total += part[c * step + DH + 1] * f;
         }
-        T* out = (T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head;
-        out[d] = (T)(total == 0.0f ? 0.0f : sum / total);
+        *(v4f*)(s_sum[grp] + d) = sum;
+        if (d == 0) s_total[grp] = total;
     }
+    __syncthreads();
+    if (threadIdx.x >= LC) return;
+    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    float total = 0.0f;
+    for (int x = 0; x < G; x++) {
+        sum += *(const v4f*)(s_sum[x] + 4 * threadIdx.x);
+        total += s_total[x];
+    }
+    store4((T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head + 4 * threadIdx.x, sum * (total == 0.0f ? 0.0f : 1.0f / total), vec);
 }
 
 struct RowsPlan {
@@ -508,7 +682,7 @@ RowsPlan rows_plan(const KvAttnArgs& a) {
     p.chunk_tiles = tiles;
     if (p.waves > 1) {
         // enough workgroups to fill the chip, each with four tiles a wave at least
-        const int want = std::max(1, 2048 / std::max(1, p.units));
+        const int want = std::max(1, 2048 / p.units);
         p.chunk_tiles = std::max(16, (tiles + want - 1) / want);
     }
     p.chunks = std::max(1, (tiles + p.chunk_tiles - 1) / p.chunk_tiles);
@@ -525,21 +699,22 @@ hipError_t launch_kv_read(const KvRowsArgs& a, hipStream_t s) { return launch_ro
 size_t kv_attention_ws_bytes(const KvAttnArgs& a) {
     const RowsPlan p = rows_plan(a);
     if (p.chunks <= 1) return 0;
-    return (size_t)p.chunks * p.units * std::min(16, a.T * a.group) * (a.c.dh + 2) * 4;
+    return (size_t)p.chunks * p.units * std::min(16, a.T * a.group) * (a.c.dh + 4) * 4;
 }
 
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
     const RowsPlan p = rows_plan(a);
+    const int vec = rows_aligned(a.q, a.type) && rows_aligned(a.out, a.type);
     return by_width(a.c.dh, [&](auto w) {
         constexpr int DH = decltype(w)::value;
         return by_real(a.type, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
             if (p.waves == 1) {
-                hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, 1>), dim3((p.units + 3) / 4), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles);
+                hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, 1>), dim3((p.units + 3) / 4), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
             } else {
-                hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, 4>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles);
+                hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, 4>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
                 if (p.chunks > 1)
-                    hipLaunchKernelGGL((kv_attention_join_kernel<DH, T>), dim3(p.units), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles);
+                    hipLaunchKernelGGL((kv_attention_join_kernel<DH, T>), dim3(p.units, std::min(16, a.T * a.group)), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
             }
             return hipGetLastError();
         });
