@@ -223,60 +223,107 @@ __device__ __forceinline__ float sum_groups(float v) {
 constexpr int kTile = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// A tile of 32 slots as one lane of a wave holds it. K: two products of 16 keys, lane i holding slot 8 (i >> 2) + 4 h + (i & 3) of
-// the tile in product h, so that the scores of slots 8 g .. 8 g + 7 come out in lane group g. V: those eight slots, the lane's
-// channels of each.
+// One 16-byte (4-byte) load per lane from global memory straight into LDS: lane L's bytes land at LDS offset lds + 16 L (4 L).
+// Inline assembly, with the waits written out (vm_wait), because the compiler would wait for all such loads before any LDS
+// read. The LDS address goes through M0 (its write needs a wait state before its use). No register receives anything.
+__device__ __forceinline__ void lds_load16(const uint8_t* p, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "m0", "memory");
+}
+__device__ __forceinline__ void lds_load4(const uint8_t* p, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "m0", "memory");
+}
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+
+// A tile of 32 slots of one head in LDS: K's rows, V's rows, their scales, in DH / 32 loads of 1 KiB and one of 256 bytes (which
+// the scales of narrower heads do not fill). The order is chosen against bank conflicts: of K, block b of slot j stands at
+// place b ^ f(j) of its row (DH 128; f from bits 1 and 3 of j, in which the eight slots that eight lanes read together differ
+// besides bit 0), of V slot j's row is row j ^ ((j >> 3) & 3) (the four lane groups read slots eight apart).
 template <int DH>
 struct KvTile {
     using W = Width<DH>;
-    uint32_t k[2][W::KS];
-    uint32_t ks[2][W::KW];
-    uint32_t v[W::chunks][8];
-    uint32_t vs[2 * W::NB];
+    static constexpr int row = DH / 2, half = 32 * row, o_scales = 2 * half, bytes = o_scales + 256;
+    static constexpr int loads = W::KS + 1;
 
-    __device__ __forceinline__ void load(const uint8_t* kb, const uint8_t* ksb, const uint8_t* vb, const uint8_t* vsb, int j0, int i, int g) {
-        kb += (size_t)j0 * (DH / 2);
-        vb += (size_t)j0 * (DH / 2);
-        ksb += (size_t)j0 * W::NB;
-        vsb += (size_t)j0 * W::NB;
+    __device__ static __forceinline__ int k_place(int j) { return DH == 128 ? ((j >> 1) & 1) | ((j >> 2) & 2) : 0; }
+
+    // What each lane loads of the tile at slot 0 of the cache's first plane: addresses, to which (plane * cap + slot) rows are added.
+    struct Source {
+        const uint8_t* codes[W::KS];
+        const uint8_t* scales;
+        __device__ __forceinline__ void set(const KvCache& c, int lane) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int key = (i >> 2) * 8 + 4 * h + (i & 3);
-            const uint8_t* p = kb + key * (DH / 2) + (W::kEven ? (DH / 8) * g : 4 * g);
-            if constexpr (DH == 128) *(u32x4*)k[h] = *(const u32x4*)p;
-            else if constexpr (DH == 64) *(u32x2*)k[h] = *(const u32x2*)p;
+            for (int x = 0; x < W::KS; x++) {
+                const int at = 1024 * x + 16 * lane;
+                if (at < half) {
+                    const int j = at / row, b = at % row / 16;
+                    codes[x] = c.k + j * row + 16 * (b ^ k_place(j));
+                } else {
+                    const int j = (at - half) / row;
+                    codes[x] = c.v + (j ^ ((j >> 3) & 3)) * row + (at - half) % row;
+                }
+            }
+            const int at = 4 * (lane & (16 * W::NB - 1 | (W::NB == 3 ? 63 : 0)));
+            const int in = W::NB == 3 ? min(at, 188) : at;  // (lanes past the scales repeat one)
+            scales = in < 32 * W::NB ? c.ks + in : c.vs + in - 32 * W::NB;
+        }
+        __device__ __forceinline__ void load(size_t slot, uint32_t lds) const {
+#pragma unroll
+            for (int x = 0; x < W::KS; x++) lds_load16(codes[x] + slot * row, lds + 1024 * x);
+            lds_load4(scales + slot * W::NB, lds + o_scales);
+        }
+    };
+
+    // Product h of the scores: lane i holds slot 8 (i >> 2) + 4 h + (i & 3), so that the scores of slots 8 g .. 8 g + 7 come out in
+    // lane group g.
+    struct Key {
+        uint32_t w[W::KS], s[W::KW];
+        __device__ __forceinline__ void read(const uint8_t* p, int h, int i, int g) {
+            const int j = (i >> 2) * 8 + 4 * h + (i & 3);
+            const uint8_t* q = p + j * row;
+            if constexpr (DH == 128) *(u32x4*)w = *(const u32x4*)(q + 16 * (g ^ k_place(j)));
+            else if constexpr (DH == 64) *(u32x2*)w = *(const u32x2*)(q + 8 * g);
             else
 #pragma unroll
-                for (int s = 0; s < W::KS; s++) k[h][s] = *(const uint32_t*)(p + 16 * s);
+                for (int x = 0; x < W::KS; x++) w[x] = *(const uint32_t*)(q + 16 * x + 4 * g);
 #pragma unroll
-            for (int x = 0; x < W::KW; x++) ks[h][x] = ksb[key * W::NB + (W::kEven ? (DH / 4) * g / 32 : x)];
+            for (int x = 0; x < W::KW; x++) s[x] = p[o_scales + j * W::NB + (W::kEven ? (DH / 4) * g / 32 : x)];
         }
+    };
+    // Slots 8 g .. 8 g + 7, the lane's channels of each.
+    struct Value {
+        uint32_t w[W::chunks][8];
+        uint32_t s[2 * W::NB];
+        __device__ __forceinline__ void read(const uint8_t* p, int i, int g) {
 #pragma unroll
-        for (int c = 0; c < W::chunks; c++) {
-            const uint8_t* p = vb + 8 * g * (DH / 2) + (W::base(c) + i * W::E(c)) / 2;
+            for (int c = 0; c < W::chunks; c++)
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                v[c][e] = W::E(c) == 8 ? *(const uint32_t*)(p + e * (DH / 2)) : W::E(c) == 4 ? *(const uint16_t*)(p + e * (DH / 2)) : p[e * (DH / 2)];
+                for (int e = 0; e < 8; e++) {
+                    const uint8_t* q = p + half + (8 * g + (e ^ g)) * row + (W::base(c) + i * W::E(c)) / 2;
+                    w[c][e] = W::E(c) == 8 ? *(const uint32_t*)q : W::E(c) == 4 ? *(const uint16_t*)q : *q;
+                }
+#pragma unroll
+            for (int x = 0; x < W::NB; x++) *(u32x2*)(s + 2 * x) = *(const u32x2*)(p + o_scales + 32 * W::NB + 8 * g * W::NB + 8 * x);
         }
-#pragma unroll
-        for (int x = 0; x < W::NB; x++) *(u32x2*)(vs + 2 * x) = *(const u32x2*)(vsb + 8 * g * W::NB + 8 * x);
-    }
-    // The scale byte of slot 8 g + e for block b, and the scale for a conversion (b of this lane's channels in chunk c).
-    __device__ __forceinline__ uint32_t v_byte(int e, int b) const {
-        const int at = e * W::NB + b;
-        return (vs[at >> 2] >> (8 * (at & 3))) & 255;
-    }
-    __device__ __forceinline__ float v_scale(int c, int e, int i) const {
-        if constexpr (DH == 128) return scale_at(vs[e], 8 * (i >> 2) + 9);
-        else if constexpr (DH == 64) return scale_at(vs[e >> 1], 16 * (e & 1) + 8 * (i >> 3) + 9);
-        else if constexpr (DH == 32) return scale_at(vs[e >> 2], scale_shift(e & 3));
-        else {
-            if (c == 1) return scale_at(vs[(3 * e + 2) >> 2], scale_shift((3 * e + 2) & 3));
-            const int at = 3 * e;  // this byte or the next
-            const float lo = scale_at(vs[at >> 2], scale_shift(at & 3)), hi = scale_at(vs[(at + 1) >> 2], scale_shift((at + 1) & 3));
-            return i & 8 ? hi : lo;
+        // The scale byte of slot 8 g + e for block b, and the scale for a conversion (of this lane's channels in chunk c).
+        __device__ __forceinline__ uint32_t byte(int e, int b) const {
+            const int at = e * W::NB + b;
+            return (s[at >> 2] >> (8 * (at & 3))) & 255;
         }
-    }
+        __device__ __forceinline__ float scale(int c, int e, int i) const {
+            if constexpr (DH == 128) return scale_at(s[e], 8 * (i >> 2) + 9);
+            else if constexpr (DH == 64) return scale_at(s[e >> 1], 16 * (e & 1) + 8 * (i >> 3) + 9);
+            else if constexpr (DH == 32) return scale_at(s[e >> 2], scale_shift(e & 3));
+            else {
+                if (c == 1) return scale_at(s[(3 * e + 2) >> 2], scale_shift((3 * e + 2) & 3));
+                const int at = 3 * e;  // this byte or the next
+                const float lo = scale_at(s[at >> 2], scale_shift(at & 3)), hi = scale_at(s[(at + 1) >> 2], scale_shift((at + 1) & 3));
+                return i & 8 ? hi : lo;
+            }
+        }
+    };
 };
 
 // Two elements of word w (byte b), scaled, as bf16.
@@ -346,32 +393,42 @@ struct RowState {
     }
 };
 
-// One tile for 16 rows. Scores leave the matrix cores with lane (i, g) holding row i and slots 8 g .. 8 g + 7 of the tile, the very
-// layout in which the second product takes the probabilities: they never leave their lane. V comes into its layout (one
-// channel of eight slots in a lane) by unpacking the words of two slots and exchanging halves. CAREFUL keeps blocks of NaN
-// out of the product (they would spread over rows that do not see their key) and notes who sees them instead.
-template <int DH, class T, bool CAREFUL>
-__device__ __forceinline__ void tile_step(RowState<DH>& st, const KvTile<DH>& x, const v8bf (*qf)[Terms<T>::q], float scale,
-                                          const Seen& seen, int j0, bool whole, int i, int g) {
+// One tile of HB heads for 16 rows, column i of the products belonging to head `mine` of them. Scores leave the matrix cores with lane
+// (i, g) holding row i and slots 8 g .. 8 g + 7 of the tile, the very layout in which the second product takes the probabilities:
+// they never leave their lane. With several heads each product is formed for all rows and kept, or added, for its own: the
+// softmax between is done once for all of them. V comes into its layout (one channel of eight slots in a lane) by unpacking
+// the words of two slots and exchanging halves. CAREFUL keeps blocks of NaN out of the product (they would spread over rows that
+// do not see their key) and notes who sees them instead.
+template <int DH, class T, int HB, bool CAREFUL>
+__device__ __forceinline__ void tile_step(RowState<DH>& st, const uint8_t* tile, const v8bf (*qf)[Terms<T>::q], float scale,
+                                          const Seen& seen, int j0, bool whole, int i, int g, int mine) {
     using W = Width<DH>;
+    using Tile = KvTile<DH>;
     constexpr int QT = Terms<T>::q, PT = Terms<T>::p;
     float sc[8];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int hb = 0; hb < HB; hb++) {
 #pragma unroll
-        for (int s = 0; s < W::KS; s++) {
-            const float ks = mx4_scale(x.ks[h][W::kEven ? 0 : s]);
-            uint32_t kw[4];
+        for (int h = 0; h < 2; h++) {
+            typename Tile::Key x;
+            x.read(tile + hb * Tile::bytes, h, i, g);
+            v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int b = 0; b < 4; b++) kw[b] = unpack2(x.k[h][s], ks, b);
-            const v8bf kf = __builtin_bit_cast(v8bf, *(u32x4*)kw);
+            for (int s = 0; s < W::KS; s++) {
+                const float ks = mx4_scale(x.s[W::kEven ? 0 : s]);
+                uint32_t kw[4];
 #pragma unroll
-            for (int n = QT - 1; n >= 0; n--) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[s][n], d, 0, 0, 0);
+                for (int b = 0; b < 4; b++) kw[b] = unpack2(x.w[s], ks, b);
+                const v8bf kf = __builtin_bit_cast(v8bf, *(u32x4*)kw);
+#pragma unroll
+                for (int n = QT - 1; n >= 0; n--) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[s][n], d, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) sc[4 * h + r] = hb == 0 || mine == hb ? d[r] : sc[4 * h + r];
         }
-#pragma unroll
-        for (int r = 0; r < 4; r++) sc[4 * h + r] = d[r] * scale;
     }
+#pragma unroll
+    for (int e = 0; e < 8; e++) sc[e] *= scale;
     uint32_t sees = 255, drop = 0;
     if (!whole) {
         sees = 0;
@@ -398,44 +455,58 @@ __device__ __forceinline__ void tile_step(RowState<DH>& st, const KvTile<DH>& x,
 #pragma unroll
     for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(sc[e] - mu);
     st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-    v8bf pf[PT];
-    split_bf16<PT>(p, pf);
-    if (CAREFUL) {
+    v8bf pall[PT];
+    split_bf16<PT>(p, pall);
 #pragma unroll
-        for (int e = 0; e < 8; e++)
+    for (int hb = 0; hb < HB; hb++) {
+        typename Tile::Value x;
+        x.read(tile + hb * Tile::bytes, i, g);
+        v8bf pf[PT];
 #pragma unroll
-            for (int b = 0; b < W::NB; b++)
-                if (((sees >> e) & 1) && x.v_byte(e, b) > 252u) st.nan_blocks |= 1u << b;
-    }
+        for (int n = 0; n < PT; n++) {
+            u32x4 w = __builtin_bit_cast(u32x4, pall[n]);
+            if (HB > 1)
 #pragma unroll
-    for (int c = 0; c < W::chunks; c++) {
-        uint32_t word[8];
-        float vs[8];
+                for (int r = 0; r < 4; r++) w[r] = mine == hb ? w[r] : 0;
+            pf[n] = __builtin_bit_cast(v8bf, w);
+        }
+        if (CAREFUL) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            word[e] = x.v[c][e];
-            vs[e] = x.v_scale(c, e, i);
-            // (the writer's scales are at most 252, or 255 for NaN)
-            if ((CAREFUL && (__float_as_uint(vs[e]) >> 23 & 255) > 252u) || (!whole && (drop >> e & 1))) {
-                word[e] = 0;
-                vs[e] = 0.0f;
-            }
+            for (int e = 0; e < 8; e++)
+#pragma unroll
+                for (int b = 0; b < W::NB; b++)
+                    if (((sees >> e) & 1) && mine == hb && x.byte(e, b) > 252u) st.nan_blocks |= 1u << b;
         }
 #pragma unroll
-        for (int b = 0; b < W::E(c) / 2; b++) {
-            uint32_t lo[4], hi[4];
+        for (int c = 0; c < W::chunks; c++) {
+            uint32_t word[8];
+            float vs[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t y0 = unpack2(word[2 * e], vs[2 * e], b), y1 = unpack2(word[2 * e + 1], vs[2 * e + 1], b);
-                lo[e] = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
-                hi[e] = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
+            for (int e = 0; e < 8; e++) {
+                word[e] = x.w[c][e];
+                vs[e] = x.scale(c, e, i);
+                // (the writer's scales are at most 252, or 255 for NaN)
+                if ((CAREFUL && (__float_as_uint(vs[e]) >> 23 & 255) > 252u) || (!whole && (drop >> e & 1))) {
+                    word[e] = 0;
+                    vs[e] = 0.0f;
+                }
             }
-            const v8bf v0 = __builtin_bit_cast(v8bf, *(u32x4*)lo), v1 = __builtin_bit_cast(v8bf, *(u32x4*)hi);
-            const int d = W::d0(c) + 2 * b;
 #pragma unroll
-            for (int n = PT - 1; n >= 0; n--) {
-                st.acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pf[n], st.acc[d], 0, 0, 0);
-                st.acc[d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pf[n], st.acc[d + 1], 0, 0, 0);
+            for (int b = 0; b < W::E(c) / 2; b++) {
+                uint32_t lo[4], hi[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t y0 = unpack2(word[2 * e], vs[2 * e], b), y1 = unpack2(word[2 * e + 1], vs[2 * e + 1], b);
+                    lo[e] = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
+                    hi[e] = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
+                }
+                const v8bf v0 = __builtin_bit_cast(v8bf, *(u32x4*)lo), v1 = __builtin_bit_cast(v8bf, *(u32x4*)hi);
+                const int d = W::d0(c) + 2 * b;
+#pragma unroll
+                for (int n = PT - 1; n >= 0; n--) {
+                    st.acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pf[n], st.acc[d], 0, 0, 0);
+                    st.acc[d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pf[n], st.acc[d + 1], 0, 0, 0);
+                }
             }
         }
     }
@@ -445,22 +516,35 @@ __device__ __forceinline__ void tile_step(RowState<DH>& st, const KvTile<DH>& x,
 template <int DH>
 constexpr int kPart = DH + 4;
 
-// Few query rows: a wave takes 16 rows (the query heads of one key/value head, token after token) over a share of the tiles,
-// loading each tile while the one before is worked on. WAVES waves share the tiles of a row tile (of one chunk of them, with
-// a.chunks > 1) and add up what they have in LDS; with WAVES 1 a wave is alone with its row tile.
-template <int DH, class T, int WAVES>
+// Stages of a wave's tiles in LDS, for two workgroups of four waves a CU.
+template <int DH, int HB>
+struct Stages {
+    static constexpr int bytes = HB * KvTile<DH>::bytes;
+    static constexpr int n = std::min(4, std::max(2, 19 * 1024 / bytes));
+    static constexpr int loads = HB * KvTile<DH>::loads;
+    static constexpr int wave = n * bytes;
+    static_assert((n - 1) * loads <= 63, "");
+};
+
+// Few query rows: a wave takes up to 16 rows of one sequence over a share of the tiles: a row tile of one key/value head (its
+// query heads, token after token), or, with HB > 1, all rows of HB heads (16 or fewer). Tiles come straight into the wave's own
+// LDS stages, up to three ahead. WAVES waves share the tiles (of one chunk of them, where there are several) and add up what
+// they have in LDS; with WAVES 1 a wave is alone with its rows.
+template <int DH, class T, int HB, int WAVES>
 __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
     using W = Width<DH>;
+    using Tile = KvTile<DH>;
+    using St = Stages<DH, HB>;
     constexpr int QT = Terms<T>::q, LD = DH + 4;
-    __shared__ float s_ml[WAVES > 1 ? WAVES : 1][2][16];
-    __shared__ __align__(16) float s_o[WAVES > 1 ? WAVES * 16 * LD : 4];
+    static_assert(4 * 16 * (LD + 2) * 4 <= 4 * St::wave, "");
+    __shared__ __align__(16) uint8_t smem[4 * St::wave];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int unit = WAVES > 1 ? blockIdx.x : blockIdx.x * 4 + wave, w = WAVES > 1 ? wave : 0;
-    const int pairs = a.c.n * a.c.heads;
-    if (unit >= pairs * row_tiles) return;
+    const int blocks = (a.c.heads + HB - 1) / HB, units = a.c.n * blocks * row_tiles;
+    if (unit >= units) return;
     const int pair = row_tiles == 1 ? unit : unit / row_tiles, rt = unit - pair * row_tiles;
-    const int s = pair / a.c.heads, h = pair - s * a.c.heads;
+    const int s = pair / blocks, h0 = (pair - s * blocks) * HB;
     const SeqSpan q = seq_span(a.pos, a.counts, s, a.T);
     const int ring = a.c.cap - a.c.sinks, sinks = a.c.sinks;
     const int t_lo = rt == 0 ? 0 : rt * 16 / a.group;
@@ -478,12 +562,32 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
     const int o0 = blockIdx.y * chunk_tiles, o1 = min(n_tiles, o0 + chunk_tiles);
     if (blockIdx.y && o0 >= n_tiles) return;
 
+    typename Tile::Source src;
+    src.set(a.c, lane);
+    uint8_t* mine = smem + wave * St::wave;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)mine;
+    const size_t plane = (size_t)(s * a.c.heads + h0) * a.c.cap;
+    auto load = [&](int j0, int stage) {
+#pragma unroll
+        for (int hb = 0; hb < HB; hb++)
+            src.load(plane + (size_t)min(hb, a.c.heads - 1 - h0) * a.c.cap + j0, lds0 + stage * St::bytes + hb * Tile::bytes);
+    };
+
     // this lane's row
-    const int row = rt * 16 + i, rows = a.T * a.group;
-    const int t = a.T == 1 ? 0 : row / a.group, head = h * a.group + (row - t * a.group);
-    const bool there = row < rows && t < q.count;
+    const int rows = a.T * a.group;  // of a head
+    const int hb = HB > 1 ? i / rows : 0, row = HB > 1 ? i - hb * rows : rt * 16 + i;
+    const int t = a.T == 1 ? 0 : row / a.group, head = (h0 + hb) * a.group + (row - t * a.group);
+    const bool there = hb < HB && h0 + hb < a.c.heads && row < rows && t < q.count;
     seen.at = q.pos + t;
     v8bf qf[W::KS][QT];
+    float scale = 0.0f;
+    // the first `ahead` tiles of a pass are on their way
+    auto start = [&] {
+#pragma unroll
+        for (int x = 0; x < St::n - 1; x++)
+            if (o0 + w + x * WAVES < o1) load(tl.at(o0 + w + x * WAVES) * kTile, x);
+    };
+    start();
 #pragma unroll
     for (int st = 0; st < W::KS; st++) {
         float x[8] = {};
@@ -494,27 +598,29 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
         }
         split_bf16<QT>(x, qf[st]);
     }
-    const float scale = a.scale * kLog2e;
-    const size_t plane = (size_t)pair * a.c.cap;
-    const uint8_t* kb = a.c.k + plane * (DH / 2);
-    const uint8_t* ksb = a.c.ks + plane * W::NB;
-    const uint8_t* vb = a.c.v + plane * (DH / 2);
-    const uint8_t* vsb = a.c.vs + plane * W::NB;
+    scale = a.scale * kLog2e;
 
     RowState<DH> st;
     auto sweep = [&](auto careful) {
         st.clear();
-        int o = o0 + w;
-        if (o >= o1) return;
-        KvTile<DH> x, y;
-        int j0 = __builtin_amdgcn_readfirstlane(tl.at(o) * kTile);
-        x.load(kb, ksb, vb, vsb, j0, i, g);
-        for (; o < o1; o += WAVES) {
-            const int j1 = __builtin_amdgcn_readfirstlane(tl.at(min(o + WAVES, o1 - 1)) * kTile);
-            if (o + WAVES < o1) y.load(kb, ksb, vb, vsb, j1, i, g);
-            tile_step<DH, T, decltype(careful)::value>(st, x, qf, scale, seen, j0, seen.whole(j0), i, g);
-            x = y;
-            j0 = j1;
+        int stage = 0;
+        for (int o = o0 + w; o < o1; o += WAVES) {
+            // the tiles issued after this one: up to n - 2 now, one more below
+            const int more = (o1 - 1 - o) / WAVES;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last stage's reads are done: it is loaded anew
+            if (more >= St::n - 1) {
+                load(tl.at(o + (St::n - 1) * WAVES) * kTile, stage == 0 ? St::n - 1 : stage - 1);
+                vm_wait<(St::n - 1) * St::loads>();
+            } else if (St::n > 3 && more == 2) {
+                vm_wait<2 * St::loads>();
+            } else if (St::n > 2 && more == 1) {
+                vm_wait<St::loads>();
+            } else {
+                vm_wait<0>();
+            }
+            const int j0 = __builtin_amdgcn_readfirstlane(tl.at(o) * kTile);
+            tile_step<DH, T, HB, decltype(careful)::value>(st, mine + stage * St::bytes, qf, scale, seen, j0, seen.whole(j0), i, g, hb);
+            stage = stage == St::n - 1 ? 0 : stage + 1;
         }
     };
     sweep(std::false_type());
@@ -525,7 +631,11 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
         for (int d = 0; d < W::ND; d++)
 #pragma unroll
             for (int r = 0; r < 4; r++) bad += st.acc[d][r] * 0.0f;
-        if (__any(bad != 0.0f)) sweep(std::true_type());
+        if (__any(bad != 0.0f)) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            start();
+            sweep(std::true_type());
+        }
     }
     st.l = sum_groups(st.l);
     if (__any(st.nan_blocks)) {
@@ -540,9 +650,8 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
                     if ((st.nan_blocks >> ((W::base(c) + (4 * g + r) * W::E(c) + e) / 32)) & 1) st.acc[W::d0(c) + e][r] = NAN;
     }
     const bool split = n_tiles > chunk_tiles;
-    const int keep = min(16, rows);
-    // [chunk][unit][row][kPart]
-    float* part = a.ws + (((size_t)blockIdx.y * pairs * row_tiles + unit) * keep) * kPart<DH>;
+    // [chunk][unit][column][kPart]
+    float* part = a.ws + (((size_t)blockIdx.y * units + unit) * 16) * kPart<DH>;
     if constexpr (WAVES == 1) {
         if (!there) return;
         const float f = st.l == 0.0f ? 0.0f : 1.0f / st.l;
@@ -551,8 +660,7 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
         for (int c = 0; c < W::chunks; c++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                constexpr int EM = W::E0;
-                T v[EM];
+                T v[W::E0];
 #pragma unroll
                 for (int e = 0; e < W::E(c); e++) v[e] = (T)(st.acc[W::d0(c) + e][r] * f);
                 T* p = out + W::base(c) + (4 * g + r) * W::E(c);
@@ -571,7 +679,10 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
                 }
             }
     } else {
-        // join the waves: their sums at the largest maximum, added in the waves' order
+        // join the waves: their sums at the largest maximum, added in the waves' order (the stages are done with)
+        float* s_o = (float*)smem;                                 // [wave][column][LD]
+        float (*s_ml)[2][16] = (float (*)[2][16])(s_o + WAVES * 16 * LD);
+        __syncthreads();
         if (g == 0) {
             s_ml[w][0][i] = st.m;
             s_ml[w][1][i] = st.l;
@@ -588,27 +699,29 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
 #pragma unroll
                 for (int r = 0; r < 4; r++) s_o[(w * 16 + i) * LD + W::base(c) + (4 * g + r) * W::E(c) + e] = st.acc[W::d0(c) + e][r] * f;
         __syncthreads();
+        const int keep = min(16, HB > 1 ? HB * rows : rows - rt * 16);
         for (int x = threadIdx.x * 4; x < keep * DH; x += 256 * 4) {
-            const int r = x / DH, d = x - r * DH, rr = rt * 16 + r;
-            const int tt = a.T == 1 ? 0 : rr / a.group, hh = h * a.group + (rr - tt * a.group);
-            if (rr >= rows || tt >= q.count) break;
+            const int col = x / DH, d = x - col * DH;
+            const int hh = HB > 1 ? col / rows : 0, rr = HB > 1 ? col - hh * rows : rt * 16 + col;
+            const int tt = a.T == 1 ? 0 : rr / a.group, hd = (h0 + hh) * a.group + (rr - tt * a.group);
+            if (tt >= q.count || h0 + hh >= a.c.heads) continue;
             float most = -INFINITY, total = 0.0f;
 #pragma unroll
-            for (int y = 0; y < WAVES; y++) most = fmaxf(most, s_ml[y][0][r]);
+            for (int y = 0; y < WAVES; y++) most = fmaxf(most, s_ml[y][0][col]);
             v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int y = 0; y < WAVES; y++) {
-                total += s_ml[y][1][r] * (most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_ml[y][0][r] - most));
-                sum += *(const v4f*)(s_o + (y * 16 + r) * LD + d);
+                total += s_ml[y][1][col] * (most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_ml[y][0][col] - most));
+                sum += *(const v4f*)(s_o + (y * 16 + col) * LD + d);
             }
             if (split) {
-                *(v4f*)(part + r * kPart<DH> + d) = sum;
+                *(v4f*)(part + col * kPart<DH> + d) = sum;
                 if (d == 0) {
-                    part[r * kPart<DH> + DH] = most;
-                    part[r * kPart<DH> + DH + 1] = total;
+                    part[col * kPart<DH> + DH] = most;
+                    part[col * kPart<DH> + DH + 1] = total;
                 }
             } else {
-                store4((T*)a.out.data + s * a.out.seq + tt * a.out.token + hh * a.out.head + d, sum * (total == 0.0f ? 0.0f : 1.0f / total), vec);
+                store4((T*)a.out.data + s * a.out.seq + tt * a.out.token + hd * a.out.head + d, sum * (total == 0.0f ? 0.0f : 1.0f / total), vec);
             }
         }
     }
@@ -617,18 +730,20 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
 // Joins the chunks of a row tile that took more than one: a workgroup a row, its lanes over channels (four each) and, in as many
 // groups as fit, over the chunks, whose sums are added in a fixed order.
 template <int DH, class T>
-__global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
+__global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int hb, int row_tiles, int chunk_tiles, int vec) {
     constexpr int LC = DH / 4, G = 256 / LC;  // lanes a group, groups
     __shared__ float s_top[4];
     __shared__ __align__(16) float s_sum[G][DH + 4];
     __shared__ float s_total[G];
-    const int unit = blockIdx.x, pairs = a.c.n * a.c.heads, r = blockIdx.y;
+    const int unit = blockIdx.x, col = blockIdx.y;
+    const int blocks = (a.c.heads + hb - 1) / hb, units = a.c.n * blocks * row_tiles;
     const int pair = unit / row_tiles, rt = unit - pair * row_tiles;
-    const int s = pair / a.c.heads, h = pair - s * a.c.heads;
+    const int s = pair / blocks, h0 = (pair - s * blocks) * hb;
     const SeqSpan q = seq_span(a.pos, a.counts, s, a.T);
-    const int rows = a.T * a.group, keep = min(16, rows), row = rt * 16 + r;
-    const int t = row / a.group, head = h * a.group + (row - t * a.group);
-    if (row >= rows || t >= q.count) return;
+    const int rows = a.T * a.group;
+    const int hh = hb > 1 ? col / rows : 0, row = hb > 1 ? col - hh * rows : rt * 16 + col;
+    const int t = row / a.group, head = (h0 + hh) * a.group + (row - t * a.group);
+    if (row >= rows || t >= q.count || h0 + hh >= a.c.heads) return;
     Seen seen;
     seen.sinks = a.c.sinks; seen.ring = a.c.cap - a.c.sinks; seen.window = a.window;
     seen.last = q.end - 1;
@@ -637,8 +752,8 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, in
     seen.hi_at = q.pos + min((rt * 16 + 15) / a.group, q.count - 1);
     const int chunks = (tiles_of(seen, a.c.cap).count() + chunk_tiles - 1) / chunk_tiles;
     if (chunks <= 1) return;
-    const size_t step = (size_t)pairs * row_tiles * keep * kPart<DH>;
-    const float* part = a.ws + ((size_t)unit * keep + r) * kPart<DH>;
+    const size_t step = (size_t)units * 16 * kPart<DH>;
+    const float* part = a.ws + ((size_t)unit * 16 + col) * kPart<DH>;
     float top = -INFINITY;
     for (int c = threadIdx.x; c < chunks; c += 256) top = fmaxf(top, part[c * step + DH]);
     top = wave_max(top);
@@ -669,13 +784,16 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, in
 }
 
 struct RowsPlan {
-    int row_tiles, units, waves, chunk_tiles, chunks;
+    int hb, row_tiles, units, waves, chunk_tiles, chunks;
 };
 RowsPlan rows_plan(const KvAttnArgs& a) {
     RowsPlan p;
-    p.row_tiles = (a.T * a.group + 15) / 16;
-    p.units = a.c.n * a.c.heads * p.row_tiles;
-    // tiles a row tile can see, at most: the sinks', and the window's (or the ring's), with the ends of three runs
+    // heads a wave takes together: as many as give it 16 rows or fewer
+    const int rows = a.T * a.group, most = a.c.dh == 32 ? 8 : a.c.dh == 64 ? 4 : 2;
+    p.hb = rows * most <= 16 && a.c.heads % most == 0 ? most : rows * 2 <= 16 && a.c.heads % 2 == 0 ? 2 : 1;
+    p.row_tiles = (rows + 15) / 16;
+    p.units = a.c.n * (a.c.heads / p.hb) * p.row_tiles;
+    // tiles that a row tile can see, at most: the sinks', and the window's (or the ring's), with the ends of three runs
     const long long span = a.window > 0 ? std::min<long long>((long long)a.window + a.T, a.c.cap) : a.c.cap;
     const int tiles = (int)std::min<long long>((span + kTile - 1) / kTile + (a.c.sinks + kTile - 1) / kTile + 2, a.c.cap / kTile);
     p.waves = tiles <= 4 ? 1 : 4;
@@ -689,6 +807,20 @@ RowsPlan rows_plan(const KvAttnArgs& a) {
     return p;
 }
 
+template <int DH, class T, int HB>
+hipError_t launch_rows_attention(const KvAttnArgs& a, const RowsPlan& p, hipStream_t s) {
+    const int vec = rows_aligned(a.q, a.type) && rows_aligned(a.out, a.type);
+    if (p.waves == 1) {
+        hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 1>), dim3((p.units + 3) / 4), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
+    } else {
+        hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 4>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
+        if (p.chunks > 1)
+            hipLaunchKernelGGL((kv_attention_join_kernel<DH, T>), dim3(p.units, std::min(16, HB * a.T * a.group)), dim3(256), 0, s, a, HB,
+                               p.row_tiles, p.chunk_tiles, vec);
+    }
+    return hipGetLastError();
+}
+
 }  // namespace
 
 bool kv_head_width(int dh) { return dh == 32 || dh == 64 || dh == 96 || dh == 128; }
@@ -699,24 +831,19 @@ hipError_t launch_kv_read(const KvRowsArgs& a, hipStream_t s) { return launch_ro
 size_t kv_attention_ws_bytes(const KvAttnArgs& a) {
     const RowsPlan p = rows_plan(a);
     if (p.chunks <= 1) return 0;
-    return (size_t)p.chunks * p.units * std::min(16, a.T * a.group) * (a.c.dh + 4) * 4;
+    return (size_t)p.chunks * p.units * 16 * (a.c.dh + 4) * 4;
 }
 
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
     const RowsPlan p = rows_plan(a);
-    const int vec = rows_aligned(a.q, a.type) && rows_aligned(a.out, a.type);
     return by_width(a.c.dh, [&](auto w) {
-        constexpr int DH = decltype(w)::value;
+        constexpr int DH = decltype(w)::value, most = DH == 32 ? 8 : DH == 64 ? 4 : 2;
         return by_real(a.type, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            if (p.waves == 1) {
-                hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, 1>), dim3((p.units + 3) / 4), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
-            } else {
-                hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, 4>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
-                if (p.chunks > 1)
-                    hipLaunchKernelGGL((kv_attention_join_kernel<DH, T>), dim3(p.units, std::min(16, a.T * a.group)), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
-            }
-            return hipGetLastError();
+            if (p.hb == most) return launch_rows_attention<DH, T, most>(a, p, s);
+            if constexpr (most > 2)
+                if (p.hb == 2) return launch_rows_attention<DH, T, 2>(a, p, s);
+            return launch_rows_attention<DH, T, 1>(a, p, s);
         });
     });
 }
