@@ -3,6 +3,7 @@
 #include "mx4.hpp"
 
 #include <algorithm>
+#include <climits>
 
 #include "common.hpp"
 #include "mx4_device.hpp"
@@ -145,7 +146,7 @@ struct Tiles {
     int n0, n1, n2;      // tiles of each run
     int b1, b2;          // first tiles of the second and third
     __device__ __forceinline__ int count() const { return n0 + n1 + n2; }
-    __device__ __forceinline__ int at(int o) const { return o < n0 ? o : o < n0 + n1 ? b1 + o - n0 : b2 + o - n0 - n1; }
+    __device__ __forceinline__ int at(int o) const { return o + (o >= n0 ? b1 - n0 : 0) + (o >= n0 + n1 ? b2 - b1 - n1 : 0); }
 };
 template <class T>
 struct Terms;  // bf16 parts that hold a query element, and those that a probability is split into
@@ -184,20 +185,20 @@ __device__ __forceinline__ void split_bf16(const float x[8], v8bf out[N]) {
 }
 
 // Channels of a head as the two products take them, with i = lane & 15 and g = lane >> 4.
-//   Scores, K (16 keys a product) times q: step s of DH / 32 covers, for lane group g, channels (DH / 4) g + 8 s .. + 7, so
+//   Scores, K (16 slots a product) times q: step s of DH / 32 covers, for lane group g, channels (DH / 4) g + 8 s .. + 7, so
 //   that a lane's steps are neighbouring words of a row (DH 96: channels 32 s + 8 g, since 24 do not end with a block).
-//   Output, V^T times the probabilities: channels in chunks of 16 E, lane i owning E neighbouring ones (E 8, 4, 2): of the
-//   product's result, lane (i, g) holds row i and in element r of fragment e channel base + (4 g + r) E + e.
+//   Output, V^T times the probabilities: channels in chunks of 16 E, lane i owning E neighbouring ones (E 8, 4, 2), a pair at a
+//   time.
 template <int DH>
 struct Width {
-    static constexpr int KS = DH / 32, NB = DH / 32, ND = DH / 16;
+    static constexpr int KS = DH / 32, NB = DH / 32, NA = DH / 32;  // NA: fragments of the output, 16 pairs of channels each
     static constexpr bool kEven = DH != 96;
     static constexpr int KW = kEven ? 1 : 3;  // scale bytes a lane needs of a key
     static constexpr int chunks = DH == 96 ? 2 : 1;
     static constexpr int E0 = DH == 96 ? 4 : DH / 16;
     __host__ __device__ static constexpr int E(int c) { return c == 0 ? E0 : 2; }
     __host__ __device__ static constexpr int base(int c) { return c == 0 ? 0 : 64; }
-    __host__ __device__ static constexpr int d0(int c) { return c == 0 ? 0 : E0; }
+    __host__ __device__ static constexpr int a0(int c) { return c == 0 ? 0 : E0 / 2; }
     __device__ static int k_channel(int g, int s) { return kEven ? (DH / 4) * g + 8 * s : 32 * s + 8 * g; }
 };
 
@@ -223,14 +224,20 @@ __device__ __forceinline__ float sum_groups(float v) {
 constexpr int kTile = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// One 16-byte (4-byte) load per lane from global memory straight into LDS: lane L's bytes land at LDS offset lds + 16 L (4 L).
-// Inline assembly, with the waits written out (vm_wait), because the compiler would wait for all such loads before any LDS
-// read. The LDS address goes through M0 (its write needs a wait state before its use). No register receives anything.
+// One 16-byte (4-byte) load per lane from global memory straight into LDS: lane L's bytes land at LDS offset lds + AT + 16 L
+// (lds + 4 L). Inline assembly, with the waits written out (vm_wait), because the compiler would wait for all such loads before
+// any LDS read. The LDS address goes through M0; the s_nop covers the wait states after a vector instruction's write of the
+// scalar base and after that of M0. AT counts on both sides. No register receives anything. (nt: a tile is read once; 12 % more
+// bandwidth than without for plain reads of large arrays.)
+template <int AT>
+__device__ __forceinline__ void lds_load16(const uint8_t* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3 nt" ::"v"(off), "s"(base), "s"(lds), "i"(AT) : "m0", "memory");
+}
 __device__ __forceinline__ void lds_load16(const uint8_t* p, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "m0", "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(p), "s"(lds) : "m0", "memory");
 }
 __device__ __forceinline__ void lds_load4(const uint8_t* p, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "m0", "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dword %0, off nt" ::"v"(p), "s"(lds) : "m0", "memory");
 }
 template <int N>
 __device__ __forceinline__ void vm_wait() {
@@ -249,29 +256,41 @@ struct KvTile {
 
     __device__ static __forceinline__ int k_place(int j) { return DH == 128 ? ((j >> 1) & 1) | ((j >> 2) & 2) : 0; }
 
-    // What each lane loads of the tile at slot 0 of the cache's first plane: addresses, to which (plane * cap + slot) rows are added.
+    // What each lane loads of a tile, from the tile's place in the planes. Where a load is of K or V alone (DH 64 and 128) the place
+    // is a scalar; otherwise it is added to each lane's address.
     struct Source {
-        const uint8_t* codes[W::KS];
+        uint32_t k_off, v_off;         // within 1 KiB of K and V
+        const uint8_t* codes[W::KS];   // DH 32 and 96
         const uint8_t* scales;
         __device__ __forceinline__ void set(const KvCache& c, int lane) {
+            if constexpr (DH % 64 == 0) {
+                const int j = 16 * lane / row, b = 16 * lane % row;
+                k_off = j * row + (b ^ (16 * k_place(j)));
+                v_off = (j ^ ((j >> 3) & 3)) * row + b;
+            } else {
 #pragma unroll
-            for (int x = 0; x < W::KS; x++) {
-                const int at = 1024 * x + 16 * lane;
-                if (at < half) {
-                    const int j = at / row, b = at % row / 16;
-                    codes[x] = c.k + j * row + 16 * (b ^ k_place(j));
-                } else {
-                    const int j = (at - half) / row;
-                    codes[x] = c.v + (j ^ ((j >> 3) & 3)) * row + (at - half) % row;
+                for (int x = 0; x < W::KS; x++) {
+                    const int at = 1024 * x + 16 * lane, in = at < half ? at : at - half, j = in / row;
+                    codes[x] = at < half ? c.k + in : c.v + (j ^ ((j >> 3) & 3)) * row + in % row;
                 }
             }
-            const int at = 4 * (lane & (16 * W::NB - 1 | (W::NB == 3 ? 63 : 0)));
-            const int in = W::NB == 3 ? min(at, 188) : at;  // (lanes past the scales repeat one)
-            scales = in < 32 * W::NB ? c.ks + in : c.vs + in - 32 * W::NB;
+            const int at = min(4 * (W::NB == 3 ? lane : lane & (16 * W::NB - 1)), 64 * W::NB - 4);  // (lanes past the scales repeat some)
+            scales = at < 32 * W::NB ? c.ks + at : c.vs + at - 32 * W::NB;
         }
-        __device__ __forceinline__ void load(size_t slot, uint32_t lds) const {
+        __device__ __forceinline__ void load(const KvCache& c, size_t slot, uint32_t lds) const {
+            if constexpr (DH % 64 == 0) {
+                const uint8_t *k = c.k + slot * row, *v = c.v + slot * row;
+                lds_load16<0>(k, k_off, lds);
+                if constexpr (DH == 128) lds_load16<1024>(k, k_off, lds);
+                lds_load16<0>(v, v_off, lds + half);
+                if constexpr (DH == 128) {
+                    // (slots 16 and on: the same order, since bits 3 and 4 of a slot choose the row)
+                    lds_load16<1024>(v, v_off ^ (2 * row), lds + half);
+                }
+            } else {
 #pragma unroll
-            for (int x = 0; x < W::KS; x++) lds_load16(codes[x] + slot * row, lds + 1024 * x);
+                for (int x = 0; x < W::KS; x++) lds_load16(codes[x] + slot * row, lds + 1024 * x);
+            }
             lds_load4(scales + slot * W::NB, lds + o_scales);
         }
     };
@@ -307,6 +326,16 @@ struct KvTile {
 #pragma unroll
             for (int x = 0; x < W::NB; x++) *(u32x2*)(s + 2 * x) = *(const u32x2*)(p + o_scales + 32 * W::NB + 8 * g * W::NB + 8 * x);
         }
+        // Slot 8 g + e as zeros.
+        __device__ __forceinline__ void drop(int e) {
+#pragma unroll
+            for (int c = 0; c < W::chunks; c++) w[c][e] = 0;
+#pragma unroll
+            for (int b = 0; b < W::NB; b++) {
+                const int at = e * W::NB + b;
+                s[at >> 2] &= ~(255u << (8 * (at & 3)));
+            }
+        }
         // The scale byte of slot 8 g + e for block b, and the scale for a conversion (of this lane's channels in chunk c).
         __device__ __forceinline__ uint32_t byte(int e, int b) const {
             const int at = e * W::NB + b;
@@ -336,14 +365,18 @@ __device__ __forceinline__ uint32_t unpack2(uint32_t w, float s, int b) {
     }
 }
 
-// What a wave's rows and the slots are, for the masks. Uniform but for `at`.
+// What a wave's rows and the slots are, for the masks. Uniform but for `at` and `low`.
 struct Seen {
     int sinks, ring, window;
     int last, newest;     // the last position, and its slot in the ring (-1: none is there)
     int lo_at, hi_at;     // positions of the wave's rows
     int at;               // of this lane's row
-    __device__ __forceinline__ int position(int j) const { return j < sinks ? j : last - (newest - j + (j > newest ? ring : 0)); }
-    __device__ __forceinline__ bool held(int j, int p) const { return j < sinks ? j <= last : p >= sinks && p <= last; }
+    int low;              // the last position behind its window
+    // The position that a slot holds, if that is one of a sink or from `sinks` on.
+    __device__ __forceinline__ int position(int j) const {
+        const int back = newest - j;
+        return j < sinks ? j : last - (back + (back < 0 ? ring : 0));
+    }
     // Every row sees every slot of the tile.
     __device__ __forceinline__ bool whole(int j0) const {
         if (j0 + 31 < sinks) return j0 + 31 <= lo_at;
@@ -377,30 +410,40 @@ __device__ __forceinline__ Tiles tiles_of(const Seen& q, int cap) {
     return r;
 }
 
-// Running softmax of 16 rows, a lane's share: O^T in the second product's layout, the maximum of its row (common to the four
-// lane groups), and the sum over its own keys.
-template <int DH>
+// Running softmax of 8 rows, a lane's share: column i = lane & 15 of the products is row i >> 1; O^T in the second product's layout for
+// each of HB heads (a column's own head counts); the maximum of the row (common to the lanes that have it), and the sum over
+// the lane's own slots.
+template <int DH, int HB>
 struct RowState {
-    v4f acc[Width<DH>::ND];
+    v4f acc[HB][Width<DH>::NA];
     float m, l;
     uint32_t nan_blocks;  // careful form: bit b: a key that the row sees has NaN in channels 32 b .. 32 b + 31
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int d = 0; d < Width<DH>::ND; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int hb = 0; hb < HB; hb++)
+#pragma unroll
+            for (int d = 0; d < Width<DH>::NA; d++) acc[hb][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         m = -INFINITY;
         l = 0.0f;
         nan_blocks = 0;
     }
 };
 
-// One tile of HB heads for 16 rows, column i of the products belonging to head `mine` of them. Scores leave the matrix cores with lane
-// (i, g) holding row i and slots 8 g .. 8 g + 7 of the tile, the very layout in which the second product takes the probabilities:
-// they never leave their lane. With several heads each product is formed for all rows and kept, or added, for its own: the
-// softmax between is done once for all of them. V comes into its layout (one channel of eight slots in a lane) by unpacking
-// the words of two slots and exchanging halves. CAREFUL keeps blocks of NaN out of the product (they would spread over rows that
-// do not see their key) and notes who sees them instead.
+// One tile of HB heads for 8 rows, column i of the products belonging to head `mine` of them.
+//
+// Scores: product h of a head leaves lane (i, g) with row i >> 1 and slots 8 g + 4 h .. + 3 of the tile. With several heads each
+// product is formed for all columns and kept for its own, so that the softmax between is done once for all of them.
+//
+// Output: unpacking a byte of V gives two neighbouring channels of one slot in a register, where the product wants two
+// neighbouring entries of the sum. They are taken as such: the sum runs over (slot, channel parity), and the column of even
+// parity has the probability at the slot's even entry and zero at its odd one, the other column the reverse. A row thus has two
+// columns, which give its even and its odd channels; no value is moved between lanes or registers on the way, and the
+// probabilities stay in the lane where the scores came out.
+//
+// CAREFUL keeps blocks of NaN out of the product (they would spread over rows that do not see their key) and notes who sees them
+// instead.
 template <int DH, class T, int HB, bool CAREFUL>
-__device__ __forceinline__ void tile_step(RowState<DH>& st, const uint8_t* tile, const v8bf (*qf)[Terms<T>::q], float scale,
+__device__ __forceinline__ void tile_step(RowState<DH, HB>& st, const uint8_t* tile, const v8bf (*qf)[Terms<T>::q], float scale,
                                           const Seen& seen, int j0, bool whole, int i, int g, int mine) {
     using W = Width<DH>;
     using Tile = KvTile<DH>;
@@ -431,44 +474,55 @@ __device__ __forceinline__ void tile_step(RowState<DH>& st, const uint8_t* tile,
     for (int e = 0; e < 8; e++) sc[e] *= scale;
     uint32_t sees = 255, drop = 0;
     if (!whole) {
+        asm volatile("");  // a branch: as selects this would cost every tile
         sees = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const int j = j0 + 8 * g + e, p = seen.position(j);
-            const bool held = seen.held(j, p);
-            const bool v = held && p <= seen.at && (j < seen.sinks || seen.window <= 0 || p > seen.at - seen.window);
+            const bool held = (p >= (j < seen.sinks ? 0 : seen.sinks)) & (p <= seen.last);
+            const bool v = held & (p <= seen.at) & ((j < seen.sinks) | (p > seen.low));
             sees |= (uint32_t)v << e;
             drop |= (uint32_t)!held << e;  // never written, or lost: may hold anything
             sc[e] = v ? sc[e] : -INFINITY;
         }
     }
-    float mt = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+    const float mt = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
     if (__any(mt > st.m)) {  // rare after the first tiles
         const float mn = fmaxf(st.m, max_groups(mt)), al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : st.m - mn);
         st.m = mn;
         st.l *= al;
 #pragma unroll
-        for (int d = 0; d < W::ND; d++) st.acc[d] *= al;
+        for (int hb = 0; hb < HB; hb++)
+#pragma unroll
+            for (int d = 0; d < W::NA; d++) st.acc[hb][d] *= al;
     }
     const float mu = st.m == -INFINITY ? 0.0f : st.m;
     float p[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(sc[e] - mu);
     st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-    v8bf pall[PT];
-    split_bf16<PT>(p, pall);
+    // the probabilities in PT parts, each at its parity's half of a word
+    const uint32_t parity = i & 1 ? 0xffff0000u : 0x0000ffffu;
+    uint32_t pw[PT][8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        float x = p[e];
+#pragma unroll
+        for (int n = 0; n < PT; n++) {
+            const uint32_t both = pack_bf16(x, x);
+            pw[n][e] = both & parity;
+            if (n + 1 < PT) x -= bf16_hi(both);
+        }
+    }
 #pragma unroll
     for (int hb = 0; hb < HB; hb++) {
         typename Tile::Value x;
         x.read(tile + hb * Tile::bytes, i, g);
-        v8bf pf[PT];
+        if (!whole) {
+            asm volatile("");
 #pragma unroll
-        for (int n = 0; n < PT; n++) {
-            u32x4 w = __builtin_bit_cast(u32x4, pall[n]);
-            if (HB > 1)
-#pragma unroll
-                for (int r = 0; r < 4; r++) w[r] = mine == hb ? w[r] : 0;
-            pf[n] = __builtin_bit_cast(v8bf, w);
+            for (int e = 0; e < 8; e++)
+                if (drop >> e & 1) x.drop(e);
         }
         if (CAREFUL) {
 #pragma unroll
@@ -479,35 +533,29 @@ __device__ __forceinline__ void tile_step(RowState<DH>& st, const uint8_t* tile,
         }
 #pragma unroll
         for (int c = 0; c < W::chunks; c++) {
-            uint32_t word[8];
             float vs[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                word[e] = x.w[c][e];
                 vs[e] = x.scale(c, e, i);
                 // (the writer's scales are at most 252, or 255 for NaN)
-                if ((CAREFUL && (__float_as_uint(vs[e]) >> 23 & 255) > 252u) || (!whole && (drop >> e & 1))) {
-                    word[e] = 0;
+                if (CAREFUL && (__float_as_uint(vs[e]) >> 23 & 255) > 252u) {
+                    x.w[c][e] = 0;
                     vs[e] = 0.0f;
                 }
             }
 #pragma unroll
-            for (int b = 0; b < W::E(c) / 2; b++) {
-                uint32_t lo[4], hi[4];
+            for (int b = 0; b < W::E(c) / 2; b++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t y0 = unpack2(word[2 * e], vs[2 * e], b), y1 = unpack2(word[2 * e + 1], vs[2 * e + 1], b);
-                    lo[e] = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
-                    hi[e] = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
-                }
-                const v8bf v0 = __builtin_bit_cast(v8bf, *(u32x4*)lo), v1 = __builtin_bit_cast(v8bf, *(u32x4*)hi);
-                const int d = W::d0(c) + 2 * b;
+                for (int h = 0; h < 2; h++) {
+                    uint32_t vw[4];
 #pragma unroll
-                for (int n = PT - 1; n >= 0; n--) {
-                    st.acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pf[n], st.acc[d], 0, 0, 0);
-                    st.acc[d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pf[n], st.acc[d + 1], 0, 0, 0);
+                    for (int r = 0; r < 4; r++) vw[r] = unpack2(x.w[c][4 * h + r], vs[4 * h + r], b);
+                    const v8bf vf = __builtin_bit_cast(v8bf, *(u32x4*)vw);
+                    v4f& o = st.acc[hb][W::a0(c) + b];
+#pragma unroll
+                    for (int n = PT - 1; n >= 0; n--)
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(v8bf, *(u32x4*)(pw[n] + 4 * h)), o, 0, 0, 0);
                 }
-            }
         }
     }
 }
@@ -516,40 +564,43 @@ __device__ __forceinline__ void tile_step(RowState<DH>& st, const uint8_t* tile,
 template <int DH>
 constexpr int kPart = DH + 4;
 
+// Rows of a wave: half the columns of a product.
+constexpr int kRows = 8;
+
 // Stages of a wave's tiles in LDS, for two workgroups of four waves a CU.
 template <int DH, int HB>
 struct Stages {
     static constexpr int bytes = HB * KvTile<DH>::bytes;
-    static constexpr int n = std::min(4, std::max(2, 19 * 1024 / bytes));
+    static constexpr int n = std::min(4, std::max(2, 20 * 1024 / bytes));
     static constexpr int loads = HB * KvTile<DH>::loads;
     static constexpr int wave = n * bytes;
     static_assert((n - 1) * loads <= 63, "");
 };
 
-// Few query rows: a wave takes up to 16 rows of one sequence over a share of the tiles: a row tile of one key/value head (its
-// query heads, token after token), or, with HB > 1, all rows of HB heads (16 or fewer). Tiles come straight into the wave's own
+// Few query rows: a wave takes up to 8 rows of one sequence over a share of the tiles: a row tile of one key/value head (its
+// query heads, token after token), or, with HB > 1, all rows of HB heads (8 or fewer). Tiles come straight into the wave's own
 // LDS stages, up to three ahead. WAVES waves share the tiles (of one chunk of them, where there are several) and add up what
 // they have in LDS; with WAVES 1 a wave is alone with its rows.
 template <int DH, class T, int HB, int WAVES>
-__global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
+__global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
     using W = Width<DH>;
     using Tile = KvTile<DH>;
     using St = Stages<DH, HB>;
     constexpr int QT = Terms<T>::q, LD = DH + 4;
-    static_assert(4 * 16 * (LD + 2) * 4 <= 4 * St::wave, "");
+    static_assert(4 * kRows * (LD + 2) * 4 <= 4 * St::wave, "");
     __shared__ __align__(16) uint8_t smem[4 * St::wave];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int unit = WAVES > 1 ? blockIdx.x : blockIdx.x * 4 + wave, w = WAVES > 1 ? wave : 0;
-    const int blocks = (a.c.heads + HB - 1) / HB, units = a.c.n * blocks * row_tiles;
+    const int blocks = a.c.heads / HB, units = a.c.n * blocks * row_tiles;
     if (unit >= units) return;
     const int pair = row_tiles == 1 ? unit : unit / row_tiles, rt = unit - pair * row_tiles;
-    const int s = pair / blocks, h0 = (pair - s * blocks) * HB;
+    const int s = blocks == 1 ? pair : pair / blocks, h0 = (pair - s * blocks) * HB;
     const SeqSpan q = seq_span(a.pos, a.counts, s, a.T);
     const int ring = a.c.cap - a.c.sinks, sinks = a.c.sinks;
-    const int t_lo = rt == 0 ? 0 : rt * 16 / a.group;
+    const int t_lo = rt == 0 ? 0 : rt * kRows / a.group;
     if (t_lo >= q.count) return;
-    const int t_hi = a.T == 1 ? 0 : min((rt * 16 + 15) / a.group, q.count - 1);
+    const int t_hi = a.T == 1 ? 0 : min((rt * kRows + kRows - 1) / a.group, q.count - 1);
 
     Seen seen;
     seen.sinks = sinks; seen.ring = ring; seen.window = a.window;
@@ -564,30 +615,30 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
 
     typename Tile::Source src;
     src.set(a.c, lane);
-    uint8_t* mine = smem + wave * St::wave;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)mine;
+    uint8_t* own = smem + wave * St::wave;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)own;
     const size_t plane = (size_t)(s * a.c.heads + h0) * a.c.cap;
-    auto load = [&](int j0, int stage) {
+    auto load = [&](int o, int stage) {
+        const size_t slot = plane + tl.at(o) * kTile;
 #pragma unroll
-        for (int hb = 0; hb < HB; hb++)
-            src.load(plane + (size_t)min(hb, a.c.heads - 1 - h0) * a.c.cap + j0, lds0 + stage * St::bytes + hb * Tile::bytes);
+        for (int hb = 0; hb < HB; hb++) src.load(a.c, slot + (size_t)hb * a.c.cap, lds0 + stage * St::bytes + hb * Tile::bytes);
     };
-
-    // this lane's row
-    const int rows = a.T * a.group;  // of a head
-    const int hb = HB > 1 ? i / rows : 0, row = HB > 1 ? i - hb * rows : rt * 16 + i;
-    const int t = a.T == 1 ? 0 : row / a.group, head = (h0 + hb) * a.group + (row - t * a.group);
-    const bool there = hb < HB && h0 + hb < a.c.heads && row < rows && t < q.count;
-    seen.at = q.pos + t;
-    v8bf qf[W::KS][QT];
-    float scale = 0.0f;
-    // the first `ahead` tiles of a pass are on their way
+    // the first tiles of a pass are on their way
     auto start = [&] {
 #pragma unroll
         for (int x = 0; x < St::n - 1; x++)
-            if (o0 + w + x * WAVES < o1) load(tl.at(o0 + w + x * WAVES) * kTile, x);
+            if (o0 + w + x * WAVES < o1) load(o0 + w + x * WAVES, x);
     };
     start();
+
+    // this lane's row
+    const int rows = a.T * a.group;  // of a head
+    const int col = i >> 1, hb_own = HB > 1 ? col / rows : 0, row = HB > 1 ? col - hb_own * rows : rt * kRows + col;
+    const int t = a.T == 1 ? 0 : row / a.group, head = (h0 + hb_own) * a.group + (row - t * a.group);
+    const bool there = hb_own < HB && row < rows && t < q.count;
+    seen.at = q.pos + t;
+    seen.low = a.window > 0 ? seen.at - a.window : INT_MIN;
+    v8bf qf[W::KS][QT];
 #pragma unroll
     for (int st = 0; st < W::KS; st++) {
         float x[8] = {};
@@ -598,9 +649,9 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
         }
         split_bf16<QT>(x, qf[st]);
     }
-    scale = a.scale * kLog2e;
+    const float scale = a.scale * kLog2e;
 
-    RowState<DH> st;
+    RowState<DH, HB> st;
     auto sweep = [&](auto careful) {
         st.clear();
         int stage = 0;
@@ -609,7 +660,7 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
             const int more = (o1 - 1 - o) / WAVES;
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last stage's reads are done: it is loaded anew
             if (more >= St::n - 1) {
-                load(tl.at(o + (St::n - 1) * WAVES) * kTile, stage == 0 ? St::n - 1 : stage - 1);
+                load(o + (St::n - 1) * WAVES, stage == 0 ? St::n - 1 : stage - 1);
                 vm_wait<(St::n - 1) * St::loads>();
             } else if (St::n > 3 && more == 2) {
                 vm_wait<2 * St::loads>();
@@ -619,106 +670,134 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
                 vm_wait<0>();
             }
             const int j0 = __builtin_amdgcn_readfirstlane(tl.at(o) * kTile);
-            tile_step<DH, T, HB, decltype(careful)::value>(st, mine + stage * St::bytes, qf, scale, seen, j0, seen.whole(j0), i, g, hb);
+            tile_step<DH, T, HB, decltype(careful)::value>(st, own + stage * St::bytes, qf, scale, seen, j0, seen.whole(j0), i, g, hb_own);
             stage = stage == St::n - 1 ? 0 : stage + 1;
         }
     };
+    // the lane's sums: of its row's own head
+    v4f acc[W::NA];
+    auto pick = [&] {
+#pragma unroll
+        for (int d = 0; d < W::NA; d++) {
+            acc[d] = st.acc[0][d];
+#pragma unroll
+            for (int hb = 1; hb < HB; hb++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[d][r] = hb_own == hb ? st.acc[hb][d][r] : acc[d][r];
+        }
+    };
     sweep(std::false_type());
+    pick();
     {
         // A NaN among the sums: it may come from a value that the row does not see.
         float bad = 0.0f;
 #pragma unroll
-        for (int d = 0; d < W::ND; d++)
+        for (int d = 0; d < W::NA; d++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) bad += st.acc[d][r] * 0.0f;
+            for (int r = 0; r < 4; r++) bad += acc[d][r] * 0.0f;
         if (__any(bad != 0.0f)) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             start();
             sweep(std::true_type());
+            pick();
+            st.nan_blocks |= __shfl_xor(st.nan_blocks, 16, 64);
+            st.nan_blocks |= __shfl_xor(st.nan_blocks, 32, 64);
+#pragma unroll
+            for (int c = 0; c < W::chunks; c++)
+#pragma unroll
+                for (int b = 0; b < W::E(c) / 2; b++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if ((st.nan_blocks >> ((W::base(c) + (4 * g + r) * W::E(c)) / 32)) & 1) acc[W::a0(c) + b][r] = NAN;
         }
     }
     st.l = sum_groups(st.l);
-    if (__any(st.nan_blocks)) {
-        st.nan_blocks |= __shfl_xor(st.nan_blocks, 16, 64);
-        st.nan_blocks |= __shfl_xor(st.nan_blocks, 32, 64);
-#pragma unroll
-        for (int c = 0; c < W::chunks; c++)
-#pragma unroll
-            for (int e = 0; e < W::E(c); e++)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if ((st.nan_blocks >> ((W::base(c) + (4 * g + r) * W::E(c) + e) / 32)) & 1) st.acc[W::d0(c) + e][r] = NAN;
-    }
     const bool split = n_tiles > chunk_tiles;
     // [chunk][unit][column][kPart]
-    float* part = a.ws + (((size_t)blockIdx.y * units + unit) * 16) * kPart<DH>;
+    float* part = a.ws + (((size_t)blockIdx.y * units + unit) * kRows) * kPart<DH>;
     if constexpr (WAVES == 1) {
-        if (!there) return;
         const float f = st.l == 0.0f ? 0.0f : 1.0f / st.l;
         T* out = (T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head;
+        // Lanes 2 r and 2 r + 1 have the even and odd channels of element groups 0 .. 3: the first gets both of groups 0 and 1, the
+        // second those of groups 2 and 3.
+        const bool odd = i & 1;
 #pragma unroll
-        for (int c = 0; c < W::chunks; c++)
+        for (int c = 0; c < W::chunks; c++) {
+            float v[2][W::E0];
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                T v[W::E0];
+            for (int b = 0; b < W::E(c) / 2; b++)
 #pragma unroll
-                for (int e = 0; e < W::E(c); e++) v[e] = (T)(st.acc[W::d0(c) + e][r] * f);
-                T* p = out + W::base(c) + (4 * g + r) * W::E(c);
-                if (vec) {
-                    if (W::E(c) * sizeof(T) >= 16) {
+                for (int r = 0; r < 2; r++) {
+                    const v4f& x = acc[W::a0(c) + b];
+                    const float keep = odd ? x[2 + r] : x[r], get = dpp_move<0xB1>(odd ? x[r] : x[2 + r]);
+                    v[r][2 * b] = (odd ? get : keep) * f;
+                    v[r][2 * b + 1] = (odd ? keep : get) * f;
+                }
+            if (there) {
 #pragma unroll
-                        for (int x = 0; x < (int)(W::E(c) * sizeof(T) / 16); x++) ((u32x4*)p)[x] = ((u32x4*)v)[x];
-                    } else if (W::E(c) * sizeof(T) == 8) {
-                        *(u32x2*)p = *(u32x2*)v;
+                for (int r = 0; r < 2; r++) {
+                    T* p = out + W::base(c) + (4 * g + 2 * (i & 1) + r) * W::E(c);
+                    T u[W::E0];
+#pragma unroll
+                    for (int e = 0; e < W::E(c); e++) u[e] = (T)v[r][e];
+                    if (vec) {
+                        if (W::E(c) * sizeof(T) >= 16) {
+#pragma unroll
+                            for (int x = 0; x < (int)(W::E(c) * sizeof(T) / 16); x++) ((u32x4*)p)[x] = ((u32x4*)u)[x];
+                        } else if (W::E(c) * sizeof(T) == 8) {
+                            *(u32x2*)p = *(u32x2*)u;
+                        } else {
+                            *(uint32_t*)p = *(uint32_t*)u;
+                        }
                     } else {
-                        *(uint32_t*)p = *(uint32_t*)v;
-                    }
-                } else {
 #pragma unroll
-                    for (int e = 0; e < W::E(c); e++) p[e] = v[e];
+                        for (int e = 0; e < W::E(c); e++) p[e] = u[e];
+                    }
                 }
             }
+        }
     } else {
         // join the waves: their sums at the largest maximum, added in the waves' order (the stages are done with)
-        float* s_o = (float*)smem;                                 // [wave][column][LD]
-        float (*s_ml)[2][16] = (float (*)[2][16])(s_o + WAVES * 16 * LD);
+        float* s_o = (float*)smem;                                    // [wave][column][LD]
+        float (*s_ml)[2][kRows] = (float (*)[2][kRows])(s_o + WAVES * kRows * LD);
         __syncthreads();
-        if (g == 0) {
-            s_ml[w][0][i] = st.m;
-            s_ml[w][1][i] = st.l;
+        if (g == 0 && (i & 1) == 0) {
+            s_ml[w][0][col] = st.m;
+            s_ml[w][1][col] = st.l;
         }
         __syncthreads();
         float top = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < WAVES; x++) top = fmaxf(top, s_ml[x][0][i]);
+        for (int x = 0; x < WAVES; x++) top = fmaxf(top, s_ml[x][0][col]);
         const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - top);
 #pragma unroll
         for (int c = 0; c < W::chunks; c++)
 #pragma unroll
-            for (int e = 0; e < W::E(c); e++)
+            for (int b = 0; b < W::E(c) / 2; b++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) s_o[(w * 16 + i) * LD + W::base(c) + (4 * g + r) * W::E(c) + e] = st.acc[W::d0(c) + e][r] * f;
+                for (int r = 0; r < 4; r++)
+                    s_o[(w * kRows + col) * LD + W::base(c) + (4 * g + r) * W::E(c) + 2 * b + (i & 1)] = acc[W::a0(c) + b][r] * f;
         __syncthreads();
-        const int keep = min(16, HB > 1 ? HB * rows : rows - rt * 16);
+        const int keep = min(kRows, HB > 1 ? HB * rows : rows - rt * kRows);
         for (int x = threadIdx.x * 4; x < keep * DH; x += 256 * 4) {
-            const int col = x / DH, d = x - col * DH;
-            const int hh = HB > 1 ? col / rows : 0, rr = HB > 1 ? col - hh * rows : rt * 16 + col;
+            const int cc = x / DH, d = x - cc * DH;
+            const int hh = HB > 1 ? cc / rows : 0, rr = HB > 1 ? cc - hh * rows : rt * kRows + cc;
             const int tt = a.T == 1 ? 0 : rr / a.group, hd = (h0 + hh) * a.group + (rr - tt * a.group);
-            if (tt >= q.count || h0 + hh >= a.c.heads) continue;
+            if (tt >= q.count) continue;
             float most = -INFINITY, total = 0.0f;
 #pragma unroll
-            for (int y = 0; y < WAVES; y++) most = fmaxf(most, s_ml[y][0][col]);
+            for (int y = 0; y < WAVES; y++) most = fmaxf(most, s_ml[y][0][cc]);
             v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int y = 0; y < WAVES; y++) {
-                total += s_ml[y][1][col] * (most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_ml[y][0][col] - most));
-                sum += *(const v4f*)(s_o + (y * 16 + col) * LD + d);
+                total += s_ml[y][1][cc] * (most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_ml[y][0][cc] - most));
+                sum += *(const v4f*)(s_o + (y * kRows + cc) * LD + d);
             }
             if (split) {
-                *(v4f*)(part + col * kPart<DH> + d) = sum;
+                *(v4f*)(part + cc * kPart<DH> + d) = sum;
                 if (d == 0) {
-                    part[col * kPart<DH> + DH] = most;
-                    part[col * kPart<DH> + DH + 1] = total;
+                    part[cc * kPart<DH> + DH] = most;
+                    part[cc * kPart<DH> + DH + 1] = total;
                 }
             } else {
                 store4((T*)a.out.data + s * a.out.seq + tt * a.out.token + hd * a.out.head + d, sum * (total == 0.0f ? 0.0f : 1.0f / total), vec);
@@ -727,60 +806,55 @@ __global__ __launch_bounds__(256) void kv_attention_rows_kernel(KvAttnArgs a, in
     }
 }
 
-// Joins the chunks of a row tile that took more than one: a workgroup a row, its lanes over channels (four each) and, in as many
-// groups as fit, over the chunks, whose sums are added in a fixed order.
+// Joins the chunks of a row that took more than one: a wave a row, its lanes over channels (four each) and, in as many groups as fit,
+// over the chunks, whose sums are added in a fixed order.
 template <int DH, class T>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int hb, int row_tiles, int chunk_tiles, int vec) {
-    constexpr int LC = DH / 4, G = 256 / LC;  // lanes a group, groups
-    __shared__ float s_top[4];
-    __shared__ __align__(16) float s_sum[G][DH + 4];
-    __shared__ float s_total[G];
-    const int unit = blockIdx.x, col = blockIdx.y;
-    const int blocks = (a.c.heads + hb - 1) / hb, units = a.c.n * blocks * row_tiles;
-    const int pair = unit / row_tiles, rt = unit - pair * row_tiles;
+    constexpr int LC = DH / 4, G = 64 / LC;  // lanes a group, groups
+    const int lane = threadIdx.x & 63, col = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int unit = blockIdx.x;
+    const int blocks = a.c.heads / hb, units = a.c.n * blocks * row_tiles;
+    const int pair = row_tiles == 1 ? unit : unit / row_tiles, rt = unit - pair * row_tiles;
     const int s = pair / blocks, h0 = (pair - s * blocks) * hb;
     const SeqSpan q = seq_span(a.pos, a.counts, s, a.T);
     const int rows = a.T * a.group;
-    const int hh = hb > 1 ? col / rows : 0, row = hb > 1 ? col - hh * rows : rt * 16 + col;
+    if (col >= (hb > 1 ? hb * rows : kRows)) return;
+    const int hh = hb > 1 ? col / rows : 0, row = hb > 1 ? col - hh * rows : rt * kRows + col;
     const int t = row / a.group, head = (h0 + hh) * a.group + (row - t * a.group);
-    if (row >= rows || t >= q.count || h0 + hh >= a.c.heads) return;
+    if (row >= rows || t >= q.count) return;
     Seen seen;
     seen.sinks = a.c.sinks; seen.ring = a.c.cap - a.c.sinks; seen.window = a.window;
     seen.last = q.end - 1;
     seen.newest = seen.last >= seen.sinks ? kv_slot(seen.last, seen.sinks, seen.ring) : -1;
-    seen.lo_at = q.pos + rt * 16 / a.group;
-    seen.hi_at = q.pos + min((rt * 16 + 15) / a.group, q.count - 1);
+    seen.lo_at = q.pos + rt * kRows / a.group;
+    seen.hi_at = q.pos + min((rt * kRows + kRows - 1) / a.group, q.count - 1);
     const int chunks = (tiles_of(seen, a.c.cap).count() + chunk_tiles - 1) / chunk_tiles;
     if (chunks <= 1) return;
-    const size_t step = (size_t)units * 16 * kPart<DH>;
-    const float* part = a.ws + ((size_t)unit * 16 + col) * kPart<DH>;
+    const size_t step = (size_t)units * kRows * kPart<DH>;
+    const float* part = a.ws + ((size_t)unit * kRows + col) * kPart<DH>;
     float top = -INFINITY;
-    for (int c = threadIdx.x; c < chunks; c += 256) top = fmaxf(top, part[c * step + DH]);
+    for (int c = lane; c < chunks; c += 64) top = fmaxf(top, part[c * step + DH]);
     top = wave_max(top);
-    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-    const int grp = threadIdx.x / LC, d = (threadIdx.x - grp * LC) * 4;
-    if (grp < G) {
-        v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        float total = 0.0f;
-        for (int c = grp; c < chunks; c += G) {
-            const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[c * step + DH] - top);
-            sum += *(const v4f*)(part + c * step + d) * f;
-            total += part[c * step + DH + 1] * f;
-        }
-        *(v4f*)(s_sum[grp] + d) = sum;
-        if (d == 0) s_total[grp] = total;
-    }
-    __syncthreads();
-    if (threadIdx.x >= LC) return;
+    const float tu = top == -INFINITY ? 0.0f : top;
+    const int grp = lane / LC, d = (lane - grp * LC) * 4;
     v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
     float total = 0.0f;
-    for (int x = 0; x < G; x++) {
-        sum += *(const v4f*)(s_sum[x] + 4 * threadIdx.x);
-        total += s_total[x];
+#pragma unroll 4
+    for (int c = grp < G ? grp : chunks; c < chunks; c += G) {
+        const float f = __builtin_amdgcn_exp2f(part[c * step + DH] - tu);
+        sum += *(const v4f*)(part + c * step + d) * f;
+        total += part[c * step + DH + 1] * f;
     }
-    store4((T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head + 4 * threadIdx.x, sum * (total == 0.0f ? 0.0f : 1.0f / total), vec);
+    v4f all = sum;
+    float norm = total;
+#pragma unroll
+    for (int x = 1; x < G; x++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) all[r] += __shfl(sum[r], lane + x * LC, 64);
+        norm += __shfl(total, lane + x * LC, 64);
+    }
+    if (lane < LC)
+        store4((T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head + d, all * (norm == 0.0f ? 0.0f : 1.0f / norm), vec);
 }
 
 struct RowsPlan {
@@ -788,10 +862,10 @@ struct RowsPlan {
 };
 RowsPlan rows_plan(const KvAttnArgs& a) {
     RowsPlan p;
-    // heads a wave takes together: as many as give it 16 rows or fewer
+    // heads a wave takes together: as many as give it 8 rows or fewer
     const int rows = a.T * a.group, most = a.c.dh == 32 ? 8 : a.c.dh == 64 ? 4 : 2;
-    p.hb = rows * most <= 16 && a.c.heads % most == 0 ? most : rows * 2 <= 16 && a.c.heads % 2 == 0 ? 2 : 1;
-    p.row_tiles = (rows + 15) / 16;
+    p.hb = rows * most <= kRows && a.c.heads % most == 0 ? most : rows * 2 <= kRows && a.c.heads % 2 == 0 ? 2 : 1;
+    p.row_tiles = (rows + kRows - 1) / kRows;
     p.units = a.c.n * (a.c.heads / p.hb) * p.row_tiles;
     // tiles that a row tile can see, at most: the sinks', and the window's (or the ring's), with the ends of three runs
     const long long span = a.window > 0 ? std::min<long long>((long long)a.window + a.T, a.c.cap) : a.c.cap;
@@ -799,8 +873,9 @@ RowsPlan rows_plan(const KvAttnArgs& a) {
     p.waves = tiles <= 4 ? 1 : 4;
     p.chunk_tiles = tiles;
     if (p.waves > 1) {
-        // enough workgroups to fill the chip, each with four tiles a wave at least
-        const int want = std::max(1, 2048 / p.units);
+        // Two workgroups a CU, each with four tiles a wave at least. More, smaller chunks cost more at their ends than they even out
+        // (256 conversations, their window in one chunk or two: 28.8 or 37.7 us).
+        const int want = std::max(1, 512 / p.units);
         p.chunk_tiles = std::max(16, (tiles + want - 1) / want);
     }
     p.chunks = std::max(1, (tiles + p.chunk_tiles - 1) / p.chunk_tiles);
@@ -815,7 +890,7 @@ hipError_t launch_rows_attention(const KvAttnArgs& a, const RowsPlan& p, hipStre
     } else {
         hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 4>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
         if (p.chunks > 1)
-            hipLaunchKernelGGL((kv_attention_join_kernel<DH, T>), dim3(p.units, std::min(16, HB * a.T * a.group)), dim3(256), 0, s, a, HB,
+            hipLaunchKernelGGL((kv_attention_join_kernel<DH, T>), dim3(p.units, (std::min(kRows, HB * a.T * a.group) + 3) / 4), dim3(256), 0, s, a, HB,
                                p.row_tiles, p.chunk_tiles, vec);
     }
     return hipGetLastError();
@@ -831,7 +906,7 @@ hipError_t launch_kv_read(const KvRowsArgs& a, hipStream_t s) { return launch_ro
 size_t kv_attention_ws_bytes(const KvAttnArgs& a) {
     const RowsPlan p = rows_plan(a);
     if (p.chunks <= 1) return 0;
-    return (size_t)p.chunks * p.units * 16 * (a.c.dh + 4) * 4;
+    return (size_t)p.chunks * p.units * kRows * (a.c.dh + 4) * 4;
 }
 
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
