@@ -377,12 +377,32 @@ struct Seen {
         const int back = newest - j;
         return j < sinks ? j : last - (back + (back < 0 ? ring : 0));
     }
+    __device__ __forceinline__ bool holds(int j) const {
+        const int p = position(j);
+        return (p >= (j < sinks ? 0 : sinks)) & (p <= last);
+    }
+    __device__ __forceinline__ bool sees(int j) const {
+        const int p = position(j);
+        return (p >= (j < sinks ? 0 : sinks)) & (p <= at) & (p <= last) & ((j < sinks) | (p > low));
+    }
+    // Of a tile: its slots hold 32 positions in a row, from which on (-1: not so).
+    __device__ __forceinline__ int run(int j0) const {
+        if (j0 < sinks || (j0 <= newest && newest < j0 + 31)) return -1;
+        const int p = position(j0);
+        return p >= sinks && p + 31 <= last ? p : -1;
+    }
+    __device__ __forceinline__ bool all_held(int j0) const { return j0 + 31 < sinks ? j0 + 31 <= last : run(j0) >= 0; }
+    // No row sees a slot of the tile (it may say no where that is so).
+    __device__ __forceinline__ bool none(int j0) const {
+        if (lo_at > hi_at) return true;
+        const int p = run(j0);
+        return p >= 0 && (p > hi_at || (window > 0 && p + 31 <= lo_at - window));
+    }
     // Every row sees every slot of the tile.
     __device__ __forceinline__ bool whole(int j0) const {
         if (j0 + 31 < sinks) return j0 + 31 <= lo_at;
-        if (j0 < sinks || (j0 <= newest && newest < j0 + 31)) return false;
-        const int p = position(j0);
-        return p >= sinks && p + 31 <= lo_at && (window <= 0 || p > hi_at - window);
+        const int p = run(j0);
+        return p >= 0 && p + 31 <= lo_at && (window <= 0 || p > hi_at - window);
     }
 };
 
@@ -478,9 +498,8 @@ __device__ __forceinline__ void tile_step(RowState<DH, HB>& st, const uint8_t* t
         sees = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const int j = j0 + 8 * g + e, p = seen.position(j);
-            const bool held = (p >= (j < seen.sinks ? 0 : seen.sinks)) & (p <= seen.last);
-            const bool v = held & (p <= seen.at) & ((j < seen.sinks) | (p > seen.low));
+            const int j = j0 + 8 * g + e;
+            const bool held = seen.holds(j), v = seen.sees(j);
             sees |= (uint32_t)v << e;
             drop |= (uint32_t)!held << e;  // never written, or lost: may hold anything
             sc[e] = v ? sc[e] : -INFINITY;
@@ -807,9 +826,9 @@ __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a,
 }
 
 // Joins the chunks of a row that took more than one: a wave a row, its lanes over channels (four each) and, in as many groups as fit,
-// over the chunks, whose sums are added in a fixed order.
+// over the chunks, whose sums are added in a fixed order. Units have `per` rows.
 template <int DH, class T>
-__global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int hb, int row_tiles, int chunk_tiles, int vec) {
+__global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int per, int hb, int row_tiles, int chunk_tiles, int vec) {
     constexpr int LC = DH / 4, G = 64 / LC;  // lanes a group, groups
     const int lane = threadIdx.x & 63, col = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int unit = blockIdx.x;
@@ -818,20 +837,20 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, in
     const int s = pair / blocks, h0 = (pair - s * blocks) * hb;
     const SeqSpan q = seq_span(a.pos, a.counts, s, a.T);
     const int rows = a.T * a.group;
-    if (col >= (hb > 1 ? hb * rows : kRows)) return;
-    const int hh = hb > 1 ? col / rows : 0, row = hb > 1 ? col - hh * rows : rt * kRows + col;
+    if (col >= (hb > 1 ? hb * rows : per)) return;
+    const int hh = hb > 1 ? col / rows : 0, row = hb > 1 ? col - hh * rows : rt * per + col;
     const int t = row / a.group, head = (h0 + hh) * a.group + (row - t * a.group);
     if (row >= rows || t >= q.count) return;
     Seen seen;
     seen.sinks = a.c.sinks; seen.ring = a.c.cap - a.c.sinks; seen.window = a.window;
     seen.last = q.end - 1;
     seen.newest = seen.last >= seen.sinks ? kv_slot(seen.last, seen.sinks, seen.ring) : -1;
-    seen.lo_at = q.pos + rt * kRows / a.group;
-    seen.hi_at = q.pos + min((rt * kRows + kRows - 1) / a.group, q.count - 1);
+    seen.lo_at = q.pos + rt * per / a.group;
+    seen.hi_at = q.pos + min((rt * per + per - 1) / a.group, q.count - 1);
     const int chunks = (tiles_of(seen, a.c.cap).count() + chunk_tiles - 1) / chunk_tiles;
     if (chunks <= 1) return;
-    const size_t step = (size_t)units * kRows * kPart<DH>;
-    const float* part = a.ws + ((size_t)unit * kRows + col) * kPart<DH>;
+    const size_t step = (size_t)units * per * kPart<DH>;
+    const float* part = a.ws + ((size_t)unit * per + col) * kPart<DH>;
     float top = -INFINITY;
     for (int c = lane; c < chunks; c += 64) top = fmaxf(top, part[c * step + DH]);
     top = wave_max(top);
@@ -857,24 +876,329 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, in
         store4((T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head + d, all * (norm == 0.0f ? 0.0f : 1.0f / norm), vec);
 }
 
-struct RowsPlan {
-    int hb, row_tiles, units, waves, chunk_tiles, chunks;
+// ---- many query rows ----
+// A workgroup of four waves takes 64 CT query rows of one key/value head (the heads of its group, token after token), a wave CT
+// times 16 of them. Tiles of 32 slots come into LDS as they are, three ahead; the workgroup unpacks the next one to bf16 while
+// it works on this one, into the order in which the products take it: fragments of 16 x 32 values, 16 bytes a lane. The places
+// are exchanged (XOR of the low three bits of a lane's place) so that neither the writes of unpacking nor the reads of the
+// products meet in a bank: of K's fragment (h, s) by g and 4 (s & 1), of V's fragment d by d.
+template <int DH>
+struct Unpacked {
+    static constexpr int k = 64 * DH, bytes = 2 * k;
+    __device__ static __forceinline__ int k_lane(int i, int g) { return 16 * ((i + 16 * g) ^ g); }
+    __device__ static __forceinline__ int v_lane(int i, int g) { return k + 16 * (i + 16 * g); }
+    __device__ static __forceinline__ int k_at(int h, int s, int lane) { return (h * (DH / 32) + s) * 1024 + (lane ^ (64 * (s & 1))); }
+    __device__ static __forceinline__ int v_at(int d, int lane) { return d * 1024 + (lane ^ (16 * (d & 7))); }
 };
-RowsPlan rows_plan(const KvAttnArgs& a) {
-    RowsPlan p;
-    // heads a wave takes together: as many as give it 8 rows or fewer
+
+template <int DH, class T>
+struct Chunk {
+    static constexpr int CT = Terms<T>::q == 3 ? 1 : 2;  // (registers: the query's parts)
+    static constexpr int rows = 64 * CT;
+    static constexpr int o_raw = 2 * Unpacked<DH>::bytes, lds = o_raw + 3 * KvTile<DH>::bytes;
+};
+
+template <int DH, class T>
+__global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
+    using W = Width<DH>;
+    using Tile = KvTile<DH>;
+    using U = Unpacked<DH>;
+    using C = Chunk<DH, T>;
+    constexpr int QT = Terms<T>::q, PT = Terms<T>::p, CT = C::CT, ND = DH / 16;
+    __shared__ __align__(16) uint8_t smem[C::lds];
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int unit = blockIdx.x;
+    const int pair = unit / row_tiles, rt = unit - pair * row_tiles;
+    const int s = pair / a.c.heads, h = pair - s * a.c.heads;
+    const SeqSpan q = seq_span(a.pos, a.counts, s, a.T);
+    const int ring = a.c.cap - a.c.sinks, sinks = a.c.sinks, rows = a.T * a.group;
+    const int t_lo = rt * C::rows / a.group;
+    if (t_lo >= q.count) return;
+    const int t_hi = min((rt * C::rows + C::rows - 1) / a.group, q.count - 1);
+    Seen seen;
+    seen.sinks = sinks; seen.ring = ring; seen.window = a.window;
+    seen.last = q.end - 1;
+    seen.newest = seen.last >= sinks ? kv_slot(seen.last, sinks, ring) : -1;
+    seen.lo_at = q.pos + t_lo;
+    seen.hi_at = q.pos + t_hi;
+    const Tiles tl = tiles_of(seen, a.c.cap);
+    const int n_tiles = tl.count();
+    const int o0 = blockIdx.y * chunk_tiles, o1 = min(n_tiles, o0 + chunk_tiles);
+    if (blockIdx.y && o0 >= n_tiles) return;
+
+    // loads of a tile: wave w has numbers w, w + 4, ... of its DH / 32 KiB and the scales
+    const size_t plane = (size_t)pair * a.c.cap;
+    const uint32_t raw0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)(smem + C::o_raw);
+    const uint8_t* from[(W::KS + 4) / 4];
+#pragma unroll
+    for (int x = 0; x <= W::KS; x++)
+        if ((x & 3) == wave) {
+            if (x == W::KS) {
+                const int at = min(4 * (W::NB == 3 ? lane : lane & (16 * W::NB - 1)), 64 * W::NB - 4);
+                from[x >> 2] = at < 32 * W::NB ? a.c.ks + plane * W::NB + at : a.c.vs + plane * W::NB + at - 32 * W::NB;
+            } else {
+                const int at = 1024 * x + 16 * lane;
+                from[x >> 2] = at < Tile::half ? a.c.k + plane * Tile::row + at : a.c.v + plane * Tile::row + at - Tile::half;
+            }
+        }
+    const int mine = (W::KS + 4 - wave) / 4;  // this wave's loads of a tile
+    auto fetch = [&](int o, int slot) {
+        const size_t j0 = tl.at(o) * kTile;
+#pragma unroll
+        for (int x = 0; x <= W::KS; x++)
+            if ((x & 3) == wave) {
+                if (x == W::KS) lds_load4(from[x >> 2] + j0 * W::NB, raw0 + slot * Tile::bytes + Tile::o_scales);
+                else lds_load16(from[x >> 2] + j0 * Tile::row, raw0 + slot * Tile::bytes + 1024 * x);
+            }
+    };
+    // Unpacks the tile at slot j0. Neighbouring lanes take neighbouring words of a row, of K a word, of V those of two slots.
+    auto unpack = [&](int raw, int buf, int j0, bool careful) {
+        const uint8_t* p = smem + C::o_raw + raw * Tile::bytes;
+        uint8_t* out = smem + buf * U::bytes;
+        constexpr int words = DH / 8;
+#pragma unroll
+        for (int x = 0; x < (32 * words + 255) / 256; x++) {
+            const int at = threadIdx.x + 256 * x, j = at / words, wd = at % words;
+            if (32 * words % 256 && at >= 32 * words) break;
+            const uint32_t w = *(const uint32_t*)(p + j * Tile::row + 4 * wd);
+            const float sc = mx4_scale(p[Tile::o_scales + j * W::NB + wd / 4]);
+            u32x4 y;
+#pragma unroll
+            for (int b = 0; b < 4; b++) y[b] = unpack2(w, sc, b);
+            // the scores of slots 8 g .. 8 g + 7 come out in lane group g
+            *(u32x4*)(out + U::k_at((j >> 2) & 1, wd / 4, U::k_lane(4 * (j >> 3) + (j & 3), wd & 3))) = y;
+        }
+        const bool held = seen.all_held(j0);
+#pragma unroll
+        for (int x = 0; x < (16 * words + 255) / 256; x++) {
+            const int at = threadIdx.x + 256 * x, j = at / words * 2, wd = at % words;
+            if (16 * words % 256 && at >= 16 * words) break;
+            uint32_t w[2];
+            uint32_t sb[2];
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                w[y] = *(const uint32_t*)(p + Tile::half + (j + y) * Tile::row + 4 * wd);
+                sb[y] = p[Tile::o_scales + (32 + j + y) * W::NB + wd / 4];
+            }
+            if (!held || careful) {
+                asm volatile("");
+#pragma unroll
+                for (int y = 0; y < 2; y++)
+                    if (!seen.holds(j0 + j + y) || (careful && sb[y] > 252u)) w[y] = sb[y] = 0;
+            }
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const uint32_t y0 = unpack2(w[0], mx4_scale(sb[0]), b), y1 = unpack2(w[1], mx4_scale(sb[1]), b);
+                // channels 8 wd + 2 b and the next
+                const int at = U::v_at(wd / 2, U::v_lane(8 * (wd & 1), j >> 3)) + 2 * (j & 7);
+                *(uint32_t*)(out + (at ^ (32 * b))) = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
+                *(uint32_t*)(out + (at ^ (32 * b + 16))) = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
+            }
+        }
+    };
+
+    // this lane's rows
+    v8bf qf[CT][W::KS][QT];
+    Seen own[CT];
+    bool there[CT];
+    int t[CT], head[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const int first = rt * C::rows + (ct * 4 + wave) * 16, row = first + i;
+        t[ct] = row / a.group;
+        head[ct] = h * a.group + (row - t[ct] * a.group);
+        there[ct] = row < rows && t[ct] < q.count;
+        own[ct] = seen;
+        own[ct].lo_at = q.pos + first / a.group;
+        own[ct].hi_at = min(q.pos + (first + 15) / a.group, q.pos + q.count - 1);
+        own[ct].at = q.pos + t[ct];
+        own[ct].low = a.window > 0 ? own[ct].at - a.window : INT_MIN;
+#pragma unroll
+        for (int x = 0; x < W::KS; x++) {
+            float y[8] = {};
+            if (there[ct]) {
+                const T* p = (const T*)a.q.data + s * a.q.seq + t[ct] * a.q.token + head[ct] * a.q.head + 32 * x + 8 * g;
+                if (vec) real_load8<T, true>(p, 8, y);
+                else real_load8<T, false>(p, 8, y);
+            }
+            split_bf16<QT>(y, qf[ct][x]);
+        }
+    }
+    const float scale = a.scale * kLog2e;
+    v4f acc[CT][ND];
+    float m[CT], l[CT];
+    uint32_t nan_blocks[CT];
+
+    auto barrier = [] {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    };
+    auto wait_loads = [&](bool last) {  // all but the newest tile's, or all
+        if (last || mine == 0) vm_wait<0>();
+        else if (mine == 1) vm_wait<1>();
+        else vm_wait<2>();
+    };
+    auto work = [&](int buf, int j0, bool careful) {
+        const uint8_t* p = smem + buf * U::bytes;
+        int k_lane = U::k_lane(i, g), v_lane = U::v_lane(i, g);
+        asm volatile("" : "+v"(k_lane), "+v"(v_lane));  // (or the addresses of all fragments are kept in registers)
+        v4f d[CT][2];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) d[ct][hf] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+            for (int x = 0; x < W::KS; x++) {
+                const v8bf kf = *(const v8bf*)(p + U::k_at(hf, x, k_lane));
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                    for (int n = QT - 1; n >= 0; n--) d[ct][hf] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ct][x][n], d[ct][hf], 0, 0, 0);
+            }
+        v8bf pf[CT][PT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            float sc[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) sc[e] = d[ct][e >> 2][e & 3] * scale;
+            if (!own[ct].whole(j0)) {
+                asm volatile("");
+                uint32_t sees = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const bool v = own[ct].sees(j0 + 8 * g + e);
+                    sees |= (uint32_t)v << e;
+                    sc[e] = v ? sc[e] : -INFINITY;
+                }
+            }
+            const float mt = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+            if (__any(mt > m[ct])) {  // rare after the first tiles
+                const float mn = fmaxf(m[ct], max_groups(mt)), al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : m[ct] - mn);
+                m[ct] = mn;
+                l[ct] *= al;
+#pragma unroll
+                for (int x = 0; x < ND; x++) acc[ct][x] *= al;
+            }
+            const float mu = m[ct] == -INFINITY ? 0.0f : m[ct];
+            float pr[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) pr[e] = __builtin_amdgcn_exp2f(sc[e] - mu);
+            l[ct] += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+            split_bf16<PT>(pr, pf[ct]);
+            if (careful)
+                for (int e = 0; e < 8; e++)
+                    for (int b = 0; b < W::NB; b++)
+                        if (own[ct].sees(j0 + 8 * g + e) && a.c.vs[(plane + j0 + 8 * g + e) * W::NB + b] > 252u) nan_blocks[ct] |= 1u << b;
+        }
+#pragma unroll
+        for (int x = 0; x < ND; x++) {
+            const v8bf vf = *(const v8bf*)(p + U::v_at(x, v_lane));
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                for (int n = PT - 1; n >= 0; n--) acc[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[ct][n], acc[ct][x], 0, 0, 0);
+        }
+    };
+    auto sweep = [&](bool careful) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+#pragma unroll
+            for (int x = 0; x < ND; x++) acc[ct][x] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            m[ct] = -INFINITY;
+            l[ct] = 0.0f;
+            nan_blocks[ct] = 0;
+        }
+        const int n = o1 - o0;
+        for (int x = 0; x < min(n, 3); x++) fetch(o0 + x, x);
+        vm_wait<0>();
+        barrier();
+        if (n > 0) unpack(0, 0, tl.at(o0) * kTile, careful);
+        int raw = 0;  // of tile x
+        for (int x = 0; x < n; x++) {
+            // tile x is unpacked, tile x + 1 has landed; tile x's raw place and the other unpacked one are free
+            barrier();
+            if (x + 3 < n) fetch(o0 + x + 3, raw);
+            raw = raw == 2 ? 0 : raw + 1;
+            if (x + 1 < n) unpack(raw, (x + 1) & 1, __builtin_amdgcn_readfirstlane(tl.at(o0 + x + 1) * kTile), careful);
+            const int j0 = __builtin_amdgcn_readfirstlane(tl.at(o0 + x) * kTile);
+            bool any = false;
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) any |= !own[ct].none(j0);
+            if (any) work(x & 1, j0, careful);
+            wait_loads(x + 3 >= n);
+        }
+    };
+    sweep(false);
+    {
+        // A NaN among the sums: it may come from a value that the row does not see.
+        float bad = 0.0f;
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+            for (int x = 0; x < ND; x++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) bad += acc[ct][x][r] * 0.0f;
+        if (__syncthreads_or(bad != 0.0f)) {
+            sweep(true);
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                nan_blocks[ct] |= __shfl_xor(nan_blocks[ct], 16, 64);
+                nan_blocks[ct] |= __shfl_xor(nan_blocks[ct], 32, 64);
+#pragma unroll
+                for (int x = 0; x < ND; x++)
+                    if (nan_blocks[ct] >> (x / 2) & 1) acc[ct][x] = v4f{NAN, NAN, NAN, NAN};
+            }
+        }
+    }
+    const bool split = n_tiles > chunk_tiles;
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const float total = sum_groups(l[ct]);
+        if (!there[ct]) continue;
+        if (split) {
+            float* part = a.ws + (((size_t)blockIdx.y * gridDim.x + unit) * C::rows + (ct * 4 + wave) * 16 + i) * kPart<DH>;
+#pragma unroll
+            for (int x = 0; x < ND; x++) *(v4f*)(part + 16 * x + 4 * g) = acc[ct][x];
+            if (g == 0) {
+                part[DH] = m[ct];
+                part[DH + 1] = total;
+            }
+        } else {
+            const float f = total == 0.0f ? 0.0f : 1.0f / total;
+            T* out = (T*)a.out.data + s * a.out.seq + t[ct] * a.out.token + head[ct] * a.out.head;
+#pragma unroll
+            for (int x = 0; x < ND; x++) store4(out + 16 * x + 4 * g, acc[ct][x] * f, vec);
+        }
+    }
+}
+
+// How a call is divided: `per` rows a unit (a row tile of one head, or all rows of hb heads), `waves` sharing a unit's tiles, `chunks`
+// workgroups a unit.
+struct AttnPlan {
+    bool many;  // kv_attention_chunk_kernel
+    int per, hb, row_tiles, units, waves, chunk_tiles, chunks;
+};
+AttnPlan attn_plan(const KvAttnArgs& a) {
+    AttnPlan p;
     const int rows = a.T * a.group, most = a.c.dh == 32 ? 8 : a.c.dh == 64 ? 4 : 2;
+    p.many = rows > (getenv("KVX") ? atoi(getenv("KVX")) : 16);
+    // heads a wave takes together: as many as give it 8 rows or fewer
     p.hb = rows * most <= kRows && a.c.heads % most == 0 ? most : rows * 2 <= kRows && a.c.heads % 2 == 0 ? 2 : 1;
-    p.row_tiles = (rows + kRows - 1) / kRows;
+    p.per = p.many ? (a.type == REAL_F32 ? Chunk<32, float>::rows : Chunk<32, __bf16>::rows) : kRows;
+    p.row_tiles = (rows + p.per - 1) / p.per;
     p.units = a.c.n * (a.c.heads / p.hb) * p.row_tiles;
     // tiles that a row tile can see, at most: the sinks', and the window's (or the ring's), with the ends of three runs
-    const long long span = a.window > 0 ? std::min<long long>((long long)a.window + a.T, a.c.cap) : a.c.cap;
+    const long long span = a.window > 0 ? std::min<long long>((long long)a.window + p.per / a.group + 1, a.c.cap) : a.c.cap;
     const int tiles = (int)std::min<long long>((span + kTile - 1) / kTile + (a.c.sinks + kTile - 1) / kTile + 2, a.c.cap / kTile);
-    p.waves = tiles <= 4 ? 1 : 4;
+    p.waves = tiles <= 4 && !p.many ? 1 : 4;
     p.chunk_tiles = tiles;
     if (p.waves > 1) {
-        // Two workgroups a CU, each with four tiles a wave at least. More, smaller chunks cost more at their ends than they even out
-        // (256 conversations, their window in one chunk or two: 28.8 or 37.7 us).
+        // Two workgroups a CU, each with four tiles a wave at least (sixteen of many rows). More, smaller chunks cost more at their ends
+        // than they even out (256 conversations, their window in one chunk or two: 28.8 or 37.7 us).
         const int want = std::max(1, 512 / p.units);
         p.chunk_tiles = std::max(16, (tiles + want - 1) / want);
     }
@@ -882,18 +1206,24 @@ RowsPlan rows_plan(const KvAttnArgs& a) {
     return p;
 }
 
-template <int DH, class T, int HB>
-hipError_t launch_rows_attention(const KvAttnArgs& a, const RowsPlan& p, hipStream_t s) {
-    const int vec = rows_aligned(a.q, a.type) && rows_aligned(a.out, a.type);
-    if (p.waves == 1) {
-        hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 1>), dim3((p.units + 3) / 4), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
-    } else {
-        hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 4>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
-        if (p.chunks > 1)
-            hipLaunchKernelGGL((kv_attention_join_kernel<DH, T>), dim3(p.units, (std::min(kRows, HB * a.T * a.group) + 3) / 4), dim3(256), 0, s, a, HB,
-                               p.row_tiles, p.chunk_tiles, vec);
+template <int DH, class T>
+hipError_t launch_join(const KvAttnArgs& a, const AttnPlan& p, int vec, hipStream_t s) {
+    if (p.chunks > 1) {
+        const int cols = p.hb > 1 ? p.hb * a.T * a.group : std::min(p.per, a.T * a.group);
+        hipLaunchKernelGGL((kv_attention_join_kernel<DH, T>), dim3(p.units, (cols + 3) / 4), dim3(256), 0, s, a, p.per, p.hb, p.row_tiles,
+                           p.chunk_tiles, vec);
     }
     return hipGetLastError();
+}
+
+template <int DH, class T, int HB>
+hipError_t launch_rows_attention(const KvAttnArgs& a, const AttnPlan& p, int vec, hipStream_t s) {
+    if (p.waves == 1) {
+        hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 1>), dim3((p.units + 3) / 4), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 4>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
+    return launch_join<DH, T>(a, p, vec, s);
 }
 
 }  // namespace
@@ -904,21 +1234,31 @@ hipError_t launch_kv_write(const KvRowsArgs& a, hipStream_t s) { return launch_r
 hipError_t launch_kv_read(const KvRowsArgs& a, hipStream_t s) { return launch_rows<true>(a, s); }
 
 size_t kv_attention_ws_bytes(const KvAttnArgs& a) {
-    const RowsPlan p = rows_plan(a);
-    if (p.chunks <= 1) return 0;
-    return (size_t)p.chunks * p.units * kRows * (a.c.dh + 4) * 4;
+    size_t most = 0;
+    for (const int type : {REAL_F32, REAL_BF16}) {  // (the same for all types of a call)
+        KvAttnArgs x = a;
+        x.type = type;
+        const AttnPlan p = attn_plan(x);
+        if (p.chunks > 1) most = std::max(most, (size_t)p.chunks * p.units * p.per * (a.c.dh + 4) * 4);
+    }
+    return most;
 }
 
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
-    const RowsPlan p = rows_plan(a);
+    const AttnPlan p = attn_plan(a);
+    const int vec = rows_aligned(a.q, a.type) && rows_aligned(a.out, a.type);
     return by_width(a.c.dh, [&](auto w) {
         constexpr int DH = decltype(w)::value, most = DH == 32 ? 8 : DH == 64 ? 4 : 2;
         return by_real(a.type, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            if (p.hb == most) return launch_rows_attention<DH, T, most>(a, p, s);
+            if (p.many) {
+                hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
+                return launch_join<DH, T>(a, p, vec, s);
+            }
+            if (p.hb == most) return launch_rows_attention<DH, T, most>(a, p, vec, s);
             if constexpr (most > 2)
-                if (p.hb == 2) return launch_rows_attention<DH, T, 2>(a, p, s);
-            return launch_rows_attention<DH, T, 1>(a, p, s);
+                if (p.hb == 2) return launch_rows_attention<DH, T, 2>(a, p, vec, s);
+            return launch_rows_attention<DH, T, 1>(a, p, vec, s);
         });
     });
 }
