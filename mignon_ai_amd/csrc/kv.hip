@@ -381,7 +381,8 @@ struct Seen {
         const int p = position(j);
         return (p >= (j < sinks ? 0 : sinks)) & (p <= last);
     }
-    __device__ __forceinline__ bool sees(int j) const {
+    // A row at position at, which sees no position up to low but the sinks'.
+    __device__ __forceinline__ bool sees(int j, int at, int low) const {
         const int p = position(j);
         return (p >= (j < sinks ? 0 : sinks)) & (p <= at) & (p <= last) & ((j < sinks) | (p > low));
     }
@@ -390,13 +391,6 @@ struct Seen {
         if (j0 < sinks || (j0 <= newest && newest < j0 + 31)) return -1;
         const int p = position(j0);
         return p >= sinks && p + 31 <= last ? p : -1;
-    }
-    __device__ __forceinline__ bool all_held(int j0) const { return j0 + 31 < sinks ? j0 + 31 <= last : run(j0) >= 0; }
-    // No row sees a slot of the tile (it may say no where that is so).
-    __device__ __forceinline__ bool none(int j0) const {
-        if (lo_at > hi_at) return true;
-        const int p = run(j0);
-        return p >= 0 && (p > hi_at || (window > 0 && p + 31 <= lo_at - window));
     }
     // Every row sees every slot of the tile.
     __device__ __forceinline__ bool whole(int j0) const {
@@ -499,7 +493,7 @@ __device__ __forceinline__ void tile_step(RowState<DH, HB>& st, const uint8_t* t
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const int j = j0 + 8 * g + e;
-            const bool held = seen.holds(j), v = seen.sees(j);
+            const bool held = seen.holds(j), v = seen.sees(j, seen.at, seen.low);
             sees |= (uint32_t)v << e;
             drop |= (uint32_t)!held << e;  // never written, or lost: may hold anything
             sc[e] = v ? sc[e] : -INFINITY;
@@ -912,7 +906,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
     const int pair = unit / row_tiles, rt = unit - pair * row_tiles;
     const int s = pair / a.c.heads, h = pair - s * a.c.heads;
     const SeqSpan q = seq_span(a.pos, a.counts, s, a.T);
-    const int ring = a.c.cap - a.c.sinks, sinks = a.c.sinks, rows = a.T * a.group;
+    const int ring = a.c.cap - a.c.sinks, sinks = a.c.sinks;
     const int t_lo = rt * C::rows / a.group;
     if (t_lo >= q.count) return;
     const int t_hi = min((rt * C::rows + C::rows - 1) / a.group, q.count - 1);
@@ -927,39 +921,28 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
     const int o0 = blockIdx.y * chunk_tiles, o1 = min(n_tiles, o0 + chunk_tiles);
     if (blockIdx.y && o0 >= n_tiles) return;
 
-    // loads of a tile: wave w has numbers w, w + 4, ... of its DH / 32 KiB and the scales
+    // loads of a tile: wave w has its w'th KiB, and one wave the scales
+    constexpr int scale_wave = W::KS & 3;
     const size_t plane = (size_t)pair * a.c.cap;
     const uint32_t raw0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)(smem + C::o_raw);
-    const uint8_t* from[(W::KS + 4) / 4];
-#pragma unroll
-    for (int x = 0; x <= W::KS; x++)
-        if ((x & 3) == wave) {
-            if (x == W::KS) {
-                const int at = min(4 * (W::NB == 3 ? lane : lane & (16 * W::NB - 1)), 64 * W::NB - 4);
-                from[x >> 2] = at < 32 * W::NB ? a.c.ks + plane * W::NB + at : a.c.vs + plane * W::NB + at - 32 * W::NB;
-            } else {
-                const int at = 1024 * x + 16 * lane;
-                from[x >> 2] = at < Tile::half ? a.c.k + plane * Tile::row + at : a.c.v + plane * Tile::row + at - Tile::half;
-            }
-        }
-    const int mine = (W::KS + 4 - wave) / 4;  // this wave's loads of a tile
+    const int code_at = 1024 * wave + 16 * lane, scale_at_ = min(4 * (W::NB == 3 ? lane : lane & (16 * W::NB - 1)), 64 * W::NB - 4);
+    const uint8_t* codes = code_at < Tile::half ? a.c.k + plane * Tile::row + code_at : a.c.v + plane * Tile::row + code_at - Tile::half;
+    const uint8_t* scales = scale_at_ < 32 * W::NB ? a.c.ks + plane * W::NB + scale_at_ : a.c.vs + plane * W::NB + scale_at_ - 32 * W::NB;
     auto fetch = [&](int o, int slot) {
         const size_t j0 = tl.at(o) * kTile;
-#pragma unroll
-        for (int x = 0; x <= W::KS; x++)
-            if ((x & 3) == wave) {
-                if (x == W::KS) lds_load4(from[x >> 2] + j0 * W::NB, raw0 + slot * Tile::bytes + Tile::o_scales);
-                else lds_load16(from[x >> 2] + j0 * Tile::row, raw0 + slot * Tile::bytes + 1024 * x);
-            }
+        if (wave < W::KS) lds_load16(codes + j0 * Tile::row, raw0 + slot * Tile::bytes + 1024 * wave);
+        if (wave == scale_wave) lds_load4(scales + j0 * W::NB, raw0 + slot * Tile::bytes + Tile::o_scales);
     };
-    // Unpacks the tile at slot j0. Neighbouring lanes take neighbouring words of a row, of K a word, of V those of two slots.
-    auto unpack = [&](int raw, int buf, int j0, bool careful) {
+    // Unpacks a tile. Neighbouring lanes take neighbouring words of a row, of K a word, of V those of two slots.
+    constexpr int words = DH / 8;
+    auto unpack = [&](auto careful, int raw, int buf, int j0, bool held) {
         const uint8_t* p = smem + C::o_raw + raw * Tile::bytes;
         uint8_t* out = smem + buf * U::bytes;
-        constexpr int words = DH / 8;
+        int at0 = threadIdx.x;
+        asm volatile("" : "+v"(at0));  // (or all of the addresses below are kept in registers)
 #pragma unroll
         for (int x = 0; x < (32 * words + 255) / 256; x++) {
-            const int at = threadIdx.x + 256 * x, j = at / words, wd = at % words;
+            const int at = at0 + 256 * x, j = at / words, wd = at % words;
             if (32 * words % 256 && at >= 32 * words) break;
             const uint32_t w = *(const uint32_t*)(p + j * Tile::row + 4 * wd);
             const float sc = mx4_scale(p[Tile::o_scales + j * W::NB + wd / 4]);
@@ -969,58 +952,57 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
             // the scores of slots 8 g .. 8 g + 7 come out in lane group g
             *(u32x4*)(out + U::k_at((j >> 2) & 1, wd / 4, U::k_lane(4 * (j >> 3) + (j & 3), wd & 3))) = y;
         }
-        const bool held = seen.all_held(j0);
 #pragma unroll
         for (int x = 0; x < (16 * words + 255) / 256; x++) {
-            const int at = threadIdx.x + 256 * x, j = at / words * 2, wd = at % words;
+            const int at = at0 + 256 * x, j = at / words * 2, wd = at % words;
             if (16 * words % 256 && at >= 16 * words) break;
-            uint32_t w[2];
-            uint32_t sb[2];
+            uint32_t w[2], sb[2];
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 w[y] = *(const uint32_t*)(p + Tile::half + (j + y) * Tile::row + 4 * wd);
                 sb[y] = p[Tile::o_scales + (32 + j + y) * W::NB + wd / 4];
             }
-            if (!held || careful) {
+            if (decltype(careful)::value || !held) {
                 asm volatile("");
 #pragma unroll
                 for (int y = 0; y < 2; y++)
-                    if (!seen.holds(j0 + j + y) || (careful && sb[y] > 252u)) w[y] = sb[y] = 0;
+                    if (!seen.holds(j0 + j + y) || (decltype(careful)::value && sb[y] > 252u)) w[y] = sb[y] = 0;
             }
+            const int to = U::v_at(wd / 2, U::v_lane(8 * (wd & 1), j >> 3)) + 2 * (j & 7);
 #pragma unroll
             for (int b = 0; b < 4; b++) {
-                const uint32_t y0 = unpack2(w[0], mx4_scale(sb[0]), b), y1 = unpack2(w[1], mx4_scale(sb[1]), b);
                 // channels 8 wd + 2 b and the next
-                const int at = U::v_at(wd / 2, U::v_lane(8 * (wd & 1), j >> 3)) + 2 * (j & 7);
-                *(uint32_t*)(out + (at ^ (32 * b))) = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
-                *(uint32_t*)(out + (at ^ (32 * b + 16))) = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
+                const uint32_t y0 = unpack2(w[0], mx4_scale(sb[0]), b), y1 = unpack2(w[1], mx4_scale(sb[1]), b);
+                *(uint32_t*)(out + (to ^ (32 * b))) = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
+                *(uint32_t*)(out + (to ^ (32 * b + 16))) = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
             }
         }
     };
 
     // this lane's rows
     v8bf qf[CT][W::KS][QT];
-    Seen own[CT];
-    bool there[CT];
-    int t[CT], head[CT];
+    int at[CT], low[CT], lo[CT], hi[CT];  // its position and the last one behind its window; the wave's first and last positions
+    const int first = rt * C::rows + wave * 16 + i;
+    auto token = [&](int ct) { return (first + 64 * ct) / a.group; };
+    auto row_of = [&](const KvRows& r, int ct) {
+        const int row = first + 64 * ct, t = token(ct);
+        return s * r.seq + t * r.token + (h * a.group + (row - t * a.group)) * r.head;
+    };
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        const int first = rt * C::rows + (ct * 4 + wave) * 16, row = first + i;
-        t[ct] = row / a.group;
-        head[ct] = h * a.group + (row - t[ct] * a.group);
-        there[ct] = row < rows && t[ct] < q.count;
-        own[ct] = seen;
-        own[ct].lo_at = q.pos + first / a.group;
-        own[ct].hi_at = min(q.pos + (first + 15) / a.group, q.pos + q.count - 1);
-        own[ct].at = q.pos + t[ct];
-        own[ct].low = a.window > 0 ? own[ct].at - a.window : INT_MIN;
+        const int r0 = rt * C::rows + wave * 16 + 64 * ct;
+        lo[ct] = q.pos + r0 / a.group;
+        hi[ct] = min(q.pos + (r0 + 15) / a.group, q.pos + q.count - 1);
+        at[ct] = q.pos + token(ct);
+        low[ct] = a.window > 0 ? at[ct] - a.window : INT_MIN;
+        const bool there = token(ct) < q.count;
+        const T* p = (const T*)a.q.data + row_of(a.q, ct) + 8 * g;
 #pragma unroll
         for (int x = 0; x < W::KS; x++) {
             float y[8] = {};
-            if (there[ct]) {
-                const T* p = (const T*)a.q.data + s * a.q.seq + t[ct] * a.q.token + head[ct] * a.q.head + 32 * x + 8 * g;
-                if (vec) real_load8<T, true>(p, 8, y);
-                else real_load8<T, false>(p, 8, y);
+            if (there) {
+                if (vec) real_load8<T, true>(p + 32 * x, 8, y);
+                else real_load8<T, false>(p + 32 * x, 8, y);
             }
             split_bf16<QT>(y, qf[ct][x]);
         }
@@ -1035,15 +1017,16 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     };
-    auto wait_loads = [&](bool last) {  // all but the newest tile's, or all
-        if (last || mine == 0) vm_wait<0>();
-        else if (mine == 1) vm_wait<1>();
-        else vm_wait<2>();
-    };
-    auto work = [&](int buf, int j0, bool careful) {
+    // run: the position of the tile's first slot, where its slots hold 32 positions in a row
+    auto work = [&](auto careful, int buf, int j0, int run) {
+        bool none = true;
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++)
+            none &= lo[ct] > hi[ct] || (run >= 0 && (run > hi[ct] || (a.window > 0 && run + 31 <= lo[ct] - a.window)));
+        if (none) return;
         const uint8_t* p = smem + buf * U::bytes;
         int k_lane = U::k_lane(i, g), v_lane = U::v_lane(i, g);
-        asm volatile("" : "+v"(k_lane), "+v"(v_lane));  // (or the addresses of all fragments are kept in registers)
+        asm volatile("" : "+v"(k_lane), "+v"(v_lane));
         v4f d[CT][2];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++)
@@ -1065,14 +1048,16 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
             float sc[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) sc[e] = d[ct][e >> 2][e & 3] * scale;
-            if (!own[ct].whole(j0)) {
+            const bool whole = run >= 0 && run + 31 <= lo[ct] && (a.window <= 0 || run > hi[ct] - a.window);
+            if (!whole) {
                 asm volatile("");
-                uint32_t sees = 0;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const bool v = own[ct].sees(j0 + 8 * g + e);
-                    sees |= (uint32_t)v << e;
+                    const bool v = seen.sees(j0 + 8 * g + e, at[ct], low[ct]);
                     sc[e] = v ? sc[e] : -INFINITY;
+                    if (decltype(careful)::value && v)
+                        for (int b = 0; b < W::NB; b++)
+                            if (a.c.vs[(plane + j0 + 8 * g + e) * W::NB + b] > 252u) nan_blocks[ct] |= 1u << b;
                 }
             }
             const float mt = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
@@ -1089,10 +1074,6 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
             for (int e = 0; e < 8; e++) pr[e] = __builtin_amdgcn_exp2f(sc[e] - mu);
             l[ct] += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
             split_bf16<PT>(pr, pf[ct]);
-            if (careful)
-                for (int e = 0; e < 8; e++)
-                    for (int b = 0; b < W::NB; b++)
-                        if (own[ct].sees(j0 + 8 * g + e) && a.c.vs[(plane + j0 + 8 * g + e) * W::NB + b] > 252u) nan_blocks[ct] |= 1u << b;
         }
 #pragma unroll
         for (int x = 0; x < ND; x++) {
@@ -1103,7 +1084,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
                 for (int n = PT - 1; n >= 0; n--) acc[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[ct][n], acc[ct][x], 0, 0, 0);
         }
     };
-    auto sweep = [&](bool careful) {
+    auto sweep = [&](auto careful) {
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
 #pragma unroll
@@ -1113,26 +1094,31 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
             nan_blocks[ct] = 0;
         }
         const int n = o1 - o0;
+        if (n <= 0) return;
         for (int x = 0; x < min(n, 3); x++) fetch(o0 + x, x);
         vm_wait<0>();
         barrier();
-        if (n > 0) unpack(0, 0, tl.at(o0) * kTile, careful);
+        int j0 = tl.at(o0) * kTile, run = seen.run(j0);
+        unpack(careful, 0, 0, j0, run >= 0);
         int raw = 0;  // of tile x
         for (int x = 0; x < n; x++) {
             // tile x is unpacked, tile x + 1 has landed; tile x's raw place and the other unpacked one are free
             barrier();
             if (x + 3 < n) fetch(o0 + x + 3, raw);
             raw = raw == 2 ? 0 : raw + 1;
-            if (x + 1 < n) unpack(raw, (x + 1) & 1, __builtin_amdgcn_readfirstlane(tl.at(o0 + x + 1) * kTile), careful);
-            const int j0 = __builtin_amdgcn_readfirstlane(tl.at(o0 + x) * kTile);
-            bool any = false;
-#pragma unroll
-            for (int ct = 0; ct < CT; ct++) any |= !own[ct].none(j0);
-            if (any) work(x & 1, j0, careful);
-            wait_loads(x + 3 >= n);
+            const int j1 = tl.at(o0 + min(x + 1, n - 1)) * kTile, run1 = seen.run(j1);
+            if (x + 1 < n) unpack(careful, raw, (x + 1) & 1, j1, run1 >= 0);
+            // (the careful form asks for every slot of every tile)
+            work(careful, x & 1, j0, decltype(careful)::value ? -1 : run);
+            j0 = j1;
+            run = run1;
+            // all but this step's loads have landed
+            if (x + 3 >= n) vm_wait<0>();
+            else if (W::KS == 4 && wave == scale_wave) vm_wait<2>();
+            else vm_wait<1>();
         }
     };
-    sweep(false);
+    sweep(std::false_type());
     {
         // A NaN among the sums: it may come from a value that the row does not see.
         float bad = 0.0f;
@@ -1143,7 +1129,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
 #pragma unroll
                 for (int r = 0; r < 4; r++) bad += acc[ct][x][r] * 0.0f;
         if (__syncthreads_or(bad != 0.0f)) {
-            sweep(true);
+            sweep(std::true_type());
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 nan_blocks[ct] |= __shfl_xor(nan_blocks[ct], 16, 64);
@@ -1158,7 +1144,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         const float total = sum_groups(l[ct]);
-        if (!there[ct]) continue;
+        if (token(ct) >= q.count) continue;
         if (split) {
             float* part = a.ws + (((size_t)blockIdx.y * gridDim.x + unit) * C::rows + (ct * 4 + wave) * 16 + i) * kPart<DH>;
 #pragma unroll
@@ -1169,7 +1155,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
             }
         } else {
             const float f = total == 0.0f ? 0.0f : 1.0f / total;
-            T* out = (T*)a.out.data + s * a.out.seq + t[ct] * a.out.token + head[ct] * a.out.head;
+            T* out = (T*)a.out.data + row_of(a.out, ct);
 #pragma unroll
             for (int x = 0; x < ND; x++) store4(out + 16 * x + 4 * g, acc[ct][x] * f, vec);
         }
