@@ -12,6 +12,7 @@ namespace mg {
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 // What a sequence's call covers: token t < count sits at position pos + t, the cache holds positions below `end`.
@@ -871,45 +872,41 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, in
 }
 
 // ---- many query rows ----
-// A workgroup of four waves takes 64 CT query rows of one key/value head (the heads of its group, token after token), a wave CT
-// times 16 of them. Tiles of 32 slots come into LDS as they are, three ahead; the workgroup unpacks the next one to bf16 while
-// it works on this one, into the order in which the products take it: fragments of 16 x 32 values, 16 bytes a lane. The places
-// are exchanged (XOR of the low three bits of a lane's place) so that neither the writes of unpacking nor the reads of the
-// products meet in a bank: of K's fragment (h, s) by g and 4 (s & 1), of V's fragment d by d.
+// A workgroup of four waves takes 128 query rows of one key/value head (the heads of its group, token after token), a wave 32 of
+// them. Tiles of 32 slots come into LDS as they are, three ahead; the workgroup unpacks the next one to bf16 while it works on
+// this one, into the order in which the products of 32 x 32 x 16 take it: fragments of 32 x 16 values, 16 bytes a lane. With
+// i = lane & 31 and g = lane >> 5, K's fragment s has slot i, channels 16 s + 8 g .. + 7; the scores of row i and slots
+// (r & 3) + 8 (r >> 2) + 4 g, r < 16, come out in the lane, which is how the second product takes the probabilities: of V's
+// fragments 2 d and 2 d + 1, channel 32 d + i, entries r < 8 and r >= 8. The places are exchanged (XOR of the low three bits of a
+// lane's place) so that the writes of unpacking and the reads of the products do not meet in a bank: of K's fragment s by g and
+// 2 (s & 3), of V's by 4 g and d & 3.
 template <int DH>
 struct Unpacked {
     static constexpr int k = 64 * DH, bytes = 2 * k;
-    __device__ static __forceinline__ int k_lane(int i, int g) { return 16 * ((i + 16 * g) ^ g); }
-    __device__ static __forceinline__ int v_lane(int i, int g) { return k + 16 * (i + 16 * g); }
-    __device__ static __forceinline__ int k_at(int h, int s, int lane) { return (h * (DH / 32) + s) * 1024 + (lane ^ (64 * (s & 1))); }
-    __device__ static __forceinline__ int v_at(int d, int lane) { return d * 1024 + (lane ^ (16 * (d & 7))); }
+    __device__ static __forceinline__ int k_lane(int i, int g) { return 16 * ((i + 32 * g) ^ g); }
+    __device__ static __forceinline__ int v_lane(int i, int g) { return k + 16 * ((i + 32 * g) ^ (4 * g)); }
+    __device__ static __forceinline__ int k_at(int s, int lane) { return s * 1024 + (lane ^ (32 * (s & 3))); }
+    __device__ static __forceinline__ int v_at(int d, int half, int lane) { return (2 * d + half) * 1024 + (lane ^ (16 * (d & 3))); }
 };
-
-template <int DH, class T>
-struct Chunk {
-    static constexpr int CT = Terms<T>::q == 3 ? 1 : 2;  // (registers: the query's parts)
-    static constexpr int rows = 64 * CT;
-    static constexpr int o_raw = 2 * Unpacked<DH>::bytes, lds = o_raw + 3 * KvTile<DH>::bytes;
-};
+constexpr int kManyRows = 128;
 
 template <int DH, class T>
 __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
     using W = Width<DH>;
     using Tile = KvTile<DH>;
     using U = Unpacked<DH>;
-    using C = Chunk<DH, T>;
-    constexpr int QT = Terms<T>::q, PT = Terms<T>::p, CT = C::CT, ND = DH / 16;
-    __shared__ __align__(16) uint8_t smem[C::lds];
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    constexpr int QT = Terms<T>::q, PT = Terms<T>::p, KF = DH / 16, ND = DH / 32, o_raw = 2 * U::bytes;
+    __shared__ __align__(16) uint8_t smem[o_raw + 3 * Tile::bytes];
+    const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int unit = blockIdx.x;
     const int pair = unit / row_tiles, rt = unit - pair * row_tiles;
     const int s = pair / a.c.heads, h = pair - s * a.c.heads;
     const SeqSpan q = seq_span(a.pos, a.counts, s, a.T);
     const int ring = a.c.cap - a.c.sinks, sinks = a.c.sinks;
-    const int t_lo = rt * C::rows / a.group;
+    const int t_lo = rt * kManyRows / a.group;
     if (t_lo >= q.count) return;
-    const int t_hi = min((rt * C::rows + C::rows - 1) / a.group, q.count - 1);
+    const int t_hi = min((rt * kManyRows + kManyRows - 1) / a.group, q.count - 1);
     Seen seen;
     seen.sinks = sinks; seen.ring = ring; seen.window = a.window;
     seen.last = q.end - 1;
@@ -924,7 +921,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
     // loads of a tile: wave w has its w'th KiB, and one wave the scales
     constexpr int scale_wave = W::KS & 3;
     const size_t plane = (size_t)pair * a.c.cap;
-    const uint32_t raw0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)(smem + C::o_raw);
+    const uint32_t raw0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)(smem + o_raw);
     const int code_at = 1024 * wave + 16 * lane, scale_at_ = min(4 * (W::NB == 3 ? lane : lane & (16 * W::NB - 1)), 64 * W::NB - 4);
     const uint8_t* codes = code_at < Tile::half ? a.c.k + plane * Tile::row + code_at : a.c.v + plane * Tile::row + code_at - Tile::half;
     const uint8_t* scales = scale_at_ < 32 * W::NB ? a.c.ks + plane * W::NB + scale_at_ : a.c.vs + plane * W::NB + scale_at_ - 32 * W::NB;
@@ -936,7 +933,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
     // Unpacks a tile. Neighbouring lanes take neighbouring words of a row, of K a word, of V those of two slots.
     constexpr int words = DH / 8;
     auto unpack = [&](auto careful, int raw, int buf, int j0, bool held) {
-        const uint8_t* p = smem + C::o_raw + raw * Tile::bytes;
+        const uint8_t* p = smem + o_raw + raw * Tile::bytes;
         uint8_t* out = smem + buf * U::bytes;
         int at0 = threadIdx.x;
         asm volatile("" : "+v"(at0));  // (or all of the addresses below are kept in registers)
@@ -949,8 +946,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
             u32x4 y;
 #pragma unroll
             for (int b = 0; b < 4; b++) y[b] = unpack2(w, sc, b);
-            // the scores of slots 8 g .. 8 g + 7 come out in lane group g
-            *(u32x4*)(out + U::k_at((j >> 2) & 1, wd / 4, U::k_lane(4 * (j >> 3) + (j & 3), wd & 3))) = y;
+            *(u32x4*)(out + U::k_at(wd / 2, U::k_lane(j, wd & 1))) = y;
         }
 #pragma unroll
         for (int x = 0; x < (16 * words + 255) / 256; x++) {
@@ -968,7 +964,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
                 for (int y = 0; y < 2; y++)
                     if (!seen.holds(j0 + j + y) || (decltype(careful)::value && sb[y] > 252u)) w[y] = sb[y] = 0;
             }
-            const int to = U::v_at(wd / 2, U::v_lane(8 * (wd & 1), j >> 3)) + 2 * (j & 7);
+            const int to = U::v_at(wd / 4, j >> 4, U::v_lane(8 * (wd & 3), (j >> 2) & 1)) + 2 * ((j & 3) + (j >> 3 & 1) * 4);
 #pragma unroll
             for (int b = 0; b < 4; b++) {
                 // channels 8 wd + 2 b and the next
@@ -979,38 +975,32 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
         }
     };
 
-    // this lane's rows
-    v8bf qf[CT][W::KS][QT];
-    int at[CT], low[CT], lo[CT], hi[CT];  // its position and the last one behind its window; the wave's first and last positions
-    const int first = rt * C::rows + wave * 16 + i;
-    auto token = [&](int ct) { return (first + 64 * ct) / a.group; };
-    auto row_of = [&](const KvRows& r, int ct) {
-        const int row = first + 64 * ct, t = token(ct);
-        return s * r.seq + t * r.token + (h * a.group + (row - t * a.group)) * r.head;
-    };
+    // this lane's row
+    const int row = rt * kManyRows + wave * 32 + i, t = row / a.group, head = h * a.group + (row - t * a.group);
+    const bool there = t < q.count;
+    // its position and the last one behind its window; the wave's first and last positions
+    const int at = q.pos + t, low = a.window > 0 ? at - a.window : INT_MIN;
+    const int r0 = rt * kManyRows + wave * 32, lo = q.pos + r0 / a.group, hi = min(q.pos + (r0 + 31) / a.group, q.pos + q.count - 1);
+    // the factor's sign, or zero, goes to the query, so that the largest product is the largest score
+    const float sign = a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f, scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
+    v8bf qf[KF][QT];
+    {
+        const T* p = (const T*)a.q.data + s * a.q.seq + t * a.q.token + head * a.q.head + 8 * g;
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        const int r0 = rt * C::rows + wave * 16 + 64 * ct;
-        lo[ct] = q.pos + r0 / a.group;
-        hi[ct] = min(q.pos + (r0 + 15) / a.group, q.pos + q.count - 1);
-        at[ct] = q.pos + token(ct);
-        low[ct] = a.window > 0 ? at[ct] - a.window : INT_MIN;
-        const bool there = token(ct) < q.count;
-        const T* p = (const T*)a.q.data + row_of(a.q, ct) + 8 * g;
-#pragma unroll
-        for (int x = 0; x < W::KS; x++) {
+        for (int x = 0; x < KF; x++) {
             float y[8] = {};
             if (there) {
-                if (vec) real_load8<T, true>(p + 32 * x, 8, y);
-                else real_load8<T, false>(p + 32 * x, 8, y);
+                if (vec) real_load8<T, true>(p + 16 * x, 8, y);
+                else real_load8<T, false>(p + 16 * x, 8, y);
             }
-            split_bf16<QT>(y, qf[ct][x]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] *= sign;
+            split_bf16<QT>(y, qf[x]);
         }
     }
-    const float scale = a.scale * kLog2e;
-    v4f acc[CT][ND];
-    float m[CT], l[CT];
-    uint32_t nan_blocks[CT];
+    v16f acc[ND];
+    float m, l;
+    uint32_t nan_blocks;
 
     auto barrier = [] {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -1019,80 +1009,70 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
     };
     // run: the position of the tile's first slot, where its slots hold 32 positions in a row
     auto work = [&](auto careful, int buf, int j0, int run) {
-        bool none = true;
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++)
-            none &= lo[ct] > hi[ct] || (run >= 0 && (run > hi[ct] || (a.window > 0 && run + 31 <= lo[ct] - a.window)));
-        if (none) return;
+        if (lo > hi || (run >= 0 && (run > hi || (a.window > 0 && run + 31 <= lo - a.window)))) return;  // no row sees it
         const uint8_t* p = smem + buf * U::bytes;
         int k_lane = U::k_lane(i, g), v_lane = U::v_lane(i, g);
         asm volatile("" : "+v"(k_lane), "+v"(v_lane));
-        v4f d[CT][2];
+        v16f d = {};
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++)
+        for (int x = 0; x < KF; x++) {
+            const v8bf kf = *(const v8bf*)(p + U::k_at(x, k_lane));
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) d[ct][hf] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-            for (int x = 0; x < W::KS; x++) {
-                const v8bf kf = *(const v8bf*)(p + U::k_at(hf, x, k_lane));
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int n = QT - 1; n >= 0; n--) d[ct][hf] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ct][x][n], d[ct][hf], 0, 0, 0);
-            }
-        v8bf pf[CT][PT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            float sc[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) sc[e] = d[ct][e >> 2][e & 3] * scale;
-            const bool whole = run >= 0 && run + 31 <= lo[ct] && (a.window <= 0 || run > hi[ct] - a.window);
-            if (!whole) {
-                asm volatile("");
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const bool v = seen.sees(j0 + 8 * g + e, at[ct], low[ct]);
-                    sc[e] = v ? sc[e] : -INFINITY;
-                    if (decltype(careful)::value && v)
-                        for (int b = 0; b < W::NB; b++)
-                            if (a.c.vs[(plane + j0 + 8 * g + e) * W::NB + b] > 252u) nan_blocks[ct] |= 1u << b;
-                }
-            }
-            const float mt = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
-            if (__any(mt > m[ct])) {  // rare after the first tiles
-                const float mn = fmaxf(m[ct], max_groups(mt)), al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : m[ct] - mn);
-                m[ct] = mn;
-                l[ct] *= al;
-#pragma unroll
-                for (int x = 0; x < ND; x++) acc[ct][x] *= al;
-            }
-            const float mu = m[ct] == -INFINITY ? 0.0f : m[ct];
-            float pr[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) pr[e] = __builtin_amdgcn_exp2f(sc[e] - mu);
-            l[ct] += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
-            split_bf16<PT>(pr, pf[ct]);
+            for (int n = QT - 1; n >= 0; n--) d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[x][n], d, 0, 0, 0);
         }
+        const bool whole = run >= 0 && run + 31 <= lo && (a.window <= 0 || run > hi - a.window);
+        if (!whole) {
+            asm volatile("");
 #pragma unroll
-        for (int x = 0; x < ND; x++) {
-            const v8bf vf = *(const v8bf*)(p + U::v_at(x, v_lane));
-#pragma unroll
-            for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                for (int n = PT - 1; n >= 0; n--) acc[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[ct][n], acc[ct][x], 0, 0, 0);
+            for (int r = 0; r < 16; r++) {
+                const int j = j0 + (r & 3) + 8 * (r >> 2) + 4 * g;
+                const bool v = seen.sees(j, at, low);
+                d[r] = v ? d[r] : -INFINITY;
+                if (decltype(careful)::value && v)
+                    for (int b = 0; b < W::NB; b++)
+                        if (a.c.vs[(plane + j) * W::NB + b] > 252u) nan_blocks |= 1u << b;
+            }
         }
+        float mt = d[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) mt = fmaxf(mt, d[r]);
+        // (in units of the score's power of two; a row that sees nothing here stays as it is)
+        mt = mt == -INFINITY ? -INFINITY : mt * scale;
+        if (__any(mt > m)) {  // rare after the first tiles
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+            const float mn = fmaxf(m, fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])));
+            const float al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : m - mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int x = 0; x < ND; x++) acc[x] *= al;
+        }
+        const float mu = m == -INFINITY ? 0.0f : m;
+        float pr[16];
+#pragma unroll
+        for (int r = 0; r < 16; r++) pr[r] = __builtin_amdgcn_exp2f(fmaf(d[r], scale, -mu));
+        float sum[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) sum[r] = (pr[r] + pr[4 + r]) + (pr[8 + r] + pr[12 + r]);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        v8bf pf[2][PT];
+        split_bf16<PT>(pr, pf[0]);
+        split_bf16<PT>(pr + 8, pf[1]);
+#pragma unroll
+        for (int x = 0; x < ND; x++)
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const v8bf vf = *(const v8bf*)(p + U::v_at(x, hf, v_lane));
+#pragma unroll
+                for (int n = PT - 1; n >= 0; n--) acc[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[hf][n], acc[x], 0, 0, 0);
+            }
     };
     auto sweep = [&](auto careful) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-#pragma unroll
-            for (int x = 0; x < ND; x++) acc[ct][x] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            m[ct] = -INFINITY;
-            l[ct] = 0.0f;
-            nan_blocks[ct] = 0;
-        }
+        for (int x = 0; x < ND; x++) acc[x] = v16f{};
+        m = -INFINITY;
+        l = 0.0f;
+        nan_blocks = 0;
         const int n = o1 - o0;
         if (n <= 0) return;
         for (int x = 0; x < min(n, 3); x++) fetch(o0 + x, x);
@@ -1123,42 +1103,41 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
         // A NaN among the sums: it may come from a value that the row does not see.
         float bad = 0.0f;
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++)
+        for (int x = 0; x < ND; x++)
 #pragma unroll
-            for (int x = 0; x < ND; x++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) bad += acc[ct][x][r] * 0.0f;
+            for (int r = 0; r < 16; r++) bad += acc[x][r] * 0.0f;
         if (__syncthreads_or(bad != 0.0f)) {
             sweep(std::true_type());
+            nan_blocks |= __shfl_xor(nan_blocks, 32, 64);
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) {
-                nan_blocks[ct] |= __shfl_xor(nan_blocks[ct], 16, 64);
-                nan_blocks[ct] |= __shfl_xor(nan_blocks[ct], 32, 64);
+            for (int x = 0; x < ND; x++)
+                if (nan_blocks >> x & 1)
 #pragma unroll
-                for (int x = 0; x < ND; x++)
-                    if (nan_blocks[ct] >> (x / 2) & 1) acc[ct][x] = v4f{NAN, NAN, NAN, NAN};
-            }
+                    for (int r = 0; r < 16; r++) acc[x][r] = NAN;
         }
     }
-    const bool split = n_tiles > chunk_tiles;
+    const float total = l + __shfl_xor(l, 32, 64);
+    if (!there) return;
+    // lane (i, g): row i, channels 32 x + 8 r + 4 g .. + 3
+    if (n_tiles > chunk_tiles) {
+        float* part = a.ws + (((size_t)blockIdx.y * gridDim.x + unit) * kManyRows + wave * 32 + i) * kPart<DH>;
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        const float total = sum_groups(l[ct]);
-        if (token(ct) >= q.count) continue;
-        if (split) {
-            float* part = a.ws + (((size_t)blockIdx.y * gridDim.x + unit) * C::rows + (ct * 4 + wave) * 16 + i) * kPart<DH>;
+        for (int x = 0; x < ND; x++)
 #pragma unroll
-            for (int x = 0; x < ND; x++) *(v4f*)(part + 16 * x + 4 * g) = acc[ct][x];
-            if (g == 0) {
-                part[DH] = m[ct];
-                part[DH + 1] = total;
-            }
-        } else {
-            const float f = total == 0.0f ? 0.0f : 1.0f / total;
-            T* out = (T*)a.out.data + row_of(a.out, ct);
-#pragma unroll
-            for (int x = 0; x < ND; x++) store4(out + 16 * x + 4 * g, acc[ct][x] * f, vec);
+            for (int r = 0; r < 4; r++)
+                *(v4f*)(part + 32 * x + 8 * r + 4 * g) = v4f{acc[x][4 * r], acc[x][4 * r + 1], acc[x][4 * r + 2], acc[x][4 * r + 3]};
+        if (g == 0) {
+            part[DH] = m;
+            part[DH + 1] = total;
         }
+    } else {
+        const float f = total == 0.0f ? 0.0f : 1.0f / total;
+        T* out = (T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head;
+#pragma unroll
+        for (int x = 0; x < ND; x++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                store4(out + 32 * x + 8 * r + 4 * g, v4f{acc[x][4 * r], acc[x][4 * r + 1], acc[x][4 * r + 2], acc[x][4 * r + 3]} * f, vec);
     }
 }
 
@@ -1174,7 +1153,7 @@ AttnPlan attn_plan(const KvAttnArgs& a) {
     p.many = rows > (getenv("KVX") ? atoi(getenv("KVX")) : 16);
     // heads a wave takes together: as many as give it 8 rows or fewer
     p.hb = rows * most <= kRows && a.c.heads % most == 0 ? most : rows * 2 <= kRows && a.c.heads % 2 == 0 ? 2 : 1;
-    p.per = p.many ? (a.type == REAL_F32 ? Chunk<32, float>::rows : Chunk<32, __bf16>::rows) : kRows;
+    p.per = p.many ? kManyRows : kRows;
     p.row_tiles = (rows + p.per - 1) / p.per;
     p.units = a.c.n * (a.c.heads / p.hb) * p.row_tiles;
     // tiles that a row tile can see, at most: the sinks', and the window's (or the ring's), with the ends of three runs
@@ -1220,14 +1199,8 @@ hipError_t launch_kv_write(const KvRowsArgs& a, hipStream_t s) { return launch_r
 hipError_t launch_kv_read(const KvRowsArgs& a, hipStream_t s) { return launch_rows<true>(a, s); }
 
 size_t kv_attention_ws_bytes(const KvAttnArgs& a) {
-    size_t most = 0;
-    for (const int type : {REAL_F32, REAL_BF16}) {  // (the same for all types of a call)
-        KvAttnArgs x = a;
-        x.type = type;
-        const AttnPlan p = attn_plan(x);
-        if (p.chunks > 1) most = std::max(most, (size_t)p.chunks * p.units * p.per * (a.c.dh + 4) * 4);
-    }
-    return most;
+    const AttnPlan p = attn_plan(a);
+    return p.chunks > 1 ? (size_t)p.chunks * p.units * p.per * (a.c.dh + 4) * 4 : 0;
 }
 
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {

@@ -119,8 +119,9 @@ def test_decode(heads, group, dh, cap, sinks, window, lens, t):
     p.fill(lens, 7, t=t)
     q = _rows((len(lens), 1, heads * group, dh), 3, t, 2.0)
     p.check(q, np.asarray(lens) - 1, window=window)
-    # an idle sequence, and another scale
-    p.check(q, np.asarray(lens) - [1, 0, 1, 0], [1, 0, 1, 0], window, 0.25)
+    # an idle sequence, and other scales
+    for scale in (0.25, -0.25, 0.0):
+        p.check(q, np.asarray(lens) - [1, 0, 1, 0], [1, 0, 1, 0], window, scale)
 
 
 @pytest.mark.parametrize("dh", [32, 64, 96, 128])
@@ -133,7 +134,9 @@ def test_chunks(dh, t, T, group, sinks, window):
     lens = np.array([T, T + 3, 200 if T < 200 else T])
     counts = np.array([T, T // 2, T])
     p.fill(lens, 11, t=t)
-    p.check(_rows((n, T, heads * group, dh), 5, t, 2.0), lens - counts, counts, window)
+    q = _rows((n, T, heads * group, dh), 5, t, 2.0)
+    for scale in (None, -0.25, 0.0):
+        p.check(q, lens - counts, counts, window, scale)
 
 
 @pytest.mark.parametrize("t", list(P_BITS))
