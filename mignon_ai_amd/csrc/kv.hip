@@ -930,47 +930,59 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
         if (wave < W::KS) lds_load16(codes + j0 * Tile::row, raw0 + slot * Tile::bytes + 1024 * wave);
         if (wave == scale_wave) lds_load4(scales + j0 * W::NB, raw0 + slot * Tile::bytes + Tile::o_scales);
     };
-    // Unpacks a tile. Neighbouring lanes take neighbouring words of a row, of K a word, of V those of two slots.
-    constexpr int words = DH / 8;
+    // Unpacks a tile. Neighbouring lanes take neighbouring words of a row, of K a word, of V those of two slots; where they come from
+    // and go to is found once.
+    constexpr int words = DH / 8, NK = (32 * words + 255) / 256, NV = (16 * words + 255) / 256;
+    int k_to[NK], v_from[NV], v_scale[NV], v_slot[NV], v_to[NV];
+#pragma unroll
+    for (int x = 0; x < NK; x++) {
+        const int n = threadIdx.x + 256 * x, j = n / words, wd = n % words;
+        k_to[x] = U::k_at(wd / 2, U::k_lane(j, wd & 1));
+    }
+#pragma unroll
+    for (int x = 0; x < NV; x++) {
+        const int n = threadIdx.x + 256 * x, j = n / words * 2, wd = n % words;
+        v_from[x] = Tile::half + j * Tile::row + 4 * wd;
+        v_scale[x] = Tile::o_scales + (32 + j) * W::NB + wd / 4;
+        v_slot[x] = j;
+        v_to[x] = U::v_at(wd / 4, j >> 4, U::v_lane(8 * (wd & 3), (j >> 2) & 1)) + 2 * ((j & 3) + (j >> 3 & 1) * 4);
+    }
     auto unpack = [&](auto careful, int raw, int buf, int j0, bool held) {
         const uint8_t* p = smem + o_raw + raw * Tile::bytes;
         uint8_t* out = smem + buf * U::bytes;
-        int at0 = threadIdx.x;
-        asm volatile("" : "+v"(at0));  // (or all of the addresses below are kept in registers)
 #pragma unroll
-        for (int x = 0; x < (32 * words + 255) / 256; x++) {
-            const int at = at0 + 256 * x, j = at / words, wd = at % words;
-            if (32 * words % 256 && at >= 32 * words) break;
-            const uint32_t w = *(const uint32_t*)(p + j * Tile::row + 4 * wd);
-            const float sc = mx4_scale(p[Tile::o_scales + j * W::NB + wd / 4]);
+        for (int x = 0; x < NK; x++) {
+            if (32 * words % 256 && threadIdx.x + 256 * x >= 32 * words) break;
+            const int n = threadIdx.x + 256 * x;  // (words and scales lie in the lanes' order)
+            const uint32_t w = *(const uint32_t*)(p + 4 * n);
+            const float sc = mx4_scale(p[Tile::o_scales + n / 4]);
             u32x4 y;
 #pragma unroll
             for (int b = 0; b < 4; b++) y[b] = unpack2(w, sc, b);
-            *(u32x4*)(out + U::k_at(wd / 2, U::k_lane(j, wd & 1))) = y;
+            *(u32x4*)(out + k_to[x]) = y;
         }
 #pragma unroll
-        for (int x = 0; x < (16 * words + 255) / 256; x++) {
-            const int at = at0 + 256 * x, j = at / words * 2, wd = at % words;
-            if (16 * words % 256 && at >= 16 * words) break;
+        for (int x = 0; x < NV; x++) {
+            if (16 * words % 256 && threadIdx.x + 256 * x >= 16 * words) break;
             uint32_t w[2], sb[2];
 #pragma unroll
             for (int y = 0; y < 2; y++) {
-                w[y] = *(const uint32_t*)(p + Tile::half + (j + y) * Tile::row + 4 * wd);
-                sb[y] = p[Tile::o_scales + (32 + j + y) * W::NB + wd / 4];
+                w[y] = *(const uint32_t*)(p + v_from[x] + y * Tile::row);
+                sb[y] = p[v_scale[x] + y * W::NB];
             }
             if (decltype(careful)::value || !held) {
                 asm volatile("");
 #pragma unroll
                 for (int y = 0; y < 2; y++)
-                    if (!seen.holds(j0 + j + y) || (decltype(careful)::value && sb[y] > 252u)) w[y] = sb[y] = 0;
+                    if (!seen.holds(j0 + v_slot[x] + y) || (decltype(careful)::value && sb[y] > 252u)) w[y] = sb[y] = 0;
             }
-            const int to = U::v_at(wd / 4, j >> 4, U::v_lane(8 * (wd & 3), (j >> 2) & 1)) + 2 * ((j & 3) + (j >> 3 & 1) * 4);
+            const float s0 = mx4_scale(sb[0]), s1 = mx4_scale(sb[1]);
 #pragma unroll
             for (int b = 0; b < 4; b++) {
                 // channels 8 wd + 2 b and the next
-                const uint32_t y0 = unpack2(w[0], mx4_scale(sb[0]), b), y1 = unpack2(w[1], mx4_scale(sb[1]), b);
-                *(uint32_t*)(out + (to ^ (32 * b))) = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
-                *(uint32_t*)(out + (to ^ (32 * b + 16))) = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
+                const uint32_t y0 = unpack2(w[0], s0, b), y1 = unpack2(w[1], s1, b);
+                *(uint32_t*)(out + (v_to[x] ^ (32 * b))) = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
+                *(uint32_t*)(out + (v_to[x] ^ (32 * b + 16))) = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
             }
         }
     };
