@@ -1162,7 +1162,9 @@ struct AttnPlan {
 AttnPlan attn_plan(const KvAttnArgs& a) {
     AttnPlan p;
     const int rows = a.T * a.group, most = a.c.dh == 32 ? 8 : a.c.dh == 64 ? 4 : 2;
-    p.many = rows > (getenv("KVX") ? atoi(getenv("KVX")) : 16);
+    // (32 conversations of 4096 positions, 32 heads of 128 over 8, 24 and 32 rows a head: 88 and 115 us eight rows a wave, 109 us in
+    // both with many; 64 of 2048, fp32 heads of 64: 65 and 84, 93 and 94)
+    p.many = rows > 32;
     // heads a wave takes together: as many as give it 8 rows or fewer
     p.hb = rows * most <= kRows && a.c.heads % most == 0 ? most : rows * 2 <= kRows && a.c.heads % 2 == 0 ? 2 : 1;
     p.per = p.many ? kManyRows : kRows;

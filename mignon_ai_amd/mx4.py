@@ -17,7 +17,8 @@ import numpy as np
 from ._lib import MG_BF16, MG_F16, MG_F32, MG_PTR_DEVICE, KvCache, KvRows, MignonError, check, lib, ptr
 
 _HOST_TYPES = {np.dtype(np.float32): MG_F32, np.dtype(np.float16): MG_F16}
-_device_types = {}
+_torch = None     # (imported with the first call on tensors: the host functions do not need it)
+_reals, _u8, _i32 = {}, None, None
 
 
 def _invalid(msg: str):
@@ -29,43 +30,48 @@ def padded(K: int) -> int:
     return (K + 127) // 128 * 128
 
 
-def _type(t):
-    if not _device_types:
-        import torch
-        _device_types.update({torch.float32: MG_F32, torch.float16: MG_F16, torch.bfloat16: MG_BF16, torch.uint8: -1,
-                              torch.int32: -2})
-    return _device_types.get(t.dtype)
+def _tensors():
+    global _torch, _u8, _i32
+    import torch
+    _reals.update({torch.float32: MG_F32, torch.float16: MG_F16, torch.bfloat16: MG_BF16})
+    _torch, _u8, _i32 = torch, torch.uint8, torch.int32
 
 
 def _launch(who, fn, stream, tensors, args):
     """fn(*args, stream) with the tensors' device as the current one, on `stream` (default: torch's current stream there)."""
-    import torch
     dev = tensors[0].get_device()
     for t in tensors:
         if t.get_device() != dev or dev < 0:
             _invalid(f"{who}: tensors on one GPU are needed")
-    if torch.cuda.current_device() != dev:
-        with torch.cuda.device(dev):
+    if _torch.cuda.current_device() != dev:
+        with _torch.cuda.device(dev):
             return _launch(who, fn, stream, tensors, args)
-    rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
+    rc = fn(*args, _torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
     if rc < 0:
         check(rc)
 
 
 def _real(who, t, name):
-    """The type and row stride of a matrix of reals."""
-    ty = _type(t)
-    if ty is None or ty < 0:
+    """The type, shape and row stride of a matrix of reals."""
+    if _torch is None:
+        _tensors()
+    ty = _reals.get(t.dtype)
+    if ty is None:
         _invalid(f"{who}: {name} is float32, float16 or bfloat16")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        _invalid(f"{who}: {name} is a matrix with neighbouring elements in its rows")
+    if t.dim() != 2:
+        _invalid(f"{who}: {name} is a matrix")
     M, K = t.shape
-    return ty, M, K, t.stride(0) if M > 1 else K
+    ld, one = t.stride()
+    if K > 1 and one != 1:
+        _invalid(f"{who}: {name} has neighbouring elements in its rows")
+    return ty, M, K, ld if M > 1 else K
 
 
 def _rows4(who, codes, scales, name):
     """Rows and padded elements of a 4-bit matrix."""
-    if _type(codes) != -1 or _type(scales) != -1 or codes.dim() != 2 or scales.dim() != 2:
+    if _torch is None:
+        _tensors()
+    if codes.dtype is not _u8 or scales.dtype is not _u8 or codes.dim() != 2 or scales.dim() != 2:
         _invalid(f"{who}: {name}'s codes and scales are uint8 matrices")
     (M, b), (m, s) = codes.shape, scales.shape
     if M != m or b != 16 * s or b % 64 or b == 0 or not codes.is_contiguous() or not scales.is_contiguous():
@@ -141,8 +147,8 @@ def mx4_gemm_device(A, As, W, Ws, C, stream=None):
     """mg_mx4_gemm on torch CUDA tensors: C [M][N] = A W^T (float32, float16 or bfloat16, contiguous)."""
     M, Kp = _rows4("mx4_gemm_device", A, As, "A")
     N, Kw = _rows4("mx4_gemm_device", W, Ws, "W")
-    ty = _type(C)
-    if ty is None or ty < 0 or C.shape != (M, N) or Kp != Kw or not C.is_contiguous():
+    ty = _reals.get(C.dtype)
+    if ty is None or C.shape != (M, N) or Kp != Kw or not C.is_contiguous():
         _invalid("mx4_gemm_device: A [M][K], W [N][K] and a contiguous C [M][N] of reals are needed")
     _launch("mx4_gemm_device", lib().mg_mx4_gemm, stream, (A, As, W, Ws, C),
             (A.data_ptr(), As.data_ptr(), M, Kp, W.data_ptr(), Ws.data_ptr(), N, C.data_ptr(), ty, MG_PTR_DEVICE))
@@ -155,14 +161,16 @@ class KVCache:
 
     def __init__(self, k, k_scales, v, v_scales, sinks: int = 0):
         self.k, self.k_scales, self.v, self.v_scales = k, k_scales, v, v_scales
+        if _torch is None:
+            _tensors()
         for t in (k, k_scales, v, v_scales):
-            if _type(t) != -1 or t.dim() != 4 or not t.is_contiguous() or not t.is_cuda or t.device != k.device:
+            if t.dtype is not _u8 or t.dim() != 4 or not t.is_contiguous() or not t.is_cuda or t.device != k.device:
                 _invalid("KVCache: planes are contiguous uint8 tensors of four dimensions on one GPU")
         n, heads, cap, half = k.shape
         if v.shape != k.shape or k_scales.shape != (n, heads, cap, half // 16) or v_scales.shape != k_scales.shape:
             _invalid("KVCache: codes are [n][heads][capacity][head_dim / 2], scales [n][heads][capacity][head_dim / 32]")
         self.n, self.heads, self.capacity, self.head_dim, self.sinks = n, heads, cap, 2 * half, int(sinks)
-        self.device = k.device
+        self.device, self._shape = k.device, (n,)
         self._c = KvCache(n, heads, 2 * half, cap, self.sinks, k.data_ptr(), k_scales.data_ptr(), v.data_ptr(),
                           v_scales.data_ptr())
         self._p = ctypes.addressof(self._c)
@@ -190,16 +198,17 @@ class KVCache:
         return need
 
     def _rows(self, who, t, name, heads):
-        ty = _type(t)
-        if ty is None or ty < 0 or t.dim() != 4 or t.shape[0] != self.n or t.shape[3] != self.head_dim or t.stride(3) != 1 \
-                or (heads is not None and t.shape[2] != heads):
-            _invalid(f"{who}: {name} is [n][T][heads][head_dim] of float32, float16 or bfloat16, channels side by side")
-        s = t.stride()
-        return ty, KvRows(t.data_ptr(), s[0], s[1], s[2])
+        ty = _reals.get(t.dtype)
+        if ty is not None and t.dim() == 4:
+            n, _, h, d = t.shape
+            seq, token, head, one = t.stride()
+            if n == self.n and d == self.head_dim and one == 1 and (heads is None or h == heads):
+                return ty, KvRows(t.data_ptr(), seq, token, head)
+        _invalid(f"{who}: {name} is [n][T][heads][head_dim] of float32, float16 or bfloat16, channels side by side")
 
     def _ints(self, who, *arrays):
         for a in arrays:
-            if a is not None and (_type(a) != -2 or a.shape != (self.n,) or not a.is_contiguous()):
+            if a is not None and (a.dtype is not _i32 or a.shape != self._shape or not a.is_contiguous()):
                 _invalid(f"{who}: positions, counts and lengths are int32 [n]")
 
     def _two(self, who, k, v, pos, *ints):
