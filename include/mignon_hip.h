@@ -118,6 +118,14 @@ int mg_forward_batch(mg_model* m, const int32_t* ids, int B, int T, float* logit
  * min(max_context, context) when context > 0. State lives in device memory, constant per session. */
 int mg_sessions_create(mg_model* m, int n, int context, mg_sessions** out);
 
+/* No counterpart in the reference: a set whose key and value rings are held in microscaled 4-bit blocks (see mg_kv_write), half a
+ * byte and 1/32 per element instead of three or four, whatever MG_OPT_KV_RINGS says. Keys and values are rounded as they are
+ * written (to within a quarter of the largest of their 32 neighbours, most of them far closer), and decode steps attend over
+ * the rounded ones; prefill attends over the prompt's own, so that the logits after a prompt are those of any set. Steps run
+ * layer by layer or in tiles of 16 sessions, with the attention between. Heads of width 32, 64, 96 or 128;
+ * MG_ERR_UNSUPPORTED otherwise. All mg_sessions_* calls take the set. */
+int mg_sessions_create_mx4(mg_model* m, int n, int context, mg_sessions** out);
+
 /* quantSession.Prefill for every session at once (internal/quant/session.go:30-39): prompts
  * [n][max_len] with lengths lens[n] (1..max_len); prompts longer than the window keep their last
  * window tokens. Outputs describe the next token after each prompt:

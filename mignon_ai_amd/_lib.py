@@ -86,6 +86,7 @@ SIGNATURES = {
     "mg_model_call": (_int, [_vp, _vp, _int, _vp]),
     "mg_forward_batch": (_int, [_vp, _vp, _int, _int, _vp, _vp, _vp, _vp, _int]),
     "mg_sessions_create": (_int, [_vp, _int, _int, ctypes.POINTER(_vp)]),
+    "mg_sessions_create_mx4": (_int, [_vp, _int, _int, ctypes.POINTER(_vp)]),
     "mg_sessions_prefill": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _int]),
     "mg_sessions_step": (_int, [_vp, _vp, _vp, _vp, _vp, _int]),
     "mg_sessions_step_noalloc": (_int, [_vp, _vp, _vp, _vp, _vp]),

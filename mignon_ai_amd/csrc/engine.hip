@@ -287,6 +287,11 @@ struct mg_sessions {
     // kscale/vscale, or fp32 rows
     bool kv_packed = false;
     mg::DevBuf kscale, vscale;
+    // or microscaled 4-bit rows (mg_sessions_create_mx4): codes in kring/vring, scale bytes in kscale/vscale, one cache of
+    // n x heads x kv_cap slots (the ring rounded up to tiles) for every attention block; and the decode attention's workspace
+    bool kv_mx4 = false;
+    int kv_cap = 0;
+    mg::DevBuf kv_ws;
     mg::DevBuf sample_ws;  // the sampler's exponentials and row sums
     // stop-token bookkeeping of mg_sessions_decode_greedy_until: per-session reply length, the stopped
     // count, and a ring of pinned host slots the count is copied to after each step (one event each)
@@ -347,6 +352,53 @@ bool kv_rings_packed(const mg_model* m, int n) {
     AttnStepArgs a;
     a.S = 1; a.D = m->D; a.Dp = m->Dp; a.heads = m->heads; a.window = m->window; a.cap = m->cap;
     return attention_step_rows_fits(a);
+}
+
+// The 4-bit cache of attention block ab of a set. A step writes and attends in two launches and puts the output's limbs in a
+// third, where the other formats take one: that costs small sets (16 sessions of two blocks of 4 heads of 32 and 64 slots: 48 ->
+// 89 us a step, most of it the lost one-workgroup step), and 4096 sessions gain what their rings are smaller by (three blocks of
+// 8 heads of 32: 411 -> 271 us; four of 6 heads of 64: 1299 -> 824).
+KvCache mx4_cache(mg_sessions* s, int ab) {
+    const mg_model* m = s->m;
+    KvCache c;
+    c.n = s->n; c.heads = m->heads; c.dh = m->D / m->heads; c.cap = s->kv_cap;
+    const size_t rows = (size_t)ab * s->n * m->heads * s->kv_cap;
+    c.k = s->kring.as<uint8_t>() + rows * (c.dh / 2); c.ks = s->kscale.as<uint8_t>() + rows * (c.dh / 32);
+    c.v = s->vring.as<uint8_t>() + rows * (c.dh / 2); c.vs = s->vscale.as<uint8_t>() + rows * (c.dh / 32);
+    return c;
+}
+
+// Rows of q, k or v (which = 0, 1, 2) in the projection's output [n][T][3 D].
+KvRows qkv_rows(const mg_model* m, const float* qkv, int T, int which) {
+    KvRows r;
+    r.data = const_cast<float*>(qkv) + (size_t)which * m->D;
+    r.seq = 3LL * m->D * T; r.token = 3LL * m->D; r.head = m->D / m->heads;
+    return r;
+}
+
+// Writes the keys and values of T tokens a session (lens[i] of them; null: T) from position pos[i] (null: 0) on.
+void mx4_write(mg_sessions* s, int ab, const float* qkv, int T, const int32_t* pos, const int32_t* lens, hipStream_t st) {
+    KvRowsArgs a;
+    a.c = mx4_cache(s, ab); a.T = T; a.pos = pos; a.counts = lens;
+    a.k = qkv_rows(s->m, qkv, T, 1); a.v = qkv_rows(s->m, qkv, T, 2);
+    HIPCHECK(launch_kv_write(a, st));
+}
+
+// One decode position's attention for every session into att [n][Dp], its key and value written before.
+KvAttnArgs mx4_attention(mg_sessions* s, int ab, const float* qkv, float* att) {
+    const mg_model* m = s->m;
+    KvAttnArgs a;
+    a.c = mx4_cache(s, ab); a.T = 1; a.pos = s->pos.as<int32_t>();
+    a.q = qkv_rows(m, qkv, 1, 0);
+    a.out.data = att; a.out.seq = a.out.token = m->Dp; a.out.head = m->D / m->heads;
+    a.window = m->window > 0 ? std::min(m->window, m->cap) : m->cap;
+    a.scale = 1.0f / std::sqrt((float)(m->D / m->heads));
+    a.ws = s->kv_ws.as<float>();
+    return a;
+}
+void mx4_attend(mg_sessions* s, int ab, const float* qkv, float* att, hipStream_t st) {
+    mx4_write(s, ab, qkv, 1, s->pos.as<int32_t>(), nullptr, st);
+    HIPCHECK(launch_kv_attention(mx4_attention(s, ab, qkv, att), st));
 }
 
 // The K/V rings of attention block ab of a set: packed words and scales, or fp32 rows.
@@ -1005,7 +1057,10 @@ void run_body(mg_model* m, const BodyCtx& c, hipStream_t s) {
             } else {
                 gemm(m, EPI_F32, g, s);
             }
-            if (!fused && c.step) {
+            if (!fused && c.step && c.sess->kv_mx4) {
+                ProfScope ps(m->prof, K_ATTN_STEP, s);
+                mx4_attend(c.sess, ab, w.qkv.as<float>(), w.att.as<float>(), s);
+            } else if (!fused && c.step) {
                 AttnStepArgs aa;
                 aa.S = M; aa.D = D; aa.Dp = Dp; aa.heads = m->heads; aa.window = m->window; aa.cap = m->cap;
                 aa.pos = c.sess->pos.as<int32_t>(); aa.qkv = w.qkv.as<float>();
@@ -1025,7 +1080,9 @@ void run_body(mg_model* m, const BodyCtx& c, hipStream_t s) {
                     ProfScope ps(m->prof, K_EXPORT, s);
                     AttnStepArgs r;
                     ring_args(c.sess, ab, r);
-                    if (c.sess->kv_packed)
+                    if (c.sess->kv_mx4)
+                        mx4_write(c.sess, ab, w.qkv.as<float>(), c.T, nullptr, c.lens, s);
+                    else if (c.sess->kv_packed)
                         HIPCHECK(launch_export_kv_packed(c.B, c.T, D, m->heads, m->cap, c.lens, w.qkv.as<float>(),
                                                          r.kpack, r.vpack, r.kscale, r.vscale, s, c.row0));
                     else
@@ -1787,11 +1844,53 @@ void clear_sessions(mg_sessions* s) {
     HIPCHECK(launch_fill_f32(s->g.as<float>(), (long long)(s->g.n / 4), 0.0f, m->stream));
     HIPCHECK(launch_fill_f32(s->kring.as<float>(), (long long)(s->kring.n / 4), 0.0f, m->stream));
     HIPCHECK(launch_fill_f32(s->vring.as<float>(), (long long)(s->vring.n / 4), 0.0f, m->stream));
+    if (s->kv_mx4) {
+        HIPCHECK(launch_fill_f32(s->kscale.as<float>(), (long long)(s->kscale.n / 4), 0.0f, m->stream));
+        HIPCHECK(launch_fill_f32(s->vscale.as<float>(), (long long)(s->vscale.n / 4), 0.0f, m->stream));
+    }
     if (s->kv_packed) {  // zero words decode to zero under any scale; the scales start at 1
         HIPCHECK(launch_fill_f32(s->kscale.as<float>(), (long long)(s->kscale.n / 4), 1.0f, m->stream));
         HIPCHECK(launch_fill_f32(s->vscale.as<float>(), (long long)(s->vscale.n / 4), 1.0f, m->stream));
     }
     HIPCHECK(launch_fill_i32(s->pos.as<int32_t>(), s->n, 0, m->stream));
+}
+
+int create_sessions(mg_model* m, int n, int context, bool mx4, mg_sessions** out) {
+    *out = nullptr;
+    Guard gd(m);
+    std::unique_ptr<mg_sessions> s(new mg_sessions());
+    s->m = m;
+    s->n = n;
+    s->window = (context > 0 && context < m->max_context) ? context : m->max_context;
+    const size_t Dp = m->Dp, D = m->D;
+    s->norm_ring.ensure(std::max<size_t>(16, (size_t)m->nbs * n * m->ring * Dp * 4));
+    s->g.ensure(std::max<size_t>(16, (size_t)m->nbs * n * Dp * 4));
+    s->kv_mx4 = mx4 && m->nattn > 0;
+    s->kv_packed = !s->kv_mx4 && kv_rings_packed(m, n);
+    if (s->kv_mx4) {
+        s->kv_cap = round_up(m->cap, 32);
+        const size_t rows = (size_t)m->nattn * n * s->kv_cap * D;
+        s->kring.ensure(rows / 2);
+        s->vring.ensure(rows / 2);
+        s->kscale.ensure(rows / 32);
+        s->vscale.ensure(rows / 32);
+        s->kv_ws.ensure(kv_attention_ws_bytes(mx4_attention(s.get(), 0, nullptr, nullptr)));
+    } else {
+        // packed: 3 bytes per element and a 4-byte scale per (head, slot) row; fp32: 4 bytes per element
+        const size_t ring_bytes = (size_t)m->nattn * n * m->cap * D * (s->kv_packed ? 3 : 4);
+        s->kring.ensure(std::max<size_t>(16, ring_bytes));
+        s->vring.ensure(std::max<size_t>(16, ring_bytes));
+    }
+    if (s->kv_packed) {
+        s->kscale.ensure(std::max<size_t>(16, (size_t)m->nattn * n * m->heads * m->cap * 4));
+        s->vscale.ensure(std::max<size_t>(16, (size_t)m->nattn * n * m->heads * m->cap * 4));
+    }
+    s->pos.ensure((size_t)n * 4);
+    s->next_ids.ensure((size_t)n * 4);
+    clear_sessions(s.get());
+    HIPCHECK(hipStreamSynchronize(m->stream));
+    *out = s.release();
+    return MG_OK;
 }
 
 }  // namespace
@@ -1800,30 +1899,19 @@ int mg_sessions_create(mg_model* m, int n, int context, mg_sessions** out) {
     return guarded([&] {
         require(m && out, "mg_sessions_create: null argument");
         require(n > 0, "mg_sessions_create: n must be positive");
-        *out = nullptr;
-        Guard gd(m);
-        std::unique_ptr<mg_sessions> s(new mg_sessions());
-        s->m = m;
-        s->n = n;
-        s->window = (context > 0 && context < m->max_context) ? context : m->max_context;
-        const size_t Dp = m->Dp, D = m->D;
-        s->norm_ring.ensure(std::max<size_t>(16, (size_t)m->nbs * n * m->ring * Dp * 4));
-        s->g.ensure(std::max<size_t>(16, (size_t)m->nbs * n * Dp * 4));
-        s->kv_packed = kv_rings_packed(m, n);
-        // packed: 3 bytes per element and a 4-byte scale per (head, slot) row; fp32: 4 bytes per element
-        const size_t ring_bytes = (size_t)m->nattn * n * m->cap * D * (s->kv_packed ? 3 : 4);
-        s->kring.ensure(std::max<size_t>(16, ring_bytes));
-        s->vring.ensure(std::max<size_t>(16, ring_bytes));
-        if (s->kv_packed) {
-            s->kscale.ensure(std::max<size_t>(16, (size_t)m->nattn * n * m->heads * m->cap * 4));
-            s->vscale.ensure(std::max<size_t>(16, (size_t)m->nattn * n * m->heads * m->cap * 4));
-        }
-        s->pos.ensure((size_t)n * 4);
-        s->next_ids.ensure((size_t)n * 4);
-        clear_sessions(s.get());
-        HIPCHECK(hipStreamSynchronize(m->stream));
-        *out = s.release();
-        return MG_OK;
+        return create_sessions(m, n, context, false, out);
+    });
+}
+
+int mg_sessions_create_mx4(mg_model* m, int n, int context, mg_sessions** out) {
+    return guarded([&] {
+        require(m && out, "mg_sessions_create_mx4: null argument");
+        require(n > 0, "mg_sessions_create_mx4: n must be positive");
+        if (m->nattn > 0 && !kv_head_width(m->D / m->heads))
+            throw Error(MG_ERR_UNSUPPORTED, "mg_sessions_create_mx4: attention heads of width " + std::to_string(m->D / m->heads) +
+                                                " (32, 64, 96 and 128 are there)");
+        require((long long)n * m->max_context * std::max(m->heads, 1) < (1LL << 31), "mg_sessions_create_mx4: too many rows");
+        return create_sessions(m, n, context, true, out);
     });
 }
 
@@ -1892,8 +1980,9 @@ void prefill_device(mg_sessions* s, const int32_t* prompts_d, const int32_t* len
     w.tmp.ensure((size_t)S * Tw * 4);
     int32_t* ids_w = w.tmp.as<int32_t>();
     int32_t* lens_w = w.lens.as<int32_t>();
-    const bool seq = seq_usable(m, S, Tw);
-    const int packed = seq ? 0 : prefill_packed_rows(m, S, max_len, Tw, lens_h, s->window);
+    // (rows of a 4-bit cache are written from the layered kernels' rows, one prompt as long as the other)
+    const bool seq = !s->kv_mx4 && seq_usable(m, S, Tw);
+    const int packed = seq || s->kv_mx4 ? 0 : prefill_packed_rows(m, S, max_len, Tw, lens_h, s->window);
     int32_t* row0 = packed ? w.tgt.as<int32_t>() : nullptr;  // (no targets in a prefill)
     if (packed) {
         hipLaunchKernelGGL(pack_rows_kernel, dim3(1), dim3(1024), 0, st, S, max_len, s->window, lens_d, row0);
@@ -1947,6 +2036,7 @@ bool step1_args_fill(mg_sessions* s, const int32_t* ids_d, float* logits_d, cons
 bool step1_args(mg_sessions* s, const int32_t* ids_d, float* logits_d, const HeadCombineArgs& hc, Step1Args& a) {
     mg_model* m = s->m;
     const int mode = option(OPT_STEP_KERNEL);
+    if (s->kv_mx4) return false;  // (its attention reads the other ring formats)
     if (mode == 1 || mode == 3 || (mode == 0 && s->n > kStep1MaxSessions) || !m->s1blocks) return false;
     return step1_args_fill(s, ids_d, logits_d, hc, a) && step1_fits(a);
 }
@@ -2006,7 +2096,7 @@ bool tile_args(mg_sessions* s, const int32_t* ids_d, float* logits_d, const Head
     if (!(mode == 3 || mode == 0) || !m->s1blocks) return false;
     Step1Args& b = a;
     if (!step1_args_fill(s, ids_d, logits_d, hc, b)) return false;
-    if (m->nattn && !attention_step_rows_fits(step_attn_args(s, 0))) return false;
+    if (m->nattn && !s->kv_mx4 && !attention_step_rows_fits(step_attn_args(s, 0))) return false;
     return tile_step_fits(a);
 }
 
@@ -2039,8 +2129,14 @@ void step_device(mg_sessions* s, const int32_t* ids_d, float* logits_d, HeadComb
             int next = ta.seg_out ? ta.seg_block + 1 : ta.seg_block;
             while (next < (int)m->blocks.size() && !m->blocks[next].attn) next++;
             if (next >= (int)m->blocks.size()) break;
-            {
-                // the segment ended with block next's projection: its attention, output limbs to w.nl/w.ns
+            // the segment ended with block next's projection: its attention, output limbs to w.nl/w.ns
+            if (s->kv_mx4) {
+                {
+                    ProfScope ps(m->prof, K_ATTN_STEP, st);
+                    mx4_attend(s, ab, w.qkv.as<float>(), w.att.as<float>(), st);
+                }
+                row_call(m, S, ROW_SRC, nullptr, w.att.as<float>(), m->Dp, nullptr, nullptr, nullptr, true, st);
+            } else {
                 AttnStepArgs aa = step_attn_args(s, ab);
                 aa.done = hc.done;
                 ProfScope ps(m->prof, K_ATTN_STEP, st);
@@ -2468,6 +2564,9 @@ long long mg_sessions_device_bytes(const mg_sessions* s) {
     if (!s) return -1;
     const mg_model* m = s->m;
     // packed rings: 3 bytes per element and a 4-byte scale per (head, slot) row of each ring
+    // 4-bit: half a byte per element and a byte per 32
+    if (s->kv_mx4)
+        return (long long)m->nbs * (m->ring + 1) * m->Dp * 4 + (long long)m->nattn * 2 * s->kv_cap * (m->D / 2 + m->D / 32) + 8;
     const long long rings = s->kv_packed ? (long long)m->nattn * 2 * m->cap * ((long long)m->D * 3 + m->heads * 4)
                                          : (long long)m->nattn * 2 * m->cap * m->D * 4;
     return (long long)m->nbs * (m->ring + 1) * m->Dp * 4 + rings + 8;

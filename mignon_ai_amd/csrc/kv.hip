@@ -21,7 +21,7 @@ struct SeqSpan {
 };
 __device__ __forceinline__ SeqSpan seq_span(const int32_t* pos, const int32_t* counts, int s, int T) {
     SeqSpan r;
-    r.pos = min(max(pos[s], -kKvMaxPos), kKvMaxPos);
+    r.pos = pos ? min(max(pos[s], -kKvMaxPos), kKvMaxPos) : 0;
     r.count = counts ? min(max(counts[s], 0), T) : T;
     r.end = r.pos + r.count;
     return r;

@@ -48,7 +48,7 @@ struct KvCache {
     uint8_t* v = nullptr;
     uint8_t* vs = nullptr;
 };
-// Token t < counts[s] (null: T) of sequence s sits at position pos[s] + t.
+// Token t < counts[s] (null: T) of sequence s sits at position pos[s] (null: 0) + t.
 struct KvRowsArgs {
     KvCache c;
     KvRows k, v;

@@ -142,15 +142,19 @@ class Model:
     def new_session(self, context_size: int = 0) -> "Session":
         return Session(self, context_size)
 
-    def sessions(self, n: int, context_size: int = 0) -> "Sessions":
-        return Sessions(self, n, context_size)
+    def sessions(self, n: int, context_size: int = 0, kv: str | None = None) -> "Sessions":
+        """kv: None (the ring format of engine_option("kv_rings")) or "mx4" (4-bit rings, mg_sessions_create_mx4)."""
+        return Sessions(self, n, context_size, kv)
 
 
 class Sessions:
-    def __init__(self, model: Model, n: int, context_size: int = 0):
+    def __init__(self, model: Model, n: int, context_size: int = 0, kv: str | None = None):
         self.model = model
+        if kv not in (None, "mx4"):
+            raise ValueError(f"kv is None or \"mx4\", not {kv!r}")
         h = ctypes.c_void_p()
-        check(lib().mg_sessions_create(model.handle, int(n), int(context_size), ctypes.byref(h)))
+        create = lib().mg_sessions_create if kv is None else lib().mg_sessions_create_mx4
+        check(create(model.handle, int(n), int(context_size), ctypes.byref(h)))
         self._h = h
         self.n = n
 
