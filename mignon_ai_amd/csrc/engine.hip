@@ -1312,6 +1312,7 @@ bool kv_attention_args(const char* who, const mg_kv_cache_t* c, int q_heads, int
     REQUIRE((long long)c->n * T * q_heads < (1LL << 31), std::string(who) + ": too many rows");
     a.T = T; a.group = q_heads / c->heads;
     a.window = window >= kKvMaxPos ? 0 : std::max(window, 0);  // positions are below kKvMaxPos: such a window hides nothing
+    REQUIRE(kv_attention_fits(a), std::string(who) + ": too many rows");
     return true;
 }
 

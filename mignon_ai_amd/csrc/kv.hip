@@ -1241,6 +1241,11 @@ size_t kv_attention_ws_bytes(const KvAttnArgs& a) {
     return p.chunks > 1 ? (size_t)p.chunks * p.units * p.per * (a.c.dh + 4) * 4 : 0;
 }
 
+bool kv_attention_fits(const KvAttnArgs& a) {
+    const AttnPlan p = attn_plan(a);
+    return (p.waves == 1 ? (p.units + 3) / 4 : p.units) < 1 << 24;  // a launch's 2^32 lanes
+}
+
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
     const AttnPlan p = attn_plan(a);
     const int vec = rows_aligned(a.q, a.type) && rows_aligned(a.out, a.type);

@@ -73,6 +73,7 @@ struct KvAttnArgs {
 constexpr int kKvMaxPos = 1 << 30;
 bool kv_head_width(int dh);       // 32, 64, 96 or 128
 size_t kv_attention_ws_bytes(const KvAttnArgs& a);
+bool kv_attention_fits(const KvAttnArgs& a);  // a launch takes it
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s);
 
 }  // namespace mg

@@ -62,8 +62,8 @@ def _real(who, t, name):
         _invalid(f"{who}: {name} is a matrix")
     M, K = t.shape
     ld, one = t.stride()
-    if K > 1 and one != 1:
-        _invalid(f"{who}: {name} has neighbouring elements in its rows")
+    if (K > 1 and one != 1) or M >> 31 or K >> 31:
+        _invalid(f"{who}: {name} has neighbouring elements in its rows, and fewer than 2^31 each way")
     return ty, M, K, ld if M > 1 else K
 
 
@@ -74,7 +74,7 @@ def _rows4(who, codes, scales, name):
     if codes.dtype is not _u8 or scales.dtype is not _u8 or codes.dim() != 2 or scales.dim() != 2:
         _invalid(f"{who}: {name}'s codes and scales are uint8 matrices")
     (M, b), (m, s) = codes.shape, scales.shape
-    if M != m or b != 16 * s or b % 64 or b == 0 or not codes.is_contiguous() or not scales.is_contiguous():
+    if M != m or b != 16 * s or b % 64 or b == 0 or M >> 31 or b >> 30 or not codes.is_contiguous() or not scales.is_contiguous():
         _invalid(f"{who}: {name}'s codes are [M][Kp / 2] and its scales [M][Kp / 32], contiguous, Kp a multiple of 128")
     return M, 2 * b
 
@@ -167,13 +167,15 @@ class KVCache:
             if t.dtype is not _u8 or t.dim() != 4 or not t.is_contiguous() or not t.is_cuda or t.device != k.device:
                 _invalid("KVCache: planes are contiguous uint8 tensors of four dimensions on one GPU")
         n, heads, cap, half = k.shape
+        if max(k.shape) >> 30 or not 0 <= int(sinks) < max(cap, 1):
+            _invalid("KVCache: fewer than 2^30 each way, and sinks fewer than the capacity")
         if v.shape != k.shape or k_scales.shape != (n, heads, cap, half // 16) or v_scales.shape != k_scales.shape:
             _invalid("KVCache: codes are [n][heads][capacity][head_dim / 2], scales [n][heads][capacity][head_dim / 32]")
         self.n, self.heads, self.capacity, self.head_dim, self.sinks = n, heads, cap, 2 * half, int(sinks)
         self.device, self._shape = k.device, (n,)
         self._c = KvCache(n, heads, 2 * half, cap, self.sinks, k.data_ptr(), k_scales.data_ptr(), v.data_ptr(),
                           v_scales.data_ptr())
-        self._p = ctypes.addressof(self._c)
+        self._p, self._planes = ctypes.addressof(self._c), (k, k_scales, v, v_scales)
         self._need = {}
         self._workspace(heads, 1, 0)  # refuses what the calls would refuse
 
@@ -200,9 +202,9 @@ class KVCache:
     def _rows(self, who, t, name, heads):
         ty = _reals.get(t.dtype)
         if ty is not None and t.dim() == 4:
-            n, _, h, d = t.shape
+            n, T, h, d = t.shape
             seq, token, head, one = t.stride()
-            if n == self.n and d == self.head_dim and one == 1 and (heads is None or h == heads):
+            if n == self.n and d == self.head_dim and one == 1 and (h == heads if heads else h < 1 << 30) and T < 1 << 30:
                 return ty, KvRows(t.data_ptr(), seq, token, head)
         _invalid(f"{who}: {name} is [n][T][heads][head_dim] of float32, float16 or bfloat16, channels side by side")
 
@@ -222,14 +224,14 @@ class KVCache:
         """mg_kv_write: new rows k, v [n][T][heads][head_dim] (any strides but the last) at positions pos[s] + t, of which the
         first counts[s] (default T) are there. pos, counts: int32 [n]."""
         ty, kr, vr = self._two("KVCache.write", k, v, pos, counts)
-        _launch("KVCache.write", lib().mg_kv_write, None, (self.k, k, v, pos) + (() if counts is None else (counts,)),
+        _launch("KVCache.write", lib().mg_kv_write, None, (self._planes[0], k, v, pos) + (() if counts is None else (counts,)),
                 (self._p, ctypes.addressof(kr), ctypes.addressof(vr), ty, k.shape[1], pos.data_ptr(), ptr(counts)))
 
     def read(self, k, v, pos, counts=None, lens=None):
         """mg_kv_read: the rows at positions pos[s] + t into k, v; lens [n]: the sequences' lengths (default pos + counts)."""
         ty, kr, vr = self._two("KVCache.read", k, v, pos, counts, lens)
         more = tuple(a for a in (counts, lens) if a is not None)
-        _launch("KVCache.read", lib().mg_kv_read, None, (self.k, k, v, pos) + more,
+        _launch("KVCache.read", lib().mg_kv_read, None, (self._planes[0], k, v, pos) + more,
                 (self._p, ctypes.addressof(kr), ctypes.addressof(vr), ty, k.shape[1], pos.data_ptr(), ptr(counts), ptr(lens)))
 
     def attention(self, q, out, pos, counts=None, window: int = 0, scale: float | None = None):
@@ -240,10 +242,10 @@ class KVCache:
         if ty != to or q.shape != out.shape or pos is None:
             _invalid("KVCache.attention: q and out have one shape and type, and positions are given")
         self._ints("KVCache.attention", pos, counts)
-        T, q_heads = q.shape[1], q.shape[2]
+        T, q_heads, window = q.shape[1], q.shape[2], min(max(int(window), 0), 1 << 30)
         need = self._workspace(q_heads, T, window)
-        ws = self.k.new_empty(need) if need else None
-        _launch("KVCache.attention", lib().mg_kv_attention, None, (self.k, q, out, pos) + (() if counts is None else (counts,)),
+        ws = self._planes[0].new_empty(need) if need else None
+        _launch("KVCache.attention", lib().mg_kv_attention, None, (self._planes[0], q, out, pos) + (() if counts is None else (counts,)),
                 (self._p, ctypes.addressof(qr), ctypes.addressof(orow), ty, q_heads, T, pos.data_ptr(), ptr(counts), window,
                  self.head_dim ** -0.5 if scale is None else scale, ptr(ws), need))
         return out

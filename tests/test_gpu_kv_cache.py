@@ -324,3 +324,35 @@ def test_refusals():
                 lambda: c.attention(q.double(), q.double(), pos), lambda: c.attention(q, torch.zeros((2, 1, 4, 64), device="cuda"), pos)):
         with pytest.raises(MignonError):
             bad()
+
+
+def test_sizes_that_the_interface_cannot_hold_are_refused():
+    """Shapes of tensors that stand for more elements than they have, and windows past 32 bits."""
+    c = KVCache.empty(1, 2, 32, 64)
+    wide = torch.zeros(1, 1, 2, 32, device="cuda").expand(1, (1 << 32) + 1, 2, 32)
+    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for call in (lambda: c.write(wide, wide, pos), lambda: c.read(wide, wide, pos), lambda: c.attention(wide, wide, pos)):
+        with pytest.raises(MignonError):
+            call()
+    for sinks in (-1, 64, (1 << 32) + 1):
+        with pytest.raises(MignonError):
+            KVCache.empty(1, 2, 32, 64, sinks=sinks)
+    x = torch.randn(1, 40, 2, 32, device="cuda")
+    c.write(x, x, pos)
+    q = torch.randn(1, 40, 2, 32, device="cuda")
+    whole = c.attention(q, torch.empty_like(q), pos)
+    for window in ((1 << 32) + 1, 1 << 31, -(1 << 33), np.int64(40)):
+        assert torch.equal(c.attention(q, torch.empty_like(q), pos, window=window), whole)
+
+
+def test_a_cache_keeps_its_planes():
+    """The tensors a cache was made of live as long as it, whatever becomes of its attributes."""
+    c, d = KVCache.empty(1, 2, 32, 64), KVCache.empty(1, 2, 32, 64)
+    x = torch.randn(1, 3, 2, 32, device="cuda")
+    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+    c.write(x, x, pos)
+    d.write(x, x, pos)
+    c.k = c.v = None
+    junk = [torch.full((1, 2, 64, 16), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    assert torch.equal(c.attention(x, torch.empty_like(x), pos), d.attention(x, torch.empty_like(x), pos))
+    del junk

@@ -79,3 +79,11 @@ def test_call_refusals():
     # nothing to do
     assert L.mg_kv_write(a(_cache(n=0)), a(r), a(r), 0, 1, p, None, None) == 0
     assert L.mg_kv_attention(a(c), a(r), a(r), 0, 4, 0, p, None, 0, 1.0, None, 0, None) == 0
+
+
+def test_calls_of_more_rows_than_a_launch_has_lanes():
+    L, a = _lib.lib(), ctypes.addressof
+    assert L.mg_kv_attention_workspace(a(_cache(n=1 << 25, heads=1)), 1, 1, 0) == 0  # a wave a sequence, four a workgroup
+    assert L.mg_kv_attention_workspace(a(_cache(n=1 << 26, heads=1)), 1, 1, 0) == INVALID
+    assert L.mg_kv_attention_workspace(a(_cache(n=(1 << 24) - 1, heads=1, capacity=4096)), 1, 1, 0) == 0  # a workgroup a sequence
+    assert L.mg_kv_attention_workspace(a(_cache(n=1 << 24, heads=1, capacity=4096)), 1, 1, 0) == INVALID
