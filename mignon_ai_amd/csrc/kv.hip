@@ -32,7 +32,9 @@ __device__ __forceinline__ int kv_slot(int p, int sinks, int ring) { return p < 
 // One launch for keys and values (blockIdx.z), a workgroup for 256 / (DH / 8) tokens of U heads (blockIdx.y): DH / 8 lanes a row, four
 // to a block, a lane's U rows loaded before the first is worked on. Tokens that follow each other fill whole lines of codes and
 // scales, and a token's heads are read side by side (32768 tokens of 8 bf16 heads of 128 written: one head a
-// workgroup 53 us, four 44; read back 28 and 27).
+// workgroup 53 us, four 44; read back 28 and 27). Bound by memory: 16 prompts of 1 to 2048 such tokens, 55 MB each way, 16.6 us
+// (3.3 TB/s) and 13 (4.2); a decode step's 4096 tokens of 8 fp32 heads of 32 take 4.9 and 5.7 us, the latency of position, row and
+// store after each other.
 struct RowsSpot {
     int s, t, slot;  // slot -1: nothing there (a write: no row; a read: zeros), t -1: no row
 };
@@ -619,6 +621,12 @@ struct Stages {
 // query heads, token after token), or, with HB > 1, all rows of HB heads (8 or fewer). Tiles come straight into the wave's own
 // LDS stages, up to three ahead. WAVES waves share the tiles (of one chunk of them, where there are several) and add up what
 // they have in LDS; with WAVES 1 a wave is alone with its rows.
+//
+// Bound by reading the cache, with the unpacking close behind. 32 conversations of 16384 positions (8 heads of 128, four query
+// heads each, bf16): 5.8 TB/s; of 1 to 16384 positions, 276 MB, 72 us with the join (3.8 TB/s: the lengths do not divide evenly
+// over the chip); 256 windows of 1000 (8 heads of 64, two query heads each, fp16, 109 MB) 29 us; 4096 windows of 64 (8 fp32 heads
+// of 32, 57 MB) 24 us, where a wave's life is mostly its first tiles' latency; one conversation of 30000 (33 MB) 18 us with the
+// join, the latency of a chunk's sixteen tiles and of a second launch.
 template <int DH, class T, int HB, int WAVES>
 __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
     using W = Width<DH>;
@@ -845,7 +853,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a,
 }
 
 // Joins the chunks of a row that took more than one: a wave a row, its lanes over channels (four each) and, in as many groups as fit,
-// over the chunks, whose sums are added in a fixed order. Units have `per` rows.
+// over the chunks, whose sums are added in a fixed order. Units have `per` rows. (4.6 us for 32 conversations of 32 query heads, 6 for
+// the 59 chunks of one long one: its latency.)
 template <int DH, class T>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int per, int hb, int row_tiles, int chunk_tiles, int vec) {
     constexpr int LC = DH / 4, G = 64 / LC;  // lanes a group, groups
@@ -904,6 +913,11 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, in
 // fragments 2 d and 2 d + 1, channel 32 d + i, entries r < 8 and r >= 8. The places are exchanged (XOR of the low three bits of a
 // lane's place) so that the writes of unpacking and the reads of the products do not meet in a bank: of K's fragment s by g and
 // 2 (s & 3), of V's by 4 g and d & 3.
+//
+// Bound by issuing instructions: 2 x 1024 tokens of 32 query heads over 8 of 128 with 6000 positions in sight, bf16: 273 us, 421
+// TFLOP/s of scores and output (the output's products are done twice, for the probabilities' two parts; a quarter of the time is
+// matrix units', somewhat over half of all cycles issue something). With one part, probabilities held to 8 bits, 252 against 291
+// us then, and an error of 2.0e-3 instead of 1.7e-3 of bf16 outputs: not taken.
 template <int DH>
 struct Unpacked {
     static constexpr int k = 64 * DH, bytes = 2 * k;
@@ -946,9 +960,9 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
     constexpr int scale_wave = W::KS & 3;
     const size_t plane = (size_t)pair * a.c.cap;
     const uint32_t raw0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)(smem + o_raw);
-    const int code_at = 1024 * wave + 16 * lane, scale_at_ = min(4 * (W::NB == 3 ? lane : lane & (16 * W::NB - 1)), 64 * W::NB - 4);
+    const int code_at = 1024 * wave + 16 * lane, scales_from = min(4 * (W::NB == 3 ? lane : lane & (16 * W::NB - 1)), 64 * W::NB - 4);
     const uint8_t* codes = code_at < Tile::half ? a.c.k + plane * Tile::row + code_at : a.c.v + plane * Tile::row + code_at - Tile::half;
-    const uint8_t* scales = scale_at_ < 32 * W::NB ? a.c.ks + plane * W::NB + scale_at_ : a.c.vs + plane * W::NB + scale_at_ - 32 * W::NB;
+    const uint8_t* scales = scales_from < 32 * W::NB ? a.c.ks + plane * W::NB + scales_from : a.c.vs + plane * W::NB + scales_from - 32 * W::NB;
     auto fetch = [&](int o, int slot) {
         const size_t j0 = tl.at(o) * kTile;
         if (wave < W::KS) lds_load16(codes + j0 * Tile::row, raw0 + slot * Tile::bytes + 1024 * wave);
