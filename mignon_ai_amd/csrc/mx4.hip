@@ -216,28 +216,30 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_split_kernel(Mx4GemmArgs 
 
 // ---- Large products ----
 // A workgroup of WN x WM waves computes TN channels x TM rows, each wave its FN x FM fragments of 16 x 16, in steps of 128
-// elements of K. A step's codes come into one of four LDS slots, three steps ahead; the scales of four steps (16 bytes a row)
-// come at once into one of two. What the loads cost is lines touched, not bytes: four neighbouring lanes take the 64 bytes of
-// a row. A fragment is 16 rows of 64 bytes in LDS, a row's four blocks exchanged by (row >> 1) & 3 so that eight lanes reading
-// one block of eight rows touch all banks.
+// elements of K. The codes of two steps, a line of 128 bytes a row, come into one of the LDS slots at once, those of the next
+// pairs while a pair is worked on; the scales of four steps (16 bytes a row) into one of two. What the loads cost is lines
+// touched, not bytes: eight neighbouring lanes take the line of a row. A fragment is 16 rows of 128 bytes in LDS, a row's eight
+// blocks exchanged by row & 7 so that eight lanes reading one block of eight rows touch all banks. Two slots, or four where the
+// tile is small and its steps are short.
 //
 // In a step each channel fragment is read anew for the next step right after its products were issued, so that only the row
 // fragments need two sets of registers.
 //
-// 16384 x 4096 x 4096 into bf16: 176 us, 3.1 PFLOP/s, three times what a large bf16 product reaches on this card (1.07). The
-// instruction alone, on random data in registers, reaches 5.8 to 6.4 (9 and more on zeros: its rate is bound by power). At its
-// nominal rate a step of a 256 x 256 tile takes 1024 cycles of a CU's matrix units, and the step's LDS traffic (96 KiB read by the
-// waves, 32 KiB written by the loads, 128 bytes a cycle) as many: the two have to overlap fully, which is why the tile is not
-// smaller where there are enough of them (128 x 128 tiles: 252 us), and more accumulators do not fit the registers.
-template <int TN_, int TM_, int WN_, int WM_>
+// 16384 x 4096 x 4096 into bf16: 153 us, 3.6 PFLOP/s; 8192 x 8192 x 8192 266 us, 4.1: four times what a large bf16 product reaches on
+// this card (1.07). The instruction alone, on random data in registers, reaches 5.8 to 6.4 (9 and more on zeros: its rate is bound
+// by power). Of the 153 us some 100 are the products; the rest is what does not overlap with them: a tile's first loads and its
+// output, which all workgroups write at about the same time (20 us at the rate of a fill). At the instruction's nominal rate a step of
+// a 256 x 256 tile takes 1024 cycles of a CU's matrix units, and the step's LDS traffic (96 KiB read by the waves, 32 KiB written by the
+// loads, 128 bytes a cycle) as many, so the tile is as large as registers allow (128 x 128 tiles: 191 us). Steps loaded one by one, 64
+// bytes a row, took 5 us more, and an output of 32 bytes a row and store, straight from the registers, 12 more.
+template <int TN_, int TM_, int WN_, int WM_, int SLOTS_>
 struct MxTile {
-    static constexpr int TN = TN_, TM = TM_, WN = WN_, WM = WM_;
+    static constexpr int TN = TN_, TM = TM_, WN = WN_, WM = WM_, kSlots = SLOTS_;
     static constexpr int NW = WN * WM, FN = TN / 16 / WN, FM = TM / 16 / WM;
-    static constexpr int kSlots = 4;
-    static constexpr int loads = (TN + TM) / 16 / NW;  // of a wave: codes of a step, and scales of four steps
-    static constexpr int slot = (TN + TM) * 64, o_scale = kSlots * slot, scale_slot = (TN + TM) * 16;
-    static constexpr int lds = o_scale + 2 * scale_slot;
-    static_assert((TN + TM) / 16 % NW == 0 && FM <= FN, "");
+    static constexpr int loads = (TN + TM) / 16 / NW;  // of a wave: fragments whose codes and scales it loads
+    static constexpr int slot = (TN + TM) * 128, o_scale = kSlots * slot, scale_slot = (TN + TM) * 16;
+    static constexpr int ahead = kSlots == 2 ? 2 : kSlots - 1, o_out = o_scale + 2 * scale_slot, lds = o_out + NW * 2048;
+    static_assert((TN + TM) / 16 % NW == 0 && FM <= FN && FN % 2 == 0 && (kSlots == 2 || kSlots == 4) && lds <= 160 * 1024, "");
 };
 
 template <class S, class T>
@@ -251,40 +253,47 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a,
     const int band = tile / (8 * tiles_m), in_band = tile - band * 8 * tiles_m;
     const int width = min(8, tiles_n - 8 * band);
     const int n0 = (8 * band + in_band % width) * S::TN, m0 = in_band / width * S::TM;
-    const int steps = a.Kp / 128;
+    const int steps = a.Kp / 128, pairs = (steps + 1) / 2;
     const long long row = a.Kp / 2, srow = a.Kp / 32;
 
     // this wave's loads: 16 rows each, first of W, then of A (rows past the end: the last one, whose results are not stored)
     const uint8_t* cb[S::loads];
     const uint8_t* sb[S::loads];
-    uint32_t co[S::loads], so[S::loads];
+    uint32_t co[S::loads][2], so[S::loads];
+    const uint32_t block = (L & 7) ^ (L >> 3), tail = 16 * (block & 4);
 #pragma unroll
     for (int j = 0; j < S::loads; j++) {
         const int f = wave * S::loads + j;
         const bool w = f < S::TN / 16;
         const int first = w ? n0 + 16 * f : m0 + 16 * (f - S::TN / 16), last = (w ? a.N : a.M) - 1;
-        const int r0 = min(first, last), r = min(first + (L >> 2), last) - r0;
+        const int r0 = min(first, last);
         cb[j] = (w ? a.W : a.A) + r0 * row;
-        co[j] = (uint32_t)(r * row) + 16 * ((L & 3) ^ ((L >> 3) & 3));
         sb[j] = (w ? a.Ws : a.As) + r0 * srow;
-        so[j] = (uint32_t)(r * srow);
-    }
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem + wave * S::loads * 1024;
-    const uint32_t lds1 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem + S::o_scale + wave * S::loads * 256;
-    // past the last step it is loaded again: the count of loads in flight stays the same
-    auto fetch = [&](int k, int slot) {
-        const long long at = 64LL * min(k, steps - 1);
 #pragma unroll
-        for (int j = 0; j < S::loads; j++) lds_load16(cb[j] + at, co[j], lds0 + slot * S::slot + 1024 * j);
+        for (int h = 0; h < 2; h++) co[j][h] = (uint32_t)((min(first + 8 * h + (L >> 3), last) - r0) * row) + 16 * block;
+        so[j] = (uint32_t)((min(first + (L >> 2), last) - r0) * srow);
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem + wave * S::loads * 2048;
+    const uint32_t lds1 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem + S::o_scale + wave * S::loads * 256;
+    // Past the last pair it is loaded again: the count of loads in flight stays the same. Of a pair with one step that one is loaded
+    // twice.
+    auto fetch = [&](int p, int slot) {
+        const int q = min(p, pairs - 1);
+        const uint32_t cut = 2 * q + 1 < steps ? 0 : tail;
+#pragma unroll
+        for (int j = 0; j < S::loads; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) lds_load16(cb[j] + 128LL * q, co[j][h] - cut, lds0 + slot * S::slot + 2048 * j + 1024 * h);
     };
     auto fetch_scales = [&](int c, int slot) {
         const uint32_t at = 4 * min(4 * c + (L & 3), steps - 1);
 #pragma unroll
         for (int j = 0; j < S::loads; j++) lds_load4(sb[j], so[j] + at, lds1 + slot * S::scale_slot + 256 * j);
     };
-    const int lane_at = (L & 15) * 64 + (((L >> 4) ^ ((L >> 1) & 3)) << 4);
-    auto read_w = [&](int slot, int i) { return *(const uint4*)(smem + slot * S::slot + (wn * S::FN + i) * 1024 + lane_at); };
-    auto read_a = [&](int slot, int j) { return *(const uint4*)(smem + slot * S::slot + (S::TN / 16 + wm * S::FM + j) * 1024 + lane_at); };
+    // of the first step of a pair; of the second: ^ 64
+    const int lane_at = (L & 15) * 128 + (((L >> 4) ^ (L & 7)) << 4);
+    auto read_w = [&](int at, int i) { return *(const uint4*)(smem + at + (wn * S::FN + i) * 2048); };
+    auto read_a = [&](int at, int j) { return *(const uint4*)(smem + at + (S::TN / 16 + wm * S::FM + j) * 2048); };
     // the scale bytes of a lane's block in four steps, one a byte (the instruction picks one)
     const uint32_t pick = (L >> 4) | (((L >> 4) + 4) << 8) | 0x0c0c0000u;
     auto read_scale = [&](int slot, int r) {
@@ -304,22 +313,26 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a,
 #pragma unroll
         for (int j = 0; j < S::FM; j++) as[j] = read_scale(slot, S::TN + (wm * S::FM + j) * 16);
     };
-    // Only the matrix products and LDS reads of the wave itself cross a barrier: a slot is overwritten two barriers after it was
-    // read, and its reads were waited for by the products between.
     auto barrier = [&] {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    // Step k = 4 c + s. Its row fragments are in af[s & 1], its channel fragments in wf; those of step k + 1 have landed in LDS.
+    // Step k = 4 c + s. Its row fragments are in af[s & 1], its channel fragments in wf, those of step k + 1 are read from LDS. The
+    // second step of a pair waits until the next pair has landed (and scales that were asked for before it) and until every wave has
+    // read this one, and loads a slot anew.
     auto step = [&](auto sc, int c) {
         constexpr int s = decltype(sc)::value;
-        const int k = 4 * c + s;
-        vm_wait<(s == 1 ? 2 : 1) * S::loads>();  // (of the step before this: its codes, and the next scales where it was the first)
-        barrier();
-        if (s == 0) fetch_scales(c + 1, (c + 1) & 1);
-        fetch(k + 3, (s + 3) & 3);
-        constexpr int next = (s + 1) & 3;
+        const int pair = 2 * c + (s >> 1);
+        if (s & 1) {
+            // (with more slots than two the one loaded anew was read in the pair before)
+            if (S::kSlots == 2) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            vm_wait<2 * (S::ahead - 2) * S::loads>();
+            barrier();
+            if (s == 1) fetch_scales(c + 1, (c + 1) & 1);
+            fetch(pair + S::ahead, (pair + S::ahead) % S::kSlots);
+        }
+        const int at = (lane_at ^ (s & 1 ? 0 : 64)) + (pair + (s & 1)) % S::kSlots * S::slot;
 #pragma unroll
         for (int i = 0; i < S::FN; i++) {
             const v8i w = {(int)wf[i].x, (int)wf[i].y, (int)wf[i].z, (int)wf[i].w, 0, 0, 0, 0};
@@ -329,8 +342,8 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a,
                 const v8i x = {(int)q.x, (int)q.y, (int)q.z, (int)q.w, 0, 0, 0, 0};
                 acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc[i][j], 4, 4, s, ws[i], s, as[j]);
             }
-            if (i < S::FM) af[(s + 1) & 1][i] = read_a(next, i);
-            wf[i] = read_w(next, i);
+            if (i < S::FM) af[(s + 1) & 1][i] = read_a(at, i);
+            wf[i] = read_w(at, i);
             __builtin_amdgcn_sched_group_barrier(0x008, S::FM, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             if (i < S::FM) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
@@ -339,15 +352,13 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a,
         if (s == 3) scales((c + 1) & 1);
     };
     fetch_scales(0, 0);
-    fetch(0, 0);
-    fetch(1, 1);
-    fetch(2, 2);
-    vm_wait<2 * S::loads>();
+    for (int p = 0; p < S::ahead; p++) fetch(p, p);
+    vm_wait<2 * (S::ahead - 2) * S::loads>();
     barrier();
 #pragma unroll
-    for (int j = 0; j < S::FM; j++) af[0][j] = read_a(0, j);
+    for (int j = 0; j < S::FM; j++) af[0][j] = read_a(lane_at, j);
 #pragma unroll
-    for (int i = 0; i < S::FN; i++) wf[i] = read_w(0, i);
+    for (int i = 0; i < S::FN; i++) wf[i] = read_w(lane_at, i);
     scales(0);
     const int whole = steps / 4, rest = steps - 4 * whole;
     for (int c = 0; c < whole; c++) {
@@ -361,17 +372,38 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a,
     if (rest > 2) step(std::integral_constant<int, 2>(), whole);
     vm_wait<0>();
 
-    // lane L: rows m0 + ... + (L & 15), four channels from 4 (L >> 4)
+    // Fragments leave through LDS, 16 rows of up to 128 bytes at a time, so that stores write whole lines. Lane L has row L & 15 and
+    // four channels from 4 (L >> 4) of a fragment.
+    uint8_t* mine = smem + S::o_out + wave * 2048;
+    constexpr int group = std::min(S::FN, 128 / (16 * (int)sizeof(T)));  // fragments side by side
+    constexpr int lanes = group * (int)sizeof(T), each = 16 / (int)sizeof(T);  // of a row, 16 bytes each
 #pragma unroll
-    for (int j = 0; j < S::FM; j++) {
-        const int m = m0 + (wm * S::FM + j) * 16 + (L & 15);
-        if (m >= a.M) continue;
+    for (int j = 0; j < S::FM; j++)
 #pragma unroll
-        for (int i = 0; i < S::FN; i++) {
-            const int n = n0 + (wn * S::FN + i) * 16 + 4 * (L >> 4);
-            store4((T*)a.C + (long long)m * a.N + n, acc[i][j], a.N - n, vec);
+        for (int i0 = 0; i0 < S::FN; i0 += group) {
+            const int m = m0 + (wm * S::FM + j) * 16, n = n0 + (wn * S::FN + i0) * 16;
+            if (vec == 2) {
+#pragma unroll
+                for (int i = 0; i < group; i++) {
+                    const int at = 4 * (int)sizeof(T) * (4 * i + (L >> 4)), r = L & 15;
+                    store4((T*)(mine + r * 128 + (at ^ (16 * (r & 7)))), acc[i0 + i][j], 4, 1);
+                }
+                asm volatile("" ::: "memory");  // (read as another type)
+#pragma unroll
+                for (int h = 0; h < lanes / 4; h++) {
+                    const int r = h * (64 / lanes) + L / lanes, x = L % lanes;
+                    const uint4 v = *(const uint4*)(mine + r * 128 + 16 * (x ^ (r & 7)));
+                    if (m + r < a.M && n + x * each < a.N) *(uint4*)((T*)a.C + (long long)(m + r) * a.N + n + x * each) = v;
+                }
+                asm volatile("" ::: "memory");
+            } else if (m + (L & 15) < a.M) {
+#pragma unroll
+                for (int i = 0; i < group; i++) {
+                    const int c = n + 16 * i + 4 * (L >> 4);
+                    store4((T*)a.C + (long long)(m + (L & 15)) * a.N + c, acc[i0 + i][j], a.N - c, vec);
+                }
+            }
         }
-    }
 }
 
 // Allows a kernel dynamic LDS above the default limit, once per device.
@@ -388,6 +420,9 @@ hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& allow
 // Runs of four channels of C can be stored at once.
 template <class T>
 int vec4(const Mx4GemmArgs& a) { return a.N % 4 == 0 && (uintptr_t)a.C % (4 * sizeof(T)) == 0; }
+// 2: and sixteen bytes.
+template <class T>
+int vec16(const Mx4GemmArgs& a) { return a.N * sizeof(T) % 16 == 0 && (uintptr_t)a.C % 16 == 0 ? 2 : vec4<T>(a); }
 
 template <class S, class T>
 hipError_t launch_lds_gemm(const Mx4GemmArgs& a, hipStream_t s) {
@@ -395,7 +430,7 @@ hipError_t launch_lds_gemm(const Mx4GemmArgs& a, hipStream_t s) {
     if (const hipError_t e = allow_lds((const void*)mx4_gemm_lds_kernel<S, T>, S::lds, allowed); e != hipSuccess) return e;
     const int tn = (a.N + S::TN - 1) / S::TN, tm = (a.M + S::TM - 1) / S::TM;
     if ((long long)tn * tm >= 1 << 22) return hipErrorInvalidValue;  // beyond a launch's 2^32 lanes with the widest workgroup
-    hipLaunchKernelGGL((mx4_gemm_lds_kernel<S, T>), dim3(xcd_grid(tn * tm)), dim3(S::NW * 64), S::lds, s, a, tn, tm, vec4<T>(a));
+    hipLaunchKernelGGL((mx4_gemm_lds_kernel<S, T>), dim3(xcd_grid(tn * tm)), dim3(S::NW * 64), S::lds, s, a, tn, tm, vec16<T>(a));
     return hipGetLastError();
 }
 
@@ -449,9 +484,9 @@ hipError_t launch_mx4_gemm(const Mx4GemmArgs& a, hipStream_t s) {
     return by_real(a.type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         if (a.M <= 16) return launch_split_gemm<MxSplit<1, 1, 8>, T>(a, s);
-        if (takes(256)) return launch_lds_gemm<MxTile<256, 256, 2, 4>, T>(a, s);
-        if (takes(128)) return launch_lds_gemm<MxTile<128, 128, 2, 2>, T>(a, s);
-        if (takes(64)) return launch_lds_gemm<MxTile<64, 64, 2, 2>, T>(a, s);
+        if (takes(256)) return launch_lds_gemm<MxTile<256, 256, 2, 4, 2>, T>(a, s);
+        if (takes(128)) return launch_lds_gemm<MxTile<128, 128, 2, 2, 2>, T>(a, s);
+        if (takes(64)) return launch_lds_gemm<MxTile<64, 64, 2, 2, 4>, T>(a, s);
         return launch_split_gemm<MxSplit<2, 2, 8>, T>(a, s);
     });
 }

@@ -195,3 +195,18 @@ def test_refusals():
     flat = torch.zeros(4 * 64 + 16, dtype=torch.uint8, device="cuda")
     with pytest.raises(MignonError, match="misaligned"):
         mx4_quantize_device(x, flat[1:257].view(4, 64), scales)
+
+
+@pytest.mark.parametrize("M,K,N", [(3600, 128, 3700), (3841, 384, 3712), (3700, 640, 3601), (3600, 1000, 3704), (3585, 1025, 3590),
+                                   (1001, 1152, 1024), (1000, 128, 1030), (1030, 384, 1004), (2050, 896, 2056), (2048, 128, 2052)])
+@pytest.mark.parametrize("t", TYPES)
+def test_product_of_large_matrices(M, K, N, t):
+    """Tiles of every size with whole and cut edges, odd and even numbers of steps, and outputs of every alignment."""
+    (A, As), (W, Ws) = _operands(M, K, N, M + K + N)
+    C = torch.full((M + 1, N), 9.0, dtype=t, device="cuda")
+    mx4_gemm_device(*(torch.from_numpy(a).cuda() for a in (A, As, W, Ws)), C[:M])
+    a, w = (torch.from_numpy(R.values(*x)).cuda() for x in ((A, As), (W, Ws)))
+    want, size = a @ w.T, a.abs() @ w.abs().T
+    tol = K * 2.0 ** -23 * size + torch.finfo(t).eps / 2 * want.abs() + (2.0 ** -25 if t == torch.float16 else 0)
+    assert bool(((C[:M].double() - want).abs() <= tol).all())
+    assert bool((C[M] == 9.0).all())
