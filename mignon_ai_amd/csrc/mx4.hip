@@ -13,6 +13,7 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t Any16 __attribute__((ext_vector_type(4), may_alias));  // sixteen bytes of any type
 
 // ---- Quantisation and reading back ----
 // A workgroup of 256 lanes covers 256 / LC rows by 8 LC columns (LC lanes a row, four to a block, eight elements each): a lane
@@ -225,12 +226,12 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_split_kernel(Mx4GemmArgs 
 // In a step each channel fragment is read anew for the next step right after its products were issued, so that only the row
 // fragments need two sets of registers.
 //
-// 16384 x 4096 x 4096 into bf16: 153 us, 3.6 PFLOP/s; 8192 x 8192 x 8192 266 us, 4.1: four times what a large bf16 product reaches on
+// 16384 x 4096 x 4096 into bf16: 157 us, 3.5 PFLOP/s; 8192 x 8192 x 8192 270 us, 4.1: four times what a large bf16 product reaches on
 // this card (1.07). The instruction alone, on random data in registers, reaches 5.8 to 6.4 (9 and more on zeros: its rate is bound
-// by power). Of the 153 us some 100 are the products; the rest is what does not overlap with them: a tile's first loads and its
+// by power). Of the 157 us some 100 are the products; the rest is what does not overlap with them: a tile's first loads and its
 // output, which all workgroups write at about the same time (20 us at the rate of a fill). At the instruction's nominal rate a step of
 // a 256 x 256 tile takes 1024 cycles of a CU's matrix units, and the step's LDS traffic (96 KiB read by the waves, 32 KiB written by the
-// loads, 128 bytes a cycle) as many, so the tile is as large as registers allow (128 x 128 tiles: 191 us). Steps loaded one by one, 64
+// loads, 128 bytes a cycle) as many, so the tile is as large as registers allow (128 x 128 tiles: 194 us). Steps loaded one by one, 64
 // bytes a row, took 5 us more, and an output of 32 bytes a row and store, straight from the registers, 12 more.
 template <int TN_, int TM_, int WN_, int WM_, int SLOTS_>
 struct MxTile {
@@ -388,14 +389,12 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a,
                     const int at = 4 * (int)sizeof(T) * (4 * i + (L >> 4)), r = L & 15;
                     store4((T*)(mine + r * 128 + (at ^ (16 * (r & 7)))), acc[i0 + i][j], 4, 1);
                 }
-                asm volatile("" ::: "memory");  // (read as another type)
 #pragma unroll
                 for (int h = 0; h < lanes / 4; h++) {
                     const int r = h * (64 / lanes) + L / lanes, x = L % lanes;
-                    const uint4 v = *(const uint4*)(mine + r * 128 + 16 * (x ^ (r & 7)));
-                    if (m + r < a.M && n + x * each < a.N) *(uint4*)((T*)a.C + (long long)(m + r) * a.N + n + x * each) = v;
+                    const Any16 v = *(const Any16*)(mine + r * 128 + 16 * (x ^ (r & 7)));
+                    if (m + r < a.M && n + x * each < a.N) *(Any16*)((T*)a.C + (long long)(m + r) * a.N + n + x * each) = v;
                 }
-                asm volatile("" ::: "memory");
             } else if (m + (L & 15) < a.M) {
 #pragma unroll
                 for (int i = 0; i < group; i++) {
@@ -474,9 +473,10 @@ hipError_t launch_mx4_gemm(const Mx4GemmArgs& a, hipStream_t s) {
     if (a.M <= 0 || a.N <= 0 || a.Kp <= 0 || a.Kp % 128) return hipErrorInvalidValue;
     // The largest tile of which there are enough for three quarters of the 256 CUs and which the shape fills to four fifths;
     // where even those of 64 x 64 are too few, K is split. us at M x N x K, 256 / 128 / 64 tiles, split 32 x 32 and 16 x 16:
-    //   16384 x 4096 x 4096: 185 252 383;     2048 x 2048 x 4096: 36.8 18.2 27.5 57;    1001 x 2048 x 1152: 17.5 8.5 6.4 10.6 15.4
-    //   256 x 4096 x 4096: 33.5 15.2 9.3 14.5 19.6;    128 x 4096 x 4096: 30 14.9 8.3 7.9 10.8;    300 x 300 x 8192: 52 24 12.6 5.6 6.9
-    //   8 x 4096 x 4096: 26 13 7.6 4.8 3.5;    16 x 8192 x 4096: 27 13 7.8 5.3 4.5
+    //   16384 x 4096 x 4096: 158 194 296;     3584 x 3584 x 4096: 38 46;    4096 x 2048 x 4096: 35 28;    4096 x 4096 x 384: 12.5 14 22.5
+    //   2048 x 2048 x 4096: 31 19.5 21.9 56;    1536 x 1024 x 2048: - 10.3 7.3;    1001 x 2048 x 1152: 12.2 7.8 6.1 10.6 15.4
+    //   256 x 4096 x 4096: 28 15.9 9.1 14.5 19.5;    128 x 4096 x 4096: 28 15.6 8.4 8 10.9;    300 x 300 x 8192: 51 27 13.3 5.6 5.4
+    //   8 x 4096 x 4096: 27 15 8 3.9 3;    16 x 8192 x 4096: 27 15 8.2 4.6 3.9
     const auto takes = [&](int tile) {
         const long long n = (a.N + tile - 1) / tile, m = (a.M + tile - 1) / tile;
         return n * m >= 192 && (tile == 64 || 4.0 * n * m * tile * tile <= 5.0 * a.M * a.N);
