@@ -907,17 +907,18 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, in
 // ---- many query rows ----
 // A workgroup of four waves takes 128 query rows of one key/value head (the heads of its group, token after token), a wave 32 of
 // them. Tiles of 32 slots come into LDS as they are, three ahead; the workgroup unpacks the next one to bf16 while it works on
-// this one, into the order in which the products of 32 x 32 x 16 take it: fragments of 32 x 16 values, 16 bytes a lane. With
+// this one (with HALVES 2, four more waves do the same with every other tile, and the two sums are joined in LDS), into the order in
+// which the products of 32 x 32 x 16 take it: fragments of 32 x 16 values, 16 bytes a lane. With
 // i = lane & 31 and g = lane >> 5, K's fragment s has slot i, channels 16 s + 8 g .. + 7; the scores of row i and slots
 // (r & 3) + 8 (r >> 2) + 4 g, r < 16, come out in the lane, which is how the second product takes the probabilities: of V's
 // fragments 2 d and 2 d + 1, channel 32 d + i, entries r < 8 and r >= 8. The places are exchanged (XOR of the low three bits of a
 // lane's place) so that the writes of unpacking and the reads of the products do not meet in a bank: of K's fragment s by g and
 // 2 (s & 3), of V's by 4 g and d & 3.
 //
-// Bound by issuing instructions: 2 x 1024 tokens of 32 query heads over 8 of 128 with 6000 positions in sight, bf16: 273 us, 421
-// TFLOP/s of scores and output (the output's products are done twice, for the probabilities' two parts; a quarter of the time is
-// matrix units', somewhat over half of all cycles issue something). With one part, probabilities held to 8 bits, 252 against 291
-// us then, and an error of 2.0e-3 instead of 1.7e-3 of bf16 outputs: not taken.
+// Bound by issuing instructions: 2 x 1024 tokens of 32 query heads over 8 of 128, lengths up to 8192 and 6000 positions in sight, bf16:
+// 244 us, 473 TFLOP/s of scores and output (the output's products are done twice, for the probabilities' two parts; with four
+// waves a quarter of the time was matrix units', somewhat over half of all cycles issued something). With one part, probabilities
+// held to 8 bits, 252 us instead of 291 with four waves, and an error of 2.0e-3 instead of 1.7e-3 of bf16 outputs: not taken.
 template <int DH>
 struct Unpacked {
     static constexpr int k = 64 * DH, bytes = 2 * k;
@@ -928,15 +929,18 @@ struct Unpacked {
 };
 constexpr int kManyRows = 128;
 
-template <int DH, class T>
-__global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
+template <int DH, class T, int HALVES>
+__global__ __launch_bounds__(256 * HALVES, 2) void kv_attention_chunk_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
     using W = Width<DH>;
     using Tile = KvTile<DH>;
     using U = Unpacked<DH>;
-    constexpr int QT = Terms<T>::q, PT = Terms<T>::p, KF = DH / 16, ND = DH / 32, o_raw = 2 * U::bytes;
-    __shared__ __align__(16) uint8_t smem[o_raw + 3 * Tile::bytes];
+    constexpr int QT = Terms<T>::q, PT = Terms<T>::p, KF = DH / 16, ND = DH / 32, o_raw = 2 * U::bytes, per_half = o_raw + 3 * Tile::bytes;
+    constexpr int o_join = HALVES > 1 ? 4 * 16 * ND * 64 * 4 : 0;  // four waves' sums, then their maxima and sums of probabilities
+    __shared__ __align__(16) uint8_t both[std::max(HALVES * per_half, o_join + 4 * 32 * 8)];
     const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int half = HALVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0, tid = threadIdx.x - 256 * half;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint8_t* smem = both + half * per_half;
     const int unit = blockIdx.x;
     const int pair = unit / row_tiles, rt = unit - pair * row_tiles;
     const int s = pair / a.c.heads, h = pair - s * a.c.heads;
@@ -974,12 +978,12 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
     int k_to[NK], v_from[NV], v_scale[NV], v_slot[NV], v_to[NV];
 #pragma unroll
     for (int x = 0; x < NK; x++) {
-        const int n = threadIdx.x + 256 * x, j = n / words, wd = n % words;
+        const int n = tid + 256 * x, j = n / words, wd = n % words;
         k_to[x] = U::k_at(wd / 2, U::k_lane(j, wd & 1));
     }
 #pragma unroll
     for (int x = 0; x < NV; x++) {
-        const int n = threadIdx.x + 256 * x, j = n / words * 2, wd = n % words;
+        const int n = tid + 256 * x, j = n / words * 2, wd = n % words;
         v_from[x] = Tile::half + j * Tile::row + 4 * wd;
         v_scale[x] = Tile::o_scales + (32 + j) * W::NB + wd / 4;
         v_slot[x] = j;
@@ -990,8 +994,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
         uint8_t* out = smem + buf * U::bytes;
 #pragma unroll
         for (int x = 0; x < NK; x++) {
-            if (32 * words % 256 && threadIdx.x + 256 * x >= 32 * words) break;
-            const int n = threadIdx.x + 256 * x;  // (words and scales lie in the lanes' order)
+            if (32 * words % 256 && tid + 256 * x >= 32 * words) break;
+            const int n = tid + 256 * x;  // (words and scales lie in the lanes' order)
             const uint32_t w = *(const uint32_t*)(p + 4 * n);
             const float sc = mx4_scale(p[Tile::o_scales + n / 4]);
             u32x4 y;
@@ -1001,7 +1005,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
         }
 #pragma unroll
         for (int x = 0; x < NV; x++) {
-            if (16 * words % 256 && threadIdx.x + 256 * x >= 16 * words) break;
+            if (16 * words % 256 && tid + 256 * x >= 16 * words) break;
             uint32_t w[2], sb[2];
 #pragma unroll
             for (int y = 0; y < 2; y++) {
@@ -1123,20 +1127,21 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
         m = -INFINITY;
         l = 0.0f;
         nan_blocks = 0;
-        const int n = o1 - o0;
-        if (n <= 0) return;
-        for (int x = 0; x < min(n, 3); x++) fetch(o0 + x, x);
+        if (o1 <= o0) return;
+        const int first = o0 + half, n = (o1 - first + HALVES - 1) / HALVES;  // this half's tiles; the other's may be one more
+        for (int x = 0; x < min(n, 3); x++) fetch(first + HALVES * x, x);
         vm_wait<0>();
         barrier();
-        int j0 = tl.at(o0) * kTile, run = seen.run(j0);
-        unpack(careful, 0, 0, j0, run >= 0);
+        int j0 = tl.at(min(first, o1 - 1)) * kTile, run = seen.run(j0);
+        if (HALVES == 1 || n > 0) unpack(careful, 0, 0, j0, run >= 0);
         int raw = 0;  // of tile x
-        for (int x = 0; x < n; x++) {
+        for (int x = 0; x < (o1 - o0 + HALVES - 1) / HALVES; x++) {
             // tile x is unpacked, tile x + 1 has landed; tile x's raw place and the other unpacked one are free
             barrier();
-            if (x + 3 < n) fetch(o0 + x + 3, raw);
+            if (HALVES > 1 && x >= n) break;  // (the last time around)
+            if (x + 3 < n) fetch(first + HALVES * (x + 3), raw);
             raw = raw == 2 ? 0 : raw + 1;
-            const int j1 = tl.at(o0 + min(x + 1, n - 1)) * kTile, run1 = seen.run(j1);
+            const int j1 = tl.at(first + HALVES * min(x + 1, n - 1)) * kTile, run1 = seen.run(j1);
             if (x + 1 < n) unpack(careful, raw, (x + 1) & 1, j1, run1 >= 0);
             // (the careful form asks for every slot of every tile)
             work(careful, x & 1, j0, decltype(careful)::value ? -1 : run);
@@ -1166,7 +1171,33 @@ __global__ __launch_bounds__(256, 2) void kv_attention_chunk_kernel(KvAttnArgs a
                     for (int r = 0; r < 16; r++) acc[x][r] = NAN;
         }
     }
-    const float total = l + __shfl_xor(l, 32, 64);
+    float total = l + __shfl_xor(l, 32, 64);
+    if constexpr (HALVES > 1) {
+        // the halves' sums, at the larger maximum
+        float* s_o = (float*)both + wave * 16 * ND * 64 + lane;
+        float* s_ml = (float*)(both + o_join) + (wave * 32 + i) * 2;
+        __syncthreads();
+        if (half) {
+#pragma unroll
+            for (int x = 0; x < ND; x++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s_o[(16 * x + r) * 64] = acc[x][r];
+            if (g == 0) {
+                s_ml[0] = m;
+                s_ml[1] = total;
+            }
+        }
+        __syncthreads();
+        if (half) return;
+        const float m1 = s_ml[0], top = fmaxf(m, m1), tu = top == -INFINITY ? 0.0f : top;
+        const float f0 = __builtin_amdgcn_exp2f(m - tu), f1 = __builtin_amdgcn_exp2f(m1 - tu);
+        m = top;
+        total = total * f0 + s_ml[1] * f1;
+#pragma unroll
+        for (int x = 0; x < ND; x++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[x][r] = acc[x][r] * f0 + s_o[(16 * x + r) * 64] * f1;
+    }
     if (!there) return;
     // lane (i, g): row i, channels 32 x + 8 r + 4 g .. + 3
     if (n_tiles > chunk_tiles) {
@@ -1211,12 +1242,18 @@ AttnPlan attn_plan(const KvAttnArgs& a) {
     // tiles that a row tile can see, at most: the sinks', and the window's (or the ring's), with the ends of three runs
     const long long span = a.window > 0 ? std::min<long long>((long long)a.window + p.per / a.group + 1, a.c.cap) : a.c.cap;
     const int tiles = (int)std::min<long long>((span + kTile - 1) / kTile + (a.c.sinks + kTile - 1) / kTile + 2, a.c.cap / kTile);
-    p.waves = tiles <= 4 && !p.many ? 1 : 4;
+    // Many rows, eight waves, four for every other tile, where no more than two workgroups of four a CU would be there: they all
+    // start at once, and nothing takes the place of one that ends early (us, four waves and eight, bf16 heads of 128 but where said:
+    // 2 x 1024 tokens over 8192 positions, 512 workgroups, lengths of 8192 and less 267 and 229, both 8192 365 and 409; 16 x 256
+    // tokens, fp16 heads of 64, unequal lengths, 256 workgroups 72 and 54; 4 x 512, fp32, equal, 256 workgroups 239 and 220; 64
+    // tokens, 4 workgroups 26 and 22; and where more are waiting, 8 x 512 tokens over 4096, 1024 workgroups 455 and 523; with two tiles
+    // to share, 256 x 64 tokens, 10 and 14)
+    p.waves = p.many ? (p.units <= 512 && tiles >= 16 ? 8 : 4) : tiles <= 4 ? 1 : 4;
     p.chunk_tiles = tiles;
     if (p.waves > 1) {
-        // Two workgroups a CU, each with four tiles a wave at least (sixteen of many rows). More, smaller chunks cost more at their ends
+        // Two workgroups a CU (one of eight waves), each with four tiles a wave at least (sixteen a workgroup of many rows). More, smaller chunks cost more at their ends
         // than they even out (256 conversations, their window in one chunk or two: 28.8 or 37.7 us).
-        const int want = std::max(1, 512 / p.units);
+        const int want = std::max(1, (p.waves == 8 ? 256 : 512) / p.units);
         p.chunk_tiles = std::max(16, (tiles + want - 1) / want);
     }
     p.chunks = std::max(1, (tiles + p.chunk_tiles - 1) / p.chunk_tiles);
@@ -1268,7 +1305,9 @@ hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
         return by_real(a.type, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
             if (p.many) {
-                hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
+                const dim3 grid(p.units, p.chunks);
+                if (p.waves == 8) hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T, 2>), grid, dim3(512), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
+                else hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T, 1>), grid, dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
                 return launch_join<DH, T>(a, p, vec, s);
             }
             if (p.hb == most) return launch_rows_attention<DH, T, most>(a, p, vec, s);

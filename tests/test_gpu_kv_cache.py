@@ -356,3 +356,17 @@ def test_a_cache_keeps_its_planes():
     junk = [torch.full((1, 2, 64, 16), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
     assert torch.equal(c.attention(x, torch.empty_like(x), pos), d.attention(x, torch.empty_like(x), pos))
     del junk
+
+
+@pytest.mark.parametrize("dh", [32, 64, 96, 128])
+@pytest.mark.parametrize("t", list(P_BITS))
+@pytest.mark.parametrize("L,cap,window,sinks", [(481, 512, 0, 0), (700, 1152, 90, 5), (1100, 1152, 520, 33), (1300, 1152, 0, 7)])
+def test_many_rows_over_long_histories(dh, t, L, cap, window, sinks):
+    """Tiles shared by the two halves of a workgroup, odd and even numbers of them, one of them with nothing to see for some rows;
+    lengths apart, one of them of a single token."""
+    n, T, H, G = 3, 35, 2, 2
+    lens = np.array([L, 31, 1])
+    p = Pair(n, H, dh, cap, sinks)
+    p.fill(lens, dh, T=256, t=t)
+    counts = np.minimum(lens, T)
+    p.check(_rows((n, T, H * G, dh), 9, t, 2.0), lens - counts, counts, window)
