@@ -48,7 +48,7 @@ __device__ __forceinline__ RowsSpot rows_spot(const KvRowsArgs& a, int m) {
     return {s, t < q.count ? t : -1, held ? kv_slot(p, a.c.sinks, ring) : -1};
 }
 
-template <int DH, class T, bool VEC, int U>
+template <int DH, class T, int U>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvRowsArgs a) {
     constexpr int LR = DH / 8, rows = 256 / LR;
     const int tokens = a.c.n * a.T, h0 = blockIdx.y * U, row_in = threadIdx.x / LR, l = threadIdx.x % LR;
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvRowsArgs a) {
         float v[U][8];
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (h0 + u < a.c.heads) real_load8<T, VEC>(from + (h0 + u) * x.head, 8, v[u]);
+            if (h0 + u < a.c.heads) real_load8<T>(from + (h0 + u) * x.head, 8, v[u]);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (h0 + u >= a.c.heads) break;
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvRowsArgs a) {
     }
 }
 
-template <int DH, class T, bool VEC, int U>
+template <int DH, class T, int U>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvRowsArgs a) {
     constexpr int LR = DH / 8, rows = 256 / LR;
     const int tokens = a.c.n * a.T, h0 = blockIdx.y * U, row_in = threadIdx.x / LR, l = threadIdx.x % LR;
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRowsArgs a) {
             if (h0 + u >= a.c.heads) break;
             float v[8];
             mx4_unpack8(w[u], mx4_scale(sb[u]), v);
-            real_store8<T, VEC>(to + (h0 + u) * x.head, 8, v);
+            real_store8<T>(to + (h0 + u) * x.head, 8, v);
         }
     }
 }
@@ -128,7 +128,6 @@ template <bool READ>
 hipError_t launch_rows(const KvRowsArgs& a, hipStream_t s) {
     const int rows = 256 / (a.c.dh / 8);
     const long long groups = ((long long)a.c.n * a.T + rows - 1) / rows;
-    const bool vec = rows_aligned(a.k, a.type) && rows_aligned(a.v, a.type);
     // four heads a lane where that leaves four workgroups a CU
     const bool many = groups * a.c.heads >= 2048;
     const dim3 grid((unsigned)std::min<long long>(groups, 1 << 16), many ? (a.c.heads + 3) / 4 : a.c.heads, 2);
@@ -136,17 +135,13 @@ hipError_t launch_rows(const KvRowsArgs& a, hipStream_t s) {
         constexpr int DH = decltype(w)::value;
         return by_real(a.type, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            const auto go = [&](auto v, auto u) {
-                constexpr bool V = decltype(v)::value;
+            const auto go = [&](auto u) {
                 constexpr int U = decltype(u)::value;
-                if constexpr (READ) hipLaunchKernelGGL((kv_read_kernel<DH, T, V, U>), grid, dim3(256), 0, s, a);
-                else hipLaunchKernelGGL((kv_write_kernel<DH, T, V, U>), grid, dim3(256), 0, s, a);
+                if constexpr (READ) hipLaunchKernelGGL((kv_read_kernel<DH, T, U>), grid, dim3(256), 0, s, a);
+                else hipLaunchKernelGGL((kv_write_kernel<DH, T, U>), grid, dim3(256), 0, s, a);
                 return hipGetLastError();
             };
-            using One = std::integral_constant<int, 1>;
-            using Four = std::integral_constant<int, 4>;
-            if (vec) return many ? go(std::true_type(), Four()) : go(std::true_type(), One());
-            return many ? go(std::false_type(), Four()) : go(std::false_type(), One());
+            return many ? go(std::integral_constant<int, 4>()) : go(std::integral_constant<int, 1>());
         });
     });
 }
@@ -688,11 +683,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a,
 #pragma unroll
     for (int st = 0; st < W::KS; st++) {
         float x[8] = {};
-        if (there) {
-            const T* p = (const T*)a.q.data + s * a.q.seq + t * a.q.token + head * a.q.head + W::k_channel(g, st);
-            if (vec) real_load8<T, true>(p, 8, x);
-            else real_load8<T, false>(p, 8, x);
-        }
+        if (there) real_load8<T>((const T*)a.q.data + s * a.q.seq + t * a.q.token + head * a.q.head + W::k_channel(g, st), 8, x);
         split_bf16<QT>(x, qf[st]);
     }
     const float scale = a.scale * kLog2e;
@@ -1043,10 +1034,7 @@ __global__ __launch_bounds__(256 * HALVES, 2) void kv_attention_chunk_kernel(KvA
 #pragma unroll
         for (int x = 0; x < KF; x++) {
             float y[8] = {};
-            if (there) {
-                if (vec) real_load8<T, true>(p + 16 * x, 8, y);
-                else real_load8<T, false>(p + 16 * x, 8, y);
-            }
+            if (there) real_load8<T>(p + 16 * x, 8, y);
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] *= sign;
             split_bf16<QT>(y, qf[x]);
@@ -1299,7 +1287,7 @@ bool kv_attention_fits(const KvAttnArgs& a) {
 
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
     const AttnPlan p = attn_plan(a);
-    const int vec = rows_aligned(a.q, a.type) && rows_aligned(a.out, a.type);
+    const int vec = rows_aligned(a.out, a.type);
     return by_width(a.c.dh, [&](auto w) {
         constexpr int DH = decltype(w)::value, most = DH == 32 ? 8 : DH == 64 ? 4 : 2;
         return by_real(a.type, [&](auto* t) {

@@ -23,7 +23,7 @@ typedef uint32_t Any16 __attribute__((ext_vector_type(4), may_alias));  // sixte
 constexpr int kRowLanes = 256;
 constexpr int kMaxGridY = 32768;
 
-template <class T, bool VEC>
+template <class T>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(Mx4RowsArgs a, int lc_log2) {
     const int lanes = ((a.K + 127) / 128) * 16;  // lanes a row
     const int rows = kRowLanes >> lc_log2;
@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(Mx4RowsArgs a, int lc
     for (long long m = (long long)blockIdx.x * rows + row_in; m < a.M; m += (long long)gridDim.x * rows) {
         for (int c = (blockIdx.y << lc_log2) + c_in; c < lanes; c += gridDim.y << lc_log2) {
             float x[8];
-            real_load8<T, VEC>((const T*)a.x + m * a.ld + 8 * c, a.K - 8 * c, x);
+            real_load8<T>((const T*)a.x + m * a.ld + 8 * c, a.K - 8 * c, x);
             uint32_t s;
             const uint32_t w = mx4_block(x, s);
             *(uint32_t*)(a.codes + m * lanes * 4 + 4 * c) = w;
@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(Mx4RowsArgs a, int lc
     }
 }
 
-template <class T, bool VEC>
+template <class T>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(Mx4RowsArgs a, int lc_log2) {
     const int lanes = ((a.K + 127) / 128) * 16;
     const int rows = kRowLanes >> lc_log2;
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(Mx4RowsArgs a, int 
         for (int c = (blockIdx.y << lc_log2) + c_in; 8 * c < a.K; c += gridDim.y << lc_log2) {
             float x[8];
             mx4_unpack8(*(const uint32_t*)(a.codes + m * lanes * 4 + 4 * c), mx4_scale(a.scales[m * (lanes >> 2) + (c >> 2)]), x);
-            real_store8<T, VEC>((T*)a.y + m * a.ld + 8 * c, a.K - 8 * c, x);
+            real_store8<T>((T*)a.y + m * a.ld + 8 * c, a.K - 8 * c, x);
         }
     }
 }
@@ -448,11 +448,9 @@ hipError_t launch_split_gemm(const Mx4GemmArgs& a, hipStream_t s) {
 hipError_t launch_mx4_quantize(const Mx4RowsArgs& a, hipStream_t s) {
     if (a.M <= 0 || a.K <= 0) return hipErrorInvalidValue;
     const RowsGrid g = rows_grid(a.M, ((a.K + 127) / 128) * 16);
-    const bool vec = (uintptr_t)a.x % 16 == 0 && a.ld * real_size(a.type) % 16 == 0;
     return by_real(a.type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (vec) hipLaunchKernelGGL((mx4_quantize_kernel<T, true>), g.grid, dim3(256), 0, s, a, g.lc_log2);
-        else hipLaunchKernelGGL((mx4_quantize_kernel<T, false>), g.grid, dim3(256), 0, s, a, g.lc_log2);
+        hipLaunchKernelGGL((mx4_quantize_kernel<T>), g.grid, dim3(256), 0, s, a, g.lc_log2);
         return hipGetLastError();
     });
 }
@@ -460,11 +458,9 @@ hipError_t launch_mx4_quantize(const Mx4RowsArgs& a, hipStream_t s) {
 hipError_t launch_mx4_dequantize(const Mx4RowsArgs& a, hipStream_t s) {
     if (a.M <= 0 || a.K <= 0) return hipErrorInvalidValue;
     const RowsGrid g = rows_grid(a.M, ((a.K + 127) / 128) * 16);
-    const bool vec = (uintptr_t)a.y % 16 == 0 && a.ld * real_size(a.type) % 16 == 0;
     return by_real(a.type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (vec) hipLaunchKernelGGL((mx4_dequantize_kernel<T, true>), g.grid, dim3(256), 0, s, a, g.lc_log2);
-        else hipLaunchKernelGGL((mx4_dequantize_kernel<T, false>), g.grid, dim3(256), 0, s, a, g.lc_log2);
+        hipLaunchKernelGGL((mx4_dequantize_kernel<T>), g.grid, dim3(256), 0, s, a, g.lc_log2);
         return hipGetLastError();
     });
 }
