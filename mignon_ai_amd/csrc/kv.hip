@@ -109,11 +109,6 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRowsArgs a) {
     }
 }
 
-bool rows_aligned(const KvRows& r, int type) {
-    const int e = real_size(type);
-    return (uintptr_t)r.data % 16 == 0 && r.seq * e % 16 == 0 && r.token * e % 16 == 0 && r.head * e % 16 == 0;
-}
-
 template <class F>
 auto by_width(int dh, F&& f) {
     switch (dh) {
@@ -144,21 +139,6 @@ hipError_t launch_rows(const KvRowsArgs& a, hipStream_t s) {
             return many ? go(std::integral_constant<int, 4>()) : go(std::integral_constant<int, 1>());
         });
     });
-}
-
-// Four neighbouring channels; vec: aligned.
-template <class T>
-__device__ __forceinline__ void store4(T* p, v4f v, int vec) {
-    T t[4];
-#pragma unroll
-    for (int r = 0; r < 4; r++) t[r] = (T)v[r];
-    if (vec) {
-        if constexpr (sizeof(T) == 4) *(uint4*)p = *(uint4*)t;
-        else *(uint2*)p = *(uint2*)t;
-    } else {
-#pragma unroll
-        for (int r = 0; r < 4; r++) p[r] = t[r];
-    }
 }
 
 // ---- attention -----------------------------------------------------------------------------------------------------
@@ -623,7 +603,7 @@ struct Stages {
 // of 32, 57 MB) 24 us, where a wave's life is mostly its first tiles' latency; one conversation of 30000 (33 MB) 18 us with the
 // join, the latency of a chunk's sixteen tiles and of a second launch.
 template <int DH, class T, int HB, int WAVES>
-__global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
+__global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles) {
     using W = Width<DH>;
     using Tile = KvTile<DH>;
     using St = Stages<DH, HB>;
@@ -774,21 +754,14 @@ __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a,
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     T* p = out + W::base(c) + (4 * g + 2 * (i & 1) + r) * W::E(c);
-                    T u[W::E0];
-#pragma unroll
-                    for (int e = 0; e < W::E(c); e++) u[e] = (T)v[r][e];
-                    if (vec) {
-                        if (W::E(c) * sizeof(T) >= 16) {
-#pragma unroll
-                            for (int x = 0; x < (int)(W::E(c) * sizeof(T) / 16); x++) ((u32x4*)p)[x] = ((u32x4*)u)[x];
-                        } else if (W::E(c) * sizeof(T) == 8) {
-                            *(u32x2*)p = *(u32x2*)u;
-                        } else {
-                            *(uint32_t*)p = *(uint32_t*)u;
-                        }
+                    const float* from = v[r];
+                    if (W::E(c) == 8) {
+                        real_store8<T>(p, 8, from);
+                    } else if (W::E(c) == 4) {
+                        real_store4(p, from, 4);
                     } else {
-#pragma unroll
-                        for (int e = 0; e < W::E(c); e++) p[e] = u[e];
+                        const T u[2] = {(T)from[0], (T)from[1]};
+                        __builtin_memcpy(p, u, sizeof(u));
                     }
                 }
             }
@@ -837,7 +810,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a,
                     part[cc * kPart<DH> + DH + 1] = total;
                 }
             } else {
-                store4((T*)a.out.data + s * a.out.seq + tt * a.out.token + hd * a.out.head + d, sum * (total == 0.0f ? 0.0f : 1.0f / total), vec);
+                real_store4((T*)a.out.data + s * a.out.seq + tt * a.out.token + hd * a.out.head + d, sum * (total == 0.0f ? 0.0f : 1.0f / total), 4);
             }
         }
     }
@@ -847,7 +820,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a,
 // over the chunks, whose sums are added in a fixed order. Units have `per` rows. (4.6 us for 32 conversations of 32 query heads, 6 for
 // the 59 chunks of one long one: its latency.)
 template <int DH, class T>
-__global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int per, int hb, int row_tiles, int chunk_tiles, int vec) {
+__global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int per, int hb, int row_tiles, int chunk_tiles) {
     constexpr int LC = DH / 4, G = 64 / LC;  // lanes a group, groups
     const int lane = threadIdx.x & 63, col = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int unit = blockIdx.x;
@@ -892,7 +865,7 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, in
         norm += __shfl(total, lane + x * LC, 64);
     }
     if (lane < LC)
-        store4((T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head + d, all * (norm == 0.0f ? 0.0f : 1.0f / norm), vec);
+        real_store4((T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head + d, all * (norm == 0.0f ? 0.0f : 1.0f / norm), 4);
 }
 
 // ---- many query rows ----
@@ -921,7 +894,7 @@ struct Unpacked {
 constexpr int kManyRows = 128;
 
 template <int DH, class T, int HALVES>
-__global__ __launch_bounds__(256 * HALVES, 2) void kv_attention_chunk_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles, int vec) {
+__global__ __launch_bounds__(256 * HALVES, 2) void kv_attention_chunk_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles) {
     using W = Width<DH>;
     using Tile = KvTile<DH>;
     using U = Unpacked<DH>;
@@ -1206,7 +1179,7 @@ __global__ __launch_bounds__(256 * HALVES, 2) void kv_attention_chunk_kernel(KvA
         for (int x = 0; x < ND; x++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                store4(out + 32 * x + 8 * r + 4 * g, v4f{acc[x][4 * r], acc[x][4 * r + 1], acc[x][4 * r + 2], acc[x][4 * r + 3]} * f, vec);
+                real_store4(out + 32 * x + 8 * r + 4 * g, v4f{acc[x][4 * r], acc[x][4 * r + 1], acc[x][4 * r + 2], acc[x][4 * r + 3]} * f, 4);
     }
 }
 
@@ -1249,23 +1222,23 @@ AttnPlan attn_plan(const KvAttnArgs& a) {
 }
 
 template <int DH, class T>
-hipError_t launch_join(const KvAttnArgs& a, const AttnPlan& p, int vec, hipStream_t s) {
+hipError_t launch_join(const KvAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (p.chunks > 1) {
         const int cols = p.hb > 1 ? p.hb * a.T * a.group : std::min(p.per, a.T * a.group);
         hipLaunchKernelGGL((kv_attention_join_kernel<DH, T>), dim3(p.units, (cols + 3) / 4), dim3(256), 0, s, a, p.per, p.hb, p.row_tiles,
-                           p.chunk_tiles, vec);
+                           p.chunk_tiles);
     }
     return hipGetLastError();
 }
 
 template <int DH, class T, int HB>
-hipError_t launch_rows_attention(const KvAttnArgs& a, const AttnPlan& p, int vec, hipStream_t s) {
+hipError_t launch_rows_attention(const KvAttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (p.waves == 1) {
-        hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 1>), dim3((p.units + 3) / 4), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
+        hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 1>), dim3((p.units + 3) / 4), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 4>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
-    return launch_join<DH, T>(a, p, vec, s);
+    hipLaunchKernelGGL((kv_attention_rows_kernel<DH, T, HB, 4>), dim3(p.units, p.chunks), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles);
+    return launch_join<DH, T>(a, p, s);
 }
 
 }  // namespace
@@ -1287,21 +1260,20 @@ bool kv_attention_fits(const KvAttnArgs& a) {
 
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
     const AttnPlan p = attn_plan(a);
-    const int vec = rows_aligned(a.out, a.type);
     return by_width(a.c.dh, [&](auto w) {
         constexpr int DH = decltype(w)::value, most = DH == 32 ? 8 : DH == 64 ? 4 : 2;
         return by_real(a.type, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
             if (p.many) {
                 const dim3 grid(p.units, p.chunks);
-                if (p.waves == 8) hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T, 2>), grid, dim3(512), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
-                else hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T, 1>), grid, dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles, vec);
-                return launch_join<DH, T>(a, p, vec, s);
+                if (p.waves == 8) hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T, 2>), grid, dim3(512), 0, s, a, p.row_tiles, p.chunk_tiles);
+                else hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T, 1>), grid, dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles);
+                return launch_join<DH, T>(a, p, s);
             }
-            if (p.hb == most) return launch_rows_attention<DH, T, most>(a, p, vec, s);
+            if (p.hb == most) return launch_rows_attention<DH, T, most>(a, p, s);
             if constexpr (most > 2)
-                if (p.hb == 2) return launch_rows_attention<DH, T, 2>(a, p, vec, s);
-            return launch_rows_attention<DH, T, 1>(a, p, vec, s);
+                if (p.hb == 2) return launch_rows_attention<DH, T, 2>(a, p, s);
+            return launch_rows_attention<DH, T, 1>(a, p, s);
         });
     });
 }

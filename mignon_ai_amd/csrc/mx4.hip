@@ -83,22 +83,6 @@ __device__ __forceinline__ void vm_wait() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
 }
 
-// Four neighbouring channels of a row, `left` of which exist; vec: such a run is aligned.
-template <class T>
-__device__ __forceinline__ void store4(T* out, v4f v, int left, int vec) {
-    if (vec && left >= 4) {
-        T t[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) t[r] = (T)v[r];
-        if constexpr (sizeof(T) == 4) *(uint4*)out = *(uint4*)t;
-        else *(uint2*)out = *(uint2*)t;
-    } else {
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            if (r < left) out[r] = (T)v[r];
-    }
-}
-
 // A workgroup of up to NW waves computes 16 FN channels x 16 FM rows, each wave over its own share of K, and adds the waves' sums in
 // LDS, in the waves' order: for products with too few tiles to fill the chip, whose time is the latency of a tile's steps
 // (1 x 384 by 8192 channels 2.8 us, of which the steps are one round trip to memory; 8 x 4096 by 4096 3.5). A
@@ -112,7 +96,7 @@ struct MxSplit {
 };
 
 template <class S, class T>
-__global__ __launch_bounds__(S::NW * 64) void mx4_gemm_split_kernel(Mx4GemmArgs a, int vec) {
+__global__ __launch_bounds__(S::NW * 64) void mx4_gemm_split_kernel(Mx4GemmArgs a) {
     extern __shared__ uint8_t smem[];
     constexpr int FN = S::FN, FM = S::FM, F = S::F;
     const int L = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -211,7 +195,7 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_split_kernel(Mx4GemmArgs 
         for (int w = 1; w < waves; w++) sum += part[(w * FN * FM + f) * 64 + L];
         const int i = f / FM, j = f - i * FM;
         const int m = m0 + 16 * j + (L & 15), n = n0 + 16 * i + 4 * (L >> 4);
-        if (m < a.M) store4((T*)a.C + (long long)m * a.N + n, sum, a.N - n, vec);
+        if (m < a.M) real_store4((T*)a.C + (long long)m * a.N + n, sum, a.N - n);
     }
 }
 
@@ -244,7 +228,7 @@ struct MxTile {
 };
 
 template <class S, class T>
-__global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a, int tiles_n, int tiles_m, int vec) {
+__global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a, int tiles_n, int tiles_m) {
     extern __shared__ uint8_t smem[];
     const int L = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wn = wave % S::WN, wm = wave / S::WN;
@@ -383,23 +367,24 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a,
 #pragma unroll
         for (int i0 = 0; i0 < S::FN; i0 += group) {
             const int m = m0 + (wm * S::FM + j) * 16, n = n0 + (wn * S::FN + i0) * 16;
-            if (vec == 2) {
 #pragma unroll
-                for (int i = 0; i < group; i++) {
-                    const int at = 4 * (int)sizeof(T) * (4 * i + (L >> 4)), r = L & 15;
-                    store4((T*)(mine + r * 128 + (at ^ (16 * (r & 7)))), acc[i0 + i][j], 4, 1);
-                }
+            for (int i = 0; i < group; i++) {
+                const int at = 4 * (int)sizeof(T) * (4 * i + (L >> 4)), r = L & 15;
+                T v[4];
 #pragma unroll
-                for (int h = 0; h < lanes / 4; h++) {
-                    const int r = h * (64 / lanes) + L / lanes, x = L % lanes;
-                    const Any16 v = *(const Any16*)(mine + r * 128 + 16 * (x ^ (r & 7)));
-                    if (m + r < a.M && n + x * each < a.N) *(Any16*)((T*)a.C + (long long)(m + r) * a.N + n + x * each) = v;
-                }
-            } else if (m + (L & 15) < a.M) {
+                for (int e = 0; e < 4; e++) v[e] = (T)acc[i0 + i][j][e];
+                __builtin_memcpy(__builtin_assume_aligned(mine + r * 128 + (at ^ (16 * (r & 7))), sizeof(v)), v, sizeof(v));
+            }
 #pragma unroll
-                for (int i = 0; i < group; i++) {
-                    const int c = n + 16 * i + 4 * (L >> 4);
-                    store4((T*)a.C + (long long)(m + (L & 15)) * a.N + c, acc[i0 + i][j], a.N - c, vec);
+            for (int h = 0; h < lanes / 4; h++) {
+                const int r = h * (64 / lanes) + L / lanes, x = L % lanes, left = a.N - n - x * each;
+                const T* v = (const T*)(mine + r * 128 + 16 * (x ^ (r & 7)));
+                T* out = (T*)a.C + (long long)(m + r) * a.N + n + x * each;
+                if (m + r >= a.M) continue;
+                if (left >= each) {
+                    *(typename Raw16<sizeof(T)>::type*)out = *(const Any16*)v;
+                } else {
+                    for (int e = 0; e < left; e++) out[e] = v[e];
                 }
             }
         }
@@ -416,20 +401,13 @@ hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& allow
     return e;
 }
 
-// Runs of four channels of C can be stored at once.
-template <class T>
-int vec4(const Mx4GemmArgs& a) { return a.N % 4 == 0 && (uintptr_t)a.C % (4 * sizeof(T)) == 0; }
-// 2: and sixteen bytes.
-template <class T>
-int vec16(const Mx4GemmArgs& a) { return a.N * sizeof(T) % 16 == 0 && (uintptr_t)a.C % 16 == 0 ? 2 : vec4<T>(a); }
-
 template <class S, class T>
 hipError_t launch_lds_gemm(const Mx4GemmArgs& a, hipStream_t s) {
     static std::atomic<uint64_t> allowed{0};
     if (const hipError_t e = allow_lds((const void*)mx4_gemm_lds_kernel<S, T>, S::lds, allowed); e != hipSuccess) return e;
     const int tn = (a.N + S::TN - 1) / S::TN, tm = (a.M + S::TM - 1) / S::TM;
     if ((long long)tn * tm >= 1 << 22) return hipErrorInvalidValue;  // beyond a launch's 2^32 lanes with the widest workgroup
-    hipLaunchKernelGGL((mx4_gemm_lds_kernel<S, T>), dim3(xcd_grid(tn * tm)), dim3(S::NW * 64), S::lds, s, a, tn, tm, vec16<T>(a));
+    hipLaunchKernelGGL((mx4_gemm_lds_kernel<S, T>), dim3(xcd_grid(tn * tm)), dim3(S::NW * 64), S::lds, s, a, tn, tm);
     return hipGetLastError();
 }
 
@@ -439,7 +417,7 @@ hipError_t launch_split_gemm(const Mx4GemmArgs& a, hipStream_t s) {
     if (const hipError_t e = allow_lds((const void*)mx4_gemm_split_kernel<S, T>, S::lds, allowed); e != hipSuccess) return e;
     const int waves = std::min(S::NW, (a.Kp / 128 + 3) / 4);
     const dim3 grid((a.N + 16 * S::FN - 1) / (16 * S::FN), (a.M + 16 * S::FM - 1) / (16 * S::FM));
-    hipLaunchKernelGGL((mx4_gemm_split_kernel<S, T>), grid, dim3(64 * waves), waves * S::wave_lds, s, a, vec4<T>(a));
+    hipLaunchKernelGGL((mx4_gemm_split_kernel<S, T>), grid, dim3(64 * waves), waves * S::wave_lds, s, a);
     return hipGetLastError();
 }
 

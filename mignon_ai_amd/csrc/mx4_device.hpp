@@ -12,6 +12,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace mg {
 
 typedef float mx_v2f __attribute__((ext_vector_type(2)));
@@ -85,6 +87,26 @@ __device__ __forceinline__ void real_store8(T* p, int left, const float x[8]) {
 #pragma unroll
         for (int e = 0; e < 8; e++)
             if (e < left) p[e] = (T)x[e];
+    }
+}
+
+// Four neighbouring elements of a row from floats, `left` of which exist, with the element's alignment alone.
+template <class T, class V>
+__device__ __forceinline__ void real_store4(T* p, const V& v, int left) {
+    typedef uint32_t R4 __attribute__((ext_vector_type(4), aligned(4), may_alias));
+    typedef uint32_t R2 __attribute__((ext_vector_type(2), aligned(2), may_alias));
+    using R = std::conditional_t<sizeof(T) == 4, R4, R2>;
+    T t[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) t[r] = (T)v[r];
+    if (left >= 4) {
+        R w;
+        __builtin_memcpy(&w, t, sizeof(t));
+        *(R*)p = w;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (r < left) p[r] = t[r];
     }
 }
 
