@@ -18,8 +18,8 @@ typedef uint32_t Any16 __attribute__((ext_vector_type(4), may_alias));  // sixte
 // ---- Quantisation and reading back ----
 // A workgroup of 256 lanes covers 256 / LC rows by 8 LC columns (LC lanes a row, four to a block, eight elements each): a lane
 // reads 16 or 32 bytes and a wave writes whole lines of codes; the block's largest magnitude takes two exchanges among four
-// lanes, so an element is read once and kept in registers. Bound by memory: 16384 x 4096 bf16, 170 MB each way, 34 us quantised
-// (5.1 TB/s) and 37 read back (4.6), where a large copy reaches 4.8; 16 x 384 fp32 2.3 and 2.4 us, a launch.
+// lanes, so an element is read once and kept in registers. Bound by memory: 16384 x 4096 bf16, 170 MB each way, 33 us quantised
+// (5.2 TB/s) and 26 read back (6.5), where a large copy reaches 4.8; 16 x 384 fp32 2.2 and 2.3 us, a launch.
 constexpr int kRowLanes = 256;
 constexpr int kMaxGridY = 32768;
 
@@ -210,9 +210,9 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_split_kernel(Mx4GemmArgs 
 // In a step each channel fragment is read anew for the next step right after its products were issued, so that only the row
 // fragments need two sets of registers.
 //
-// 16384 x 4096 x 4096 into bf16: 157 us, 3.5 PFLOP/s; 8192 x 8192 x 8192 270 us, 4.1: four times what a large bf16 product reaches on
+// 16384 x 4096 x 4096 into bf16: 153 us, 3.6 PFLOP/s; 8192 x 8192 x 8192 270 us, 4.1: four times what a large bf16 product reaches on
 // this card (1.07). The instruction alone, on random data in registers, reaches 5.8 to 6.4 (9 and more on zeros: its rate is bound
-// by power). Of the 157 us some 100 are the products; the rest is what does not overlap with them: a tile's first loads and its
+// by power). Of the 153 us some 100 are the products; the rest is what does not overlap with them: a tile's first loads and its
 // output, which all workgroups write at about the same time (20 us at the rate of a fill). At the instruction's nominal rate a step of
 // a 256 x 256 tile takes 1024 cycles of a CU's matrix units, and the step's LDS traffic (96 KiB read by the waves, 32 KiB written by the
 // loads, 128 bytes a cycle) as many, so the tile is as large as registers allow (128 x 128 tiles: 194 us). Steps loaded one by one, 64

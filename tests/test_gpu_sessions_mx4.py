@@ -172,3 +172,22 @@ def test_models_without_attention_and_refusals(restore):
         m.sessions(0, kv="mx4")
     with pytest.raises(MignonError, match="width 24"):
         Model(uniform_model_bytes(_spec(24, 2, 8, 32), 5, 0.1)).sessions(2, kv="mx4")
+
+
+def test_steps_without_allocation(restore):
+    """step_noalloc, its workspace in the library's own memory, gives what a step gives."""
+    import torch
+    m, V = Model(model_bytes("c3")), synth.CONFIGS["c3"]["spec"].V
+    S = 21
+    p = synth.token_ids(6, "mx4:na", (S, 30), V)
+    a, b = m.sessions(S, kv="mx4"), m.sessions(S, kv="mx4")
+    a.prefill(p)
+    b.prefill(p)
+    for i in range(3):
+        ids = torch.from_numpy(p[:, i].copy()).cuda()
+        lg, am, pb = (torch.empty(s, dtype=t, device="cuda") for s, t in (((S, V), torch.float32), (S, torch.int32), (S, torch.float64)))
+        b.step_noalloc(ids, lg, am, pb)
+        m.sync()
+        want = a.step(p[:, i])
+        for x, y in zip(want, (lg, am, pb)):
+            assert np.array_equal(x, y.cpu().numpy())
