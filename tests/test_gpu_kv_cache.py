@@ -370,3 +370,26 @@ def test_many_rows_over_long_histories(dh, t, L, cap, window, sinks):
     p.fill(lens, dh, T=256, t=t)
     counts = np.minimum(lens, T)
     p.check(_rows((n, T, H * G, dh), 9, t, 2.0), lens - counts, counts, window)
+
+
+def test_two_streams_at_once():
+    """Calls that need workspaces, on two streams at the same time, over one cache: each gives what it gives alone."""
+    c = KVCache.empty(2, 2, 64, 8192)
+    for p in (c.k, c.v):
+        p.random_(0, 256)
+    for p in (c.k_scales, c.v_scales):
+        p.random_(120, 126)
+    qs = [_rows((2, T, 4, 64), T, torch.float16) for T in (1, 1, 40, 40)]
+    pos = [_ints([8192 - q.shape[1], 5000]) for q in qs]
+    alone = [c.attention(q, torch.empty_like(q), p) for q, p in zip(qs, pos)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(5):
+        outs = [torch.empty_like(q) for q in qs]
+        torch.cuda.synchronize()
+        for s, q, o, p in zip(streams, qs, outs, pos):
+            with torch.cuda.stream(s):
+                c.attention(q, o, p)
+        torch.cuda.synchronize()
+        for a, b in zip(alone, outs):
+            assert torch.equal(a, b)

@@ -78,15 +78,11 @@ def _unsure(x):
     return r, [(t, c, y) for (t, c), y in other.items()]
 
 
-@pytest.mark.parametrize("dh,heads,window,context", [(32, 2, 16, 48), (64, 3, 0, 40), (96, 2, 33, 64), (128, 1, 5, 32),
-                                                     (32, 2, 0, 64)])
-def test_steps_attend_over_the_rounded_rows(restore, dh, heads, window, context):
-    spec = _spec(dh, heads, window, context)
+def _against_ref(spec, S, P, lens, n):
     data = uniform_model_bytes(spec, 5, 0.1)
     rm, m = O.read_model(data), Model(data)
     context = O.OracleModel(rm).max_context  # (a context of less than 64 tokens counts as 128)
-    S, P, n = 3, 11, 60
-    lens = np.array([11, 4, 1], np.int32)
+    lens = np.array(lens, np.int32)
     prompts = synth.token_ids(7, "mx4:p", (S, P), spec.V)
     steps = synth.token_ids(7, "mx4:s", (n, S), spec.V)
     ss = m.sessions(S, kv="mx4")
@@ -110,6 +106,18 @@ def test_steps_attend_over_the_rounded_rows(restore, dh, heads, window, context)
                         tol = tol + np.abs(ref.logits(t, alt, v) - want if which == 0 else ref.logits(t, k, alt) - want)
             worst = (np.abs(got[i][s] - want) / tol).max()
             assert worst <= 1, f"session {s}, step {i}: {worst} of the tolerance"
+
+
+@pytest.mark.parametrize("dh,heads,window,context", [(32, 2, 16, 48), (64, 3, 0, 40), (96, 2, 33, 64), (128, 1, 5, 32),
+                                                     (32, 2, 0, 64)])
+def test_steps_attend_over_the_rounded_rows(restore, dh, heads, window, context):
+    _against_ref(_spec(dh, heads, window, context), 3, 11, [11, 4, 1], 60)
+
+
+@pytest.mark.parametrize("dh,heads,window,context", [(32, 2, 16, 64), (64, 1, 33, 100), (96, 1, 3, 64), (128, 1, 64, 96)])
+def test_prompts_longer_than_the_ring(restore, dh, heads, window, context):
+    """Of a prompt's rows that share a slot the later one is kept."""
+    _against_ref(_spec(dh, heads, window, context), 4, 70 if context > 64 else 60, [60, 35, 33, 5], 12)
 
 
 @pytest.mark.parametrize("cfg,S", [("c3", 5), ("c4", 37), ("c5", 300)])
