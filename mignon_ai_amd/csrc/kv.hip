@@ -892,6 +892,10 @@ struct Unpacked {
     __device__ static __forceinline__ int v_at(int d, int half, int lane) { return (2 * d + half) * 1024 + (lane ^ (16 * (d & 3))); }
 };
 constexpr int kManyRows = 128;
+// Scores as powers of two. The running maximum is a rounded product, from which the others may differ by half its step before they are
+// rounded: below kFar 2^-5, in every term of the row alike, from 2^33 on more than a power can hold. A row whose maximum is so far
+// from zero is gone over again (as for NaN, below) with scores rounded as the maximum was, so that none is above it.
+constexpr float kFar = 1 << 20;
 
 template <int DH, class T, int HALVES>
 __global__ __launch_bounds__(256 * HALVES, 2) void kv_attention_chunk_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles) {
@@ -1065,7 +1069,8 @@ __global__ __launch_bounds__(256 * HALVES, 2) void kv_attention_chunk_kernel(KvA
         const float mu = m == -INFINITY ? 0.0f : m;
         float pr[16];
 #pragma unroll
-        for (int r = 0; r < 16; r++) pr[r] = __builtin_amdgcn_exp2f(fmaf(d[r], scale, -mu));
+        for (int r = 0; r < 16; r++)
+            pr[r] = __builtin_amdgcn_exp2f(decltype(careful)::value && fabsf(mu) >= kFar ? d[r] * scale - mu : fmaf(d[r], scale, -mu));
         float sum[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) sum[r] = (pr[r] + pr[4 + r]) + (pr[8 + r] + pr[12 + r]);
@@ -1116,13 +1121,13 @@ __global__ __launch_bounds__(256 * HALVES, 2) void kv_attention_chunk_kernel(KvA
     };
     sweep(std::false_type());
     {
-        // A NaN among the sums: it may come from a value that the row does not see.
+        // A NaN among the sums: it may come from a value that the row does not see. Or scores far from zero.
         float bad = 0.0f;
 #pragma unroll
         for (int x = 0; x < ND; x++)
 #pragma unroll
             for (int r = 0; r < 16; r++) bad += acc[x][r] * 0.0f;
-        if (__syncthreads_or(bad != 0.0f)) {
+        if (__syncthreads_or(bad != 0.0f || (m != -INFINITY && fabsf(m) >= kFar))) {
             sweep(std::true_type());
             nan_blocks |= __shfl_xor(nan_blocks, 32, 64);
 #pragma unroll
