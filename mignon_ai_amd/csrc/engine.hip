@@ -2641,10 +2641,10 @@ int mg_quantize_f32(const float* w, long long n, int8_t* q, float* scale, int fl
 int mg_mx4_quantize(const void* x, int type, int M, int K, long long ldx, uint8_t* codes, uint8_t* scales, int flags,
                     void* stream) {
     return guarded([&] {
-        REQUIRE(x && codes && scales, "mg_mx4_quantize: null argument");
         REQUIRE(real_type(type), "mg_mx4_quantize: unknown type");
         REQUIRE(M >= 0 && K > 0 && K <= kMx4MaxK && ldx >= K, "mg_mx4_quantize: bad shape");
-        if (M == 0) return MG_OK;
+        if (M == 0) return MG_OK;  // (an empty tensor has no address)
+        REQUIRE(x && codes && scales, "mg_mx4_quantize: null argument");
         hipStream_t st = (hipStream_t)stream;
         const bool dev = flags & MG_PTR_DEVICE;
         const size_t e = real_size(type), kp = round_up(K, 128), nc = M * (kp / 2), ns = M * (kp / 32);
@@ -2673,10 +2673,10 @@ int mg_mx4_quantize(const void* x, int type, int M, int K, long long ldx, uint8_
 int mg_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* y, int type, long long ldy, int flags,
                       void* stream) {
     return guarded([&] {
-        REQUIRE(y && codes && scales, "mg_mx4_dequantize: null argument");
         REQUIRE(real_type(type), "mg_mx4_dequantize: unknown type");
         REQUIRE(M >= 0 && K > 0 && K <= kMx4MaxK && ldy >= K, "mg_mx4_dequantize: bad shape");
         if (M == 0) return MG_OK;
+        REQUIRE(y && codes && scales, "mg_mx4_dequantize: null argument");
         hipStream_t st = (hipStream_t)stream;
         const bool dev = flags & MG_PTR_DEVICE;
         const size_t e = real_size(type), kp = round_up(K, 128), nc = M * (kp / 2), ns = M * (kp / 32);
@@ -2699,10 +2699,10 @@ int mg_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K,
 int mg_mx4_gemm(const uint8_t* A, const uint8_t* As, int M, int K, const uint8_t* W, const uint8_t* Ws, int N, void* C,
                 int type, int flags, void* stream) {
     return guarded([&] {
-        REQUIRE(A && As && W && Ws && C, "mg_mx4_gemm: null argument");
         REQUIRE(real_type(type), "mg_mx4_gemm: unknown type");
         REQUIRE(M >= 0 && K > 0 && K <= kMx4MaxK && N > 0 && N <= kMx4MaxK, "mg_mx4_gemm: bad shape");
         if (M == 0) return MG_OK;
+        REQUIRE(A && As && W && Ws && C, "mg_mx4_gemm: null argument");
         hipStream_t st = (hipStream_t)stream;
         const bool dev = flags & MG_PTR_DEVICE;
         const size_t e = real_size(type), kp = round_up(K, 128), out = (size_t)M * N * e;

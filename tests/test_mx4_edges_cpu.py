@@ -1,0 +1,16 @@
+"""The 4-bit calls' C ABI on a machine without a GPU: calls without rows, and sizes that no launch takes."""
+from mignon_ai_amd import _lib
+
+INVALID = _lib.MG_ERR_INVALID
+
+
+def test_matrices_without_rows_need_no_memory():
+    """An empty tensor has no address. What such a call says about types and shapes is checked all the same."""
+    L = _lib.lib()
+    q = lambda M=0, K=64, ty=0: L.mg_mx4_quantize(None, ty, M, K, K, None, None, _lib.MG_PTR_DEVICE, None)  # noqa: E731
+    d = lambda M=0, K=64, ty=0: L.mg_mx4_dequantize(None, None, M, K, None, ty, K, _lib.MG_PTR_DEVICE, None)  # noqa: E731
+    g = lambda M=0, K=64, ty=0: L.mg_mx4_gemm(None, None, M, K, None, None, 8, None, ty, _lib.MG_PTR_DEVICE, None)  # noqa: E731
+    for f in (q, d, g):
+        assert f() == 0
+        for bad in (dict(K=0), dict(ty=7), dict(M=-1), dict(M=1)):
+            assert f(**bad) == INVALID, bad
