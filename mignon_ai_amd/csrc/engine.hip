@@ -2709,6 +2709,7 @@ int mg_mx4_gemm(const uint8_t* A, const uint8_t* As, int M, int K, const uint8_t
         Staging sg;
         Mx4GemmArgs a;
         a.M = M; a.N = N; a.Kp = (int)kp; a.type = type;
+        REQUIRE(mx4_gemm_fits(a), "mg_mx4_gemm: too many rows and channels");
         a.A = dev ? A : sg.in(A, M * (kp / 2), st);
         a.As = dev ? As : sg.in(As, M * (kp / 32), st);
         a.W = dev ? W : sg.in(W, N * (kp / 2), st);

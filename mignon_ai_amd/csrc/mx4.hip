@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <type_traits>
 
 #include "common.hpp"
@@ -406,7 +407,6 @@ hipError_t launch_lds_gemm(const Mx4GemmArgs& a, hipStream_t s) {
     static std::atomic<uint64_t> allowed{0};
     if (const hipError_t e = allow_lds((const void*)mx4_gemm_lds_kernel<S, T>, S::lds, allowed); e != hipSuccess) return e;
     const int tn = (a.N + S::TN - 1) / S::TN, tm = (a.M + S::TM - 1) / S::TM;
-    if ((long long)tn * tm >= 1 << 22) return hipErrorInvalidValue;  // beyond a launch's 2^32 lanes with the widest workgroup
     hipLaunchKernelGGL((mx4_gemm_lds_kernel<S, T>), dim3(xcd_grid(tn * tm)), dim3(S::NW * 64), S::lds, s, a, tn, tm);
     return hipGetLastError();
 }
@@ -443,25 +443,42 @@ hipError_t launch_mx4_dequantize(const Mx4RowsArgs& a, hipStream_t s) {
     });
 }
 
+namespace {
+// The largest tile of which there are enough for three quarters of the 256 CUs and which the shape fills to four fifths;
+// where even those of 64 x 64 are too few (0), K is split. us at M x N x K, 256 / 128 / 64 tiles, split 32 x 32 and 16 x 16:
+//   16384 x 4096 x 4096: 158 194 296;     3584 x 3584 x 4096: 38 46;    4096 x 2048 x 4096: 35 28;    4096 x 4096 x 384: 12.5 14 22.5
+//   2048 x 2048 x 4096: 31 19.5 21.9 56;    1536 x 1024 x 2048: - 10.3 7.3;    1001 x 2048 x 1152: 12.2 7.8 6.1 10.6 15.4
+//   256 x 4096 x 4096: 28 15.9 9.1 14.5 19.5;    128 x 4096 x 4096: 28 15.6 8.4 8 10.9;    300 x 300 x 8192: 51 27 13.3 5.6 5.4
+//   8 x 4096 x 4096: 27 15 8 3.9 3;    16 x 8192 x 4096: 27 15 8.2 4.6 3.9
+int gemm_tile(const Mx4GemmArgs& a) {
+    if (a.M <= 16) return 0;
+    for (const int tile : {256, 128, 64}) {
+        const long long n = (a.N + tile - 1) / tile, m = ((long long)a.M + tile - 1) / tile;
+        if (n * m >= 192 && (tile == 64 || 4.0 * n * m * tile * tile <= 5.0 * a.M * a.N)) return tile;
+    }
+    return 0;
+}
+}  // namespace
+
+// A launch has fewer than 2^32 lanes (and whole eights of workgroups); a tile's rows past the last one have numbers, too.
+bool mx4_gemm_fits(const Mx4GemmArgs& a) {
+    const int tile = gemm_tile(a);
+    if (!tile) return true;
+    const long long n = (a.N + tile - 1) / tile, m = ((long long)a.M + tile - 1) / tile;
+    return n * m <= (tile == 256 ? 1 << 23 : 1 << 24) - 8 && a.M < INT_MAX - 256;
+}
+
 hipError_t launch_mx4_gemm(const Mx4GemmArgs& a, hipStream_t s) {
-    if (a.M <= 0 || a.N <= 0 || a.Kp <= 0 || a.Kp % 128) return hipErrorInvalidValue;
-    // The largest tile of which there are enough for three quarters of the 256 CUs and which the shape fills to four fifths;
-    // where even those of 64 x 64 are too few, K is split. us at M x N x K, 256 / 128 / 64 tiles, split 32 x 32 and 16 x 16:
-    //   16384 x 4096 x 4096: 158 194 296;     3584 x 3584 x 4096: 38 46;    4096 x 2048 x 4096: 35 28;    4096 x 4096 x 384: 12.5 14 22.5
-    //   2048 x 2048 x 4096: 31 19.5 21.9 56;    1536 x 1024 x 2048: - 10.3 7.3;    1001 x 2048 x 1152: 12.2 7.8 6.1 10.6 15.4
-    //   256 x 4096 x 4096: 28 15.9 9.1 14.5 19.5;    128 x 4096 x 4096: 28 15.6 8.4 8 10.9;    300 x 300 x 8192: 51 27 13.3 5.6 5.4
-    //   8 x 4096 x 4096: 27 15 8 3.9 3;    16 x 8192 x 4096: 27 15 8.2 4.6 3.9
-    const auto takes = [&](int tile) {
-        const long long n = (a.N + tile - 1) / tile, m = (a.M + tile - 1) / tile;
-        return n * m >= 192 && (tile == 64 || 4.0 * n * m * tile * tile <= 5.0 * a.M * a.N);
-    };
+    if (a.M <= 0 || a.N <= 0 || a.Kp <= 0 || a.Kp % 128 || !mx4_gemm_fits(a)) return hipErrorInvalidValue;
     return by_real(a.type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         if (a.M <= 16) return launch_split_gemm<MxSplit<1, 1, 8>, T>(a, s);
-        if (takes(256)) return launch_lds_gemm<MxTile<256, 256, 2, 4, 2>, T>(a, s);
-        if (takes(128)) return launch_lds_gemm<MxTile<128, 128, 2, 2, 2>, T>(a, s);
-        if (takes(64)) return launch_lds_gemm<MxTile<64, 64, 2, 2, 4>, T>(a, s);
-        return launch_split_gemm<MxSplit<2, 2, 8>, T>(a, s);
+        switch (gemm_tile(a)) {
+            case 256: return launch_lds_gemm<MxTile<256, 256, 2, 4, 2>, T>(a, s);
+            case 128: return launch_lds_gemm<MxTile<128, 128, 2, 2, 2>, T>(a, s);
+            case 64: return launch_lds_gemm<MxTile<64, 64, 2, 2, 4>, T>(a, s);
+            default: return launch_split_gemm<MxSplit<2, 2, 8>, T>(a, s);
+        }
     });
 }
 

@@ -33,6 +33,7 @@ struct Mx4GemmArgs {
     void* C = nullptr;            // [M][N]
     int type = REAL_F32;
 };
+bool mx4_gemm_fits(const Mx4GemmArgs& a);  // a launch takes it
 hipError_t launch_mx4_gemm(const Mx4GemmArgs& a, hipStream_t s);
 
 // Rows of a cache call: element (sequence s, token t, head h, channel d) at data + s * seq + t * token + h * head + d.

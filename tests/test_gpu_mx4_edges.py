@@ -21,3 +21,17 @@ def test_matrices_without_rows():
         mx4_gemm_device(*rows, *_device4(5, 300), torch.empty((0, 5), device="cuda"))
     with pytest.raises(MignonError):
         mx4_quantize_device(x, *_device4(0, 300))
+
+
+def test_product_of_more_than_four_million_tiles():
+    """2^28 rows of one step by one tile's channels: the last rows' products in their place, and nothing behind them."""
+    M, K, N = (1 << 28) + 70, 128, 64
+    A, As = torch.zeros((M, K // 2), dtype=torch.uint8, device="cuda"), torch.full((M, K // 32), 127, dtype=torch.uint8, device="cuda")
+    W, Ws = torch.full((N, K // 2), 0x22, dtype=torch.uint8, device="cuda"), torch.full((N, K // 32), 127, dtype=torch.uint8, device="cuda")
+    Ws += torch.arange(N, dtype=torch.uint8, device="cuda")[:, None] % 8
+    A[-3:] = 0x24  # pairs of 2 and 1
+    C = torch.full((M + 1, N), 9.0, dtype=torch.bfloat16, device="cuda")
+    mx4_gemm_device(A, As, W, Ws, C[:M])
+    want = 192 * 2.0 ** (torch.arange(N, device="cuda") % 8)
+    assert bool((C[M - 3:M].float() == want).all()) and bool((C[M] == 9.0).all())
+    assert all(not bool(c.any()) for c in C[:M - 3].split(1 << 26))

@@ -14,3 +14,11 @@ def test_matrices_without_rows_need_no_memory():
         assert f() == 0
         for bad in (dict(K=0), dict(ty=7), dict(M=-1), dict(M=1)):
             assert f(**bad) == INVALID, bad
+
+
+def test_products_of_more_tiles_than_a_launch_has_lanes():
+    """The refusal names its cause and comes before the device is touched."""
+    L, p = _lib.lib(), 1 << 20
+    for M, N in (((1 << 30) + 1, 64), ((1 << 31) - 1, 8), ((1 << 31) - 1, 1 << 12), (1 << 27, 1 << 24)):
+        assert L.mg_mx4_gemm(p, p, M, 128, p, p, N, p, 0, _lib.MG_PTR_DEVICE, None) == INVALID, (M, N)
+        assert b"mg_mx4_gemm: too many" in L.mg_last_error()
