@@ -925,8 +925,9 @@ __global__ __launch_bounds__(256 * HALVES, 2) void kv_attention_chunk_kernel(KvA
     seen.hi_at = q.pos + t_hi;
     const Tiles tl = tiles_of(seen, a.c.cap);
     const int n_tiles = tl.count();
-    const int o0 = blockIdx.y * chunk_tiles, o1 = min(n_tiles, o0 + chunk_tiles);
-    if (blockIdx.y && o0 >= n_tiles) return;
+    // (four waves have their rows to themselves: only eight are given a chunk of the tiles)
+    const int o0 = HALVES > 1 ? blockIdx.y * chunk_tiles : 0, o1 = HALVES > 1 ? min(n_tiles, o0 + chunk_tiles) : n_tiles;
+    if (HALVES > 1 && blockIdx.y && o0 >= n_tiles) return;
 
     // loads of a tile: wave w has its w'th KiB, and one wave the scales
     constexpr int scale_wave = W::KS & 3;
@@ -1166,7 +1167,7 @@ __global__ __launch_bounds__(256 * HALVES, 2) void kv_attention_chunk_kernel(KvA
     }
     if (!there) return;
     // lane (i, g): row i, channels 32 x + 8 r + 4 g .. + 3
-    if (n_tiles > chunk_tiles) {
+    if (HALVES > 1 && n_tiles > chunk_tiles) {
         float* part = a.ws + (((size_t)blockIdx.y * gridDim.x + unit) * kManyRows + wave * 32 + i) * kPart<DH>;
 #pragma unroll
         for (int x = 0; x < ND; x++)
@@ -1216,9 +1217,10 @@ AttnPlan attn_plan(const KvAttnArgs& a) {
     // to share, 256 x 64 tokens, 10 and 14)
     p.waves = p.many ? (p.units <= 512 && tiles >= 16 ? 8 : 4) : tiles <= 4 ? 1 : 4;
     p.chunk_tiles = tiles;
-    if (p.waves > 1) {
-        // Two workgroups a CU (one of eight waves), each with four tiles a wave at least (sixteen a workgroup of many rows). More, smaller chunks cost more at their ends
-        // than they even out (256 conversations, their window in one chunk or two: 28.8 or 37.7 us).
+    if (p.many ? p.waves == 8 : p.waves > 1) {
+        // Two workgroups a CU (one of eight waves), each with four tiles a wave at least (sixteen a workgroup of many rows). More,
+        // smaller chunks cost more at their ends than they even out (256 conversations, their window in one chunk or two: 28.8 or
+        // 37.7 us). Many rows on four waves have more workgroups than that, or few tiles.
         const int want = std::max(1, (p.waves == 8 ? 256 : 512) / p.units);
         p.chunk_tiles = std::max(16, (tiles + want - 1) / want);
     }
@@ -1270,9 +1272,11 @@ hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
         return by_real(a.type, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
             if (p.many) {
-                const dim3 grid(p.units, p.chunks);
-                if (p.waves == 8) hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T, 2>), grid, dim3(512), 0, s, a, p.row_tiles, p.chunk_tiles);
-                else hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T, 1>), grid, dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles);
+                if (p.waves == 4) {
+                    hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T, 1>), dim3(p.units), dim3(256), 0, s, a, p.row_tiles, p.chunk_tiles);
+                    return hipGetLastError();
+                }
+                hipLaunchKernelGGL((kv_attention_chunk_kernel<DH, T, 2>), dim3(p.units, p.chunks), dim3(512), 0, s, a, p.row_tiles, p.chunk_tiles);
                 return launch_join<DH, T>(a, p, s);
             }
             if (p.hb == most) return launch_rows_attention<DH, T, most>(a, p, s);
