@@ -46,3 +46,43 @@ def test_scores_far_apart(form, t, dh, group, power):
             tol = np.abs(want) * (2.0 ** -P_BITS[t] + 2.0 ** -21 + torch.finfo(t).eps / 2)
             assert (np.abs(got[0, i, h] - want) <= tol).all(), (i, h, got[0, i, h], want)
     assert sure >= 0.9 * T * H * group
+
+
+# tokens a sequence, capacity, length, window
+SPOILT = {"wave": (1, 64, 60, 20), "waves": (1, 1024, 900, 400), "waves_wrapped": (1, 512, 700, 380), "waves_joined": (1, 8192, 5000, 4000),
+          "rows": (9, 256, 200, 70), "many": (40, 128, 100, 30), "many_halves": (40, 1024, 900, 380), "many_wrapped": (40, 512, 700, 380),
+          "many_joined": (40, 8192, 5000, 4000)}
+
+
+@pytest.mark.parametrize("form", list(SPOILT))
+@pytest.mark.parametrize("t", list(P_BITS))
+@pytest.mark.parametrize("dh", [32, 64, 96, 128])
+def test_nan_reaches_only_the_rows_that_see_it(form, t, dh):
+    """Blocks of NaN and infinity next to the window's end, where some rows have lost them, further on, and where only the last rows
+    have them; slots that were never written are NaN in both caches. What does not see them has the same bits as without."""
+    T, cap, L, window = SPOILT[form]
+    n, H, G, lo = 3, 2, 2, L - T - window + 1  # the first row's first position
+    k, v = _rows((n, L, H, dh), 1), _rows((n, L, H, dh), 2)
+    plain, spoilt = Pair(n, H, dh, cap), Pair(n, H, dh, cap)
+    plain.c.write(k, v, _ints([0] * n))
+    keys = [(0, lo - 1, 0), (1, L - T + T // 2, 0)]  # sequence, position, head
+    values = [(0, lo - 1, 1, dh - 1), (0, lo + T // 3, 0, 0), (2, L - T + T // 2, 1, dh - 32), (2, lo + window // 2, 0, dh // 2),
+              (2, min(lo + window // 2 + 32, L - 1), 1, 31), (1, L - 1, 1, dh - 1)]  # and channel
+    for i, (s, p, h) in enumerate(keys):
+        k[s, p, h, 7 * i] = (np.nan, -np.inf)[i]
+    for i, (s, p, h, c) in enumerate(values):
+        v[s, p, h, c] = (np.inf, np.nan, -np.inf)[i % 3]
+    spoilt.c.write(k, v, _ints([0] * n))
+    q = _rows((n, T, H * G, dh), 3, t)
+    a, b = (x.c.attention(q, torch.full_like(q, 55.0), _ints([L - T] * n), window=window) for x in (plain, spoilt))
+    bad = np.zeros(q.shape, bool)
+    for i in range(T):
+        p = L - T + i
+        for s, j, h in keys:
+            bad[s, i, h * G:(h + 1) * G] |= p - window < j <= p
+        for s, j, h, c in values:
+            bad[s, i, h * G:(h + 1) * G, c // 32 * 32:c // 32 * 32 + 32] |= p - window < j <= p
+    bad = torch.from_numpy(bad).cuda()
+    assert bool(torch.isfinite(a).all())
+    assert torch.equal(torch.isnan(b), bad)
+    assert torch.equal(b[~bad], a[~bad])
