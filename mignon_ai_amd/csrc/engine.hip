@@ -2565,9 +2565,10 @@ long long mg_sessions_device_bytes(const mg_sessions* s) {
     if (!s) return -1;
     const mg_model* m = s->m;
     // packed rings: 3 bytes per element and a 4-byte scale per (head, slot) row of each ring
-    // 4-bit: half a byte per element and a byte per 32
+    // 4-bit: half a byte per element and a byte per 32, and a share of the decode attention's workspace
     if (s->kv_mx4)
-        return (long long)m->nbs * (m->ring + 1) * m->Dp * 4 + (long long)m->nattn * 2 * s->kv_cap * (m->D / 2 + m->D / 32) + 8;
+        return (long long)m->nbs * (m->ring + 1) * m->Dp * 4 + (long long)m->nattn * 2 * s->kv_cap * (m->D / 2 + m->D / 32) +
+               ((long long)s->kv_ws.n + s->n - 1) / s->n + 8;
     const long long rings = s->kv_packed ? (long long)m->nattn * 2 * m->cap * ((long long)m->D * 3 + m->heads * 4)
                                          : (long long)m->nattn * 2 * m->cap * m->D * 4;
     return (long long)m->nbs * (m->ring + 1) * m->Dp * 4 + rings + 8;

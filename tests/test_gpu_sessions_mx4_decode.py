@@ -3,8 +3,8 @@ set holds."""
 import numpy as np
 import pytest
 
-from helpers import model_bytes
-from mignon_ai_amd import Model, engine_option, synth
+from helpers import model_bytes, uniform_model_bytes
+from mignon_ai_amd import Model, _lib, engine_option, synth
 from test_gpu_sampling import _replay
 
 pytestmark = pytest.mark.gpu
@@ -60,3 +60,19 @@ def test_sampled_replies(restore, kernel):
     want = _replay(Mx4(m), prompts, lens, G, seeds, *args, set(stops))
     ids, counts = m.sessions(S, kv="mx4").decode_sample(prompts, G, seeds, *args, stops, lens)
     assert [ids[i, :counts[i]].tolist() for i in range(S)] == want and counts.min() < G
+
+
+def test_device_bytes_count_the_attention_workspace():
+    """Few sessions of a long window split their histories, for which the set holds memory: a share of it is each session's."""
+    import ctypes
+    heads, dh, context = 2, 32, 4096
+    m = Model(uniform_model_bytes(synth.ModelSpec(V=64, D=heads * dh, H=64, blocks=[synth.BlockSpec(1, 2, 1)], heads=heads, window=0,
+                                                  context=context), 5, 0.1))
+
+    def workspace(n):
+        c = _lib.KvCache(n, heads, dh, context, 0, *(4 * (1 << 20,)))
+        return _lib.lib().mg_kv_attention_workspace(ctypes.addressof(c), heads, 1, context)
+
+    assert workspace(3) > 0 and workspace(600) == 0
+    a, b = (m.sessions(n, kv="mx4").device_bytes() for n in (3, 600))
+    assert a - b == -(-workspace(3) // 3)
