@@ -1204,7 +1204,7 @@ AttnPlan attn_plan(const KvAttnArgs& a) {
     // heads a wave takes together: as many as give it 8 rows or fewer
     p.hb = rows * most <= kRows && a.c.heads % most == 0 ? most : rows * 2 <= kRows && a.c.heads % 2 == 0 ? 2 : 1;
     p.per = p.many ? kManyRows : kRows;
-    p.row_tiles = (rows + p.per - 1) / p.per;
+    p.row_tiles = (rows - 1) / p.per + 1;  // (rows are fewer than 2^31, but not by a tile)
     p.units = a.c.n * (a.c.heads / p.hb) * p.row_tiles;
     // tiles that a row tile can see, at most: the sinks', and the window's (or the ring's), with the ends of three runs
     const long long span = a.window > 0 ? std::min<long long>((long long)a.window + p.per / a.group + 1, a.c.cap) : a.c.cap;

@@ -1,4 +1,6 @@
 """The 4-bit calls' C ABI on a machine without a GPU: calls without rows, and sizes that no launch takes."""
+import ctypes
+
 from mignon_ai_amd import _lib
 
 INVALID = _lib.MG_ERR_INVALID
@@ -22,3 +24,13 @@ def test_products_of_more_tiles_than_a_launch_has_lanes():
     for M, N in (((1 << 30) + 1, 64), ((1 << 31) - 1, 8), ((1 << 31) - 1, 1 << 12), (1 << 27, 1 << 24)):
         assert L.mg_mx4_gemm(p, p, M, 128, p, p, N, p, 0, _lib.MG_PTR_DEVICE, None) == INVALID, (M, N)
         assert b"mg_mx4_gemm: too many" in L.mg_last_error()
+
+
+def test_attention_of_nearly_two_to_the_31_rows():
+    """A last tile of rows that would pass 2^31 is refused like any call of too many."""
+    c = _lib.KvCache(1, 1, 32, 64, 0, *(4 * (1 << 20,)))
+    ws = lambda T, heads: _lib.lib().mg_kv_attention_workspace(ctypes.addressof(c), heads, T, 0)  # noqa: E731
+    assert ws((1 << 30) - 1, 2) == INVALID      # 2^31 - 2 rows
+    assert ws((1 << 30) - 64, 2) == 0           # one launch
+    assert ws((1 << 30) - 63, 2) == INVALID
+    assert ws(((1 << 31) - 1) // 7, 7) == INVALID
