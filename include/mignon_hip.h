@@ -123,7 +123,7 @@ int mg_sessions_create(mg_model* m, int n, int context, mg_sessions** out);
  * written (to within a quarter of the largest of their 32 neighbours, most of them far closer), and decode steps attend over
  * the rounded ones; prefill attends over the prompt's own, so that the logits after a prompt are those of any set. Steps run
  * layer by layer or in tiles of 16 sessions, with the attention between. Heads of width 32, 64, 96 or 128;
- * MG_ERR_UNSUPPORTED otherwise. All mg_sessions_* calls take the set. */
+ * MG_ERR_UNSUPPORTED otherwise. All mg_sessions_* calls take the set. A session's positions stay below 2^30. */
 int mg_sessions_create_mx4(mg_model* m, int n, int context, mg_sessions** out);
 
 /* quantSession.Prefill for every session at once (internal/quant/session.go:30-39): prompts
@@ -310,7 +310,7 @@ int mg_quantize_f32(const float* w, long long n, int8_t* q, float* scale, int fl
  * ties to the even code, beyond 6 to 6; a block with a NaN or an infinity is NaN (s = 255).
  * A matrix of M rows of K elements has its rows padded with zeros to Kp, the next multiple of 128: codes [M][Kp / 2] and
  * scales [M][Kp / 32]. Device pointers: codes 16-byte aligned, scales 4-byte aligned, real arrays aligned to their element.
- * Types of real arrays: */
+ * K up to 2^24. M = 0 does nothing, and needs no memory. Types of real arrays: */
 #define MG_F32 0
 #define MG_F16 1
 #define MG_BF16 2
@@ -323,7 +323,8 @@ int mg_mx4_quantize(const void* x, int type, int M, int K, long long ldx, uint8_
 int mg_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* y, int type, long long ldy, int flags,
                       void* stream);
 /* C[m][n] = sum_k A[m][k] W[n][k] for two 4-bit matrices A [M][K] and W [N][K] (both padded as above), summed in fp32 and
- * rounded once to C's type: the 4-bit counterpart of mg_gemm_i8. C [M][N]. */
+ * rounded once to C's type: the 4-bit counterpart of mg_gemm_i8. C [M][N], N up to 2^24, of fewer than 2^24 tiles of 64 x 64 to
+ * 128 x 128 (2^23 of 256 x 256 for large products). */
 int mg_mx4_gemm(const uint8_t* A, const uint8_t* As, int M, int K, const uint8_t* W, const uint8_t* Ws, int N, void* C,
                 int type, int flags, void* stream);
 
@@ -332,7 +333,9 @@ int mg_mx4_gemm(const uint8_t* A, const uint8_t* As, int M, int K, const uint8_t
  * Position p < sinks (0 <= sinks < capacity) has slot p for good; a later one has slot sinks + (p - sinks) % ring, with
  * ring = capacity - sinks: of the positions below a sequence's length, the cache holds the first `sinks` and the last `ring`.
  * Planes, 16-byte aligned: k and v codes [n][heads][capacity][head_dim / 2], k_scales and v_scales
- * [n][heads][capacity][head_dim / 32]. Memory of any contents may be used: what was not written is not seen.
+ * [n][heads][capacity][head_dim / 32]. Memory of any contents may be used: what was not written is not seen. What is seen was
+ * written by mg_kv_write, or has no scale bytes but its (up to 252, and 255): 253 and 254 stand for numbers past fp32's range, and
+ * attention may take a block with them as NaN.
  * The caller owns the planes and keeps count of the positions. All pointers of these calls but the structs are device
  * pointers; the calls enqueue work on `stream`, allocate nothing and can be captured. */
 typedef struct {
@@ -357,10 +360,11 @@ int mg_kv_read(const mg_kv_cache_t* cache, const mg_kv_rows_t* k, const mg_kv_ro
 /* Causal attention of query rows [n][T][q_heads][head_dim] (q_heads a multiple of the cache's heads; query head i reads head
  * i / (q_heads / heads)) over the cache, after the call's own keys were written: sequence s has length pos[s] + counts[s], and
  * the row at position p sees the held positions j <= p with j > p - window, or any if window <= 0, and those with j < sinks.
- * out = sum softmax(scale q.k) v, zeros for a row that sees nothing; statistics and sums in fp32. Rows past counts[s] are left
- * as they are. A NaN or infinity in a key or value reaches the rows that see it only. workspace: device memory of
- * mg_kv_attention_workspace bytes, 16-byte aligned, for this call alone until it has run (calls that may overlap, and captured
- * graphs that may, need one each); may be NULL where that is 0. */
+ * out = sum softmax(scale q.k) v, zeros for a row that sees nothing; scores, statistics and sums in fp32, probabilities held to 24
+ * bits for the product with v (MG_F32) or to 16 (MG_F16, MG_BF16). Rows past counts[s] are left as they are. A NaN or infinity in a
+ * key or value reaches the rows that see it only. workspace: device memory of mg_kv_attention_workspace bytes, 16-byte aligned, for
+ * this call alone until it has run (calls that may overlap, and captured graphs that may, need one each); may be NULL where that
+ * is 0. */
 long long mg_kv_attention_workspace(const mg_kv_cache_t* cache, int q_heads, int T, int window);
 int mg_kv_attention(const mg_kv_cache_t* cache, const mg_kv_rows_t* q, const mg_kv_rows_t* out, int type, int q_heads, int T,
                     const int32_t* pos, const int32_t* counts, int window, float scale, void* workspace,

@@ -356,8 +356,8 @@ bool kv_rings_packed(const mg_model* m, int n) {
 
 // The 4-bit cache of attention block ab of a set. A step writes and attends in two launches and puts the output's limbs in a
 // third, where the other formats take one: that costs small sets (16 sessions of two blocks of 4 heads of 32 and 64 slots: 48 ->
-// 89 us a step, most of it the lost one-workgroup step), and 4096 sessions gain what their rings are smaller by (three blocks of
-// 8 heads of 32: 411 -> 271 us; four of 6 heads of 64: 1299 -> 824).
+// 88 us a step, most of it the lost one-workgroup step), and 4096 sessions gain what their rings are smaller by (three blocks of
+// 8 heads of 32: 412 -> 271 us; four of 6 heads of 64: 1303 -> 821).
 KvCache mx4_cache(mg_sessions* s, int ab) {
     const mg_model* m = s->m;
     KvCache c;

@@ -32,9 +32,9 @@ __device__ __forceinline__ int kv_slot(int p, int sinks, int ring) { return p < 
 // One launch for keys and values (blockIdx.z), a workgroup for 256 / (DH / 8) tokens of U heads (blockIdx.y): DH / 8 lanes a row, four
 // to a block, a lane's U rows loaded before the first is worked on. Tokens that follow each other fill whole lines of codes and
 // scales, and a token's heads are read side by side (32768 tokens of 8 bf16 heads of 128 written: one head a
-// workgroup 53 us, four 44; read back 28 and 27). Bound by memory: 16 prompts of 1 to 2048 such tokens, 55 MB each way, 16.6 us
-// (3.3 TB/s) and 13 (4.2); a decode step's 4096 tokens of 8 fp32 heads of 32 take 4.9 and 5.7 us, the latency of position, row and
-// store after each other.
+// workgroup 53 us, four 44; read back 28 and 27). Bound by memory: 16 prompts of 1 to 2048 such tokens, 55 MB each way, 16 us
+// (3.5 TB/s) and 13 (4.2); a decode step's 4096 tokens of 8 fp32 heads of 32 take 4.9 and 5.3 us, the latency of position, row and
+// store after each other (of a write's row only the place depends on the position: it could be asked for at once).
 struct RowsSpot {
     int s, t, slot;  // slot -1: nothing there (a write: no row; a read: zeros), t -1: no row
 };
@@ -598,10 +598,10 @@ struct Stages {
 // they have in LDS; with WAVES 1 a wave is alone with its rows.
 //
 // Bound by reading the cache, with the unpacking close behind. 32 conversations of 16384 positions (8 heads of 128, four query
-// heads each, bf16): 5.8 TB/s; of 1 to 16384 positions, 276 MB, 72 us with the join (3.8 TB/s: the lengths do not divide evenly
-// over the chip); 256 windows of 1000 (8 heads of 64, two query heads each, fp16, 109 MB) 29 us; 4096 windows of 64 (8 fp32 heads
-// of 32, 57 MB) 24 us, where a wave's life is mostly its first tiles' latency; one conversation of 30000 (33 MB) 18 us with the
-// join, the latency of a chunk's sixteen tiles and of a second launch.
+// heads each, bf16): 101 us, 5.6 TB/s; of 1 to 16384 positions, 276 MB, 71 us (3.9 TB/s: the lengths do not divide evenly over the
+// chip) and 4.5 for the join; 256 windows of 1000 (8 heads of 64, two query heads each, fp16, 109 MB) 29 us; 4096 windows of 64 (8 fp32 heads
+// of 32, 57 MB) 24 us, where a wave's life is mostly its first tiles' latency; one conversation of 30000 (33 MB) 13 us and 6 for the
+// join: two heads a wave make 236 workgroups of it, where 512 have room, each with sixteen tiles one after another.
 template <int DH, class T, int HB, int WAVES>
 __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles) {
     using W = Width<DH>;
@@ -817,7 +817,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a,
 }
 
 // Joins the chunks of a row that took more than one: a wave a row, its lanes over channels (four each) and, in as many groups as fit,
-// over the chunks, whose sums are added in a fixed order. Units have `per` rows. (4.6 us for 32 conversations of 32 query heads, 6 for
+// over the chunks, whose sums are added in a fixed order. Units have `per` rows. (4.5 us for 32 conversations of 32 query heads, 6 for
 // the 59 chunks of one long one: its latency.)
 template <int DH, class T>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, int per, int hb, int row_tiles, int chunk_tiles) {
@@ -880,9 +880,11 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(KvAttnArgs a, in
 // 2 (s & 3), of V's by 4 g and d & 3.
 //
 // Bound by issuing instructions: 2 x 1024 tokens of 32 query heads over 8 of 128, lengths up to 8192 and 6000 positions in sight, bf16:
-// 244 us, 473 TFLOP/s of scores and output (the output's products are done twice, for the probabilities' two parts; 68 % of all
-// cycles issue something, the matrix units are busy for 28 %). With one part, probabilities
-// held to 8 bits, 252 us instead of 291 with four waves, and an error of 2.0e-3 instead of 1.7e-3 of bf16 outputs: not taken.
+// 243 us between other calls, 252 in a row of forty, 473 and 457 TFLOP/s of scores and output (the output's products are done twice,
+// for the probabilities' two parts; 68 % of all cycles issue something, the matrix units are busy for 28 %). With one part,
+// probabilities held to 8 bits, 13 % less with four waves, and an error of 2.0e-3 instead of 1.7e-3 of bf16 outputs: not taken.
+// fp32 and fp16 rows of 128 channels do not fit the registers whole (40 to 48 of them go to memory and back, one of fp16): 2 x 1024
+// tokens over 8192 positions each take 695 and 537 us where bf16 takes 492.
 template <int DH>
 struct Unpacked {
     static constexpr int k = 64 * DH, bytes = 2 * k;
@@ -1198,8 +1200,8 @@ struct AttnPlan {
 AttnPlan attn_plan(const KvAttnArgs& a) {
     AttnPlan p;
     const int rows = a.T * a.group, most = a.c.dh == 32 ? 8 : a.c.dh == 64 ? 4 : 2;
-    // (32 conversations of 4096 positions, 32 heads of 128 over 8, 24 and 32 rows a head: 88 and 115 us eight rows a wave, 109 us in
-    // both with many; 64 of 2048, fp32 heads of 64: 65 and 84, 93 and 94)
+    // (32 conversations of 4096 positions, 32 heads of 128 over 8, bf16, 24 and 32 rows a head: 90 and 120 us eight rows a wave, 129
+    // in both with many; 64 of 2048, fp32 heads of 64: 62 and 88, 124 in both)
     p.many = rows > 32;
     // heads a wave takes together: as many as give it 8 rows or fewer
     p.hb = rows * most <= kRows && a.c.heads % most == 0 ? most : rows * 2 <= kRows && a.c.heads % 2 == 0 ? 2 : 1;
@@ -1210,17 +1212,18 @@ AttnPlan attn_plan(const KvAttnArgs& a) {
     const long long span = a.window > 0 ? std::min<long long>((long long)a.window + p.per / a.group + 1, a.c.cap) : a.c.cap;
     const int tiles = (int)std::min<long long>((span + kTile - 1) / kTile + (a.c.sinks + kTile - 1) / kTile + 2, a.c.cap / kTile);
     // Many rows, eight waves, four for every other tile, where no more than two workgroups of four a CU would be there: they all
-    // start at once, and nothing takes the place of one that ends early (us, four waves and eight, bf16 heads of 128 but where said:
-    // 2 x 1024 tokens over 8192 positions, 512 workgroups, lengths of 8192 and less 267 and 229, both 8192 365 and 409; 16 x 256
-    // tokens, fp16 heads of 64, unequal lengths, 256 workgroups 72 and 54; 4 x 512, fp32, equal, 256 workgroups 239 and 220; 64
-    // tokens, 4 workgroups 26 and 22; and where more are waiting, 8 x 512 tokens over 4096, 1024 workgroups 455 and 523; with two tiles
-    // to share, 256 x 64 tokens, 10 and 14)
+    // start at once, and nothing takes the place of one that ends early. The lengths are not known here: unequal ones gain, equal ones
+    // that fill the card lose a few percent (us, four waves and eight, in rows of forty, bf16 heads of 128 but where said: 2 x 1024
+    // tokens, 512 workgroups, over up to 8192 positions 360 and 298, over 8192 each 452 and 492, the same in fp16 497 and 537, in fp32
+    // 780 and 695; 16 x 256 tokens over up to 4096, fp16 heads of 64, 256 workgroups 148 and 102; 4 x 512 over 4096 each, fp32 heads of
+    // 64, 256 workgroups 228 and 240; 64 tokens over 2048, 4 workgroups 94 and 28; and where more are waiting, 8 x 512 tokens over 4096,
+    // 1024 workgroups 509 and 523; with two tiles to share, 256 x 64 tokens, heads of 64, 36 and 58)
     p.waves = p.many ? (p.units <= 512 && tiles >= 16 ? 8 : 4) : tiles <= 4 ? 1 : 4;
     p.chunk_tiles = tiles;
     if (p.many ? p.waves == 8 : p.waves > 1) {
         // Two workgroups a CU (one of eight waves), each with four tiles a wave at least (sixteen a workgroup of many rows). More,
-        // smaller chunks cost more at their ends than they even out (256 conversations, their window in one chunk or two: 28.8 or
-        // 37.7 us). Many rows on four waves have more workgroups than that, or few tiles.
+        // smaller chunks cost more at their ends than they even out (256 conversations, their window in one chunk or two: 29 or
+        // 38 us). Many rows on four waves have more workgroups than that, or few tiles.
         const int want = std::max(1, (p.waves == 8 ? 256 : 512) / p.units);
         p.chunk_tiles = std::max(16, (tiles + want - 1) / want);
     }

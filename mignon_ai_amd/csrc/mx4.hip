@@ -19,8 +19,8 @@ typedef uint32_t Any16 __attribute__((ext_vector_type(4), may_alias));  // sixte
 // ---- Quantisation and reading back ----
 // A workgroup of 256 lanes covers 256 / LC rows by 8 LC columns (LC lanes a row, four to a block, eight elements each): a lane
 // reads 16 or 32 bytes and a wave writes whole lines of codes; the block's largest magnitude takes two exchanges among four
-// lanes, so an element is read once and kept in registers. Bound by memory: 16384 x 4096 bf16, 170 MB each way, 33 us quantised
-// (5.2 TB/s) and 26 read back (6.5), where a large copy reaches 4.8; 16 x 384 fp32 2.2 and 2.3 us, a launch.
+// lanes, so an element is read once and kept in registers. Bound by memory: 16384 x 4096 bf16, 170 MB each way, 35 us quantised
+// (4.8 TB/s) and 26 read back (6.5), where a large copy reaches 4.9; 16 x 384 fp32 2.2 and 2.3 us, a launch.
 constexpr int kRowLanes = 256;
 constexpr int kMaxGridY = 32768;
 
@@ -211,13 +211,14 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_split_kernel(Mx4GemmArgs 
 // In a step each channel fragment is read anew for the next step right after its products were issued, so that only the row
 // fragments need two sets of registers.
 //
-// 16384 x 4096 x 4096 into bf16: 153 us, 3.6 PFLOP/s; 8192 x 8192 x 8192 270 us, 4.1: four times what a large bf16 product reaches on
-// this card (1.07). The instruction alone, on random data in registers, reaches 5.8 to 6.4 (9 and more on zeros: its rate is bound
-// by power). Of the 153 us some 100 are the products; the rest is what does not overlap with them: a tile's first loads and its
-// output, which all workgroups write at about the same time (20 us at the rate of a fill). At the instruction's nominal rate a step of
-// a 256 x 256 tile takes 1024 cycles of a CU's matrix units, and the step's LDS traffic (96 KiB read by the waves, 32 KiB written by the
-// loads, 128 bytes a cycle) as many, so the tile is as large as registers allow (128 x 128 tiles: 194 us). Steps loaded one by one, 64
-// bytes a row, took 5 us more, and an output of 32 bytes a row and store, straight from the registers, 12 more.
+// 16384 x 4096 x 4096 into bf16: 154 us between other calls, 172 in a row of forty, where power holds the clock down (3.6 and 3.2
+// PFLOP/s); 8192 x 8192 x 8192 303 us in such a row, 3.6: three times what a large bf16 product reaches on this card (1.26). The
+// instruction alone, on random data in registers, reaches 5.8 to 6.4 (9 and more on zeros), which is 86 to 95 us for the products; the
+// rest is what does not overlap with them: a tile's first loads and its output, which all workgroups write at about the same time
+// (20 us at the rate of a fill). At the instruction's nominal rate a step of a 256 x 256 tile takes 1024 cycles of a CU's matrix units,
+// and the step's LDS traffic (96 KiB read by the waves, 32 KiB written by the loads, 128 bytes a cycle) as many, so the tile is as
+// large as registers allow (the table at gemm_tile has the smaller ones). Steps loaded one by one, 64 bytes a row, took 3 % longer,
+// and an output of 32 bytes a row and store, straight from the registers, 8 %.
 template <int TN_, int TM_, int WN_, int WM_, int SLOTS_>
 struct MxTile {
     static constexpr int TN = TN_, TM = TM_, WN = WN_, WM = WM_, kSlots = SLOTS_;
@@ -445,11 +446,12 @@ hipError_t launch_mx4_dequantize(const Mx4RowsArgs& a, hipStream_t s) {
 
 namespace {
 // The largest tile of which there are enough for three quarters of the 256 CUs and which the shape fills to four fifths;
-// where even those of 64 x 64 are too few (0), K is split. us at M x N x K, 256 / 128 / 64 tiles, split 32 x 32 and 16 x 16:
-//   16384 x 4096 x 4096: 158 194 296;     3584 x 3584 x 4096: 38 46;    4096 x 2048 x 4096: 35 28;    4096 x 4096 x 384: 12.5 14 22.5
-//   2048 x 2048 x 4096: 31 19.5 21.9 56;    1536 x 1024 x 2048: - 10.3 7.3;    1001 x 2048 x 1152: 12.2 7.8 6.1 10.6 15.4
-//   256 x 4096 x 4096: 28 15.9 9.1 14.5 19.5;    128 x 4096 x 4096: 28 15.6 8.4 8 10.9;    300 x 300 x 8192: 51 27 13.3 5.6 5.4
-//   8 x 4096 x 4096: 27 15 8 3.9 3;    16 x 8192 x 4096: 27 15 8.2 4.6 3.9
+// where even those of 64 x 64 are too few (0), K is split. us at M x N x K into bf16, forty in a row, 256 / 128 / 64 tiles, split
+// 32 x 32 and 16 x 16:
+//   16384 x 4096 x 4096: 182 201 304;     3584 x 3584 x 4096: 35 43;    4096 x 2048 x 4096: 33 26;    4096 x 4096 x 384: 12.2 13.6 20.6
+//   2048 x 2048 x 4096: 30 18.7 19.8 54;    1536 x 1024 x 2048: - 10.3 7.2;    1001 x 2048 x 1152: 12 7.9 6.3 10.8 14.9
+//   256 x 4096 x 4096: 28 15.8 9.2 14.5 18.7;    128 x 4096 x 4096: 27 15.4 8.6 8.3 11.2;    300 x 300 x 8192: 49 27 13.4 5.9 6
+//   8 x 4096 x 4096: 27 14.8 8.2 4.2 3.5;    16 x 8192 x 4096: 27 15.2 8.4 5 4.3
 int gemm_tile(const Mx4GemmArgs& a) {
     if (a.M <= 16) return 0;
     for (const int tile : {256, 128, 64}) {

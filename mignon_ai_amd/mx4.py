@@ -157,7 +157,8 @@ def mx4_gemm_device(A, As, W, Ws, C, stream=None):
 class KVCache:
     """A 4-bit key/value cache (mg_kv_cache_t) over torch CUDA tensors: k and v codes [n][heads][capacity][head_dim / 2], their
     scales [n][heads][capacity][head_dim / 32], uint8. Positions below `sinks` keep their slots, later ones take turns in the
-    others. The caller keeps count of the positions. Calls are enqueued on torch's current stream of the cache's device."""
+    others. The caller keeps count of the positions, and has the rows written by `write` (the planes' first contents do not
+    matter). Calls are enqueued on torch's current stream of the cache's device."""
 
     def __init__(self, k, k_scales, v, v_scales, sinks: int = 0):
         self.k, self.k_scales, self.v, self.v_scales = k, k_scales, v, v_scales
