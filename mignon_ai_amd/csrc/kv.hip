@@ -599,9 +599,9 @@ struct Stages {
 //
 // Bound by reading the cache, with the unpacking close behind. 32 conversations of 16384 positions (8 heads of 128, four query
 // heads each, bf16): 101 us, 5.6 TB/s; of 1 to 16384 positions, 276 MB, 71 us (3.9 TB/s: the lengths do not divide evenly over the
-// chip) and 4.5 for the join; 256 windows of 1000 (8 heads of 64, two query heads each, fp16, 109 MB) 29 us; 4096 windows of 64 (8 fp32 heads
-// of 32, 57 MB) 24 us, where a wave's life is mostly its first tiles' latency; one conversation of 30000 (33 MB) 13 us and 6 for the
-// join: two heads a wave make 236 workgroups of it, where 512 have room, each with sixteen tiles one after another.
+// chip) and 4.5 for the join; 256 windows of 1000 (8 heads of 64, two query heads each, fp16, 109 MB) 29 us; 4096 windows of 64 (8
+// fp32 heads of 32, 57 MB) 24 us, where a wave's life is mostly its first tiles' latency; one conversation of 30000 (33 MB) 13 us and
+// 6 for the join: two heads a wave make 236 workgroups of it, where 512 have room, each with sixteen tiles one after another.
 template <int DH, class T, int HB, int WAVES>
 __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(KvAttnArgs a, int row_tiles, int chunk_tiles) {
     using W = Width<DH>;

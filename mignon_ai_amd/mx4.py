@@ -237,7 +237,7 @@ class KVCache:
 
     def attention(self, q, out, pos, counts=None, window: int = 0, scale: float | None = None):
         """mg_kv_attention: rows q [n][T][q_heads][head_dim] at positions pos[s] + t over the cache (their own keys written
-        already) into out, which is returned; scale: head_dim ** -0.5 if not given."""
+        already) into out (which may be q), which is returned; scale: head_dim ** -0.5 if not given."""
         ty, qr = self._rows("KVCache.attention", q, "q", None)
         to, orow = self._rows("KVCache.attention", out, "out", None)
         if ty != to or q.shape != out.shape or pos is None:

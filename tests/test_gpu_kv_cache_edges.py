@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from mignon_ai_amd import KVCache
 from test_gpu_kv_cache import P_BITS, Pair, _ints, _np, _rows
 
 pytestmark = pytest.mark.gpu
@@ -86,3 +87,37 @@ def test_nan_reaches_only_the_rows_that_see_it(form, t, dh):
     assert bool(torch.isfinite(a).all())
     assert torch.equal(torch.isnan(b), bad)
     assert torch.equal(b[~bad], a[~bad])
+
+
+@pytest.mark.parametrize("form", list(SPOILT))
+@pytest.mark.parametrize("t", list(P_BITS))
+def test_rows_replaced_by_their_outputs(form, t):
+    """out may be q itself: a row is read before anything is written in its place."""
+    T, cap, L, window = SPOILT[form]
+    n, H, G, dh = 5, 4, 2, 64
+    p = Pair(n, H, dh, cap)
+    lens = np.array([L, T, L // 2, L - 3, max(1, T // 2)])
+    counts = np.minimum(lens, T)
+    p.c.write(_rows((n, L, H, dh), 1), _rows((n, L, H, dh), 2), _ints([0] * n), _ints(lens))
+    q, pos, cnt = _rows((n, T, H * G, dh), 3, t), _ints(lens - counts), _ints(counts)
+    want = p.c.attention(q, q.clone(), pos, cnt, window=window)
+    assert torch.equal(p.c.attention(q, q, pos, cnt, window=window), want)
+
+
+def test_counts_outside_the_call_and_sequences_without_tokens():
+    """Counts are taken as 0..T; calls on no sequences or no tokens do nothing."""
+    p = Pair(3, 2, 64, 64)
+    k, v = _rows((3, 10, 2, 64), 1), _rows((3, 10, 2, 64), 2)
+    p.c.write(k, v, _ints([0, 0, 0]), _ints([99, -5, 10]))
+    q = _rows((3, 10, 4, 64), 3)
+    out = p.c.attention(q, torch.full_like(q, 55.0), _ints([0, 0, 0]), _ints([99, -5, 10]))
+    whole = p.c.attention(q, torch.full_like(q, 55.0), _ints([0, 0, 0]), _ints([10, 0, 10]))
+    assert torch.equal(out, whole) and bool((out[1] == 55.0).all()) and bool(torch.isfinite(out).all())
+    none = KVCache.empty(0, 2, 64, 64)
+    empty = torch.empty((0, 3, 2, 64), device="cuda")
+    none.write(empty, empty, _ints([]))
+    none.read(empty, empty, _ints([]))
+    assert none.attention(empty, empty, _ints([])).shape == empty.shape
+    still = torch.empty((3, 0, 2, 64), device="cuda")
+    p.c.write(still, still, _ints([0, 0, 0]))
+    p.c.attention(still, still, _ints([0, 0, 0]))

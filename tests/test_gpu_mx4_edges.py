@@ -35,3 +35,25 @@ def test_product_of_more_than_four_million_tiles():
     want = 192 * 2.0 ** (torch.arange(N, device="cuda") % 8)
     assert bool((C[M - 3:M].float() == want).all()) and bool((C[M] == 9.0).all())
     assert all(not bool(c.any()) for c in C[:M - 3].split(1 << 26))
+
+
+@pytest.mark.parametrize("K", [1 << 24, (1 << 24) - 3])
+def test_the_longest_rows(K):
+    """Rows of as many elements as a call takes, nearly all zeros: the values and the product of what is not."""
+    M, N, Kp = 3, 5, 1 << 24
+    g = torch.Generator("cuda").manual_seed(1)
+    at = torch.randint(0, K, (200,), generator=g, device="cuda")
+    at[:3] = torch.tensor([0, K - 1, K - 40], device="cuda")
+    values = torch.tensor([0.5, 1.0, 2.0, 3.0, 4.0, 6.0, -1.5], device="cuda")
+    x = torch.zeros((M + N, K), device="cuda")
+    x[:, at] = values[torch.randint(0, 7, (M + N, 200), generator=g, device="cuda")]
+    codes, scales = _device4(M + N, K)
+    assert codes.shape[1] == Kp // 2
+    mx4_quantize_device(x, codes, scales)
+    y = torch.full_like(x, 9.0)
+    mx4_dequantize_device(codes, scales, y)
+    # (a value next to a larger one may be rounded)
+    assert int((y != 0).sum()) <= int((x != 0).sum()) and bool(((y - x).abs() <= 1).all())
+    C = torch.empty((M, N), device="cuda")
+    mx4_gemm_device(codes[:M], scales[:M], codes[M:], scales[M:], C)
+    assert torch.equal(C.double(), y[:M].double() @ y[M:].double().t().contiguous())
