@@ -362,9 +362,9 @@ int mg_kv_read(const mg_kv_cache_t* cache, const mg_kv_rows_t* k, const mg_kv_ro
  * the row at position p sees the held positions j <= p with j > p - window, or any if window <= 0, and those with j < sinks.
  * out = sum softmax(scale q.k) v, zeros for a row that sees nothing; scores, statistics and sums in fp32, probabilities held to 24
  * bits for the product with v (MG_F32) or to 16 (MG_F16, MG_BF16). Rows past counts[s] are left as they are, and out may be q
- * itself. A NaN or infinity in a key or value reaches the rows that see it only. workspace: device memory of mg_kv_attention_workspace bytes, 16-byte aligned, for
- * this call alone until it has run (calls that may overlap, and captured graphs that may, need one each); may be NULL where that
- * is 0. */
+ * itself. A NaN or infinity in a key or value reaches the rows that see it only. workspace: device memory of
+ * mg_kv_attention_workspace bytes, 16-byte aligned, for this call alone until it has run (calls that may overlap, and captured
+ * graphs that may, need one each); may be NULL where that is 0. */
 long long mg_kv_attention_workspace(const mg_kv_cache_t* cache, int q_heads, int T, int window);
 int mg_kv_attention(const mg_kv_cache_t* cache, const mg_kv_rows_t* q, const mg_kv_rows_t* out, int type, int q_heads, int T,
                     const int32_t* pos, const int32_t* counts, int window, float scale, void* workspace,
