@@ -370,6 +370,40 @@ int mg_kv_attention(const mg_kv_cache_t* cache, const mg_kv_rows_t* q, const mg_
                     const int32_t* pos, const int32_t* counts, int window, float scale, void* workspace,
                     long long workspace_bytes, void* stream);
 
+/* Sequences copied, forked, reordered and compacted: sequence i of `to` becomes sequence parents[i] of `from`, lens[i] positions long
+ * (both [to->n]), where parents[i] is in [0, from->n); elsewhere it stays as it is. What `to` holds of such a length is written, and its
+ * other slots are left as they are. from_lens [from->n]: the lengths of `from`'s sequences (NULL: as long as what becomes of them); a
+ * position that `from` no longer holds, or never held, becomes zeros, as mg_kv_read reads it. `from` NULL or `to` itself: in place, as if
+ * from a copy taken before, for at most 16384 sequences. Otherwise the caches share no memory and may differ in n, capacity and sinks.
+ * Ended sequences need no call: a place is free once nothing asks for it. */
+int mg_kv_gather(const mg_kv_cache_t* to, const mg_kv_cache_t* from, const int32_t* parents, const int32_t* lens,
+                 const int32_t* from_lens, void* stream);
+/* mg_kv_attention for sequences that go on from shared prefixes, each of which is read once for all of its sequences. `prefix` holds
+ * prefix->n of them, with the cache's heads and head_dim: sequences starts[g] .. starts[g + 1] - 1 of the cache go on from prefix g
+ * (starts [prefix->n + 1], not decreasing; may be NULL for a single prefix, which is then that of all sequences; sequences before the
+ * first and from the last start on have none). A row sees all positions that prefix g holds of its first prefix_lens[g], whatever the
+ * window, and of its own sequence what mg_kv_attention shows it; pos counts the sequence's own positions. Numbers, q, out and workspace as
+ * there; a NaN in a prefix reaches all of its rows. */
+long long mg_kv_attention_shared_workspace(const mg_kv_cache_t* cache, const mg_kv_cache_t* prefix, int q_heads, int T, int window);
+int mg_kv_attention_shared(const mg_kv_cache_t* cache, const mg_kv_cache_t* prefix, const int32_t* prefix_lens, const int32_t* starts,
+                           const mg_kv_rows_t* q, const mg_kv_rows_t* out, int type, int q_heads, int T, const int32_t* pos,
+                           const int32_t* counts, int window, float scale, void* workspace, long long workspace_bytes, void* stream);
+
+/* ---- Log probabilities (no reference counterpart: mg_score_sequences and mg_forward_batch give those of a model's own targets) ----
+ * For n rows of logits [n][V] (row stride ld >= V elements; MG_F32, MG_F16 or MG_BF16; V up to 2^30):
+ *   logprob [n][m]      log-softmax of tokens targets [n][m] (NaN for an id outside [0, V))
+ *   entropy [n]         -sum p log p, in nats (a token of probability 0 adds nothing)
+ *   top_ids, top_logprob [n][k]  the k (0..min(V, 64)) largest logits, the likeliest first, the lowest id first among equals
+ * all optional but for targets with logprob where m > 0 and one of the last two where k > 0; statistics in fp32. A row with a NaN or a
+ * positive infinity, and one with nothing but negative infinities, has NaN for its log probabilities and entropy; NaN stands below every
+ * number in its order. Host pointers, or with MG_PTR_DEVICE device pointers: then the work is enqueued on `stream`, nothing is
+ * allocated, the call can be captured, and workspace is device memory of mg_token_logprobs_workspace bytes, 16-byte aligned, for this
+ * call alone until it has run (may be NULL where that is 0). */
+long long mg_token_logprobs_workspace(int n, int V, int k);
+int mg_token_logprobs(const void* logits, int type, int n, int V, long long ld, const int32_t* targets, int m, int k, float* logprob,
+                      float* entropy, int32_t* top_ids, float* top_logprob, void* workspace, long long workspace_bytes, int flags,
+                      void* stream);
+
 /* Engine options, no reference counterpart: where two implementations of a stage exist, which one runs,
  * for every model of the process. Value 0 (the default) chooses automatically. Small models (state size up
  * to 128, hidden size up to 256, heads of up to 32 over spans of up to 65 keys) run sequences of up to 128 tokens

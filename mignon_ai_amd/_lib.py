@@ -105,6 +105,11 @@ SIGNATURES = {
     "mg_kv_read": (_int, [_vp, _vp, _vp, _int, _int, _vp, _vp, _vp, _vp]),
     "mg_kv_attention_workspace": (_ll, [_vp, _int, _int, _int]),
     "mg_kv_attention": (_int, [_vp, _vp, _vp, _int, _int, _int, _vp, _vp, _int, ctypes.c_float, _vp, _ll, _vp]),
+    "mg_kv_gather": (_int, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "mg_kv_attention_shared_workspace": (_ll, [_vp, _vp, _int, _int, _int]),
+    "mg_kv_attention_shared": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp, _vp, _int, ctypes.c_float, _vp, _ll, _vp]),
+    "mg_token_logprobs_workspace": (_ll, [_int, _int, _int]),
+    "mg_token_logprobs": (_int, [_vp, _int, _int, _int, _ll, _vp, _int, _int, _vp, _vp, _vp, _vp, _vp, _ll, _int, _vp]),
     "mg_engine_option": (_int, [_int, _int]),
     "mg_score_sequences": (_int, [_vp, _vp, _vp, _int, _int, _vp]),
     "mg_tokenizer_load": (_int, [_u8p, ctypes.c_size_t, ctypes.POINTER(_vp)]),

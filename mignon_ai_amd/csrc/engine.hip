@@ -30,6 +30,7 @@
 #include "gemm.hpp"
 #include "kernels.hpp"
 #include "model_file.hpp"
+#include "logprob.hpp"
 #include "mx4.hpp"
 #include "options.hpp"
 #include "sample.hpp"
@@ -1313,6 +1314,16 @@ bool kv_attention_args(const char* who, const mg_kv_cache_t* c, int q_heads, int
     a.T = T; a.group = q_heads / c->heads;
     a.window = window >= kKvMaxPos ? 0 : std::max(window, 0);  // positions are below kKvMaxPos: such a window hides nothing
     REQUIRE(kv_attention_fits(a), std::string(who) + ": too many rows");
+    return true;
+}
+
+// The same with prefixes: as many key/value heads, of the same width.
+bool kv_shared_args(const char* who, const mg_kv_cache_t* c, const mg_kv_cache_t* prefix, int q_heads, int T, int window, KvSharedArgs& a) {
+    const bool some = kv_cache(who, prefix, 1, a.prefix);
+    if (!kv_attention_args(who, c, q_heads, T, window, a)) return false;
+    if (!some) return true;
+    REQUIRE(a.prefix.heads == a.c.heads && a.prefix.dh == a.c.dh, std::string(who) + ": a prefix of unequal heads");
+    REQUIRE(kv_shared_fits(a), std::string(who) + ": too many rows");
     return true;
 }
 
@@ -2776,6 +2787,133 @@ int mg_kv_attention(const mg_kv_cache_t* cache, const mg_kv_rows_t* q, const mg_
                 "mg_kv_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) + " needed");
         a.ws = (float*)workspace;
         HIPCHECK(launch_kv_attention(a, (hipStream_t)stream));
+        return MG_OK;
+    });
+}
+
+int mg_kv_gather(const mg_kv_cache_t* to, const mg_kv_cache_t* from, const int32_t* parents, const int32_t* lens,
+                 const int32_t* from_lens, void* stream) {
+    return guarded([&] {
+        const char* who = "mg_kv_gather";
+        KvGatherArgs a;
+        const bool any = kv_cache(who, to, 1, a.to), some = kv_cache(who, from ? from : to, 1, a.from);
+        if (!any) return MG_OK;
+        REQUIRE(parents && lens, "mg_kv_gather: null argument");
+        if (!some) return MG_OK;  // no sequence has a parent
+        REQUIRE(a.to.heads == a.from.heads && a.to.dh == a.from.dh, "mg_kv_gather: caches of unequal heads");
+        if (a.to.k == a.from.k) {
+            REQUIRE(a.to.ks == a.from.ks && a.to.v == a.from.v && a.to.vs == a.from.vs && a.to.n == a.from.n && a.to.cap == a.from.cap &&
+                        a.to.sinks == a.from.sinks,
+                    "mg_kv_gather: two caches that share some of their memory");
+        } else {
+            const KvCache* c[2] = {&a.to, &a.from};
+            std::pair<const uint8_t*, const uint8_t*> span[2][4];
+            for (int x = 0; x < 2; x++) {
+                const size_t rows = (size_t)c[x]->n * c[x]->heads * c[x]->cap, codes = rows * (c[x]->dh / 2), scales = rows * (c[x]->dh / 32);
+                span[x][0] = {c[x]->k, c[x]->k + codes};
+                span[x][1] = {c[x]->v, c[x]->v + codes};
+                span[x][2] = {c[x]->ks, c[x]->ks + scales};
+                span[x][3] = {c[x]->vs, c[x]->vs + scales};
+            }
+            for (const auto& x : span[0])
+                for (const auto& y : span[1])
+                    REQUIRE(x.first >= y.second || y.first >= x.second, "mg_kv_gather: two caches that share some of their memory");
+        }
+        a.parents = parents; a.lens = lens; a.from_lens = from_lens;
+        REQUIRE(kv_gather_fits(a), "mg_kv_gather: too many sequences");
+        HIPCHECK(launch_kv_gather(a, (hipStream_t)stream));
+        return MG_OK;
+    });
+}
+
+long long mg_kv_attention_shared_workspace(const mg_kv_cache_t* cache, const mg_kv_cache_t* prefix, int q_heads, int T, int window) {
+    long long bytes = 0;
+    const int rc = guarded([&] {
+        KvSharedArgs a;
+        if (!kv_shared_args("mg_kv_attention_shared_workspace", cache, prefix, q_heads, T, window, a)) return MG_OK;
+        bytes = (long long)(a.prefix.n ? kv_shared_ws_bytes(a) : kv_attention_ws_bytes(a));
+        return MG_OK;
+    });
+    return rc < 0 ? rc : bytes;
+}
+
+int mg_kv_attention_shared(const mg_kv_cache_t* cache, const mg_kv_cache_t* prefix, const int32_t* prefix_lens, const int32_t* starts,
+                           const mg_kv_rows_t* q, const mg_kv_rows_t* out, int type, int q_heads, int T, const int32_t* pos,
+                           const int32_t* counts, int window, float scale, void* workspace, long long workspace_bytes, void* stream) {
+    return guarded([&] {
+        const char* who = "mg_kv_attention_shared";
+        KvSharedArgs a;
+        if (!kv_shared_args(who, cache, prefix, q_heads, T, window, a)) return MG_OK;
+        REQUIRE(q && out && q->data && out->data && pos, "mg_kv_attention_shared: null argument");
+        REQUIRE(a.prefix.n == 0 || (prefix_lens && (starts || a.prefix.n == 1)), "mg_kv_attention_shared: prefixes without lengths or sequences");
+        REQUIRE(real_type(type), "mg_kv_attention_shared: unknown type");
+        REQUIRE(aligned(q->data, real_size(type)) && aligned(out->data, real_size(type)) && aligned(workspace, 16),
+                "mg_kv_attention_shared: misaligned pointer");
+        a.q = kv_rows(q); a.out = kv_rows(out);
+        a.type = type; a.pos = pos; a.counts = counts; a.scale = scale;
+        a.prefix_lens = prefix_lens; a.starts = starts;
+        const size_t need = a.prefix.n ? kv_shared_ws_bytes(a) : kv_attention_ws_bytes(a);
+        REQUIRE(need == 0 || (workspace && workspace_bytes >= 0 && (size_t)workspace_bytes >= need),
+                "mg_kv_attention_shared: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) + " needed");
+        a.ws = (float*)workspace;
+        HIPCHECK(a.prefix.n ? launch_kv_shared(a, (hipStream_t)stream) : launch_kv_attention(a, (hipStream_t)stream));
+        return MG_OK;
+    });
+}
+
+long long mg_token_logprobs_workspace(int n, int V, int k) {
+    if (n < 0 || V <= 0 || V > kLogprobMaxV || k < 0 || k > std::min(V, kMaxTop)) {
+        g_last_error = "mg_token_logprobs_workspace: bad shape";
+        return MG_ERR_INVALID;
+    }
+    LogprobArgs a;
+    a.n = n; a.V = V; a.k = k;
+    return (long long)logprob_ws_bytes(a);
+}
+
+int mg_token_logprobs(const void* logits, int type, int n, int V, long long ld, const int32_t* targets, int m, int k, float* logprob,
+                      float* entropy, int32_t* top_ids, float* top_logprob, void* workspace, long long workspace_bytes, int flags,
+                      void* stream) {
+    return guarded([&] {
+        REQUIRE(real_type(type), "mg_token_logprobs: unknown type");
+        REQUIRE(n >= 0 && V > 0 && V <= kLogprobMaxV && ld >= V && m >= 0, "mg_token_logprobs: bad shape");
+        REQUIRE(k >= 0 && k <= std::min(V, kMaxTop), "mg_token_logprobs: k is at most " + std::to_string(kMaxTop) + " and the vocabulary");
+        if (n == 0) return MG_OK;  // (an empty tensor has no address)
+        REQUIRE(logits && (m == 0 || (targets && logprob)) && (k == 0 || top_ids || top_logprob), "mg_token_logprobs: null argument");
+        hipStream_t st = (hipStream_t)stream;
+        const bool dev = flags & MG_PTR_DEVICE;
+        const size_t e = real_size(type), nm = (size_t)n * m, nk = (size_t)n * k;
+        Staging sg;
+        LogprobArgs a;
+        a.type = type; a.n = n; a.V = V; a.m = m; a.k = k; a.ld = dev ? ld : V;
+        a.x = logits; a.targets = targets; a.logprob = logprob; a.entropy = entropy; a.top_ids = top_ids; a.top_logprob = top_logprob;
+        a.ws = workspace;
+        const size_t need = logprob_ws_bytes(a);
+        if (!dev) {
+            uint8_t* x = sg.out<uint8_t>((size_t)n * V * e);
+            HIPCHECK(hipMemcpy2DAsync(x, V * e, logits, ld * e, V * e, n, hipMemcpyHostToDevice, st));
+            a.x = x;
+            a.targets = m ? sg.in(targets, nm, st) : nullptr;
+            a.logprob = m ? sg.out<float>(nm) : nullptr;
+            a.entropy = entropy ? sg.out<float>(n) : nullptr;
+            a.top_ids = k && top_ids ? sg.out<int32_t>(nk) : nullptr;
+            a.top_logprob = k && top_logprob ? sg.out<float>(nk) : nullptr;
+            a.ws = sg.out<uint8_t>(need);
+        } else {
+            REQUIRE(need == 0 || (workspace && workspace_bytes >= 0 && (size_t)workspace_bytes >= need),
+                    "mg_token_logprobs: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) + " needed");
+            REQUIRE(aligned(logits, e) && aligned(targets, 4) && aligned(logprob, 4) && aligned(entropy, 4) && aligned(top_ids, 4) &&
+                        aligned(top_logprob, 4) && aligned(workspace, 16),
+                    "mg_token_logprobs: misaligned pointer");
+        }
+        HIPCHECK(launch_logprob(a, st));
+        if (!dev) {
+            if (m) HIPCHECK(hipMemcpyAsync(logprob, a.logprob, nm * 4, hipMemcpyDeviceToHost, st));
+            if (entropy) HIPCHECK(hipMemcpyAsync(entropy, a.entropy, (size_t)n * 4, hipMemcpyDeviceToHost, st));
+            if (k && top_ids) HIPCHECK(hipMemcpyAsync(top_ids, a.top_ids, nk * 4, hipMemcpyDeviceToHost, st));
+            if (k && top_logprob) HIPCHECK(hipMemcpyAsync(top_logprob, a.top_logprob, nk * 4, hipMemcpyDeviceToHost, st));
+            HIPCHECK(hipStreamSynchronize(st));
+        }
         return MG_OK;
     });
 }

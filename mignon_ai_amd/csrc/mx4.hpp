@@ -70,11 +70,33 @@ struct KvAttnArgs {
     const int32_t* counts = nullptr;
     float* ws = nullptr;          // kv_attention_ws_bytes
 };
+// Attention over prefixes that several sequences share, besides each one's own cache (kv_shared.hip): sequences starts[g] .. starts[g + 1] - 1
+// (null: all, of one prefix) go on from prefix g, of which all that it holds of its first prefix_lens[g] positions is seen.
+struct KvSharedArgs : KvAttnArgs {
+    KvCache prefix;               // n prefixes
+    const int32_t* starts = nullptr;
+    const int32_t* prefix_lens = nullptr;
+    float* parts = nullptr;       // [chunk][row][dh + 4]: what a chunk of its prefix gave each query row (kv_attention.hpp)
+    int prefix_chunks = 0;        // at most so many chunks a prefix
+};
 // Positions are below this.
 constexpr int kKvMaxPos = 1 << 30;
 bool kv_head_width(int dh);       // 32, 64, 96 or 128
 size_t kv_attention_ws_bytes(const KvAttnArgs& a);
 bool kv_attention_fits(const KvAttnArgs& a);  // a launch takes it
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s);
+size_t kv_shared_ws_bytes(const KvSharedArgs& a);
+bool kv_shared_fits(const KvSharedArgs& a);
+hipError_t launch_kv_shared(const KvSharedArgs& a, hipStream_t s);  // workspace: a.ws
+
+// Sequence i of `to` becomes sequence parents[i] of `from` (outside its range: stays), lens[i] positions long.
+struct KvGatherArgs {
+    KvCache to, from;                    // the same planes: in place
+    const int32_t* parents = nullptr;
+    const int32_t* lens = nullptr;
+    const int32_t* from_lens = nullptr;  // null: a parent is as long as its copy
+};
+bool kv_gather_fits(const KvGatherArgs& a);
+hipError_t launch_kv_gather(const KvGatherArgs& a, hipStream_t s);
 
 }  // namespace mg

@@ -250,3 +250,46 @@ class KVCache:
                 (self._p, ctypes.addressof(qr), ctypes.addressof(orow), ty, q_heads, T, pos.data_ptr(), ptr(counts), window,
                  self.head_dim ** -0.5 if scale is None else scale, ptr(ws), need))
         return out
+
+    def gather(self, parents, lens, source: "KVCache | None" = None, source_lens=None):
+        """mg_kv_gather: sequence i becomes sequence parents[i] of `source` (default: of this cache, as if from a copy taken before),
+        lens[i] positions long; it stays where parents[i] is none of the source's. parents, lens: int32 [n]; source_lens int32
+        [source.n]: the lengths of the source's sequences, where they are longer than what is taken of them."""
+        src = self if source is None else source
+        if parents is None or lens is None:
+            _invalid("KVCache.gather: parents and lengths are given")
+        self._ints("KVCache.gather", parents, lens)
+        src._ints("KVCache.gather", source_lens)
+        more = () if source_lens is None else (source_lens,)
+        _launch("KVCache.gather", lib().mg_kv_gather, None, (self._planes[0], src._planes[0], parents, lens) + more,
+                (self._p, src._p, parents.data_ptr(), lens.data_ptr(), ptr(source_lens)))
+
+    def attention_shared(self, q, out, pos, prefix: "KVCache", prefix_lens, starts=None, counts=None, window: int = 0,
+                         scale: float | None = None):
+        """mg_kv_attention_shared: `attention` for sequences that go on from prefixes: sequences starts[g] .. starts[g + 1] - 1 from
+        sequence g of `prefix`, of whose first prefix_lens[g] positions they see all that it holds. prefix_lens int32 [prefix.n],
+        starts int32 [prefix.n + 1] (None: all go on from the only one). pos counts a sequence's own positions."""
+        who = "KVCache.attention_shared"
+        ty, qr = self._rows(who, q, "q", None)
+        to, orow = self._rows(who, out, "out", None)
+        if ty != to or q.shape != out.shape or pos is None or prefix_lens is None:
+            _invalid(f"{who}: q and out have one shape and type, positions and the prefixes' lengths are given")
+        self._ints(who, pos, counts)
+        prefix._ints(who, prefix_lens)
+        if starts is not None and (starts.dtype is not _i32 or starts.shape != (prefix.n + 1,) or not starts.is_contiguous()):
+            _invalid(f"{who}: starts are int32 [prefixes + 1]")
+        T, q_heads, window = q.shape[1], q.shape[2], min(max(int(window), 0), 1 << 30)
+        key = (q_heads, T, window, prefix.n, prefix.capacity, prefix.heads, prefix.head_dim)
+        need = self._need.get(key)
+        if need is None:
+            need = lib().mg_kv_attention_shared_workspace(self._p, prefix._p, q_heads, T, window)
+            check(-1 if need < 0 else 0)
+            if len(self._need) >= 256:
+                self._need.clear()
+            self._need[key] = need
+        ws = self._planes[0].new_empty(need) if need else None
+        more = tuple(a for a in (starts, counts) if a is not None)
+        _launch(who, lib().mg_kv_attention_shared, None, (self._planes[0], prefix._planes[0], q, out, pos, prefix_lens) + more,
+                (self._p, prefix._p, prefix_lens.data_ptr(), ptr(starts), ctypes.addressof(qr), ctypes.addressof(orow), ty, q_heads, T,
+                 pos.data_ptr(), ptr(counts), window, self.head_dim ** -0.5 if scale is None else scale, ptr(ws), need))
+        return out
