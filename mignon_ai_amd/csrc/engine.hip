@@ -2888,6 +2888,7 @@ int mg_token_logprobs(const void* logits, int type, int n, int V, long long ld, 
         a.type = type; a.n = n; a.V = V; a.m = m; a.k = k; a.ld = dev ? ld : V;
         a.x = logits; a.targets = targets; a.logprob = logprob; a.entropy = entropy; a.top_ids = top_ids; a.top_logprob = top_logprob;
         a.ws = workspace;
+        REQUIRE(logprob_fits(a), "mg_token_logprobs: too many rows");
         const size_t need = logprob_ws_bytes(a);
         if (!dev) {
             uint8_t* x = sg.out<uint8_t>((size_t)n * V * e);

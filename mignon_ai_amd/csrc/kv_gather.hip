@@ -157,8 +157,6 @@ hipError_t launch_kv_gather(const KvGatherArgs& a, hipStream_t s) {
     return by_width(a.to.dh, [&](auto w) {
         constexpr int DH = decltype(w)::value;
         if (in_place(a)) {
-            if (const hipError_t e = hipFuncSetAttribute((const void*)kv_gather_in_place_kernel<DH>, hipFuncAttributeMaxDynamicSharedMemorySize, 4 * kInPlaceMax); e != hipSuccess)
-                return e;
             const int per_wg = 64;
             const long long blocks = ((long long)a.to.cap * (DH / 2) / 16 + per_wg - 1) / per_wg;
             const dim3 grid((unsigned)std::min<long long>(blocks, std::max(1, (1 << 16) / a.to.heads)), a.to.heads * 4);

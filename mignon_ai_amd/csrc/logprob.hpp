@@ -22,6 +22,7 @@ struct LogprobArgs {
     void* ws = nullptr;                // logprob_ws_bytes
 };
 size_t logprob_ws_bytes(const LogprobArgs& a);
+bool logprob_fits(const LogprobArgs& a);  // a launch takes it
 hipError_t launch_logprob(const LogprobArgs& a, hipStream_t s);
 
 }  // namespace mg

@@ -392,17 +392,6 @@ __global__ __launch_bounds__(S::NW * 64) void mx4_gemm_lds_kernel(Mx4GemmArgs a,
         }
 }
 
-// Allows a kernel dynamic LDS above the default limit, once per device.
-hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& allowed) {
-    int dev = 0;
-    if (const hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (allowed.load() & bit) return hipSuccess;
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == hipSuccess) allowed |= bit;
-    return e;
-}
-
 template <class S, class T>
 hipError_t launch_lds_gemm(const Mx4GemmArgs& a, hipStream_t s) {
     static std::atomic<uint64_t> allowed{0};

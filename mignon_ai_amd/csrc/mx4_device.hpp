@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 namespace mg {
@@ -120,6 +121,17 @@ __device__ __forceinline__ uint32_t mx4_block(const float x[8], uint32_t& s) {
     m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false));
     s = mx4_scale_byte(m);
     return mx4_pack8(x, mx4_scale(s));
+}
+
+// Allows a kernel dynamic LDS above the default limit, once per device.
+inline hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& allowed) {
+    int dev = 0;
+    if (const hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (allowed.load() & bit) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) allowed |= bit;
+    return e;
 }
 
 // Calls f with a null pointer of the element type's C++ type.
