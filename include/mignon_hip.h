@@ -383,7 +383,7 @@ int mg_kv_gather(const mg_kv_cache_t* to, const mg_kv_cache_t* from, const int32
  * (starts [prefix->n + 1], not decreasing; may be NULL for a single prefix, which is then that of all sequences; sequences before the
  * first and from the last start on have none). A row sees all positions that prefix g holds of its first prefix_lens[g], whatever the
  * window, and of its own sequence what mg_kv_attention shows it; pos counts the sequence's own positions. Numbers, q, out and workspace as
- * there; a NaN in a prefix reaches all of its rows. */
+ * there, but that probabilities over a prefix are held to 11 bits for MG_F16 and MG_BF16; a NaN in a prefix reaches all of its rows. */
 long long mg_kv_attention_shared_workspace(const mg_kv_cache_t* cache, const mg_kv_cache_t* prefix, int q_heads, int T, int window);
 int mg_kv_attention_shared(const mg_kv_cache_t* cache, const mg_kv_cache_t* prefix, const int32_t* prefix_lens, const int32_t* starts,
                            const mg_kv_rows_t* q, const mg_kv_rows_t* out, int type, int q_heads, int T, const int32_t* pos,

@@ -163,16 +163,16 @@ constexpr int kPart = DH + 4;
 template <class A>
 constexpr bool kShared = std::is_same_v<A, KvSharedArgs>;
 
-// The tiles of a prefix, a chunk's and the chunks: at most `most`, of eight tiles or more.
+// The steps (two tiles) of a prefix, a chunk's and the chunks: at most prefix_chunks, of two steps or more.
 struct PrefixSpan {
-    int held, tiles, each, chunks;
+    int held, steps, each, chunks;
 };
 __device__ __forceinline__ PrefixSpan prefix_span(const KvSharedArgs& a, int g) {
     PrefixSpan r;
     r.held = min(max(a.prefix_lens[g], 0), a.prefix.cap);
-    r.tiles = (r.held + 31) >> 5;
-    r.each = max(8, (r.tiles + a.prefix_chunks - 1) / a.prefix_chunks);
-    r.chunks = (r.tiles + r.each - 1) / r.each;
+    r.steps = (r.held + 63) >> 6;
+    r.each = max(2, (r.steps + a.prefix_chunks - 1) / a.prefix_chunks);
+    r.chunks = (r.steps + r.each - 1) / r.each;
     return r;
 }
 // The sequences of a prefix, and the prefix of a sequence (-1: none).
@@ -204,6 +204,7 @@ struct PrefixRow {
         chunks = prefix_span(a, g).chunks;
         step = (size_t)a.c.n * a.T * heads * (DH + 4);
         at = a.parts + (((size_t)s * a.T + t) * heads + head) * (DH + 4);
+#pragma unroll 8
         for (int c = 0; c < chunks; c++) top = fmaxf(top, at[c * step + DH]);
     }
     // A chunk's factor at maximum `mu` (finite), its sum of probabilities, and neighbouring sums.
@@ -366,58 +367,63 @@ __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(A a, int row_
     // [chunk][unit][column][kPart]
     float* part = a.ws + (((size_t)blockIdx.y * units + unit) * kRows) * kPart<DH>;
     if constexpr (WAVES == 1) {
-        float total = st.l, own_f = 1.0f;
-        PrefixRow<DH> pre;
-        if constexpr (kShared<A>) {
-            pre.find(a, s, t, head, there);
-            const float top = fmaxf(st.m, pre.top);
-            pre.top = top == -INFINITY ? 0.0f : top;
-            own_f = __builtin_amdgcn_exp2f(st.m - pre.top);
-            total *= own_f;
-            for (int c = 0; c < pre.chunks; c++) total += pre.total(c) * pre.factor(c, pre.top);
-        }
-        const float f = total == 0.0f ? 0.0f : 1.0f / total;
-        T* out = (T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head;
         // Lanes 2 r and 2 r + 1 have the even and odd channels of element groups 0 .. 3: the first gets both of groups 0 and 1, the
         // second those of groups 2 and 3.
         const bool odd = i & 1;
+        float v[W::chunks][2][W::E0];
 #pragma unroll
-        for (int c = 0; c < W::chunks; c++) {
-            float v[2][W::E0];
+        for (int c = 0; c < W::chunks; c++)
 #pragma unroll
             for (int b = 0; b < W::E(c) / 2; b++)
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     const v4f& x = acc[W::a0(c) + b];
                     const float keep = odd ? x[2 + r] : x[r], get = dpp_move<0xB1>(odd ? x[r] : x[2 + r]);
-                    if constexpr (kShared<A>) {
-                        v[r][2 * b] = (odd ? get : keep) * own_f;
-                        v[r][2 * b + 1] = (odd ? keep : get) * own_f;
-                    } else {
-                        v[r][2 * b] = (odd ? get : keep) * f;
-                        v[r][2 * b + 1] = (odd ? keep : get) * f;
-                    }
+                    v[c][r][2 * b] = odd ? get : keep;
+                    v[c][r][2 * b + 1] = odd ? keep : get;
                 }
-            if constexpr (kShared<A>) {
-                for (int x = 0; x < pre.chunks; x++) {
-                    const float pf = pre.factor(x, pre.top);
+        const auto channel = [&](int c, int r) { return W::base(c) + (4 * g + 2 * (i & 1) + r) * W::E(c); };
+        float total = st.l;
+        if constexpr (kShared<A>) {
+            PrefixRow<DH> pre;
+            pre.find(a, s, t, head, there);
+            const float top = fmaxf(st.m, pre.top), mu = top == -INFINITY ? 0.0f : top, own_f = __builtin_amdgcn_exp2f(st.m - mu);
+            total *= own_f;
 #pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        const float* p = pre.sums(x, W::base(c) + (4 * g + 2 * (i & 1) + r) * W::E(c));
-#pragma unroll
-                        for (int e = 0; e < W::E(c); e++) v[r][e] += p[e] * pf;
-                    }
-                }
+            for (int c = 0; c < W::chunks; c++)
 #pragma unroll
                 for (int r = 0; r < 2; r++)
 #pragma unroll
-                    for (int e = 0; e < W::E(c); e++) v[r][e] *= f;
+                    for (int e = 0; e < W::E(c); e++) v[c][r][e] *= own_f;
+#pragma unroll 2
+            for (int x = 0; x < pre.chunks; x++) {
+                const float pf = pre.factor(x, mu);
+                total += pre.total(x) * pf;
+#pragma unroll
+                for (int c = 0; c < W::chunks; c++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        typedef float VE __attribute__((ext_vector_type(2)));
+#pragma unroll
+                        for (int e = 0; e < W::E(c); e += 2) {
+                            const VE y = *(const VE*)(pre.sums(x, channel(c, r)) + e);
+                            v[c][r][e] += y.x * pf;
+                            v[c][r][e + 1] += y.y * pf;
+                        }
+                    }
             }
-            if (there) {
+        }
+        const float f = total == 0.0f ? 0.0f : 1.0f / total;
+        T* out = (T*)a.out.data + s * a.out.seq + t * a.out.token + head * a.out.head;
+        if (there) {
+#pragma unroll
+            for (int c = 0; c < W::chunks; c++)
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    T* p = out + W::base(c) + (4 * g + 2 * (i & 1) + r) * W::E(c);
-                    const float* from = v[r];
+                    T* p = out + channel(c, r);
+                    float* from = v[c][r];
+#pragma unroll
+                    for (int e = 0; e < W::E(c); e++) from[e] *= f;
                     if (W::E(c) == 8) {
                         real_store8<T>(p, 8, from);
                     } else if (W::E(c) == 4) {
@@ -427,7 +433,6 @@ __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(A a, int row_
                         __builtin_memcpy(p, u, sizeof(u));
                     }
                 }
-            }
         }
     } else {
         // join the waves: their sums at the largest maximum, added in the waves' order (the stages are done with)
@@ -479,6 +484,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_rows_kernel(A a, int row_
                     const float top = fmaxf(most, pre.top), mu = top == -INFINITY ? 0.0f : top, own_f = __builtin_amdgcn_exp2f(most - mu);
                     sum *= own_f;
                     total *= own_f;
+#pragma unroll 8
                     for (int c = 0; c < pre.chunks; c++) {
                         const float pf = pre.factor(c, mu);
                         total += pre.total(c) * pf;

@@ -14,18 +14,61 @@ namespace {
 // workgroup takes 32 rows a wave, RW waves, over a chunk of the prefix's tiles, which come into LDS as they are, three ahead, and are
 // unpacked once for all waves while the tile before is worked on (the layouts are Unpacked's). All rows see all of a prefix, so there are
 // no masks but behind its end, and a block of NaN belongs to every row.
+//
+// For 16-bit queries values and probabilities are fp16, a probability as 2^15 times itself so that what is 2^-29 of a row's largest or less
+// loses bits, not what is 2^-14: one product an output where two bf16 parts of a probability take two, at 11 bits instead of 16. fp16
+// holds a 4-bit number exactly if its scale lies in 2^-23 .. 2^13 (bytes 104 to 140); a workgroup that meets another one (with codes that
+// are not all zero), or scores far from zero (kFar), goes over its tiles again in the careful form, which is that of kv_attention.hpp.
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t unpack2h(uint32_t w, float s, int b) {
+    switch (b) {
+        case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0));
+        case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1));
+        case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2));
+        default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3));
+    }
+}
+template <bool HALF>
+__device__ __forceinline__ uint32_t unpack2_as(uint32_t w, float s, int b) {
+    return HALF ? unpack2h(w, s, b) : unpack2(w, s, b);
+}
+__device__ __forceinline__ v16f product(v8bf a, v8bf b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v16f product(v8h a, v8h b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// What the two forms hold queries, keys, probabilities and values in, and in how many parts.
+template <class T, bool CAREFUL>
+struct Forms {
+    static constexpr bool key_half = !CAREFUL && std::is_same_v<T, _Float16>, value_half = !CAREFUL && sizeof(T) == 2;
+    using Q = std::conditional_t<key_half, v8h, v8bf>;
+    using P = std::conditional_t<value_half, v8h, v8bf>;
+    static constexpr int q = key_half ? 1 : Terms<T>::q, p = value_half ? 1 : Terms<T>::p;
+    static constexpr float lift = value_half ? 15.0f : 0.0f;  // probabilities are held 2^lift times themselves
+};
+template <int N>
+__device__ __forceinline__ void split(const float x[8], v8bf out[N]) { split_bf16<N>(x, out); }
+template <int N>
+__device__ __forceinline__ void split(const float x[8], v8h out[N]) {
+    static_assert(N == 1, "");
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{x[2 * i], x[2 * i + 1]}), v2h));
+    out[0] = __builtin_bit_cast(v8h, *(uint4*)w);
+}
+
 template <int DH, class T, int RW>
-__global__ __launch_bounds__(64 * RW, 2) void kv_prefix_kernel(KvSharedArgs a) {
+__global__ __launch_bounds__(64 * RW, sizeof(T) == 4 && DH >= 64 ? 1 : 2) void kv_prefix_kernel(KvSharedArgs a) {
     using W = Width<DH>;
-    using Tile = KvTile<DH>;
     using U = Unpacked<DH>;
-    constexpr int QT = Terms<T>::q, PT = Terms<T>::p, KF = DH / 16, ND = DH / 32, NT = 64 * RW, R = 32 * RW, o_raw = 2 * U::bytes;
-    __shared__ __align__(16) uint8_t smem[o_raw + 3 * Tile::bytes];
+    constexpr int KF = DH / 16, ND = DH / 32, NT = 64 * RW, R = 32 * RW, row_bytes = DH / 2, step = 2 * U::bytes;
+    __shared__ __align__(16) uint8_t smem[2 * step];
     const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // the row tile: of which prefix, and which of its tiles
-    const int h = blockIdx.x % a.c.heads, per = a.T * a.group;  // rows a sequence
-    int tile = blockIdx.x / a.c.heads, p = 0, first = 0;
+    // the row tile: of which prefix, and which of its tiles (numbers without one, the last, come last); the chunk and the head
+    const int h = blockIdx.x % a.c.heads, rest = blockIdx.x / a.c.heads, chunk = rest % a.prefix_chunks, per = a.T * a.group;  // rows a sequence
+    int tile = rest / a.prefix_chunks, p = 0, first = 0;
     long long rows = 0;
     for (;; p++) {
         if (p == a.prefix.n) return;
@@ -36,7 +79,7 @@ __global__ __launch_bounds__(64 * RW, 2) void kv_prefix_kernel(KvSharedArgs a) {
         tile -= tiles;
     }
     const PrefixSpan span = prefix_span(a, p);
-    const int o0 = blockIdx.y * span.each, o1 = min(span.tiles, o0 + span.each);
+    const int o0 = chunk * span.each, o1 = min(span.steps, o0 + span.each);
     if (o0 >= o1) return;
 
     // this lane's row
@@ -46,71 +89,93 @@ __global__ __launch_bounds__(64 * RW, 2) void kv_prefix_kernel(KvSharedArgs a) {
     const bool there = row < rows && t < (a.counts ? min(max(a.counts[s], 0), a.T) : a.T);
     if (!__syncthreads_or(there)) return;
 
+    // What a lane loads of a step, and where it unpacks it to: of K KV neighbouring words (of one block) of a slot, of V a word of each of two
+    // neighbouring slots.
+    constexpr int words = DH / 8, KW = 2 * kTile * words, VN = kTile * words;
+    constexpr int KV = KW >= 4 * NT ? 4 : KW >= 2 * NT ? 2 : 1, KN = KW / KV, NK = (KN + NT - 1) / NT, NV = (VN + NT - 1) / NT;
     const size_t plane = ((size_t)p * a.c.heads + h) * a.prefix.cap;
-    const uint32_t raw0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)(smem + o_raw);
-    // loads of a tile: KS of 1 KiB, one of the scales, dealt out to the waves
-    constexpr int loads = W::KS + 1, most = (loads + RW - 1) / RW;
-    const int scales_from = min(4 * (W::NB == 3 ? lane : lane & (16 * W::NB - 1)), 64 * W::NB - 4);
-    const uint8_t* scales = scales_from < 32 * W::NB ? a.prefix.ks + plane * W::NB + scales_from : a.prefix.vs + plane * W::NB + scales_from - 32 * W::NB;
-    auto fetch = [&](int o, int slot) {
-        const size_t j0 = (size_t)o * kTile;
+    const uint8_t *kp = a.prefix.k + plane * row_bytes, *vp = a.prefix.v + plane * row_bytes, *ksp = a.prefix.ks + plane * W::NB, *vsp = a.prefix.vs + plane * W::NB;
+    int k_to[NK][KV], v_to[NV];
 #pragma unroll
-        for (int x = 0; x < most; x++) {
-            const int n = wave + RW * x;
-            if (n < W::KS) {
-                const int at = 1024 * n + 16 * lane;
-                const uint8_t* from = at < Tile::half ? a.prefix.k + (plane + j0) * Tile::row + at : a.prefix.v + (plane + j0) * Tile::row + at - Tile::half;
-                lds_load16(from, raw0 + slot * Tile::bytes + 1024 * n);
-            } else if (n == W::KS) {
-                lds_load4(scales + j0 * W::NB, raw0 + slot * Tile::bytes + Tile::o_scales);
-            }
+    for (int x = 0; x < NK; x++)
+#pragma unroll
+        for (int e = 0; e < KV; e++) {
+            const int n = (tid + NT * x) * KV + e, j = n / words, wd = n % words;
+            k_to[x][e] = (j >> 5) * U::bytes + U::k_at(wd / 2, U::k_lane(j & 31, wd & 1));
         }
-    };
-    const int mine = (loads - 1 - wave) / RW + (wave < loads ? 1 : 0);  // this wave's loads of a tile
-    constexpr int words = DH / 8, NK = (32 * words + NT - 1) / NT, NV = (16 * words + NT - 1) / NT;
-    int k_to[NK], v_from[NV], v_scale[NV], v_slot[NV], v_to[NV];
-#pragma unroll
-    for (int x = 0; x < NK; x++) {
-        const int n = tid + NT * x, j = n / words, wd = n % words;
-        k_to[x] = U::k_at(wd / 2, U::k_lane(j, wd & 1));
-    }
 #pragma unroll
     for (int x = 0; x < NV; x++) {
         const int n = tid + NT * x, j = n / words * 2, wd = n % words;
-        v_from[x] = Tile::half + j * Tile::row + 4 * wd;
-        v_scale[x] = Tile::o_scales + (32 + j) * W::NB + wd / 4;
-        v_slot[x] = j;
-        v_to[x] = U::v_at(wd / 4, j >> 4, U::v_lane(8 * (wd & 3), (j >> 2) & 1)) + 2 * ((j & 3) + (j >> 3 & 1) * 4);
+        v_to[x] = (j >> 5) * U::bytes + U::v_at(wd / 4, (j >> 4) & 1, U::v_lane(8 * (wd & 3), (j >> 2) & 1)) + 2 * ((j & 3) + (j >> 3 & 1) * 4);
     }
-    auto unpack = [&](int raw, int buf, int j0) {
-        const uint8_t* from = smem + o_raw + raw * Tile::bytes;
-        uint8_t* out = smem + buf * U::bytes;
+    struct Raw {
+        uint32_t k[NK][KV], ks[NK], v[NV][2], vs[NV][2];
+    };
+    // Slots behind the prefix's end may hold anything, or not be there: the last slot stands for them, its values with zeros.
+    auto load = [&](Raw& w, int o) {
+        const int j0 = o * 2 * kTile, last = span.held - 1 - j0;
+        const uint8_t *k = kp + (size_t)j0 * row_bytes, *v = vp + (size_t)j0 * row_bytes, *ks = ksp + (size_t)j0 * W::NB, *vs = vsp + (size_t)j0 * W::NB;
 #pragma unroll
         for (int x = 0; x < NK; x++) {
-            if (32 * words % NT && tid + NT * x >= 32 * words) break;
-            const int n = tid + NT * x;  // (words and scales lie in the lanes' order)
-            const uint32_t w = *(const uint32_t*)(from + 4 * n);
-            const float sc = mx4_scale(from[Tile::o_scales + n / 4]);
-            u32x4 y;
-#pragma unroll
-            for (int b = 0; b < 4; b++) y[b] = unpack2(w, sc, b);
-            *(u32x4*)(out + k_to[x]) = y;
+            if (KN % NT && tid + NT * x >= KN) break;
+            const int n = (tid + NT * x) * KV, j = min(n / words, last), wd = n % words;
+            if constexpr (KV == 4) *(u32x4*)w.k[x] = *(const u32x4*)(k + j * row_bytes + 4 * wd);
+            else if constexpr (KV == 2) *(u32x2*)w.k[x] = *(const u32x2*)(k + j * row_bytes + 4 * wd);
+            else w.k[x][0] = *(const uint32_t*)(k + j * row_bytes + 4 * wd);
+            w.ks[x] = ks[j * W::NB + wd / 4];
         }
 #pragma unroll
         for (int x = 0; x < NV; x++) {
-            if (16 * words % NT && tid + NT * x >= 16 * words) break;
-            uint32_t w[2], sb[2];
+            if (VN % NT && tid + NT * x >= VN) break;
+            const int n = tid + NT * x, wd = n % words;
 #pragma unroll
             for (int y = 0; y < 2; y++) {
-                w[y] = *(const uint32_t*)(from + v_from[x] + y * Tile::row);
-                sb[y] = from[v_scale[x] + y * W::NB];
-                if (j0 + v_slot[x] + y >= span.held) w[y] = sb[y] = 0;  // behind the end: may hold anything
+                const int j = min(n / words * 2 + y, last);
+                w.v[x][y] = *(const uint32_t*)(v + j * row_bytes + 4 * wd);
+                w.vs[x][y] = vs[j * W::NB + wd / 4];
             }
-            const float s0 = mx4_scale(sb[0]), s1 = mx4_scale(sb[1]);
+        }
+    };
+    uint32_t low = ~0u, high = ~0u;  // of scale bytes less 1, and less 141, the least (fp16_lacks)
+    auto give = [&](auto careful, Raw& w, uint8_t* out, int o) {
+        using Fm = Forms<T, decltype(careful)::value>;
+        const int left = span.held - o * 2 * kTile;
+#pragma unroll
+        for (int x = 0; x < NK; x++) {
+            if (KN % NT && tid + NT * x >= KN) break;
+            if (Fm::key_half) {
+                low = min(low, w.ks[x] - 1u);
+                high = min(high, w.ks[x] - 141u);
+            }
+            const float sc = mx4_scale(w.ks[x]);
+#pragma unroll
+            for (int e = 0; e < KV; e++) {
+                u32x4 y;
+#pragma unroll
+                for (int b = 0; b < 4; b++) y[b] = unpack2_as<Fm::key_half>(w.k[x][e], sc, b);
+                *(u32x4*)(out + k_to[x][e]) = y;
+            }
+        }
+        if (left < 2 * kTile) {
+            asm volatile("");
+#pragma unroll
+            for (int x = 0; x < NV; x++)
+#pragma unroll
+                for (int y = 0; y < 2; y++)
+                    if ((tid + NT * x) / words * 2 + y >= left) w.v[x][y] = w.vs[x][y] = 0;
+        }
+#pragma unroll
+        for (int x = 0; x < NV; x++) {
+            if (VN % NT && tid + NT * x >= VN) break;
+            if (Fm::value_half) {
+                low = min(low, min(w.vs[x][0] - 1u, w.vs[x][1] - 1u));
+                high = min(high, min(w.vs[x][0] - 141u, w.vs[x][1] - 141u));
+            }
+            const float s0 = mx4_scale(w.vs[x][0]), s1 = mx4_scale(w.vs[x][1]);
 #pragma unroll
             for (int b = 0; b < 4; b++) {
                 // channels 8 wd + 2 b and the next
-                const uint32_t y0 = unpack2(w[0], s0, b), y1 = unpack2(w[1], s1, b);
+                const uint32_t y0 = unpack2_as<Fm::value_half>(w.v[x][0], s0, b), y1 = unpack2_as<Fm::value_half>(w.v[x][1], s1, b);
                 *(uint32_t*)(out + (v_to[x] ^ (32 * b))) = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
                 *(uint32_t*)(out + (v_to[x] ^ (32 * b + 16))) = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
             }
@@ -124,8 +189,12 @@ __global__ __launch_bounds__(64 * RW, 2) void kv_prefix_kernel(KvSharedArgs a) {
 
     // the factor's sign, or zero, goes to the query, so that the largest product is the largest score
     const float sign = a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f, scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
-    v8bf qf[KF][QT];
-    {
+    v16f acc[ND];
+    float ref, l;  // 2^-ref is in l and acc
+    auto sweep = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+        using Fm = Forms<T, CAREFUL>;
+        typename Fm::Q qf[KF][Fm::q];
         const T* q = (const T*)a.q.data + s * a.q.seq + t * a.q.token + head * a.q.head + 8 * g;
 #pragma unroll
         for (int x = 0; x < KF; x++) {
@@ -133,118 +202,158 @@ __global__ __launch_bounds__(64 * RW, 2) void kv_prefix_kernel(KvSharedArgs a) {
             if (there) real_load8<T>(q + 16 * x, 8, y);
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] *= sign;
-            split_bf16<QT>(y, qf[x]);
+            split<Fm::q>(y, qf[x]);
         }
-    }
-    v16f acc[ND];
-    float m, l;
-    auto work = [&](auto careful, int buf, int j0) {
-        const uint8_t* from = smem + buf * U::bytes;
-        int k_lane = U::k_lane(i, g), v_lane = U::v_lane(i, g);
-        asm volatile("" : "+v"(k_lane), "+v"(v_lane));
-        v16f d = {};
-#pragma unroll
-        for (int x = 0; x < KF; x++) {
-            const v8bf kf = *(const v8bf*)(from + U::k_at(x, k_lane));
-#pragma unroll
-            for (int n = QT - 1; n >= 0; n--) d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[x][n], d, 0, 0, 0);
-        }
-        if (j0 + 32 > span.held) {
-            asm volatile("");
-#pragma unroll
-            for (int r = 0; r < 16; r++)
-                if (j0 + (r & 3) + 8 * (r >> 2) + 4 * g >= span.held) d[r] = -INFINITY;
-        }
-        float mt = d[0];
-#pragma unroll
-        for (int r = 1; r < 16; r++) mt = fmaxf(mt, d[r]);
-        mt = mt == -INFINITY ? -INFINITY : mt * scale;
-        if (__any(mt > m)) {  // rare after the first tiles
-            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
-            const float mn = fmaxf(m, fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])));
-            const float al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : m - mn);
-            m = mn;
-            l *= al;
-#pragma unroll
-            for (int x = 0; x < ND; x++) acc[x] *= al;
-        }
-        const float mu = m == -INFINITY ? 0.0f : m;
-        float pr[16];
-#pragma unroll
-        for (int r = 0; r < 16; r++)
-            pr[r] = __builtin_amdgcn_exp2f(decltype(careful)::value && fabsf(mu) >= kFar ? d[r] * scale - mu : fmaf(d[r], scale, -mu));
-        float sum[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) sum[r] = (pr[r] + pr[4 + r]) + (pr[8 + r] + pr[12 + r]);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        v8bf pf[2][PT];
-        split_bf16<PT>(pr, pf[0]);
-        split_bf16<PT>(pr + 8, pf[1]);
-#pragma unroll
-        for (int x = 0; x < ND; x++)
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                const v8bf vf = *(const v8bf*)(from + U::v_at(x, hf, v_lane));
-#pragma unroll
-                for (int n = PT - 1; n >= 0; n--) acc[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[hf][n], acc[x], 0, 0, 0);
-            }
-    };
-    auto sweep = [&](auto careful) {
 #pragma unroll
         for (int x = 0; x < ND; x++) acc[x] = v16f{};
-        m = -INFINITY;
+        float m = -INFINITY;  // the largest product so far
+        ref = -Fm::lift;
         l = 0.0f;
-        const int n = o1 - o0;
-        for (int x = 0; x < min(n, 3); x++) fetch(o0 + x, x);
-        vm_wait<0>();
-        barrier();
-        unpack(0, 0, o0 * kTile);
-        int raw = 0;  // of tile x
-        for (int x = 0; x < n; x++) {
-            // tile x is unpacked, tile x + 1 has landed; tile x's raw place and the other unpacked one are free
+        Raw w;
+        // Step o, unpacked in half `buf`; the next one is unpacked meanwhile, and the one after that asked for.
+        auto work = [&](auto buf, int o) {
+            uint8_t* from = smem + decltype(buf)::value * step;
+            uint8_t* to = smem + (1 - decltype(buf)::value) * step;
+            // All fragments of a product are asked for before the first is needed, V's before the softmax: left to itself the compiler waits for
+            // them two by two.
+            constexpr bool EARLY = !CAREFUL && sizeof(T) == 2;
+            constexpr int AHEAD = DH <= 64 ? 2 : 1;
+            const auto key = [&](int u, int f) { return *(const typename Fm::Q*)(from + u * U::bytes + U::k_at(f, U::k_lane(i, g))); };
+            const auto value = [&](int u, int f) { return *(const typename Fm::P*)(from + u * U::bytes + U::v_at(f >> 1, f & 1, U::v_lane(i, g))); };
+            typename Fm::Q kf[2][KF];
+            typename Fm::P vf[2][2 * ND];
+            if (EARLY) {
+#pragma unroll
+                for (int f = 0; f < KF; f++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) kf[u][f] = key(u, f);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            v16f d[2] = {v16f{}, v16f{}};
+#pragma unroll
+            for (int f = 0; f < KF; f++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    if (!EARLY) kf[u][f] = key(u, f);
+#pragma unroll
+                    for (int n = Fm::q - 1; n >= 0; n--) d[u] = product(kf[u][f], qf[f][n], d[u]);
+                }
+            if (EARLY) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int f = 0; f < 2 * ND; f++)
+#pragma unroll
+                    for (int u = 0; u < AHEAD; u++) vf[u][f] = value(u, f);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (o + 1 < o1) give(careful, w, to, o + 1);
+            if (o + 2 < o1) load(w, o + 2);
+            const int left = span.held - o * 2 * kTile;
+            if (left < 2 * kTile) {
+                asm volatile("");
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (kTile * u + (r & 3) + 8 * (r >> 2) + 4 * g >= left) d[u][r] = -INFINITY;
+            }
+            float mt = d[0][0];
+#pragma unroll
+            for (int r = 1; r < 32; r++) mt = __builtin_elementwise_maximum(mt, d[r >> 4][r & 15]);
+            if (__any(mt > m)) {  // rare after the first steps
+                const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+                const float mn = fmaxf(m, fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])));
+                const float now = mn == -INFINITY ? -Fm::lift : mn * scale - Fm::lift;
+                const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - now);  // (0: there is nothing yet)
+                m = mn;
+                ref = now;
+                l *= al;
+#pragma unroll
+                for (int f = 0; f < ND; f++) acc[f] *= al;
+            }
+            typename Fm::P pf[2][2][Fm::p];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                float pr[16];
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    pr[r] = __builtin_amdgcn_exp2f(CAREFUL && fabsf(ref) >= kFar ? d[u][r] * scale - ref : fmaf(d[u][r], scale, -ref));
+                split<Fm::p>(pr, pf[u][0]);
+                split<Fm::p>(pr + 8, pf[u][1]);
+                if constexpr (Fm::value_half) {
+                    // (the probabilities as they are held)
+                    const v2h one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+                    for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) l = __builtin_amdgcn_fdot2(v2h{pf[u][hf][0][2 * e], pf[u][hf][0][2 * e + 1]}, one, l, false);
+                } else {
+                    float sum[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) sum[r] = (pr[r] + pr[4 + r]) + (pr[8 + r] + pr[12 + r]);
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int f = 0; f < 2 * ND; f++) {
+                    if (!EARLY || u >= AHEAD) vf[u][f] = value(u, f);
+#pragma unroll
+                    for (int n = Fm::p - 1; n >= 0; n--) acc[f >> 1] = product(vf[u][f], pf[u][f & 1][n], acc[f >> 1]);
+                }
+        };
+        load(w, o0);
+        give(careful, w, smem, o0);
+        if (o0 + 1 < o1) load(w, o0 + 1);
+        for (int o = o0; o < o1; o += 2) {
             barrier();
-            if (x + 3 < n) fetch(o0 + x + 3, raw);
-            raw = raw == 2 ? 0 : raw + 1;
-            if (x + 1 < n) unpack(raw, (x + 1) & 1, (o0 + x + 1) * kTile);
-            work(careful, x & 1, (o0 + x) * kTile);
-            // all but this step's loads have landed
-            if (x + 3 >= n || mine == 0) vm_wait<0>();
-            else if (mine == 1) vm_wait<1>();
-            else vm_wait<most>();
+            work(std::integral_constant<int, 0>(), o);
+            if (o + 1 < o1) {
+                barrier();
+                work(std::integral_constant<int, 1>(), o + 1);
+            }
         }
         barrier();
     };
     sweep(std::false_type());
-    // scores far from zero: once more, with scores rounded as the maximum was (kFar)
-    if (__syncthreads_or(m != -INFINITY && fabsf(m) >= kFar)) sweep(std::true_type());
+    if (__syncthreads_or(low < 103u || high < 114u || fabsf(ref) >= kFar)) sweep(std::true_type());
     const float total = l + __shfl_xor(l, 32, 64);
     if (!there) return;
     // lane (i, g): row i, channels 32 x + 8 r + 4 g .. + 3
     const int heads = a.c.heads * a.group;
-    float* part = a.parts + (((size_t)blockIdx.y * a.c.n + s) * a.T * heads + (size_t)t * heads + head) * kPart<DH>;
+    float* part = a.parts + (((size_t)chunk * a.c.n + s) * a.T * heads + (size_t)t * heads + head) * kPart<DH>;
 #pragma unroll
     for (int x = 0; x < ND; x++)
 #pragma unroll
         for (int r = 0; r < 4; r++)
             *(v4f*)(part + 32 * x + 8 * r + 4 * g) = v4f{acc[x][4 * r], acc[x][4 * r + 1], acc[x][4 * r + 2], acc[x][4 * r + 3]};
     if (g == 0) {
-        part[DH] = m;
+        part[DH] = total == 0.0f ? -INFINITY : ref;
         part[DH + 1] = total;
     }
 }
 
-// How a call's rows are divided among workgroups of `rows` rows, and a prefix among `chunks`. How the sequences fall to the prefixes is
-// not known here: there is room for a last, partly filled row tile each.
+// How a call's rows are divided among workgroups of `rows` rows, and a prefix among `chunks`. How the sequences fall to the prefixes, and
+// how long these are, is not known here: there is room for a last, partly filled row tile each.
+//
+// Eight waves share a workgroup's unpacking where heads are wide, rows are 16-bit and a prefix has 256 or more of a head, four elsewhere (us
+// of this kernel, four and eight waves at their best chunks, bf16 heads of 128: 1024 rows of each of 8 heads over 16384 positions, four
+// times, 304 and 277; 256 rows over 16384 40 and 35; fp16 heads of 64, 680 rows over up to 6001, 22 and 26). Workgroups for every CU, of four
+// waves three, each with two steps at least; more cost more at their ends and in the join (the 256 rows with 8, 16 and 32 chunks 76, 48 and 35,
+// with 64 each 2 steps less; the 680 rows with 4, 8, 16 chunks 30, 21.7, 22.9; 8 fp32 heads of 32, 820 rows over up to 1000, with 1, 2, 3, 4:
+// 28, 20.6, 17.8, 27.3).
 struct PrefixPlan {
     int rows, chunks;
     long long tiles;  // row tiles a head, at most
 };
 PrefixPlan prefix_plan(const KvSharedArgs& a) {
     PrefixPlan p;
-    p.rows = 128;
-    p.tiles = (long long)a.c.n * a.T * a.group / p.rows + a.prefix.n;
-    const long long units = p.tiles * a.c.heads;
-    p.chunks = (int)std::max<long long>(1, std::min<long long>(512 / units, a.prefix.cap / kTile / 8));
+    const long long all = (long long)a.c.n * a.T * a.group;  // of a head
+    p.rows = real_size(a.type) == 2 && a.c.dh >= 96 && all >= 256LL * a.prefix.n ? 256 : 128;
+    p.tiles = std::max(0LL, all - a.prefix.n) / p.rows + a.prefix.n;
+    const long long want = (p.rows == 256 ? 256 : 768) / std::max(1LL, p.tiles * a.c.heads);
+    p.chunks = (int)std::max<long long>(1, std::min<long long>(want, a.prefix.cap / (2 * kTile) / 2));
     return p;
 }
 size_t parts_bytes(const KvSharedArgs& a, const PrefixPlan& p) {
@@ -258,7 +367,8 @@ size_t kv_shared_ws_bytes(const KvSharedArgs& a) {
     return own_ws_bytes(a, attn_plan(a)) + parts_bytes(a, prefix_plan(a));
 }
 bool kv_shared_fits(const KvSharedArgs& a) {
-    return own_fits(attn_plan(a)) && prefix_plan(a).tiles * a.c.heads < 1 << 23;
+    const PrefixPlan p = prefix_plan(a);
+    return own_fits(attn_plan(a)) && p.tiles * a.c.heads * p.chunks < 1 << 23;
 }
 
 hipError_t launch_kv_shared(const KvSharedArgs& args, hipStream_t s) {
@@ -271,7 +381,14 @@ hipError_t launch_kv_shared(const KvSharedArgs& args, hipStream_t s) {
         constexpr int DH = decltype(w)::value;
         return by_real(a.type, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            hipLaunchKernelGGL((kv_prefix_kernel<DH, T, 4>), dim3((unsigned)(p.tiles * a.c.heads), p.chunks), dim3(256), 0, s, a);
+            const dim3 grid((unsigned)(p.tiles * p.chunks * a.c.heads));
+            if constexpr (sizeof(T) == 2 && DH >= 96) {
+                if (p.rows == 256) {
+                    hipLaunchKernelGGL((kv_prefix_kernel<DH, T, 8>), grid, dim3(512), 0, s, a);
+                    return hipGetLastError();
+                }
+            }
+            hipLaunchKernelGGL((kv_prefix_kernel<DH, T, 4>), grid, dim3(256), 0, s, a);
             return hipGetLastError();
         });
     });
