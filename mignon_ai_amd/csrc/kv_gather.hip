@@ -59,110 +59,154 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvGatherArgs a) {
 }
 
 // In place: as if from a copy. What a sequence's place is to hold may be another's old rows and so on around, so a workgroup takes 16 bytes
-// of a head's plane times some neighbours, of all sequences at once: it reads all that moves there into its lanes' registers, waits, and
-// writes. Nobody else touches these bytes. A lane writes what it read.
-constexpr int kLanes = 1024, kHold = 16;         // lanes a workgroup, 16-byte pieces a lane
-constexpr int kInPlaceMax = kLanes * kHold;      // sequences
+// of a head's plane, times some neighbours, of all sequences at once: it reads all that moves there into its lanes' registers, waits, and
+// writes. Nobody else touches these bytes, and a lane writes what it read. No memory beside the cache, each byte moved once.
+//
+// A lane holds HOLD pieces of 16 bytes: up to 512 sequences 256 lanes of 8, up to 16384 1024 lanes of 16 (whose pieces then lie 16 to 64 bytes
+// at a place).
+constexpr int kInPlaceMax = 1024 * 16;  // sequences
+constexpr int kInPlaceFew = 512;
 
+// Bytes of a piece one by one: up to the first slot that holds no position, or where some may have been lost (zeros).
+__device__ __forceinline__ uint8_t byte_of(const u32x4& v, uint32_t b) {
+    const uint32_t w = b < 8 ? (b < 4 ? v.x : v.y) : b < 12 ? v.z : v.w;
+    return (uint8_t)(w >> (8 * (b & 3)));
+}
 template <int RB>
-__device__ __forceinline__ void gather_columns(const KvGatherArgs& a, uint8_t* plane, int h, const uint32_t* moves, int moved, int per_wg) {
-    const size_t seq = (size_t)a.to.heads * a.to.cap * RB;
-    uint8_t* base = plane + (size_t)h * a.to.cap * RB;
-    const uint32_t columns = (uint32_t)((size_t)a.to.cap * RB / 16);
-    int shift = 0;  // 2^shift columns at once
-    while ((2 << shift) <= per_wg && ((size_t)moved << (shift + 1)) <= (size_t)kInPlaceMax) shift++;
-    const int width = 1 << shift, items = moved << shift;
-    for (uint32_t c0 = blockIdx.x * per_wg; c0 < columns; c0 += gridDim.x * per_wg) {
-        for (uint32_t c1 = c0; c1 < min(columns, c0 + per_wg); c1 += width) {
-            u32x4 x[kHold];
-            uint32_t fine = 0;
-#pragma unroll
-            for (int k = 0; k < kHold; k++) {
-                const int n = k * kLanes + threadIdx.x;
-                if (k * kLanes >= items) break;
-                if (n >= items) continue;
-                const uint32_t mv = moves[n >> shift], c = c1 + (n & (width - 1)), j = 16 * c / RB;
-                const int i = mv >> 16, parent = mv & 0xffff;
-                if (c >= columns || (int)j >= min(max(a.lens[i], 0), a.to.cap)) continue;
-                fine |= 1u << k;
-                x[k] = *(const u32x4*)(base + parent * seq + 16 * (size_t)c);
-            }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < kHold; k++) {
-                if (!(fine >> k & 1)) continue;
-                const int n = k * kLanes + threadIdx.x;
-                const uint32_t mv = moves[n >> shift], c = c1 + (n & (width - 1));
-                const int i = mv >> 16, parent = mv & 0xffff, len = min(max(a.lens[i], 0), kKvMaxPos);
-                uint8_t* to = base + i * seq + 16 * (size_t)c;
-                const GatherSlot g{a.to, a.to, len, a.from_lens ? min(max(a.from_lens[parent], 0), kKvMaxPos) : len};
-                if (!a.from_lens && (int)((16 * c + 15) / RB) < min(len, a.to.cap)) {
-                    *(u32x4*)to = x[k];
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 16; b++) {
-                        const int j = (16 * c + b) / RB;
-                        int slot;
-                        if (j < a.to.cap && g.find(j, slot)) to[b] = slot >= 0 ? (uint8_t)(x[k][b / 4] >> (8 * (b & 3))) : 0;
-                    }
-                }
-            }
-            __syncthreads();
-        }
+__device__ __forceinline__ void store_first(uint8_t* to, const u32x4& v, uint32_t first, uint32_t slots) {
+    const uint32_t n = min(16u, slots * RB - first);
+#pragma unroll 1
+    for (uint32_t b = 0; b < n; b++) to[b] = byte_of(v, b);
+}
+template <int RB>
+__device__ __forceinline__ void store_some(uint8_t* to, const u32x4& v, const GatherSlot& g, uint32_t first) {
+#pragma unroll 1
+    for (uint32_t b = 0; b < 16; b++) {
+        int slot;
+        if (g.find((int)((first + b) / RB), slot)) to[b] = slot >= 0 ? byte_of(v, b) : 0;
     }
 }
 
-template <int DH>
-__global__ __launch_bounds__(kLanes) void kv_gather_in_place_kernel(KvGatherArgs a, int per_wg) {
-    extern __shared__ uint32_t moves[];  // sequence << 16 | parent
-    __shared__ int s_count[kLanes / 64];
+template <int RB, int NT, int HOLD>
+__device__ __forceinline__ void gather_columns(const KvGatherArgs& a, uint8_t* plane, int h, const uint2* moves, int moved, uint32_t c0, int per_wg) {
+    const size_t seq = (size_t)a.to.heads * a.to.cap * RB;
+    uint8_t* base = plane + (size_t)h * a.to.cap * RB;
+    const uint32_t columns = (uint32_t)((size_t)a.to.cap * RB / 16), c_end = min(columns, c0 + per_wg);
+    int shift = 0;  // 2^shift columns at once
+    while ((2 << shift) <= per_wg && (moved << (shift + 1)) <= NT * HOLD) shift++;
+    const int width = 1 << shift, items = moved << shift;
+    for (uint32_t c1 = c0; c1 < c_end; c1 += width) {
+        u32x4 x[HOLD];
+        uint32_t fine = 0;
+#pragma unroll
+        for (int k = 0; k < HOLD; k++) {
+            const int n = k * NT + threadIdx.x;
+            if (n >= items) continue;
+            const uint2 mv = moves[n >> shift];
+            const uint32_t c = c1 + (n & (width - 1));
+            if (c >= c_end || 16 * c / RB >= mv.y) continue;
+            fine |= 1u << k;
+            x[k] = *(const u32x4*)(base + (mv.x & 0xffff) * seq + 16 * (size_t)c);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < HOLD; k++) {
+            if (!(fine >> k & 1)) continue;
+            int n = k * NT + threadIdx.x;
+            asm volatile("" : "+v"(n));  // (addresses are found again: kept, they would not fit the registers)
+            const uint2 mv = moves[n >> shift];
+            const uint32_t c = c1 + (n & (width - 1)), i = mv.x >> 16, parent = mv.x & 0xffff;
+            uint8_t* to = base + i * seq + 16 * (size_t)c;
+            if (!a.from_lens && (16 * c + 15) / RB < mv.y) {
+                *(u32x4*)to = x[k];
+            } else if (!a.from_lens) {
+                store_first<RB>(to, x[k], 16 * c, mv.y);
+            } else {
+                store_some<RB>(to, x[k], GatherSlot{a.to, a.to, min(max(a.lens[i], 0), kKvMaxPos), min(max(a.from_lens[parent], 0), kKvMaxPos)}, 16 * c);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <int DH, int NT, int HOLD>
+__global__ __launch_bounds__(NT) void kv_gather_in_place_kernel(KvGatherArgs a, int per_wg, int code_blocks, int scale_blocks) {
+    extern __shared__ uint2 moves[];  // sequence << 16 | parent; slots that hold a position
+    __shared__ int s_count[NT / 64];
     int moved = 0;
-    for (int i0 = 0; i0 < a.to.n; i0 += kLanes) {
-        const int i = i0 + threadIdx.x, parent = i < a.to.n ? a.parents[i] : -1;
+    for (int i0 = 0; i0 < a.to.n; i0 += NT) {
+        const int i = i0 + threadIdx.x, parent = i < a.to.n ? a.parents[i] : -1, len = i < a.to.n ? a.lens[i] : 0;
         // (a sequence that becomes itself, of another length, may have positions to clear)
-        const bool mv = parent >= 0 && parent < a.to.n && a.lens[i] > 0 && (parent != i || (a.from_lens && a.from_lens[i] != a.lens[i]));
+        const bool mv = parent >= 0 && parent < a.to.n && len > 0 && (parent != i || (a.from_lens && a.from_lens[i] != len));
         const uint64_t who = __ballot(mv);
         const int wave = threadIdx.x >> 6;
         __syncthreads();
         if ((threadIdx.x & 63) == 0) s_count[wave] = __popcll(who);
         __syncthreads();
         int before = moved;
-        for (int w = 0; w < kLanes / 64; w++) {
+        for (int w = 0; w < NT / 64; w++) {
             before += w < wave ? s_count[w] : 0;
             moved += s_count[w];
         }
-        if (mv) moves[before + __popcll(who & ((1ull << (threadIdx.x & 63)) - 1))] = (uint32_t)i << 16 | parent;
+        if (mv) moves[before + __popcll(who & ((1ull << (threadIdx.x & 63)) - 1))] = make_uint2((uint32_t)i << 16 | parent, min(len, a.to.cap));
     }
     __syncthreads();
     if (moved == 0) return;
-    const int h = blockIdx.y >> 2;
-    switch (blockIdx.y & 3) {
-        case 0: return gather_columns<DH / 2>(a, a.to.k, h, moves, moved, per_wg);
-        case 1: return gather_columns<DH / 2>(a, a.to.v, h, moves, moved, per_wg);
-        case 2: return gather_columns<DH / 32>(a, a.to.ks, h, moves, moved, per_wg);
-        default: return gather_columns<DH / 32>(a, a.to.vs, h, moves, moved, per_wg);
+    int b = blockIdx.x;
+    const int codes = 2 * a.to.heads * code_blocks;
+    if (b < codes) {
+        const int plane = b / code_blocks, h = plane >> 1;
+        gather_columns<DH / 2, NT, HOLD>(a, plane & 1 ? a.to.v : a.to.k, h, moves, moved, (uint32_t)(b - plane * code_blocks) * per_wg, per_wg);
+    } else {
+        b -= codes;
+        const int plane = b / scale_blocks, h = plane >> 1;
+        gather_columns<DH / 32, NT, HOLD>(a, plane & 1 ? a.to.vs : a.to.ks, h, moves, moved, (uint32_t)(b - plane * scale_blocks) * per_wg, per_wg);
     }
 }
 
 bool in_place(const KvGatherArgs& a) { return a.to.k == a.from.k; }
 
+// Columns of a workgroup: as many as it holds of all sequences twice over (fewer than all move).
+struct InPlacePlan {
+    int per_wg;
+    long long code_blocks, scale_blocks, blocks;
+};
+InPlacePlan in_place_plan(const KvGatherArgs& a) {
+    InPlacePlan p;
+    const int room = a.to.n <= kInPlaceFew ? 256 * 8 : 1024 * 16;
+    p.per_wg = 1;
+    while (p.per_wg < 256 && p.per_wg * a.to.n < room) p.per_wg *= 2;
+    const auto blocks = [&](int rb) { return ((long long)a.to.cap * rb / 16 + p.per_wg - 1) / p.per_wg; };
+    p.code_blocks = blocks(a.to.dh / 2);
+    p.scale_blocks = blocks(a.to.dh / 32);
+    p.blocks = 2 * a.to.heads * (p.code_blocks + p.scale_blocks);
+    return p;
+}
+
+template <int DH, int NT, int HOLD>
+hipError_t launch_in_place(const KvGatherArgs& a, hipStream_t s) {
+    static std::atomic<uint64_t> allowed{0};
+    if (NT > 256)
+        if (const hipError_t e = allow_lds((const void*)kv_gather_in_place_kernel<DH, NT, HOLD>, 8 * kInPlaceMax, allowed); e != hipSuccess) return e;
+    const InPlacePlan p = in_place_plan(a);
+    hipLaunchKernelGGL((kv_gather_in_place_kernel<DH, NT, HOLD>), dim3((unsigned)p.blocks), dim3(NT), 8 * a.to.n, s, a, p.per_wg, (int)p.code_blocks,
+                       (int)p.scale_blocks);
+    return hipGetLastError();
+}
+
 }  // namespace
 
+// (a launch's 2^32 lanes)
 bool kv_gather_fits(const KvGatherArgs& a) {
-    return in_place(a) ? a.to.n <= kInPlaceMax : (long long)a.to.n * a.to.heads < 1 << 23;
+    if (!in_place(a)) return (long long)a.to.n * a.to.heads < 1 << 23;
+    return a.to.n <= kInPlaceMax && in_place_plan(a).blocks < (a.to.n <= kInPlaceFew ? 1 << 24 : 1 << 22);
 }
 
 hipError_t launch_kv_gather(const KvGatherArgs& a, hipStream_t s) {
     return by_width(a.to.dh, [&](auto w) {
         constexpr int DH = decltype(w)::value;
-        if (in_place(a)) {
-            const int per_wg = 64;
-            const long long blocks = ((long long)a.to.cap * (DH / 2) / 16 + per_wg - 1) / per_wg;
-            const dim3 grid((unsigned)std::min<long long>(blocks, std::max(1, (1 << 16) / a.to.heads)), a.to.heads * 4);
-            hipLaunchKernelGGL((kv_gather_in_place_kernel<DH>), grid, dim3(kLanes), 4 * a.to.n, s, a, per_wg);
-            return hipGetLastError();
-        }
+        if (in_place(a)) return a.to.n <= kInPlaceFew ? launch_in_place<DH, 256, 8>(a, s) : launch_in_place<DH, 1024, 16>(a, s);
         const long long rows = (long long)a.to.n * a.to.heads;
         const int blocks = (int)std::max<long long>(1, std::min<long long>((a.to.cap * (DH / 32) + 255) / 256, 8192 / rows));
         hipLaunchKernelGGL((kv_gather_kernel<DH>), dim3((unsigned)rows, blocks), dim3(256), 0, s, a);
