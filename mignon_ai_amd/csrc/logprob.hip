@@ -5,10 +5,11 @@
 // one fused operation a power; sums at one r are put at another by 2^(r - r'), and at the end r's rounding, d = m c - r, is taken out
 // of log S (it cancels in the entropy).
 //
-// The k likeliest: of every 32 WAVES logits that lie in one of 64 groups of lanes, the largest; the k-th of these is at most the k-th of
-// the tile, so only what reaches it can be among the k. Numbers and ids are one 64-bit key, no two alike: at most k groups, 32 k WAVES
-// logits, reach the bound, whatever the logits are, and in ordinary rows few more than k. Later tiles are held to the bound so far, and
-// one whose lanes' maxima all fail it (most do) costs nothing more. Candidates are put in order by counting, for each, those above it.
+// The k likeliest: a wave looks at tiles of 2048 logits, 32 a lane. The k-th of the lanes' maxima is at most the k-th of the tile, so only what
+// reaches it can be among the k: in ordinary rows few more than k. Where the k-th is met by more than there is room for (many equal logits, as
+// in masked rows), numbers and ids together, one 64-bit key, no two alike, bound it: at most k lanes reach the bound then, with 32 logits
+// each. Later tiles are held to the bound so far, and one whose lanes' maxima all fail it (most do) costs nothing more. Candidates are put in
+// order by counting, for each, those above it. A wave does all that by itself; up to four share a row, and meet at its end.
 #include "logprob.hpp"
 
 #include <algorithm>
@@ -64,58 +65,66 @@ struct Raw8 {
     }
 };
 
+// Between lanes of a wave, through LDS.
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
-template <int WAVES>
-__device__ __forceinline__ void team_sync() {
-    if constexpr (WAVES > 1) __syncthreads();
-    else wave_fence();
-}
-template <int WAVES>
-__device__ __forceinline__ bool team_any(bool v) {
-    if constexpr (WAVES > 1) return __syncthreads_or(v);
-    else return __any(v);
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = min(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    return v;
 }
 
-// The candidates of a team (a wave, or four) in LDS.
-template <int WAVES>
+constexpr int kTile = 2048;  // logits of a wave's tile
+// A wave's candidates, in LDS.
 struct Top {
-    static constexpr int lanes = 64 * WAVES, each = 32 * WAVES;  // each: logits of a group in a tile
     uint64_t* keys;   // room
-    uint64_t* best;   // 64 groups' keys; the k best in order
+    uint64_t* best;   // the k best in order; lanes' keys
     int* count;
     int k, room, l;
     uint64_t bound = 1;
-    static __host__ __device__ int room_of(int k) { return each * k + 256; }
+    static __host__ __device__ int room_of(int k) { return 32 * k + 256; }
     static __host__ __device__ int bytes(int k) { return k ? 8 * (room_of(k) + 64) + 16 : 0; }
     __device__ __forceinline__ Top(uint8_t* at, int k_, int l_) : k(k_), room(room_of(k_)), l(l_) {
         keys = (uint64_t*)at;
         best = keys + room;
         count = (int*)(best + 64);
     }
-    // Raises the bound to the k-th largest of the groups' largest keys.
-    __device__ void tighten(uint64_t mine) {
-        if constexpr (WAVES > 1) {
-            // four neighbouring lanes are a group
+    // Raises the bound to the k-th largest of the lanes' maxima, or, for many, of those of their halves (of 64 maxima the 64th is met by 300
+    // of 2048 logits, of 128 by 90), by their numbers alone. A lane without numbers has none.
+    static __device__ __forceinline__ uint32_t number(float m) { return m > -INFINITY ? (uint32_t)(top_key(m, 0) >> 32) : 0u; }
+    __device__ __forceinline__ void tighten(float m0, float m1) {
+        uint32_t h0 = number(m0), h1 = number(m1), kth;
+        if (k <= 16) {
+            h0 = max(h0, h1);
+            int above = 0;
 #pragma unroll
-            for (int o = 1; o < WAVES; o *= 2) {
-                const uint64_t other = __shfl_xor((unsigned long long)mine, o, 64);
-                mine = other > mine ? other : mine;
+            for (int j = 0; j < 64; j++) above += (uint32_t)__builtin_amdgcn_readlane((int)h0, j) > h0;
+            kth = wave_min(above < k ? h0 : ~0u);
+        } else {
+            int a0 = 0, a1 = 0;
+#pragma unroll 16
+            for (int j = 0; j < 64; j++) {
+                const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)h0, j), y = (uint32_t)__builtin_amdgcn_readlane((int)h1, j);
+                a0 += (x > h0) + (y > h0);
+                a1 += (x > h1) + (y > h1);
             }
+            kth = wave_min(min(a0 < k ? h0 : ~0u, a1 < k ? h1 : ~0u));
         }
-        if (l % WAVES == 0) best[l / WAVES] = mine;
-        team_sync<WAVES>();
-        // (each wave finds it for itself)
-        const uint64_t key = best[l & 63];
+        const uint64_t key = (uint64_t)kth << 32;
+        bound = key > bound ? key : bound;
+    }
+    __device__ void tighten_exactly(uint64_t mine) {
+        best[l] = mine;
+        wave_fence();
         int above = 0;
 #pragma unroll 8
-        for (int j = 0; j < 64; j++) above += best[j] > key || (best[j] == key && j < (l & 63));  // (groups without logits are alike)
+        for (int j = 0; j < 64; j++) above += best[j] > mine || (best[j] == mine && j < l);  // (lanes without logits are alike)
         const uint64_t who = __ballot(above == k - 1);
-        const uint64_t kth = __shfl((unsigned long long)key, __ffsll((unsigned long long)who) - 1, 64);
+        const uint64_t kth = __shfl((unsigned long long)mine, __ffsll((unsigned long long)who) - 1, 64);
         bound = kth > bound ? kth : bound;
-        team_sync<WAVES>();
+        wave_fence();
     }
     __device__ __forceinline__ void push(uint64_t key) {
         if (key < bound) return;
@@ -124,46 +133,49 @@ struct Top {
     }
     // Leaves the k largest of n candidates, in order, and raises the bound to the last of them.
     __device__ int select(int n) {
-        for (int c = l; c < n; c += lanes) {
+        for (int c = l; c < n; c += 64) {
             const uint64_t key = keys[c];
             int above = 0;
 #pragma unroll 8
             for (int j = 0; j < n; j++) above += keys[j] > key;
             if (above < k) best[above] = key;
         }
-        team_sync<WAVES>();
+        wave_fence();
         const int left = min(n, k);
         if (l < left) keys[l] = best[l];
         if (l == 0) *count = left;
         if (left == k) bound = best[k - 1] > bound ? best[k - 1] : bound;
-        team_sync<WAVES>();
+        wave_fence();
         return left;
     }
 };
 
-// A team of WAVES waves takes a segment of a row, in tiles of 32 logits a lane, the next one loaded while one is worked on.
+// WAVES waves take a segment of a row, tile by tile in turns, each wave's next tile loaded while it works on one.
 template <class T, int WAVES>
 __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int splits, int segment) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float s_part[3][4];
-    constexpr int lanes = 64 * WAVES, tile = 32 * lanes, teams = 4 / WAVES;
-    const int team = WAVES > 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & (lanes - 1);
+    __shared__ uint64_t s_best[kMaxTop];
+    constexpr int lanes = 64 * WAVES, teams = 4 / WAVES;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = wave / WAVES, w = wave % WAVES;
+    const int lane = threadIdx.x & 63, l = 64 * w + lane;
     const long long unit = (long long)blockIdx.x * teams + team;
-    if (unit >= (long long)a.n * splits) return;  // (a wave by itself)
+    if (unit >= (long long)a.n * splits) return;  // (a wave by itself, or all four)
     const long long r = splits == 1 ? unit : unit / splits;
     const int part = (int)(unit - r * splits), from = part * segment, to = min(a.V, from + segment);
     const T* x = (const T*)a.x + r * a.ld;
-    Top<WAVES> top(smem + team * Top<WAVES>::bytes(a.k), a.k, l);
+    Top top(smem + wave * Top::bytes(a.k), a.k, lane);
 
     Raw8<T> next[4];
     auto fetch = [&](int v0) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int v = v0 + (j * lanes + l) * 8;
+            const int v = v0 + (j * 64 + lane) * 8;
             next[j].load(x + v, to - v);
         }
     };
-    fetch(from);
+    const int begin = from + kTile * w;
+    if (begin < to) fetch(begin);
     // a lane's target
     int target = -1;
     float x_t = NAN;
@@ -174,17 +186,21 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int splits,
     float m = -INFINITY, at = 0.0f, S = 0.0f, X = 0.0f;  // at: r
     int n = 0;                                           // candidates
     if (a.k) {
-        if (l == 0) *top.count = 0;
-        team_sync<WAVES>();
+        if (lane == 0) *top.count = 0;
+        wave_fence();
     }
-    for (int v0 = from; v0 < to; v0 += tile) {
+    for (int v0 = begin; v0 < to; v0 += kTile * WAVES) {
         float y[32];
 #pragma unroll
         for (int j = 0; j < 4; j++) next[j].get(y + 8 * j);
-        if (v0 + tile < to) fetch(v0 + tile);
-        float mt = y[0];
+        if (v0 + kTile * WAVES < to) fetch(v0 + kTile * WAVES);
+        float m0 = y[0], m1 = y[16];
 #pragma unroll
-        for (int e = 1; e < 32; e++) mt = fmaxf(mt, y[e]);
+        for (int e = 1; e < 16; e++) {
+            m0 = fmaxf(m0, y[e]);
+            m1 = fmaxf(m1, y[16 + e]);
+        }
+        const float mt = fmaxf(m0, m1);
         if (__any(mt > m)) {
             const float mn = fmaxf(m, mt), an = fmaxf(mn, -kHuge) * kLog2e, f = __builtin_amdgcn_exp2f(at - an);
             // (a lane with nothing above -kHuge adds nothing to a row that has more; S 0: there is no reference to leave)
@@ -203,50 +219,55 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int splits,
         S += (s4[0] + s4[1]) + (s4[2] + s4[3]);
         X += (x4[0] + x4[1]) + (x4[2] + x4[3]);
         if (!a.k) continue;
-        const bool first = v0 == from;
-        if (!team_any<WAVES>(first || (top.bound >> 32) == 0 || mt >= key_value(top.bound))) continue;
-        auto tighten = [&] {
-            int id = -1;
-            uint64_t key = 0;
+        const bool first = v0 == begin;
+        if (!first && !__any((top.bound >> 32) == 0 || mt >= key_value(top.bound))) continue;
+        const auto id_of = [&](int e) { return v0 + ((e >> 3) * 64 + lane) * 8 + (e & 7); };
+        // the lane's first largest logit (what is not there, behind the end, is -infinity and comes last)
+        const auto largest = [&] {
+            int at = 0;
 #pragma unroll
-            for (int e = 31; e >= 0; e--) {
-                const int v = v0 + ((e >> 3) * lanes + l) * 8 + (e & 7);
-                if (v < to) {
-                    if (y[e] == mt) id = v;
-                    else if (y[e] != y[e]) key = top_key(y[e], v);
+            for (int e = 31; e >= 0; e--) at = y[e] == mt ? e : at;
+            uint64_t key = id_of(at) < to ? top_key(mt, id_of(at)) : 0;
+            if (!(mt > -INFINITY)) {
+                // nothing but -infinity, NaN, and what is not there
+                asm volatile("");
+                key = 0;
+#pragma unroll
+                for (int e = 31; e >= 0; e--) {
+                    const uint64_t other = id_of(e) < to ? top_key(y[e], id_of(e)) : 0;
+                    key = other > key ? other : key;
                 }
             }
-            top.tighten(id >= 0 ? top_key(mt, id) : key);
+            return key;
         };
-        auto push = [&] {
+        const auto push = [&] {
+            // (NaN is not below anything: its key decides)
+            const float low = (top.bound >> 32) == 0 ? -INFINITY : key_value(top.bound);
 #pragma unroll
-            for (int e = 0; e < 32; e++) {
-                const int v = v0 + ((e >> 3) * lanes + l) * 8 + (e & 7);
-                if (v < to) top.push(top_key(y[e], v));
-            }
-            team_sync<WAVES>();
+            for (int e = 0; e < 32; e++)
+                if (!(y[e] < low) && id_of(e) < to) top.push(top_key(y[e], id_of(e)));
+            wave_fence();
+            return *top.count;
         };
-        if (first) tighten();
-        push();
-        int now = *top.count;
+        if (first) top.tighten(m0, m1);
+        int now = push();
         if (now > top.room) {
             // more than there is room for reach the bound so far: once more, with the tile's own
-            team_sync<WAVES>();
-            if (l == 0) *top.count = n;
-            team_sync<WAVES>();
+            wave_fence();
+            if (lane == 0) *top.count = n;
+            wave_fence();
             n = top.select(n);
-            tighten();
-            push();
-            now = *top.count;
+            top.tighten_exactly(largest());
+            now = push();
         }
         n = now;
-        team_sync<WAVES>();
-        if (n > 2 * a.k + 32) n = top.select(n);
+        wave_fence();
+        if (n > a.k + a.k / 2 + 8) n = top.select(n);
     }
     // the row's: lanes' sums at the largest maximum
     float most = wave_max(m);
     if constexpr (WAVES > 1) {
-        if ((l & 63) == 0) s_part[0][l >> 6] = most;
+        if (lane == 0) s_part[0][w] = most;
         __syncthreads();
         most = fmaxf(fmaxf(s_part[0][0], s_part[0][1]), fmaxf(s_part[0][2], s_part[0][3]));
     }
@@ -266,16 +287,39 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int splits,
     }
     S = wave_sum(S);
     X = wave_sum(X);
+    const uint64_t* best = top.best;
+    if (a.k) n = top.select(n);
     if constexpr (WAVES > 1) {
-        if ((l & 63) == 0) {
-            s_part[1][l >> 6] = S;
-            s_part[2][l >> 6] = X;
+        if (lane == 0) {
+            s_part[1][w] = S;
+            s_part[2][w] = X;
         }
+        if (a.k && lane < a.k && lane >= n) top.keys[lane] = 0;
         __syncthreads();
         S = (s_part[1][0] + s_part[1][1]) + (s_part[1][2] + s_part[1][3]);
         X = (s_part[2][0] + s_part[2][1]) + (s_part[2][2] + s_part[2][3]);
+        if (a.k) {
+            // the waves' lists, in order each
+            if (lane < a.k) {
+                const uint64_t key = top.keys[lane];
+                int above = lane;
+                for (int o = 1; o < WAVES; o++) {
+                    const uint64_t* other = (const uint64_t*)(smem + (w ^ o) * Top::bytes(a.k));
+                    int lo = 0, hi = a.k;  // other[lo - 1] > key >= other[hi]
+                    while (lo < hi) {
+                        const int mid = (lo + hi) >> 1;
+                        if (other[mid] > key) lo = mid + 1;
+                        else hi = mid;
+                    }
+                    above += lo;
+                }
+                if (above < a.k && key) s_best[above] = key;
+            }
+            __syncthreads();
+            n = min(a.k, to - from);
+            best = s_best;
+        }
     }
-    if (a.k) n = top.select(n);
     if (splits > 1) {
         uint8_t* out = (uint8_t*)a.ws + unit * part_bytes(a.k);
         if (most == -INFINITY) off = 0.0f;
@@ -284,7 +328,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int splits,
             *(Part*)out = Part{most, S * f, (X - off * S) * f, 0.0f};
         }
         uint64_t* keys = (uint64_t*)(out + sizeof(Part));
-        if (l < a.k) keys[l] = l < n ? top.best[l] : 0;  // (k is at most 64)
+        if (l < a.k) keys[l] = l < n ? best[l] : 0;  // (k is at most 64)
         return;
     }
     const float log_s = logf(S) - off * kLn2;
@@ -297,7 +341,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int splits,
         a.logprob[r * a.m + j] = (x_t - most) - log_s;
     }
     if (l < a.k) {
-        const uint64_t key = top.best[l];
+        const uint64_t key = best[l];
         if (a.top_ids) a.top_ids[r * a.k + l] = key_id(key);
         if (a.top_logprob) a.top_logprob[r * a.k + l] = (key_value(key) - most) - log_s;
     }
@@ -379,7 +423,7 @@ struct LogprobPlan {
 LogprobPlan logprob_plan(const LogprobArgs& a) {
     LogprobPlan p;
     p.waves = a.V <= 2048 ? 1 : 4;
-    const int tile = 2048 * p.waves, tiles = (a.V - 1) / tile + 1;
+    const int tile = kTile * p.waves, tiles = (a.V - 1) / tile + 1;
     const int want = std::min(64, std::max(1, std::min(tiles, 1024 / std::max(a.n, 1))));
     p.segment = (tiles + want - 1) / want * tile;
     p.splits = (a.V - 1) / p.segment + 1;
@@ -391,8 +435,8 @@ hipError_t launch_rows(const LogprobArgs& a, const LogprobPlan& p, hipStream_t s
     const long long units = (long long)a.n * p.splits;
     const int teams = 4 / WAVES;
     static std::atomic<uint64_t> allowed{0};
-    if (const hipError_t e = allow_lds((const void*)logprob_kernel<T, WAVES>, teams * Top<WAVES>::bytes(kMaxTop), allowed); e != hipSuccess) return e;
-    hipLaunchKernelGGL((logprob_kernel<T, WAVES>), dim3((unsigned)((units + teams - 1) / teams)), dim3(256), teams * Top<WAVES>::bytes(a.k), s, a,
+    if (const hipError_t e = allow_lds((const void*)logprob_kernel<T, WAVES>, 4 * Top::bytes(kMaxTop), allowed); e != hipSuccess) return e;
+    hipLaunchKernelGGL((logprob_kernel<T, WAVES>), dim3((unsigned)((units + teams - 1) / teams)), dim3(256), 4 * Top::bytes(a.k), s, a,
                        p.splits, p.segment);
     return hipGetLastError();
 }
