@@ -26,6 +26,8 @@ struct GatherSlot {
 };
 
 // Another cache's: a workgroup a sequence, head and stretch of slots, a lane 16 bytes of codes of K and V; then the scales, a slot a lane.
+// Bound by memory: 64 sequences of 1500 to 3000 positions, 8 heads of 128, 131 MB read and written: 23 us where the source stays in the
+// caches (5.7 TB/s), 41 from call to call of other data.
 template <int DH>
 __global__ __launch_bounds__(256) void kv_gather_kernel(KvGatherArgs a) {
     constexpr int row = DH / 2, L16 = row / 16, NB = DH / 32;
@@ -62,10 +64,12 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvGatherArgs a) {
 // of a head's plane, times some neighbours, of all sequences at once: it reads all that moves there into its lanes' registers, waits, and
 // writes. Nobody else touches these bytes, and a lane writes what it read. No memory beside the cache, each byte moved once.
 //
-// A lane holds HOLD pieces of 16 bytes: up to 512 sequences 256 lanes of 8, up to 16384 1024 lanes of 16 (whose pieces then lie 16 to 64 bytes
-// at a place).
+// A lane holds HOLD pieces of 16 bytes: up to 512 sequences 256 lanes of 8, up to 2048 512 of 8, up to 16384 1024 of 16, so that whole 64 bytes
+// of a place are taken together. us, half of the sequences becoming copies of the others, 256 x 8, 512 x 8, 1024 x 8 and 1024 x 16: 64 of 1024
+// positions (8 heads of 128) 11.3 14.1 16.5 17; 256 of 1051 (8 of 64) 22 26 29 34; 1024 of 251 (8 of 64) 46 35 33 41; 2000 of 251 (8 of 32)
+// 53 44 49 62; 4096 of 59 (8 of 32) - 51 46 45. Bound by memory for few long sequences (256 streams of 1056 slots, 111 MB read and
+// written: 5 TB/s), then by lines of which a workgroup takes a part, and by the list of moves that each makes (4096: four rounds).
 constexpr int kInPlaceMax = 1024 * 16;  // sequences
-constexpr int kInPlaceFew = 512;
 
 // Bytes of a piece one by one: up to the first slot that holds no position, or where some may have been lost (zeros).
 __device__ __forceinline__ uint8_t byte_of(const u32x4& v, uint32_t b) {
@@ -167,14 +171,15 @@ __global__ __launch_bounds__(NT) void kv_gather_in_place_kernel(KvGatherArgs a, 
 
 bool in_place(const KvGatherArgs& a) { return a.to.k == a.from.k; }
 
+int in_place_lanes(const KvGatherArgs& a) { return a.to.n <= 512 ? 256 : a.to.n <= 2048 ? 512 : 1024; }
+
 // Columns of a workgroup: as many as it holds of all sequences twice over (fewer than all move).
 struct InPlacePlan {
     int per_wg;
     long long code_blocks, scale_blocks, blocks;
 };
-InPlacePlan in_place_plan(const KvGatherArgs& a) {
+InPlacePlan in_place_plan(const KvGatherArgs& a, int room) {
     InPlacePlan p;
-    const int room = a.to.n <= kInPlaceFew ? 256 * 8 : 1024 * 16;
     p.per_wg = 1;
     while (p.per_wg < 256 && p.per_wg * a.to.n < room) p.per_wg *= 2;
     const auto blocks = [&](int rb) { return ((long long)a.to.cap * rb / 16 + p.per_wg - 1) / p.per_wg; };
@@ -187,9 +192,9 @@ InPlacePlan in_place_plan(const KvGatherArgs& a) {
 template <int DH, int NT, int HOLD>
 hipError_t launch_in_place(const KvGatherArgs& a, hipStream_t s) {
     static std::atomic<uint64_t> allowed{0};
-    if (NT > 256)
+    if (NT == 1024)
         if (const hipError_t e = allow_lds((const void*)kv_gather_in_place_kernel<DH, NT, HOLD>, 8 * kInPlaceMax, allowed); e != hipSuccess) return e;
-    const InPlacePlan p = in_place_plan(a);
+    const InPlacePlan p = in_place_plan(a, NT * HOLD);
     hipLaunchKernelGGL((kv_gather_in_place_kernel<DH, NT, HOLD>), dim3((unsigned)p.blocks), dim3(NT), 8 * a.to.n, s, a, p.per_wg, (int)p.code_blocks,
                        (int)p.scale_blocks);
     return hipGetLastError();
@@ -200,13 +205,20 @@ hipError_t launch_in_place(const KvGatherArgs& a, hipStream_t s) {
 // (a launch's 2^32 lanes)
 bool kv_gather_fits(const KvGatherArgs& a) {
     if (!in_place(a)) return (long long)a.to.n * a.to.heads < 1 << 23;
-    return a.to.n <= kInPlaceMax && in_place_plan(a).blocks < (a.to.n <= kInPlaceFew ? 1 << 24 : 1 << 22);
+    const int lanes = in_place_lanes(a);
+    return a.to.n <= kInPlaceMax && in_place_plan(a, lanes * (lanes == 1024 ? 16 : 8)).blocks < (1LL << 32) / lanes;
 }
 
 hipError_t launch_kv_gather(const KvGatherArgs& a, hipStream_t s) {
     return by_width(a.to.dh, [&](auto w) {
         constexpr int DH = decltype(w)::value;
-        if (in_place(a)) return a.to.n <= kInPlaceFew ? launch_in_place<DH, 256, 8>(a, s) : launch_in_place<DH, 1024, 16>(a, s);
+        if (in_place(a)) {
+            switch (in_place_lanes(a)) {
+                case 256: return launch_in_place<DH, 256, 8>(a, s);
+                case 512: return launch_in_place<DH, 512, 8>(a, s);
+                default: return launch_in_place<DH, 1024, 16>(a, s);
+            }
+        }
         const long long rows = (long long)a.to.n * a.to.heads;
         const int blocks = (int)std::max<long long>(1, std::min<long long>((a.to.cap * (DH / 32) + 255) / 256, 8192 / rows));
         hipLaunchKernelGGL((kv_gather_kernel<DH>), dim3((unsigned)rows, blocks), dim3(256), 0, s, a);

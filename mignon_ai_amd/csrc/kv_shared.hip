@@ -11,9 +11,18 @@ namespace {
 
 // ---- rows over a prefix --------------------------------------------------------------------------------------------
 // The rows of a prefix and key/value head are those of all its sequences, tokens and the heads of the group, one after another. A
-// workgroup takes 32 rows a wave, RW waves, over a chunk of the prefix's tiles, which come into LDS as they are, three ahead, and are
-// unpacked once for all waves while the tile before is worked on (the layouts are Unpacked's). All rows see all of a prefix, so there are
-// no masks but behind its end, and a block of NaN belongs to every row.
+// workgroup takes 32 rows a wave, RW waves, over a chunk of the prefix, in steps of 64 slots. A step's codes are loaded straight to
+// registers a step ahead, and unpacked once for all waves into one half of LDS while the waves work on the other (the layouts are
+// Unpacked's); one barrier a step. All rows see all of a prefix, so there are no masks but behind its end, and a block of NaN belongs to
+// every row.
+//
+// Bound by issuing: on this chip products and other vector instructions of a SIMD's waves take turns (8 products of 32 x 32 x 16 and 64
+// fused multiply-adds a wave, four waves a SIMD: 1541 cycles, alone 1026 and 567), so a step costs a wave its 32 products, some 130
+// other instructions and 32 powers, one after another, and its waits. Steps of 64 slots halve the waits of steps of 32: 32 x 32 tokens of 32
+// query heads over 8 of 128, 16384 positions, bf16, 211 GFLOP: 334 -> 277 us (764 TFLOP/s; a large bf16 product reaches 1131); 64
+// conversations 50 -> 35. Not kept: a tile's scores among the powers of the one before (no gain), 64 rows a wave (registers moved to and
+// fro, 503), three workgroups a CU (registers put to memory, 335), the scaled product of fp8 queries and the codes themselves (it drops
+// what is 2^-13 of the largest product: errors of 1e-4 of the sum of magnitudes).
 //
 // For 16-bit queries values and probabilities are fp16, a probability as 2^15 times itself so that what is 2^-29 of a row's largest or less
 // loses bits, not what is 2^-14: one product an output where two bf16 parts of a probability take two, at 11 bits instead of 16. fp16
