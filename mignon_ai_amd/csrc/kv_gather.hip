@@ -37,8 +37,8 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvGatherArgs a) {
     const GatherSlot g{a.to, a.from, len, a.from_lens ? min(max(a.from_lens[parent], 0), kKvMaxPos) : len};
     const size_t to = ((size_t)i * a.to.heads + h) * a.to.cap, from = ((size_t)parent * a.to.heads + h) * a.from.cap;
     const int slots = min(len, a.to.cap), step = gridDim.y * 256;
-    for (int x = blockIdx.y * 256 + threadIdx.x; x < slots * L16; x += step) {
-        const int j = x / L16, at = 16 * (x % L16);
+    for (long long x = blockIdx.y * 256 + threadIdx.x; x < (long long)slots * L16; x += step) {
+        const int j = (int)(x / L16), at = 16 * (int)(x % L16);
         int slot;
         if (!g.find(j, slot)) continue;
         u32x4 k = {}, v = {};
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvGatherArgs a) {
         *(u32x4*)(a.to.k + (to + j) * row + at) = k;
         *(u32x4*)(a.to.v + (to + j) * row + at) = v;
     }
-    for (int j = blockIdx.y * 256 + threadIdx.x; j < slots; j += step) {
+    for (int j = blockIdx.y * 256 + threadIdx.x; j < slots; j += step) {  // (slots and a step stay below 2^31)
         int slot;
         if (!g.find(j, slot)) continue;
 #pragma unroll
@@ -77,13 +77,13 @@ __device__ __forceinline__ uint8_t byte_of(const u32x4& v, uint32_t b) {
     return (uint8_t)(w >> (8 * (b & 3)));
 }
 template <int RB>
-__device__ __forceinline__ void store_first(uint8_t* to, const u32x4& v, uint32_t first, uint32_t slots) {
-    const uint32_t n = min(16u, slots * RB - first);
+__device__ __forceinline__ void store_first(uint8_t* to, const u32x4& v, uint64_t first, uint32_t slots) {
+    const uint32_t n = (uint32_t)min((uint64_t)16, (uint64_t)slots * RB - first);
 #pragma unroll 1
     for (uint32_t b = 0; b < n; b++) to[b] = byte_of(v, b);
 }
 template <int RB>
-__device__ __forceinline__ void store_some(uint8_t* to, const u32x4& v, const GatherSlot& g, uint32_t first) {
+__device__ __forceinline__ void store_some(uint8_t* to, const u32x4& v, const GatherSlot& g, uint64_t first) {
 #pragma unroll 1
     for (uint32_t b = 0; b < 16; b++) {
         int slot;
@@ -99,7 +99,7 @@ __device__ __forceinline__ void gather_columns(const KvGatherArgs& a, uint8_t* p
     int shift = 0;  // 2^shift columns at once
     while ((2 << shift) <= per_wg && (moved << (shift + 1)) <= NT * HOLD) shift++;
     const int width = 1 << shift, items = moved << shift;
-    for (uint32_t c1 = c0; c1 < c_end; c1 += width) {
+    for (uint64_t c1 = c0; c1 < c_end; c1 += width) {
         u32x4 x[HOLD];
         uint32_t fine = 0;
 #pragma unroll
@@ -107,10 +107,10 @@ __device__ __forceinline__ void gather_columns(const KvGatherArgs& a, uint8_t* p
             const int n = k * NT + threadIdx.x;
             if (n >= items) continue;
             const uint2 mv = moves[n >> shift];
-            const uint32_t c = c1 + (n & (width - 1));
+            const uint64_t c = c1 + (n & (width - 1));
             if (c >= c_end || 16 * c / RB >= mv.y) continue;
             fine |= 1u << k;
-            x[k] = *(const u32x4*)(base + (mv.x & 0xffff) * seq + 16 * (size_t)c);
+            x[k] = *(const u32x4*)(base + (mv.x & 0xffff) * seq + 16 * c);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -120,8 +120,9 @@ __device__ __forceinline__ void gather_columns(const KvGatherArgs& a, uint8_t* p
             int n = k * NT + threadIdx.x;
             asm volatile("" : "+v"(n));  // (addresses are found again: kept, they would not fit the registers)
             const uint2 mv = moves[n >> shift];
-            const uint32_t c = c1 + (n & (width - 1)), i = mv.x >> 16, parent = mv.x & 0xffff;
-            uint8_t* to = base + i * seq + 16 * (size_t)c;
+            const uint64_t c = c1 + (n & (width - 1));
+            const uint32_t i = mv.x >> 16, parent = mv.x & 0xffff;
+            uint8_t* to = base + i * seq + 16 * c;
             if (!a.from_lens && (16 * c + 15) / RB < mv.y) {
                 *(u32x4*)to = x[k];
             } else if (!a.from_lens) {

@@ -79,14 +79,32 @@ __global__ __launch_bounds__(64 * RW, sizeof(T) == 4 && DH >= 64 ? 1 : 2) void k
     const int h = blockIdx.x % a.c.heads, rest = blockIdx.x / a.c.heads, chunk = rest % a.prefix_chunks, per = a.T * a.group;  // rows a sequence
     int tile = rest / a.prefix_chunks, p = 0, first = 0;
     long long rows = 0;
-    for (;; p++) {
-        if (p == a.prefix.n) return;
-        first = prefix_first(a, p);
-        rows = (long long)max(prefix_first(a, p + 1) - first, 0) * per;
-        const int tiles = (int)((rows + R - 1) / R);
-        if (tile < tiles) break;
-        tile -= tiles;
+    for (;; p += 64) {
+        // 64 prefixes at once: their rows, their row tiles, and the tiles of those before
+        if (p >= a.prefix.n) return;
+        const int mine = p + lane, from = mine < a.prefix.n ? prefix_first(a, mine) : 0;
+        const int count = mine < a.prefix.n ? max(prefix_first(a, mine + 1) - from, 0) : 0;
+        const int tiles = (int)(((long long)count * per + R - 1) / R);
+        int until = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int before = __shfl_up(until, o, 64);
+            until += lane >= o ? before : 0;
+        }
+        const uint64_t past = __ballot(until > tile);
+        if (past) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            tile -= __shfl(until - tiles, at, 64);
+            first = __shfl(from, at, 64);
+            rows = (long long)__shfl(count, at, 64) * per;
+            p += at;
+            break;
+        }
+        tile -= __shfl(until, 63, 64);
     }
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    first = __builtin_amdgcn_readfirstlane(first);
+    p = __builtin_amdgcn_readfirstlane(p);
     const PrefixSpan span = prefix_span(a, p);
     const int o0 = chunk * span.each, o1 = min(span.steps, o0 + span.each);
     if (o0 >= o1) return;
@@ -371,9 +389,15 @@ size_t parts_bytes(const KvSharedArgs& a, const PrefixPlan& p) {
 
 }  // namespace
 
-// The parts, then the workspace of the rows' own attention.
+// The parts, then the workspace of the rows' own attention; for rows of any type.
 size_t kv_shared_ws_bytes(const KvSharedArgs& a) {
-    return own_ws_bytes(a, attn_plan(a)) + parts_bytes(a, prefix_plan(a));
+    size_t parts = 0;
+    for (const int type : {REAL_F32, REAL_BF16}) {
+        KvSharedArgs b = a;
+        b.type = type;
+        parts = std::max(parts, parts_bytes(b, prefix_plan(b)));
+    }
+    return own_ws_bytes(a, attn_plan(a)) + parts;
 }
 bool kv_shared_fits(const KvSharedArgs& a) {
     const PrefixPlan p = prefix_plan(a);

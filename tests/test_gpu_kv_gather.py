@@ -170,3 +170,19 @@ def test_refusals_of_tensors():
         c.gather(i, i, source=KVCache(c.k, c.k_scales, d.v.repeat(2, 1, 1, 1)[:3].contiguous(), c.v_scales))
     with pytest.raises(MignonError):
         c.gather(None, i)
+
+
+def test_in_place_past_2_to_28_pieces():
+    """A head's plane of more than 2^28 pieces of 16 bytes: byte offsets within it pass 32 bits."""
+    cap = (1 << 28) + 64
+    a = [torch.empty((2, 1, cap, w), dtype=torch.uint8, device="cuda") for w in (16, 1) * 2]
+    c = KVCache(*a)
+    tails = []
+    for t in a:
+        t[:, :, :1000] = torch.randint(0, 256, t[:, :, :1000].shape, dtype=torch.uint8, device="cuda")
+        t[:, :, -1000:] = torch.randint(0, 256, t[:, :, -1000:].shape, dtype=torch.uint8, device="cuda")
+        tails.append((t[:, :, :1000].clone(), t[:, :, -1000:].clone()))
+    c.gather(ints([1, 0]), ints([cap, cap - 3]))
+    for t, (first, last) in zip(a, tails):
+        assert torch.equal(t[:, :, :1000], first.flip(0))
+        assert torch.equal(t[0, :, -1000:], last[1]) and torch.equal(t[1, :, -1000:-3], last[0, :, :-3]) and torch.equal(t[1, :, -3:], last[1, :, -3:])

@@ -410,3 +410,27 @@ def test_a_beam_search():
         # fp32 throughout: twelve steps, each with logits of a few tens from sums of D products (D 2^-24 of the sum of magnitudes,
         # which |o + x| |w|, some 128 x 1 x 0.3, bounds by 50): 12 * 2 * 50 * 128 * 2^-24 = 9e-3
         assert abs(want - score[b]) <= 9e-3, (b, want, score[b])
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_many_prefixes(t):
+    """More prefixes than a wave has lanes, most of them of few sequences or none, some longer than a workgroup's rows."""
+    r = np.random.default_rng(3)
+    m, n = 150, 420
+    starts = np.sort(np.concatenate([[2], r.integers(0, n, m - 20), np.full(19, 100)]))
+    starts = np.concatenate([starts, [n - 1]])
+    starts[-30:-1] = np.minimum(starts[-30:-1], 200)  # (one prefix has the last two hundred)
+    starts = np.sort(starts)
+    own = Filled(r.integers(1, 20, n).tolist(), 1, 32, 32, 0, 1)
+    prefix = Filled(r.integers(0, 70, m).tolist(), 1, 32, 96, 0, 5)
+    q = rows((n, 1, 2, 32), 9, t)
+    check(own, prefix, starts.tolist(), q, [x - 1 for x in own.lens], [1] * n)
+
+
+def test_tokens_without_a_count_and_scale_zero():
+    """counts None: all rows; a scale of zero: all positions alike; a negative window: none."""
+    own, prefix = Filled([9, 5], 2, 32, 64, 0, 1), Filled((40,), 2, 32, 64, 0, 5)
+    q = rows((2, 3, 2, 32), 9)
+    out = own.c.attention_shared(q, torch.empty_like(q), ints([6, 2]), prefix.c, ints([40]), window=-3, scale=0.0)
+    want, tol = reference(own, prefix, [40], (0, 2), q, [6, 2], [3, 3], 0, 0.0)
+    assert (np.abs(num(out) - want) <= tol + 2.0 ** -24 * np.abs(want)).all()
