@@ -421,14 +421,19 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs a, int sp
     }
 }
 
+// A wave a row where rows are short, or so many that waves alone fill the chip (then each finds its first candidates once), four elsewhere; long
+// rows in segments where there are fewer than 512. us, a wave a row and four: 16384 rows of 1000 bf16 17.8 and 52; of 2048 fp32 with 5
+// alternatives 34 and 102, of 4096 53 and 108, of 8192 101 and 128, without 93 and 87; 4096 of 32768 with 5 105 and 100; 2048 of 8192 with 5
+// 18.8 and 22, 1024 14.9 and 11.2; 64 of 4096 13.3 and 9.1. Segments for 512 workgroups and for 2048: 512 rows of 100003 bf16 without
+// alternatives 22.6 and 26.4, with 16 50 and 63; 32 of 131072 19.6 and 19.4.
 struct LogprobPlan {
     int waves, splits, segment;
 };
 LogprobPlan logprob_plan(const LogprobArgs& a) {
     LogprobPlan p;
-    p.waves = a.V <= 2048 ? 1 : 4;
+    p.waves = a.V <= 2048 || (a.n >= 2048 && a.V <= (a.k ? 8192 : 4096)) ? 1 : 4;
     const int tile = kTile * p.waves, tiles = (a.V - 1) / tile + 1;
-    const int want = std::min(64, std::max(1, std::min(tiles, 1024 / std::max(a.n, 1))));
+    const int want = std::min(64, std::max(1, std::min(tiles, 512 / std::max(a.n, 1))));
     p.segment = (tiles + want - 1) / want * tile;
     p.splits = (a.V - 1) / p.segment + 1;
     return p;
