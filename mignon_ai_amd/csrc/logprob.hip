@@ -351,8 +351,8 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int splits,
     }
 }
 
-// A row's segments: sums at the largest maximum, and the k largest of their k largest keys each. Of `splits` lists in order, the smallest of
-// the ceil(k / splits)-th keys bounds the k-th of all.
+// A row's segments (64 at most): sums at the largest maximum, and the k largest of their k largest keys each. The k-th of the lists' first keys is
+// at most the k-th of all; few more than k reach it.
 template <class T>
 __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs a, int splits) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -387,18 +387,26 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs a, int sp
     }
     if (!a.k) return;
     uint64_t* keys = (uint64_t*)smem;
-    __shared__ uint64_t s_best[kMaxTop];
+    __shared__ uint64_t s_best[kMaxTop], s_heads[192], s_low;
     __shared__ int s_count;
     if (l == 0) s_count = 0;
-    const int deep = (a.k + splits - 1) / splits;
-    uint64_t low = ~0ull;
-    if (w < splits) low = ((const uint64_t*)(parts + w * part_bytes(a.k) + sizeof(Part)))[deep - 1];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t other = __shfl_xor((unsigned long long)low, o, 64);
-        low = other < low ? other : low;
+    // the k-th of the lists' first keys, some 2 k of them
+    const int deep = min(a.k, (2 * a.k - 1) / splits + 1), heads = splits * deep;  // k to 2 k + 63
+    uint64_t key = 0;
+    if (l < heads) {
+        const int s = l / deep;
+        key = ((const uint64_t*)(parts + s * part_bytes(a.k) + sizeof(Part)))[l - s * deep];
+        s_heads[l] = key;
     }
     __syncthreads();
+    if (l < heads) {
+        int above = 0;  // (0: no key, all alike)
+#pragma unroll 16
+        for (int j = 0; j < heads; j++) above += s_heads[j] > key || (s_heads[j] == key && j < l);
+        if (above == a.k - 1) s_low = key;
+    }
+    __syncthreads();
+    const uint64_t low = s_low;
     for (int c = l; c < splits * a.k; c += 256) {
         const int s = c / a.k;
         const uint64_t key = ((const uint64_t*)(parts + s * part_bytes(a.k) + sizeof(Part)))[c - s * a.k];
