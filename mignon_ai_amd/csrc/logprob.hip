@@ -11,9 +11,9 @@
 // each. Later tiles are held to the bound so far, and one whose lanes' maxima all fail it (most do) costs nothing more. Candidates are put in
 // order by counting, for each, those above it. A wave does all that by itself; up to four share a row, and meet at its end.
 //
-// Bound by memory without alternatives (16384 rows of 8192 fp32 logits, 537 MB: 85 to 90 us, 6.1 TB/s; 512 of 100003 bf16 26, 4 TB/s), by the
-// first tiles' candidates with them (the same 512 with 1, 5, 16 and 64 alternatives: 37 42 51 137; all four waves agreeing on a bound tile by
-// tile took 54 60 66 118), by latency for few rows (16 of 8192 with 5: 7.6; one of 131072 with 20: 12 and 4.8 to join 16 segments).
+// Bound by memory without alternatives (16384 rows of 8192 fp32 logits, 537 MB: 85 to 90 us, 6.1 TB/s; 512 of 100003 bf16 23.7, 4.3 TB/s), by the
+// first tiles' candidates with them (the same 512 with 1, 5, 16 and 64 alternatives: 37 43 52 93; all four waves agreeing on a bound tile by
+// tile took 54 60 66 118), by latency for few rows (16 of 8192 with 5: 7.6; one of 131072 with 20: 12 and 4.7 to join 16 segments).
 #include "logprob.hpp"
 
 #include <algorithm>
