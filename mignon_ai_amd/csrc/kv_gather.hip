@@ -221,7 +221,7 @@ hipError_t launch_kv_gather(const KvGatherArgs& a, hipStream_t s) {
             }
         }
         const long long rows = (long long)a.to.n * a.to.heads;
-        const int blocks = (int)std::max<long long>(1, std::min<long long>((a.to.cap * (DH / 32) + 255) / 256, 8192 / rows));
+        const int blocks = (int)std::max<long long>(1, std::min(((long long)a.to.cap * (DH / 32) + 255) / 256, 8192 / rows));
         hipLaunchKernelGGL((kv_gather_kernel<DH>), dim3((unsigned)rows, blocks), dim3(256), 0, s, a);
         return hipGetLastError();
     });
