@@ -27,7 +27,8 @@ namespace {
 // For 16-bit queries values and probabilities are fp16, a probability as 2^15 times itself so that what is 2^-29 of a row's largest or less
 // loses bits, not what is 2^-14: one product an output where two bf16 parts of a probability take two, at 11 bits instead of 16. fp16
 // holds a 4-bit number exactly if its scale lies in 2^-23 .. 2^13 (bytes 104 to 140); a workgroup that meets another one (with codes that
-// are not all zero), or scores far from zero (kFar), goes over its tiles again in the careful form, which is that of kv_attention.hpp.
+// are not all zero), or scores far from zero (a maximum of kFar or more at any step: its rounding may put a probability past what fp16, or
+// fp32, holds), goes over its tiles again in the careful form, which is that of kv_attention.hpp.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(64 * RW, sizeof(T) == 4 && DH >= 64 ? 1 : 2) void k
             }
         }
     };
-    uint32_t low = ~0u, high = ~0u;  // of scale bytes less 1, and less 141, the least (fp16_lacks)
+    uint32_t low = ~0u, high = ~0u;  // of scale bytes less 1, and less 141, the least; low is 0 once a reference was far from zero
     auto give = [&](auto careful, Raw& w, uint8_t* out, int o) {
         using Fm = Forms<T, decltype(careful)::value>;
         const int left = span.held - o * 2 * kTile;
@@ -292,6 +293,7 @@ __global__ __launch_bounds__(64 * RW, sizeof(T) == 4 && DH >= 64 ? 1 : 2) void k
                 const float mn = fmaxf(m, fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])));
                 const float now = mn == -INFINITY ? -Fm::lift : mn * scale - Fm::lift;
                 const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - now);  // (0: there is nothing yet)
+                if (fabsf(now) >= kFar) low = 0;  // (also where a nearer one follows)
                 m = mn;
                 ref = now;
                 l *= al;
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(64 * RW, sizeof(T) == 4 && DH >= 64 ? 1 : 2) void k
         barrier();
     };
     sweep(std::false_type());
-    if (__syncthreads_or(low < 103u || high < 114u || fabsf(ref) >= kFar)) sweep(std::true_type());
+    if (__syncthreads_or(low < 103u || high < 114u)) sweep(std::true_type());
     const float total = l + __shfl_xor(l, 32, 64);
     if (!there) return;
     // lane (i, g): row i, channels 32 x + 8 r + 4 g .. + 3
