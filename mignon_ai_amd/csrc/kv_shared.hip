@@ -26,9 +26,9 @@ namespace {
 //
 // For 16-bit queries values and probabilities are fp16, a probability as 2^15 times itself so that what is 2^-29 of a row's largest or less
 // loses bits, not what is 2^-14: one product an output where two bf16 parts of a probability take two, at 11 bits instead of 16. fp16
-// holds a 4-bit number exactly if its scale lies in 2^-23 .. 2^13 (bytes 104 to 140); a workgroup that meets another one (with codes that
-// are not all zero), or scores far from zero (a maximum of kFar or more at any step: its rounding may put a probability past what fp16, or
-// fp32, holds), goes over its tiles again in the careful form, which is that of kv_attention.hpp.
+// holds a 4-bit number exactly if its scale lies in 2^-23 .. 2^13 (bytes 104 to 140); a workgroup that meets another one (byte 0 with
+// codes of zero is none: those are zeros), or scores far from zero (a maximum of kFar or more at any step: its rounding may put a
+// probability past what fp16, or fp32, holds), goes over its tiles again in the careful form, which is that of kv_attention.hpp.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -164,7 +164,10 @@ __global__ __launch_bounds__(64 * RW, sizeof(T) == 4 && DH >= 64 ? 1 : 2) void k
             }
         }
     };
-    uint32_t low = ~0u, high = ~0u;  // of scale bytes less 1, and less 141, the least; low is 0 once a reference was far from zero
+    // Of scale bytes, and of them less 141, the least; byte 0 of a block of zeros (kSize: codes' bits without signs) counts as 104. low is 0
+    // once a reference was far from zero, too.
+    constexpr uint32_t kSize = 0x77777777u;
+    uint32_t low = ~0u, high = ~0u;
     auto give = [&](auto careful, Raw& w, uint8_t* out, int o) {
         using Fm = Forms<T, decltype(careful)::value>;
         const int left = span.held - o * 2 * kTile;
@@ -172,7 +175,15 @@ __global__ __launch_bounds__(64 * RW, sizeof(T) == 4 && DH >= 64 ? 1 : 2) void k
         for (int x = 0; x < NK; x++) {
             if (KN % NT && tid + NT * x >= KN) break;
             if (Fm::key_half) {
-                low = min(low, w.ks[x] - 1u);
+                uint32_t least = w.ks[x];
+                if (least == 0) {
+                    asm volatile("");  // a branch: blocks of zeros are rare
+                    uint32_t codes = 0;
+#pragma unroll
+                    for (int e = 0; e < KV; e++) codes |= w.k[x][e];
+                    least = codes & kSize ? 0 : 104;
+                }
+                low = min(low, least);
                 high = min(high, w.ks[x] - 141u);
             }
             const float sc = mx4_scale(w.ks[x]);
@@ -196,7 +207,14 @@ __global__ __launch_bounds__(64 * RW, sizeof(T) == 4 && DH >= 64 ? 1 : 2) void k
         for (int x = 0; x < NV; x++) {
             if (VN % NT && tid + NT * x >= VN) break;
             if (Fm::value_half) {
-                low = min(low, min(w.vs[x][0] - 1u, w.vs[x][1] - 1u));
+                uint32_t least = min(w.vs[x][0], w.vs[x][1]);
+                if (least == 0) {
+                    asm volatile("");
+                    least = 104;
+#pragma unroll
+                    for (int y = 0; y < 2; y++) least = min(least, w.vs[x][y] == 0 && (w.v[x][y] & kSize) == 0 ? 104u : w.vs[x][y]);
+                }
+                low = min(low, least);
                 high = min(high, min(w.vs[x][0] - 141u, w.vs[x][1] - 141u));
             }
             const float s0 = mx4_scale(w.vs[x][0]), s1 = mx4_scale(w.vs[x][1]);
@@ -346,7 +364,7 @@ __global__ __launch_bounds__(64 * RW, sizeof(T) == 4 && DH >= 64 ? 1 : 2) void k
         barrier();
     };
     sweep(std::false_type());
-    if (__syncthreads_or(low < 103u || high < 114u)) sweep(std::true_type());
+    if (__syncthreads_or(low < 104u || high < 114u)) sweep(std::true_type());
     const float total = l + __shfl_xor(l, 32, 64);
     if (!there) return;
     // lane (i, g): row i, channels 32 x + 8 r + 4 g .. + 3
