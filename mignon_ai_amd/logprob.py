@@ -25,7 +25,11 @@ def token_logprobs(logits, targets=None, k: int = 0) -> dict:
     out = {"entropy": np.empty(n, np.float32)}
     t = None
     if targets is not None:
-        shape = np.shape(targets)
+        targets = np.asarray(targets)
+        shape = targets.shape
+        if targets.dtype.kind in "iu" and targets.dtype != np.int32:
+            # (what is left of an id in 32 bits could be another's)
+            targets = np.where((targets >= 0) & (targets < V), targets.astype(np.int32), np.int32(-1))
         t = np.ascontiguousarray(targets, np.int32).reshape(n, -1) if shape[:1] == (n,) and len(shape) <= 2 and n else np.empty((0, 0), np.int32)
         if n and shape not in ((n,), t.shape):
             mx4._invalid("token_logprobs: targets are [n] or [n][m]")

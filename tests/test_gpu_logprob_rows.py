@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import many_ref as R
+from mignon_ai_amd import token_logprobs
 from test_gpu_logprob import TYPES, call, rows
 
 pytestmark = pytest.mark.gpu
@@ -143,3 +144,16 @@ def test_rows_alone_and_in_company(V):
                 a, b = one[key][0], other[key][i]
                 with np.errstate(invalid="ignore"):
                     assert ((a == b) | (np.isnan(a) & np.isnan(b)) | (np.abs(a - b) <= 2 * tol[key][i])).all(), (key, i)
+
+
+def test_ids_past_32_bits_are_outside_the_vocabulary():
+    """Host targets of any integer type: an id is what it says, not what is left of it in 32 bits."""
+    x = rows(3, 50, 1).numpy()
+    ids = np.array([[7, 2 ** 32 + 7, -2 ** 32 + 7], [3, 2 ** 31, 2 ** 63 - 1], [0, -2 ** 31 - 1, 49]], np.int64)
+    got = token_logprobs(x, ids)["logprob"]
+    want = token_logprobs(x, np.where((ids >= 0) & (ids < 50), ids, -1).astype(np.int32))["logprob"]
+    assert np.array_equal(got, want, equal_nan=True)
+    assert np.array_equal(np.isnan(got), (ids < 0) | (ids >= 50))
+    big = token_logprobs(x, np.array([2 ** 64 - 1, 2 ** 32, 5], np.uint64))["logprob"]
+    assert np.isnan(big[:2]).all() and big[2] == token_logprobs(x, [0, 0, 5])["logprob"][2]
+    assert token_logprobs(x, np.array([1, 2, 3], np.uint8))["logprob"].tolist() == token_logprobs(x, [1, 2, 3])["logprob"].tolist()
