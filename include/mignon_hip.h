@@ -391,7 +391,7 @@ int mg_kv_attention_shared(const mg_kv_cache_t* cache, const mg_kv_cache_t* pref
 
 /* ---- Log probabilities (no reference counterpart: mg_score_sequences and mg_forward_batch give those of a model's own targets) ----
  * For n rows of logits [n][V] (row stride ld >= V elements; MG_F32, MG_F16 or MG_BF16; V up to 2^30):
- *   logprob [n][m]      log-softmax of tokens targets [n][m] (NaN for an id outside [0, V))
+ *   logprob [n][m]      log-softmax of tokens targets [n][m] (NaN for an id outside [0, V)); m up to 2^30
  *   entropy [n]         -sum p log p, in nats (a token of probability 0 adds nothing)
  *   top_ids, top_logprob [n][k]  the k (0..min(V, 64)) largest logits, the likeliest first, the lowest id first among equals
  * all optional but for targets with logprob where m > 0 and one of the last two where k > 0; statistics in fp32. A row with a NaN or a

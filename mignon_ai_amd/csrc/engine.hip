@@ -2876,7 +2876,7 @@ int mg_token_logprobs(const void* logits, int type, int n, int V, long long ld, 
                       void* stream) {
     return guarded([&] {
         REQUIRE(real_type(type), "mg_token_logprobs: unknown type");
-        REQUIRE(n >= 0 && V > 0 && V <= kLogprobMaxV && ld >= V && m >= 0, "mg_token_logprobs: bad shape");
+        REQUIRE(n >= 0 && V > 0 && V <= kLogprobMaxV && ld >= V && m >= 0 && m <= kLogprobMaxTargets, "mg_token_logprobs: bad shape");
         REQUIRE(k >= 0 && k <= std::min(V, kMaxTop), "mg_token_logprobs: k is at most " + std::to_string(kMaxTop) + " and the vocabulary");
         if (n == 0) return MG_OK;  // (an empty tensor has no address)
         REQUIRE(logits && (m == 0 || (targets && logprob)) && (k == 0 || top_ids || top_logprob), "mg_token_logprobs: null argument");

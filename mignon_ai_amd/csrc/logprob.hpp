@@ -8,7 +8,7 @@
 
 namespace mg {
 
-constexpr int kMaxTop = 64, kLogprobMaxV = 1 << 30;
+constexpr int kMaxTop = 64, kLogprobMaxV = 1 << 30, kLogprobMaxTargets = 1 << 30;  // (a lane counts in steps of 256: below 2^31)
 
 struct LogprobArgs {
     const void* x = nullptr;           // logits [n][V], row stride ld elements

@@ -1,0 +1,23 @@
+"""Limits of log probabilities: what a call that is too large, or asks for a number of alternatives below zero, is told before anything touches a
+device."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import mignon_ai_amd as M
+from mignon_ai_amd import _lib
+
+
+def call(n=1, V=8, m=1, k=0):
+    buf = (ctypes.c_uint8 * 4096)()  # never read by a refused call
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    rc = _lib.lib().mg_token_logprobs(p, 0, n, V, V, p, m, k, p, p, p, p, None, 0, _lib.MG_PTR_DEVICE, None)
+    return rc, _lib.lib().mg_last_error().decode()
+
+
+@pytest.mark.parametrize("m", [2 ** 30 + 1, 2 ** 31 - 256, 2 ** 31 - 1])
+def test_targets_past_what_a_lane_counts_to(m):
+    """A lane's targets are 256 apart: its count stays below 2^31."""
+    rc, error = call(m=m)
+    assert rc == _lib.MG_ERR_INVALID and "shape" in error
