@@ -460,7 +460,12 @@ hipError_t launch_rows(const LogprobArgs& a, const LogprobPlan& p, hipStream_t s
 
 }  // namespace
 
-bool logprob_fits(const LogprobArgs& a) { return (long long)a.n * logprob_plan(a).splits < 1 << 24; }
+// (a launch's 2^32 lanes; a workgroup takes four rows of a wave each)
+bool logprob_fits(const LogprobArgs& a) {
+    const LogprobPlan p = logprob_plan(a);
+    const int teams = 4 / p.waves;
+    return ((long long)a.n * p.splits + teams - 1) / teams < 1 << 24;
+}
 size_t logprob_ws_bytes(const LogprobArgs& a) {
     const LogprobPlan p = logprob_plan(a);
     return p.splits > 1 ? (size_t)a.n * p.splits * part_bytes(a.k) : 0;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import many_ref as R
-from mignon_ai_amd import token_logprobs
+from mignon_ai_amd import token_logprobs, token_logprobs_device
 from test_gpu_logprob import TYPES, call, rows
 
 pytestmark = pytest.mark.gpu
@@ -157,3 +157,15 @@ def test_ids_past_32_bits_are_outside_the_vocabulary():
     big = token_logprobs(x, np.array([2 ** 64 - 1, 2 ** 32, 5], np.uint64))["logprob"]
     assert np.isnan(big[:2]).all() and big[2] == token_logprobs(x, [0, 0, 5])["logprob"][2]
     assert token_logprobs(x, np.array([1, 2, 3], np.uint8))["logprob"].tolist() == token_logprobs(x, [1, 2, 3])["logprob"].tolist()
+
+
+def test_more_rows_than_workgroups():
+    """2^24 short rows and more: four a workgroup."""
+    n, V = (1 << 24) + 5, 3
+    x = torch.randn((n, V), generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    entropy, ids = torch.full((n,), 77.0, device="cuda"), torch.full((n, 1), -5, dtype=torch.int32, device="cuda")
+    token_logprobs_device(x, entropy=entropy, top_ids=ids)
+    assert torch.equal(ids[:, 0].long(), x.argmax(-1))
+    p = torch.log_softmax(x.double(), -1)
+    # the statistics of three logits (R.logprobs): entropy and its parts are below 2, a logit's distance from the largest below 12
+    assert float((entropy + (p.exp() * p).sum(-1)).abs().max()) <= 2 * (chain(1) + 14 * 2.0 ** -22) * 2

@@ -21,3 +21,10 @@ def test_targets_past_what_a_lane_counts_to(m):
     """A lane's targets are 256 apart: its count stays below 2^31."""
     rc, error = call(m=m)
     assert rc == _lib.MG_ERR_INVALID and "shape" in error
+
+
+def test_rows_past_a_launch():
+    """2^24 workgroups: of four short rows, or of one."""
+    for n, V in ((2 ** 26, 8), (2 ** 24, 10000)):
+        rc, error = call(n=n, V=V)
+        assert rc == _lib.MG_ERR_INVALID and "too many rows" in error
