@@ -34,10 +34,11 @@ def token_logprobs(logits, targets=None, k: int = 0) -> dict:
         if n and shape not in ((n,), t.shape):
             mx4._invalid("token_logprobs: targets are [n] or [n][m]")
         out["logprob"] = np.empty(shape, np.float32)
-    if k:
-        out["top_ids"], out["top_logprob"] = np.empty((n, int(k)), np.int32), np.empty((n, int(k)), np.float32)
+    k = min(max(int(k), -1), 65)  # (the library refuses fewer than none and more than 64)
+    if k > 0:
+        out["top_ids"], out["top_logprob"] = np.empty((n, k), np.int32), np.empty((n, k), np.float32)
     m = 0 if t is None else t.shape[1]
-    check(lib().mg_token_logprobs(ptr(x), mx4._HOST_TYPES[x.dtype], n, V, V, ptr(t) if m else None, m, int(k),
+    check(lib().mg_token_logprobs(ptr(x), mx4._HOST_TYPES[x.dtype], n, V, V, ptr(t) if m else None, m, k,
                                   ptr(out["logprob"]) if m else None, ptr(out["entropy"]), ptr(out.get("top_ids")),
                                   ptr(out.get("top_logprob")), None, 0, 0, None))
     return out

@@ -28,3 +28,9 @@ def test_rows_past_a_launch():
     for n, V in ((2 ** 26, 8), (2 ** 24, 10000)):
         rc, error = call(n=n, V=V)
         assert rc == _lib.MG_ERR_INVALID and "too many rows" in error
+
+
+@pytest.mark.parametrize("k", [-1, -3, 65, 2 ** 32, 2 ** 32 + 1, -2 ** 32 + 1])
+def test_numbers_of_alternatives(k):
+    with pytest.raises(M.MignonError, match="k is"):
+        M.token_logprobs(np.zeros((2, 100), np.float32), k=k)
