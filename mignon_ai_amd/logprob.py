@@ -22,6 +22,8 @@ def token_logprobs(logits, targets=None, k: int = 0) -> dict:
     if x.ndim != 2 or x.shape[1] == 0:
         mx4._invalid("token_logprobs: a matrix is needed")
     n, V = x.shape
+    if n >> 31 or V >> 31:
+        mx4._invalid("token_logprobs: rows and logits of a row are fewer than 2^31")
     out = {"entropy": np.empty(n, np.float32)}
     t = None
     if targets is not None:

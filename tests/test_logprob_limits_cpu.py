@@ -34,3 +34,10 @@ def test_rows_past_a_launch():
 def test_numbers_of_alternatives(k):
     with pytest.raises(M.MignonError, match="k is"):
         M.token_logprobs(np.zeros((2, 100), np.float32), k=k)
+
+
+@pytest.mark.parametrize("shape", [(2 ** 32 + 3, 1), (2 ** 31, 1), (1, 2 ** 32 + 3), (1, 2 ** 31)])
+def test_host_arrays_past_32_bits(shape):
+    """Sizes that the library's 32 bits do not hold (memory that is never touched)."""
+    with pytest.raises(M.MignonError, match="fewer than 2\\^31"):
+        M.token_logprobs(np.zeros(shape, np.float16))
