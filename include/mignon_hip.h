@@ -374,7 +374,7 @@ int mg_kv_attention(const mg_kv_cache_t* cache, const mg_kv_rows_t* q, const mg_
  * (both [to->n]), where parents[i] is in [0, from->n); elsewhere it stays as it is. What `to` holds of such a length is written, and its
  * other slots are left as they are. from_lens [from->n]: the lengths of `from`'s sequences (NULL: as long as what becomes of them); a
  * position that `from` no longer holds, or never held, becomes zeros, as mg_kv_read reads it. `from` NULL or `to` itself: in place, as if
- * from a copy taken before, for at most 16384 sequences. Otherwise the caches share no memory and may differ in n, capacity and sinks.
+ * from a copy taken before, for at most 16384 sequences (of less than 64 GB each). Otherwise the caches share no memory and may differ in n, capacity and sinks.
  * Ended sequences need no call: a place is free once nothing asks for it. */
 int mg_kv_gather(const mg_kv_cache_t* to, const mg_kv_cache_t* from, const int32_t* parents, const int32_t* lens,
                  const int32_t* from_lens, void* stream);

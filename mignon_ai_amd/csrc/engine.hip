@@ -2820,7 +2820,7 @@ int mg_kv_gather(const mg_kv_cache_t* to, const mg_kv_cache_t* from, const int32
                     REQUIRE(x.first >= y.second || y.first >= x.second, "mg_kv_gather: two caches that share some of their memory");
         }
         a.parents = parents; a.lens = lens; a.from_lens = from_lens;
-        REQUIRE(kv_gather_fits(a), "mg_kv_gather: too many sequences");
+        REQUIRE(kv_gather_fits(a), "mg_kv_gather: too many sequences, or too long ones");
         HIPCHECK(launch_kv_gather(a, (hipStream_t)stream));
         return MG_OK;
     });

@@ -26,8 +26,9 @@ struct GatherSlot {
 };
 
 // Another cache's: a workgroup a sequence, head and stretch of slots, a lane 16 bytes of codes of K and V; then the scales, a slot a lane.
-// Bound by memory: 64 sequences of 1500 to 3000 positions, 8 heads of 128, 131 MB read and written: 23 us where the source stays in the
-// caches (5.7 TB/s), 41 from call to call of other data.
+// 64 sequences of 1500 to 3000 positions, 8 heads of 128, 131 MB read and written: 23 us where the source stays in the caches (5.7 TB/s), and
+// 41 on other data each call, where a plain copy of as many bytes takes 26: a lane asks for one pair of pieces, waits, and stores it before the
+// next, and scales go byte by byte.
 template <int DH>
 __global__ __launch_bounds__(256) void kv_gather_kernel(KvGatherArgs a) {
     constexpr int row = DH / 2, L16 = row / 16, NB = DH / 32;
@@ -67,8 +68,10 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvGatherArgs a) {
 // A lane holds HOLD pieces of 16 bytes: up to 512 sequences 256 lanes of 8, up to 2048 512 of 8, up to 16384 1024 of 16, so that whole 64 bytes
 // of a place are taken together. us, half of the sequences becoming copies of the others, 256 x 8, 512 x 8, 1024 x 8 and 1024 x 16: 64 of 1024
 // positions (8 heads of 128) 11.3 14.1 16.5 17; 256 of 1051 (8 of 64) 22 26 29 34; 1024 of 251 (8 of 64) 46 35 33 41; 2000 of 251 (8 of 32)
-// 53 44 49 62; 4096 of 59 (8 of 32) - 51 46 45. Bound by memory for few long sequences (256 streams of 1056 slots, 111 MB read and
-// written: 5 TB/s), then by lines of which a workgroup takes a part, and by the list of moves that each makes (4096: four rounds).
+// 53 44 49 62; 4096 of 59 (8 of 32) - 51 46 45. Few long sequences (256 streams of 1056 slots, half of them moving, 111 MB
+// read and written) take 22 us, 5 TB/s, where they stay in the caches, and 35 on other data each call, where a plain copy of as many bytes takes
+// 22: a workgroup asks for all it holds, 128 bytes of a place, waits, and only then writes. Many are bound by lines of which a workgroup takes
+// a part, and by the list of moves that each makes (4096: four rounds).
 constexpr int kInPlaceMax = 1024 * 16;  // sequences
 
 // Bytes of a piece one by one: up to the first slot that holds no position, or where some may have been lost (zeros).
@@ -174,7 +177,7 @@ bool in_place(const KvGatherArgs& a) { return a.to.k == a.from.k; }
 
 int in_place_lanes(const KvGatherArgs& a) { return a.to.n <= 512 ? 256 : a.to.n <= 2048 ? 512 : 1024; }
 
-// Columns of a workgroup: as many as it holds of all sequences twice over (fewer than all move).
+// Columns of a workgroup: the first power of two, up to 256, of which all sequences together fill its room (fewer than all move).
 struct InPlacePlan {
     int per_wg;
     long long code_blocks, scale_blocks, blocks;

@@ -20,7 +20,7 @@ namespace {
 // fused multiply-adds a wave, four waves a SIMD: 1541 cycles, alone 1026 and 567), so a step costs a wave its 32 products, some 130
 // other instructions and 32 powers, one after another, and its waits. Steps of 64 slots halve the waits of steps of 32: 32 x 32 tokens of 32
 // query heads over 8 of 128, 16384 positions, bf16, 211 GFLOP: 334 -> 277 us (764 TFLOP/s; a large bf16 product reaches 1131); 64
-// conversations 50 -> 35. Not kept: a tile's scores among the powers of the one before (no gain), 64 rows a wave (registers moved to and
+// conversations 50 -> 35 (the checks of scales and scores below take 1 % of either). Not kept: a tile's scores among the powers of the one before (no gain), 64 rows a wave (registers moved to and
 // fro, 503), three workgroups a CU (registers put to memory, 335), the scaled product of fp8 queries and the codes themselves (it drops
 // what is 2^-13 of the largest product: errors of 1e-4 of the sum of magnitudes).
 //
